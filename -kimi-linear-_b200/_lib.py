@@ -52,6 +52,11 @@ EXPORTED = (
     "mla_decode_fwd",
     "mla_decode_workspace_bytes",
     "mla_decode_args_size",
+    "mla_cache_append",
+    "mla_cache_read",
+    "mla_cache_attention",
+    "mla_cache_workspace_bytes",
+    "mla_cache_args_size",
     "kda_args_size",
     "kda_abi_version",
 )
@@ -193,6 +198,35 @@ class MlaDecodeArgs(ctypes.Structure):
     ]
 
 
+class MlaCacheArgs(ctypes.Structure):
+    """Mirror of ``struct MlaCacheArgs``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("io_dtype", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("KVL", ctypes.c_int32), ("DR", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("N", ctypes.c_int32), ("H", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("codes", ctypes.c_void_p), ("codes_stride", _I64x2),
+        ("scales", ctypes.c_void_p), ("scales_stride", ctypes.c_int64),
+        ("rope", ctypes.c_void_p), ("rope_stride", _I64x2),
+        ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("lens", ctypes.c_void_p),
+        ("q_start", ctypes.c_void_p),
+        ("c_kv", ctypes.c_void_p), ("c_kv_stride", ctypes.c_int64),
+        ("k_rope", ctypes.c_void_p), ("k_rope_stride", ctypes.c_int64),
+        ("q_lat", ctypes.c_void_p), ("q_lat_stride", _I64x2),
+        ("q_rope", ctypes.c_void_p), ("q_rope_stride", _I64x2),
+        ("out", ctypes.c_void_p), ("out_stride", _I64x2),
+        ("lse", ctypes.c_void_p), ("lse_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class KdaLibraryError(RuntimeError):
     """The CUDA library is missing or unusable (there is no fallback path)."""
 
@@ -229,6 +263,14 @@ def _declare(lib):
     lib.mla_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.mla_decode_args_size.argtypes = []
     lib.mla_decode_args_size.restype = ctypes.c_size_t
+    C = ctypes.POINTER(MlaCacheArgs)
+    for fn in ("mla_cache_append", "mla_cache_read", "mla_cache_attention"):
+        getattr(lib, fn).argtypes = [C, ctypes.c_void_p]
+        getattr(lib, fn).restype = ctypes.c_int
+    lib.mla_cache_workspace_bytes.argtypes = [C]
+    lib.mla_cache_workspace_bytes.restype = ctypes.c_size_t
+    lib.mla_cache_args_size.argtypes = []
+    lib.mla_cache_args_size.restype = ctypes.c_size_t
     lib.kda_backward.argtypes = [ctypes.POINTER(KdaBackwardArgs), ctypes.c_void_p]
     lib.kda_backward.restype = ctypes.c_int
     lib.kda_backward_ckpt_floats.argtypes = [ctypes.c_int] * 5
@@ -269,7 +311,8 @@ def load(path: str | None = None):
         for fn, st in (("kda_prologue_args_size", KdaPrologueArgs),
                        ("kda_epilogue_args_size", KdaEpilogueArgs),
                        ("kda_backward_args_size", KdaBackwardArgs),
-                       ("mla_decode_args_size", MlaDecodeArgs)):
+                       ("mla_decode_args_size", MlaDecodeArgs),
+                       ("mla_cache_args_size", MlaCacheArgs)):
             if getattr(lib, fn)() != ctypes.sizeof(st):
                 raise KdaLibraryError(f"{p}: {fn}() != ctypes sizeof {ctypes.sizeof(st)}")
         if lib.kda_args_size() != ctypes.sizeof(KdaArgs):

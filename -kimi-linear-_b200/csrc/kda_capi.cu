@@ -372,8 +372,10 @@ int kda_device_supported(int device) {
 int kda_device_error(int clear) {
   const int a = read_device_error(clear != 0);
   const int b = kda::mla::read_device_error(clear != 0);
-  if (a < 0 || b < 0) return -1;
-  return a ? a : b;
+  const int c = kda::cache::read_device_error(clear != 0);
+  const int d = kda::cache::read_attn_device_error(clear != 0);
+  if (a < 0 || b < 0 || c < 0 || d < 0) return -1;
+  return a ? a : b ? b : c ? c : d;
 }
 
 int kda_prologue_fwd(const KdaPrologueArgs* args, void* stream) {

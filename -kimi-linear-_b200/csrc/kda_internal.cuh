@@ -41,6 +41,10 @@ cudaError_t launch_dependent(void (*k)(Params...), dim3 grid, int threads, size_
 namespace mla {
 int read_device_error(bool clear);   // the MLA kernels' error word (mla_decode.cu)
 }
+namespace cache {
+int read_device_error(bool clear);        // latent cache append / read (mla_cache.cu)
+int read_attn_device_error(bool clear);   // latent cache attention (mla_cache_attn.cu)
+}
 
 constexpr int kRecMaxK = 256;    // recurrent kernel: K <= 256, any V
 constexpr int kSimtMaxK = 256;   // SIMT chunkwise kernel: K <= 256, any V

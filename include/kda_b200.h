@@ -9,7 +9,9 @@
  * and, around it, the fused prologue / epilogue of the KDA block
  * (kda_prologue_fwd, kda_epilogue_fwd), the gradient of the core
  * (kda_backward) and the static-buffer MLA decode step of the full-attention
- * layers (mla_decode_fwd, kimi_linear/mla.py:117-181).
+ * layers (mla_decode_fwd, kimi_linear/mla.py:117-181); and, for serving those
+ * layers, a paged latent cache in 8 bits with the attention over it
+ * (mla_cache_append, mla_cache_read, mla_cache_attention).
  *
  * Plain pointers, sizes and element strides only.  The Python host layer
  * (-kimi-linear-_b200/ops.py) keeps the reference's Python signatures and
@@ -334,6 +336,74 @@ size_t mla_decode_workspace_bytes(const MlaDecodeArgs* args);
 
 /* sizeof(MlaDecodeArgs) as compiled. */
 size_t mla_decode_args_size(void);
+
+/*
+ * Paged latent cache in 8 bits and the attention over it, for serving the MLA
+ * layers (kimi_linear/mla.py:183-288: the latent c_kv and the rope key are all
+ * that a layer caches per token).  No counterpart in the reference, which
+ * caches 16-bit latents contiguously.
+ *
+ * The pool holds num_pages pages of page_size tokens.  A token is KVL e4m3
+ * codes, DR rope channels in the 16-bit type and one power-of-two scale s:
+ *   e = max(least e1: amax|c| <= 448 2^e1, least e2: amax|k_rope| <= 2^15 2^e2, -100)
+ *   s = 2^e (NaN when a value of the token is not finite)
+ *   code = e4m3(c / s), rope = 16-bit(k_rope / s), both rounded to nearest even
+ * Sequence b holds lens[b] tokens, its last n_b new: n_b = q_start[b + 1] -
+ * q_start[b], or N / B when q_start is NULL.  New token i of b sits at position
+ * p = lens[b] - n_b + i: slot p % page_size of page block_table[b, p / page_size].
+ *
+ * mla_cache_append: writes codes, scale and rope of c_kv [N, KVL], k_rope
+ *   [N, DR] into their slots.  Tokens with p < 0 are skipped.
+ * mla_cache_read: c_kv, k_rope (outputs) = code s, rope s in the 16-bit type;
+ *   zeros for tokens with p < 0.
+ * mla_cache_attention: for each new token and head, over positions 0 .. p,
+ *   score = scale (q_lat . c + q_rope . k_rope), out = softmax(score) c,
+ *   lse = ln sum exp(score) (may be NULL).  A row that sees nothing: out = 0,
+ *   lse = -inf.  Needs mla_cache_workspace_bytes() of device scratch.
+ *
+ * A position past the table's max_pages or a page outside the pool sets the
+ * device error word (6) where it is met: append skips the token, read gives
+ * zeros, attention ignores positions past the table and gives NaN for a
+ * sequence with a visible page outside the pool.
+ *
+ * Requires 16-bit io_dtype, KVL in {128, 256, 384, 512}, DR in {0, 64},
+ * page_size a power of two from 16 to 1024, num_pages * page_size < 2^31.  Codes and rope rows are unit-stride and start
+ * on 16-byte boundaries; scales have a unit token stride.
+ */
+typedef struct MlaCacheArgs {
+  int32_t abi_version;
+  int32_t io_dtype;            /* c_kv, k_rope, q_lat, q_rope, out and the pool's rope part */
+  int32_t num_pages, page_size, KVL, DR;
+  int32_t B, N, H, max_pages;  /* H: attention only */
+  float scale;                 /* attention only */
+  int32_t reserved;
+  /* pool: strides in elements (page, token); scales: page stride */
+  void* codes;  int64_t codes_stride[2];
+  float* scales; int64_t scales_stride;
+  void* rope;   int64_t rope_stride[2];
+  const int32_t* block_table; int64_t table_stride;   /* [B, max_pages] */
+  const int32_t* lens;                                /* [B] */
+  const int32_t* q_start;                             /* [B + 1] or NULL */
+  /* append (inputs) / read (outputs): row strides in elements */
+  void* c_kv;   int64_t c_kv_stride;
+  void* k_rope; int64_t k_rope_stride;
+  /* attention: (token, head) strides in elements; lse: token stride */
+  const void* q_lat;  int64_t q_lat_stride[2];
+  const void* q_rope; int64_t q_rope_stride[2];
+  void* out;          int64_t out_stride[2];
+  float* lse;         int64_t lse_stride;
+  void* workspace;    size_t workspace_bytes;   /* 256-byte aligned */
+} MlaCacheArgs;
+
+int mla_cache_append(const MlaCacheArgs* args, void* stream);
+int mla_cache_read(const MlaCacheArgs* args, void* stream);
+int mla_cache_attention(const MlaCacheArgs* args, void* stream);
+
+/* device workspace of mla_cache_attention (0 = none, or invalid sizes). */
+size_t mla_cache_workspace_bytes(const MlaCacheArgs* args);
+
+/* sizeof(MlaCacheArgs) as compiled. */
+size_t mla_cache_args_size(void);
 
 /* sizeof(KdaArgs) as compiled, for FFI layout checks. */
 size_t kda_args_size(void);
