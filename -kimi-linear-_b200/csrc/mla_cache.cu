@@ -155,7 +155,7 @@ int validate(const MlaCacheArgs* a) {
     return KDA_ERR_SHAPE;
   if (a->num_pages < 1 || (int64_t)a->num_pages * a->page_size >= (1ll << 31)) return KDA_ERR_SHAPE;
   if (a->B < 0 || a->N < 0 || a->max_pages < 0 || a->max_pages > (1 << 24)) return KDA_ERR_SHAPE;
-  if ((int64_t)a->max_pages * a->page_size >= (1ll << 31)) return KDA_ERR_SHAPE;
+  if ((int64_t)a->max_pages * a->page_size > (1ll << 30)) return KDA_ERR_SHAPE;
   if (a->B == 0 || a->N == 0) return KDA_OK;               // nothing to do
   if (a->q_start == nullptr && a->N % a->B != 0) return KDA_ERR_SHAPE;
   if (!a->codes || !a->scales || (a->DR && !a->rope) || !a->lens ||
@@ -164,13 +164,13 @@ int validate(const MlaCacheArgs* a) {
   if (!aligned16(a->codes) || a->codes_stride[0] % 16 || a->codes_stride[1] % 16 ||
       reinterpret_cast<uintptr_t>(a->scales) % 4)
     return KDA_ERR_ALIGNMENT;
-  if (a->codes_stride[0] < 0 || a->codes_stride[1] < a->KVL || a->scales_stride < 0 ||
+  if (a->codes_stride[0] < (a->num_pages > 1) || a->codes_stride[1] < a->KVL || a->scales_stride < 0 ||
       a->table_stride < 0)
     return KDA_ERR_STRIDE;
   if (a->DR) {
     if (!aligned16(a->rope) || a->rope_stride[0] % 8 || a->rope_stride[1] % 8)
       return KDA_ERR_ALIGNMENT;
-    if (a->rope_stride[0] < 0 || a->rope_stride[1] < a->DR) return KDA_ERR_STRIDE;
+    if (a->rope_stride[0] < (a->num_pages > 1) || a->rope_stride[1] < a->DR) return KDA_ERR_STRIDE;
   }
   return KDA_OK;
 }
@@ -225,7 +225,7 @@ int run_tokens(const MlaCacheArgs* a, bool append, void* stream) {
 int validate_attention(const MlaCacheArgs* a) {
   const int st = validate(a);
   if (st != KDA_OK) return st;
-  if (a->H < 0 || a->H > 1024 || (int64_t)a->N * a->H >= (1ll << 31)) return KDA_ERR_SHAPE;
+  if (a->H < 0 || a->H > 1024 || (int64_t)a->N * a->H > (1ll << 30)) return KDA_ERR_SHAPE;
   if (a->B == 0 || a->N == 0 || a->H == 0) return KDA_OK;
   if (!a->q_lat || !a->out || (a->DR && !a->q_rope)) return KDA_ERR_NULL_POINTER;
   if (reinterpret_cast<uintptr_t>(a->q_lat) % 2 || reinterpret_cast<uintptr_t>(a->q_rope) % 2 ||

@@ -61,7 +61,7 @@ __device__ __forceinline__ void locate(const CacheParams& p, int n, int& b, int&
     b = lo;
     new_tokens(p, b, first, count);
   }
-  pos = n - first < count ? p.lens[b] - count + (n - first) : -1;
+  pos = n - first < count ? max(p.lens[b], 0) - count + (n - first) : -1;
 }
 
 // Page of position pos of sequence b, or -1 where the table or the pool ends.

@@ -367,7 +367,8 @@ size_t mla_decode_args_size(void);
  * sequence with a visible page outside the pool.
  *
  * Requires 16-bit io_dtype, KVL in {128, 256, 384, 512}, DR in {0, 64},
- * page_size a power of two from 16 to 1024, num_pages * page_size < 2^31.  Codes and rope rows are unit-stride and start
+ * page_size a power of two from 16 to 1024, num_pages * page_size < 2^31, max_pages *
+ * page_size and N * H at most 2^30.  Codes and rope rows are unit-stride and start
  * on 16-byte boundaries; scales have a unit token stride.
  */
 typedef struct MlaCacheArgs {
