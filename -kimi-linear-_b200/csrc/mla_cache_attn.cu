@@ -44,42 +44,41 @@ __device__ int g_attn_device_error = 0;
 namespace {
 
 constexpr int TILE = 128;                  // positions per tile (MMA M)
-constexpr int kThreads = 192;              // warps 0-3 softmax, 4 loads, 5 MMA issue
-constexpr int kMaxStages = 8;
+constexpr int CHUNK = TILE * 128;          // bytes of 128 positions x 128 bytes
+constexpr int kThreads = 320;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue
+constexpr int kMaxRing = 14;
 constexpr int kSmemMax = 232448;           // 227 KB per block
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kBias = 6.f;               // P carries 2^6 ...
-constexpr float kSlack = 2.f;              // ... and may outgrow the maximum by 2^2 (2^8 < 448)
+constexpr float kBias = 4.f;               // P carries 2^4 ...
+constexpr float kSlack = 4.f;              // ... and may outgrow the maximum by 2^4 (2^8 < 448)
+constexpr float kUnset = -1e30f;           // maximum of a row that has seen nothing
 
 // e4m3 terms of a query and of a softmax weight
-template <typename T> constexpr int kTerms = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
+template <typename T> constexpr int kQTerms = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
+constexpr int NP = 3;
 
 template <typename T, int R, int NCH>
 struct Cfg {
-  static constexpr int NT = kTerms<T>;
-  static constexpr int N = NT * R;                       // columns of S and of one O chunk
-  static constexpr int O_COLS = NCH * N;
-  static constexpr int SBUF = O_COLS + 2 * N <= 512 ? 2 : 1;
-  static_assert(O_COLS + SBUF * N <= 512, "TMEM columns");
-  static constexpr int CHUNK = TILE * 128;               // bytes of 128 positions x 128 channels
-  static constexpr int Q_BYTES = NCH * N * 128;
-  static constexpr int QR_BYTES = R * 128;
-  static constexpr int P_BYTES = N * 128;
+  static constexpr int NQ = kQTerms<T>;
+  static constexpr int NS = NQ * R, NO = NP * R;         // columns of S and of one O chunk
+  static constexpr int SBUF = NCH * NO + 2 * NS <= 512 ? 2 : 1;
+  static_assert(NCH * NO + SBUF * NS <= 512, "TMEM columns");
 };
 
-// Shared memory besides the stages (4 KB: barriers, rows; 1 KB: alignment), and
-// the stages that fit beside it.
+// Shared memory besides the ring (4 KB: barriers, rows; 1 KB: alignment), and the
+// chunks that fit beside it.  The order of the products needs the codes of one
+// tile and all of the next at once.
 constexpr int kFixedBytes = 4096 + 1024;
-int stage_bytes(int kvl, int dr) { return (kvl / 128 + (dr ? 1 : 0)) * TILE * 128; }
-int fixed_bytes(int kvl, int terms, int R) {
-  return kFixedBytes + terms * R * (kvl + 128) + R * 128;
+int fixed_bytes(int kvl, int q_terms, int R) {
+  return kFixedBytes + q_terms * R * kvl + R * 128 + 2 * NP * R * 128;
 }
-int stages(int kvl, int dr, int terms, int R) {
-  const int n = (kSmemMax - fixed_bytes(kvl, terms, R)) / stage_bytes(kvl, dr);
-  return n < kMaxStages ? n : kMaxStages;
+int ring_chunks(int kvl, int q_terms, int R) {
+  const int n = (kSmemMax - fixed_bytes(kvl, q_terms, R)) / CHUNK;
+  return n < kMaxRing ? n : kMaxRing;
 }
+int ring_least(int kvl, int dr) { return 2 * (kvl / 128) + (dr ? 1 : 0); }
 
 // Where a range of tiles starts inside a group; what cache_join_kernel reads.
 struct Cut {
@@ -92,7 +91,7 @@ struct Work {
   float* part;     // [2 ranges][R][KVL] fp32: slot 2 c: group begun before range c; 2 c + 1: left unfinished
   float* lse2;     // [2 ranges][R] log2 of the sum of a part
   Cut* cuts;       // [ranges]
-  int stages;
+  int ring;        // chunks of the ring
 };
 
 // ---------------------------------------------------------------------------
@@ -194,14 +193,39 @@ struct Walk {
 // ---------------------------------------------------------------------------
 // PTX used only here
 // ---------------------------------------------------------------------------
+// The issuing warp runs its loops with all lanes, and each instruction elects one
+// lane itself: the operands then stay in uniform registers.  One instruction of 128 x
+// 32 x 32 takes 41 cycles this way (49 with N = 64: reading its operands from shared
+// memory), 80 or 143 from a branch that one lane takes.
 // D[tmem] = A[smem] B[smem] (+ D): 8-bit operands, fp32 accumulation
-__device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                       uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x;\n\t"
+      "elect.sync x|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D += A B, 16-bit operands of one type
+__device__ __forceinline__ void mma_half(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                         uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x;\n\t"
+      "elect.sync x|e, 0xffffffff;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc)
+      : "memory");
+}
+// arrive on `bar` once the warp's products so far have completed
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 x;\n\t"
+      "elect.sync x|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          ptx::smem_u32(bar))
       : "memory");
 }
 // Shared-memory descriptor of 128-byte rows with the 128-byte swizzle (eight
@@ -213,9 +237,9 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {
          (static_cast<uint64_t>(2) << 61);
 }
 // Instruction descriptors: fp32 accumulator; e4m3 operands, or `fmt` 0 = f16, 1 = bf16
-__host__ __device__ constexpr uint32_t idesc(int N, bool a_m_major, uint32_t fmt) {
+__host__ __device__ constexpr uint32_t idesc(int N, bool a_m_major, bool b_n_major, uint32_t fmt) {
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_m_major ? 1u : 0u) << 15) |
-         (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
+         ((b_n_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
 }
 // largest of the 32 lanes' values (NaN ignored)
 __device__ __forceinline__ float warp_max(float x) {
@@ -278,51 +302,80 @@ __device__ __forceinline__ float join(const float* t, int stride) {   // t[0] + 
 }
 
 struct Shared {            // at the end of dynamic shared memory
-  uint64_t full[kMaxStages], empty[kMaxStages];
-  uint64_t s_full[2], s_empty[2], p_full, o_done, q_ready, drain;
+  uint64_t full[kMaxRing], empty[kMaxRing];
+  uint64_t s_full[2], s_empty[2], p_full[2], o_done[4], m_full[2], q_ready, drain;
   uint32_t tmem;
   int abort_flag;
-  int64_t scan[8];
+  int changed[2];          // the tile of this parity moved the maxima
+  int64_t scan[kThreads / 32];
   int64_t base;            // where the range starts: count at which sequence b starts
   int b;
-  float q_scale[32];       // per row: 2^e scale log2e
-  int seen[32];            // per row: positions that it sees
-  float red[2][4][32];     // per warp and row: maxima (two tiles in turn), sums
+  // per row of the group
+  float q_scale[32];       // 2^e scale log2e
+  float m[32];             // running maximum less kBias
+  float mb[2][32];         // the same as of each softmax group's last tile
+  float alpha[2][32];      // what its sums (and O) are rescaled by
+  int seen[32];            // positions that it sees
+  int64_t out[32], lse[32];  // where its results go
+  float red[8][32];        // per warp and row: maxima, sums
 };
-static_assert(sizeof(Shared) <= 4096, "room for barriers and rows");
+static_assert(sizeof(Shared) <= kFixedBytes - 1024, "room for barriers and rows");
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// sums of v[0 .. R - 1] over the warp: lane i < R (and i + R) gets the sum of v[i]
+template <int R>
+__device__ __forceinline__ float warp_sums(float (&v)[R], int lane) {
+#pragma unroll
+  for (int n = R / 2; n >= 1; n /= 2) {
+    const bool up = lane & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+    }
+  }
+#pragma unroll
+  for (int o = R; o < 32; o <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
 
 template <typename T, int R, int NCH>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUtensorMap map_codes,
                   const __grid_constant__ CUtensorMap map_rope) {
   using C = Cfg<T, R, NCH>;
-  constexpr int NT = C::NT, N = C::N;
+  constexpr int NQ = C::NQ, NS = C::NS, NO = C::NO;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stage_size = (NCH + (p.DR ? 1 : 0)) * C::CHUNK;
-  uint8_t* q_s = sm + w.stages * stage_size;
-  uint8_t* qr_s = q_s + C::Q_BYTES;
-  uint8_t* p_s = qr_s + C::QR_BYTES;
-  Shared& sh = *reinterpret_cast<Shared*>(p_s + C::P_BYTES);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* q_s = sm + w.ring * CHUNK;
+  uint8_t* qr_s = q_s + NCH * NS * 128;
+  uint8_t* p_s = qr_s + R * 128;                // two buffers
+  Shared& sh = *reinterpret_cast<Shared*>(p_s + 2 * NO * 128);
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int ring = w.ring, tile_chunks = NCH + (p.DR ? 1 : 0);
 
   if (tid == 0) {
-    for (int i = 0; i < w.stages; ++i) {
+    for (int i = 0; i < ring; ++i) {
       ptx::mbar_init(&sh.full[i], 1);
       ptx::mbar_init(&sh.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&sh.s_full[i], 1);
       ptx::mbar_init(&sh.s_empty[i], 128);
+      ptx::mbar_init(&sh.p_full[i], 128);
+      ptx::mbar_init(&sh.o_done[i], 1);
+      ptx::mbar_init(&sh.o_done[i + 2], 1);
+      ptx::mbar_init(&sh.m_full[i], 128);
     }
-    ptx::mbar_init(&sh.p_full, 128);
-    ptx::mbar_init(&sh.o_done, 1);
-    ptx::mbar_init(&sh.q_ready, 128);
+    ptx::mbar_init(&sh.q_ready, 256);
     ptx::mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 5) ptx::tmem_alloc(&sh.tmem, 512);
+  if (warp == 9) ptx::tmem_alloc(&sh.tmem, 512);
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
 
@@ -360,10 +413,10 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       sh.b = b;
       sh.base = before;
     }
-    // the group that this range starts inside of, for cache_join_kernel
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
+    // the group that this range starts inside of, for cache_join_kernel
     if (tid == 0) {
       Cut cut{-1, 0, 0, 0};
       if (u0 < u1 && blockIdx.x > 0) {
@@ -386,20 +439,21 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     }
   }
   const uint32_t tmem = sh.tmem;
-  const uint32_t tm_s = tmem + C::O_COLS;       // S buffers after the O chunks
+  const uint32_t tm_s = tmem + NCH * NO;        // S buffers after the O chunks
   volatile int* ab = &sh.abort_flag;
   Walk<R> walk(p, sh.b, sh.base, u0, u1);
   Segment seg;
 
-  if (warp == 4) {
-    // ======== loads: boxes of one page (at most 128 positions) x 128 channels
-    int stage = 0, round = 0, issued = 0;
+  if (warp == 8) {
+    // ======== loads: boxes of one page (at most 128 positions) x 128 bytes into a
+    // ring of 16 KB chunks; a tile is its rope chunk, then its code chunks
+    int slot = 0, round = 0, issued = 0;
     const int box_rows = min(p.page_size, TILE), boxes = TILE / box_rows;
     bool ok = true;
     while (ok && walk.next(seg)) {
       const int seen = seen_by<R>(p, walk.s, seg.g * R + R - 1);
       if (seen == 0) continue;
-      for (int t = seg.t0; t < seg.t1; ++t) {
+      for (int t = seg.t0; t < seg.t1 && ok; ++t) {
         const int pos = t * TILE;
         const int nbox = min(boxes, (seen - pos + box_rows - 1) / box_rows);
         int page = p.num_pages;                 // outside: the copy fills in zeros
@@ -407,96 +461,107 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           const int x = page_of(p, seg.b, pos + lane * box_rows);
           if (x >= 0) page = x;
         }
-        if (round > 0 && !wait(&sh.empty[stage], (round - 1) & 1, ab)) { ok = false; break; }
-        uint8_t* dst = sm + stage * stage_size;
-        if (lane == 0) {
-          ptx::mbar_arrive_expect_tx(&sh.full[stage],
-                                     nbox * box_rows * 128 * (NCH + (p.DR ? 1 : 0)));
+        const int at = p.page_size > TILE ? pos & (p.page_size - 1) : 0;
+        for (int c = p.DR ? -1 : 0; c < NCH; ++c) {
+          if (round > 0 && !wait(&sh.empty[slot], (round - 1) & 1, ab)) { ok = false; break; }
+          if (lane == 0) ptx::mbar_arrive_expect_tx(&sh.full[slot], nbox * box_rows * 128);
+          __syncwarp();
+          uint8_t* dst = sm + slot * CHUNK + lane * box_rows * 128;
+          if (lane < nbox) {
+            if (c < 0) ptx::tma_load_3d(dst, &map_rope, 0, at, page, &sh.full[slot]);
+            else ptx::tma_load_3d(dst, &map_codes, c * 128, at, page, &sh.full[slot]);
+          }
+          ++issued;
+          if (++slot == ring) { slot = 0; ++round; }
         }
-        __syncwarp();
-        if (lane < nbox) {
-          const int row = pos & (p.page_size - 1) & ~(box_rows - 1);
-          const int at = p.page_size >= TILE ? row : 0;
-#pragma unroll
-          for (int c = 0; c < NCH; ++c)
-            ptx::tma_load_3d(dst + c * C::CHUNK + lane * box_rows * 128, &map_codes, c * 128, at,
-                             page, &sh.full[stage]);
-          if (p.DR)
-            ptx::tma_load_3d(dst + NCH * C::CHUNK + lane * box_rows * 128, &map_rope, 0, at, page,
-                             &sh.full[stage]);
-        }
-        ++issued;
-        if (++stage == w.stages) { stage = 0; ++round; }
       }
     }
     if (*ab) {                                  // copies in flight land before the block ends
-      for (int i = max(0, issued - w.stages); i < issued; ++i) {
+      for (int i = max(0, issued - ring); i < issued; ++i) {
         const uint64_t t0 = ptx::globaltimer_ns();
-        while (!ptx::mbar_try_wait(&sh.full[i % w.stages], (i / w.stages) & 1) &&
+        while (!ptx::mbar_try_wait(&sh.full[i % ring], (i / ring) & 1) &&
                ptx::globaltimer_ns() - t0 < kWaitNs) {
         }
       }
     }
     __syncwarp();
-  } else if (warp == 5) {
-    // ======== MMA issue: S of tile i + 1 ahead of O of tile i
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc(N, false, 0), id_o = idesc(N, true, 0);
-      constexpr uint32_t id_r = idesc(R, false, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+  } else if (warp == 9) {
+    // ======== MMA issue: S of tile k + 1 ahead of O of tile k
+    {
+      constexpr uint32_t id_s = idesc(NS, false, false, 0), id_o = idesc(NO, true, true, 0);
+      constexpr uint32_t id_r = idesc(R, false, false, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+      const uint32_t sm0 = ptx::smem_u32(sm);
       const uint64_t dq = sdesc_sw128(ptx::smem_u32(q_s)), dqr = sdesc_sw128(ptx::smem_u32(qr_s));
-      const uint64_t dp = sdesc_sw128(ptx::smem_u32(p_s));
-      int k = 0;                                // tiles so far
-      int stage = 0, round = 0, segs = 0;
+      // P: 16 rows x 8 positions a core matrix, 128 bytes on along the positions,
+      // 2048 along the rows
+      const uint64_t dp = ptx::sdesc(ptx::smem_u32(p_s), 128, TILE * 16);
+      int k = 0, segs = 0;
+      int slot = 0, round = 0;                  // of the next chunk that S reads
+      int oslot = 0;                            // of the next chunk that O reads
       bool ok = true;
-      auto issue_o = [&](int i, int st, bool first) {          // O += codes^T P of tile i
-        if (!wait(&sh.p_full, i & 1, ab)) return false;
+      auto issue_o = [&](int i, bool first) {   // O += codes^T P of tile i
+        const int par = i & 1;
+        if (!wait(&sh.p_full[par], (i >> 1) & 1, ab)) return false;
         ptx::tc_fence_after();
-        const uint64_t dv = sdesc_sw128(ptx::smem_u32(sm + st * stage_size));
+        if (p.DR && ++oslot == ring) oslot = 0;
+        uint64_t dv[NCH];
+        int at[NCH];
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
+        for (int c = 0; c < NCH; ++c) {
+          at[c] = oslot;
+          dv[c] = sdesc_sw128(sm0 + oslot * CHUNK);
+          if (++oslot == ring) oslot = 0;
+        }
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8_ss(tmem + c * N, dv + ((c * C::CHUNK + kk * 4096) >> 4), dp + ((kk * 32) >> 4),
-                      id_o, !(first && kk == 0));
-        ptx::tc_commit(&sh.empty[st]);
-        ptx::tc_commit(&sh.o_done);
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int c = 0; c < NCH; ++c)
+            mma_f8(tmem + c * NO, dv[c] + ((kk * 4096) >> 4),
+                      dp + ((par * NO * 128 + kk * 512) >> 4), id_o, !(first && kk == 0));
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) commit(&sh.empty[at[c]]);
+        commit(&sh.o_done[i & 3]);
         return true;
       };
       while (ok && walk.next(seg)) {
         if (seen_by<R>(p, walk.s, seg.g * R + R - 1) == 0) continue;
         if (!wait(&sh.q_ready, segs & 1, ab)) break;
         ++segs;
-        int prev = 0;
-        for (int t = seg.t0; t < seg.t1 && ok; ++t) {
-          const int buf = C::SBUF == 2 ? (k & 1) : 0, use = C::SBUF == 2 ? (k >> 1) : k;
-          if (!wait(&sh.full[stage], round & 1, ab) ||
-              (use > 0 && !wait(&sh.s_empty[buf], (use - 1) & 1, ab))) { ok = false; break; }
-          ptx::tc_fence_after();
-          const uint32_t st0 = ptx::smem_u32(sm + stage * stage_size);
-          const uint64_t dk = sdesc_sw128(st0);
-          const uint32_t d = tm_s + buf * N;
-#pragma unroll
-          for (int c = 0; c < NCH; ++c)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_f8_ss(d, dk + ((c * C::CHUNK + kk * 32) >> 4),
-                        dq + ((c * N * 128 + kk * 32) >> 4), id_s, c + kk > 0);
+        for (int t = seg.t0; t < seg.t1; ++t) {
+          const int before = k - C::SBUF;       // the tile whose scores were here
+          if (before >= 0 && !wait(&sh.s_empty[before & 1], (before >> 1) & 1, ab)) { ok = false; break; }
+          const uint32_t d = tm_s + (C::SBUF == 2 ? (k & 1) * NS : 0);
+          const int rope_slot = slot;
           if (p.DR) {
+            if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
+            if (++slot == ring) { slot = 0; ++round; }
+          }
+          for (int c = 0; c < NCH; ++c) {
+            if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
+            ptx::tc_fence_after();
+            const uint64_t dk = sdesc_sw128(sm0 + slot * CHUNK);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              ptx::mma_f16_ss(d, dk + ((NCH * C::CHUNK + kk * 32) >> 4), dqr + ((kk * 32) >> 4),
-                              id_r, 1);
+              mma_f8(d, dk + ((kk * 32) >> 4), dq + ((c * NS * 128 + kk * 32) >> 4), id_s,
+                        c + kk > 0);
+            if (++slot == ring) { slot = 0; ++round; }
           }
-          ptx::tc_commit(&sh.s_full[buf]);
-          if (t > seg.t0) ok = issue_o(k - 1, prev, t - 1 == seg.t0);
-          prev = stage;
+          if (!ok) break;
+          if (p.DR) {
+            const uint64_t dk = sdesc_sw128(sm0 + rope_slot * CHUNK);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_half(d, dk + ((kk * 32) >> 4), dqr + ((kk * 32) >> 4), id_r);
+            commit(&sh.empty[rope_slot]);
+          }
+          commit(&sh.s_full[k & 1]);
+          if (t > seg.t0 && !issue_o(k - 1, t - 1 == seg.t0)) { ok = false; break; }
           ++k;
-          if (++stage == w.stages) { stage = 0; ++round; }
         }
-        if (ok) ok = issue_o(k - 1, prev, seg.t1 - 1 == seg.t0);
+        if (ok) ok = issue_o(k - 1, seg.t1 - 1 == seg.t0);
       }
       if (*ab) {                                // products in flight end before TMEM is freed
-        ptx::tc_commit(&sh.drain);
+        commit(&sh.drain);
         const uint64_t t0 = ptx::globaltimer_ns();
         while (!ptx::mbar_try_wait(&sh.drain, 0) && ptx::globaltimer_ns() - t0 < kWaitNs) {
         }
@@ -504,87 +569,33 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     }
     __syncwarp();
   } else {
-    // ======== softmax: thread = position of the tile = TMEM lane
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    const int tt = warp * 32 + lane;
+    // ======== softmax: two groups of four warps take the tiles in turn; thread =
+    // position of the tile = TMEM lane
+    const int wg = warp >> 2;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const int tt = tid & 127;
     int k = 0;
     bool failed = false;
+    // The products of tile i are in O.  A wait tells a barrier's phase only from its
+    // neighbours; each group waits for its own last tile's products, so with four
+    // barriers the phase asked for is the one under way or the one just ended.
+    auto o_done = [&](int i) { return wait(&sh.o_done[i & 3], (i >> 2) & 1, ab); };
     while (!failed && walk.next(seg)) {
       const int row0 = seg.g * R, rows = min(R, (int)((int64_t)walk.s.n * p.H - row0));
       const int seen = seen_by<R>(p, walk.s, row0 + R - 1);
       const int seen0 = seen_by<R>(p, walk.s, row0);
       if (seen == 0) {                          // nobody sees anything
-        for (int i = tid; i < rows * p.KVL; i += 128) {
-          const int row = row0 + i / p.KVL;
-          T* o = static_cast<T*>(p.out) + (int64_t)(walk.s.first + row / p.H) * p.o_s[0] +
-                 (int64_t)(row % p.H) * p.o_s[1];
-          st(o + i % p.KVL, 0.f);
+        for (int r = warp; r < rows; r += 8) {
+          const int64_t n = walk.s.first + (row0 + r) / p.H, h = (row0 + r) % p.H;
+          T* o = static_cast<T*>(p.out) + n * p.o_s[0] + h * p.o_s[1];
+          for (int c = lane; c < p.KVL; c += 32) st(o + c, 0.f);
+          if (lane == 0 && p.lse) p.lse[n * p.lse_s + h] = -INFINITY;
         }
-        if (tid < rows && p.lse)
-          p.lse[(int64_t)(walk.s.first + (row0 + tid) / p.H) * p.lse_s + (row0 + tid) % p.H] = -INFINITY;
         continue;
       }
       if (tid == 0 && walk.s.off + walk.s.n > walk.s.cap) atomicExch(&g_attn_device_error, kErrOutside);
-      // ---- queries: scaled by a power of two, split into e4m3 terms (rows past the end: zeros)
-#pragma unroll 1
-      for (int r = warp; r < R; r += 4) {
-        const int row = row0 + r;
-        const bool live = r < rows;
-        const int64_t n = walk.s.first + row / p.H, h = row % p.H;
-        const T* ql = static_cast<const T*>(p.q_lat) + n * p.ql_s[0] + h * p.ql_s[1];
-        float x[NCH][4], y[2] = {0.f, 0.f};     // channels 128 c + 4 lane + i; rope 2 lane + i
-        uint32_t amax = 0, rmax = 0;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[c][i] = 0.f;
-        if (live) {
-#pragma unroll
-          for (int c = 0; c < NCH; ++c) {
-            if (p.vec) {
-              ld4(ql + c * 128 + 4 * lane, x[c]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x[c][i] = ld(ql + c * 128 + 4 * lane + i);
-            }
-          }
-          if (p.DR) {
-            const T* qr = static_cast<const T*>(p.q_rope) + n * p.qr_s[0] + h * p.qr_s[1];
-            y[0] = ld(qr + 2 * lane);
-            y[1] = ld(qr + 2 * lane + 1);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < NCH; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) amax = max(amax, abs_bits(x[c][i]));
-        rmax = max(abs_bits(y[0]), abs_bits(y[1]));
-        const int e = scale_exp(warp_max_u32(amax), warp_max_u32(rmax));
-        const float inv = pow2i(-e);
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[c][i] *= inv;
-          uint32_t t[NT];
-          split4<NT>(x[c], t);
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-            *reinterpret_cast<uint32_t*>(q_s + c * N * 128 + swz(j * R + r, 4 * lane)) = t[j];
-        }
-        if (p.DR) {
-          T* d = reinterpret_cast<T*>(qr_s + swz(r, 4 * lane));
-          st(d, y[0] * inv);
-          st(d + 1, y[1] * inv);
-        }
-        if (lane == 0) {
-          sh.q_scale[r] = pow2i(e) * p.scale * kLog2e;
-          sh.seen[r] = live ? seen_by<R>(p, walk.s, row) : seen;
-        }
-      }
-      ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(&sh.q_ready);
-      asm volatile("bar.sync 1, 128;" ::: "memory");      // q_scale and seen are written
-      // ---- scale of this thread's position, a tile ahead, its page two tiles ahead
+      // ---- scale of this thread's position, its page a tile before that
+      const int t_mine = seg.t0 + ((k ^ wg) & 1);          // this group's first tile
       auto page_at = [&](int t) {
         const int pos = t * TILE + tt;
         return t < seg.t1 && pos < seen ? page_of(p, seg.b, pos) : -2;
@@ -597,160 +608,284 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         }
         return p.scales[(int64_t)page * p.scales_s + ((t * TILE + tt) & (p.page_size - 1))];
       };
-      float s_next = scale_at(seg.t0, page_at(seg.t0));
-      int page_next = page_at(seg.t0 + 1);
-      float l[R], m_row = -INFINITY;            // m_row: running maximum of row `lane`
+      const int page_first = page_at(t_mine);
+      int page_next = page_at(t_mine + 2);
+      // ---- queries: scaled by a power of two, split into e4m3 terms (rows past the end: zeros)
+      {
+        constexpr int RW = R / 8;               // rows of a warp: warp + 8 i
+        uint2 raw[RW][NCH];                     // channels 128 c + 4 lane + j
+        uint32_t raw_r[RW];                     // rope 2 lane + j
+        const T *ql[RW], *qr[RW];
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {          // (rows past the end: the last one's)
+          const int row = row0 + min(warp + 8 * i, rows - 1);
+          const int64_t n = walk.s.first + row / p.H, h = row % p.H;
+          ql[i] = static_cast<const T*>(p.q_lat) + n * p.ql_s[0] + h * p.ql_s[1] + 4 * lane;
+          qr[i] = static_cast<const T*>(p.q_rope) + n * p.qr_s[0] + h * p.qr_s[1] + 2 * lane;
+          raw_r[i] = 0;
+        }
+        if (p.vec) {
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) raw[i][c] = *reinterpret_cast<const uint2*>(ql[i] + c * 128);
+            if (p.DR) raw_r[i] = *reinterpret_cast<const uint32_t*>(qr[i]);
+          }
+        } else {
+          const auto bits = [](const T* q) { return (uint32_t)*reinterpret_cast<const uint16_t*>(q); };
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+              const T* q = ql[i] + c * 128;
+              raw[i][c] = make_uint2(bits(q) | bits(q + 1) << 16, bits(q + 2) | bits(q + 3) << 16);
+            }
+            if (p.DR) raw_r[i] = bits(qr[i]) | bits(qr[i] + 1) << 16;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+          const int r = warp + 8 * i;
+          const bool live = r < rows;
+          float x[NCH][4], y[2];
+          uint32_t amax = 0;
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            const T* v = reinterpret_cast<const T*>(&raw[i][c]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[c][j] = live ? ld(v + j) : 0.f;
+              amax = max(amax, abs_bits(x[c][j]));
+            }
+          }
+          const T* v = reinterpret_cast<const T*>(&raw_r[i]);
+          y[0] = live ? ld(v) : 0.f;
+          y[1] = live ? ld(v + 1) : 0.f;
+          const uint32_t rmax = max(abs_bits(y[0]), abs_bits(y[1]));
+          const int e = scale_exp(warp_max_u32(amax), warp_max_u32(rmax));
+          const float inv = pow2i(-e);
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[c][j] *= inv;
+            uint32_t term[NQ];
+            split4<NQ>(x[c], term);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+              *reinterpret_cast<uint32_t*>(q_s + c * NS * 128 + swz(j * R + r, 4 * lane)) = term[j];
+          }
+          if (p.DR) {
+            T* d = reinterpret_cast<T*>(qr_s + swz(r, 4 * lane));
+            st(d, y[0] * inv);
+            st(d + 1, y[1] * inv);
+          }
+          if (lane == 0) {
+            const int row = row0 + r;
+            const int64_t n = walk.s.first + row / p.H, h = row % p.H;
+            sh.q_scale[r] = pow2i(e) * p.scale * kLog2e;
+            sh.seen[r] = r < rows ? seen_by<R>(p, walk.s, row) : seen;
+            sh.m[r] = sh.mb[0][r] = sh.mb[1][r] = kUnset;
+            sh.out[r] = n * p.o_s[0] + h * p.o_s[1];
+            sh.lse[r] = n * p.lse_s + h;
+          }
+        }
+      }
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(&sh.q_ready);
+      float s_next = scale_at(t_mine, page_first);
+      float ls_next = log2f(s_next), rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
+      bar_sync(3, 256);                         // the rows' figures are written
+      float l[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) l[r] = 0.f;
       for (int t = seg.t0; t < seg.t1; ++t, ++k) {
-        const float s = s_next;
-        s_next = scale_at(t + 1, page_next);
-        page_next = page_at(t + 2);
-        const int buf = C::SBUF == 2 ? (k & 1) : 0, use = C::SBUF == 2 ? (k >> 1) : k;
+        const int par = k & 1;
+        if (par != wg) continue;
+        // log2 of the position's scale and its reciprocal (a NaN scale: NaN reaches
+        // the sum through P, where the row sees the position)
+        const float s = s_next, ls = ls_next, rs = rs_next;
+        s_next = scale_at(t + 2, page_next);
+        page_next = page_at(t + 4);
+        const int buf = C::SBUF == 2 ? par : 0;
         const int pos = t * TILE + tt;
-        if (!wait(&sh.s_full[buf], use & 1, ab)) failed = true;
+        if (!wait(&sh.s_full[par], (k >> 1) & 1, ab)) failed = true;
         ptx::tc_fence_after();
-        float z[N];
-        ptx::tmem_ld<N>(tm_s + buf * N + lane_base, z);
-        ptx::tmem_wait_ld();
+        float a[R];
+#pragma unroll
+        for (int g = 0; g < R; g += 16) {       // 16 rows at a time: registers
+          float z[NQ * 16];
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+            ptx::tmem_ld16(tm_s + buf * NS + j * R + g + lane_base, z + 16 * j);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            a[g + r] = fmaf(join<NQ>(z + r, 16), sh.q_scale[g + r] * s, ls);
+        }
         ptx::tc_fence_before();
-        ptx::mbar_arrive(&sh.s_empty[buf]);
+        ptx::mbar_arrive(&sh.s_empty[par]);
+        if (t * TILE + TILE > seen0) {          // some row does not see the whole tile
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (pos >= sh.seen[r]) a[r] = -INFINITY;
+        }
         // positions that nobody sees, or that are NaN as a whole, must not meet
         // a weight of zero: their codes become zeros
         if (pos >= seen || s != s) {
-          uint8_t* row = sm + ((k % w.stages) * stage_size) + tt * 128;
+          int at = (int)(((int64_t)k * tile_chunks + tile_chunks - NCH) % ring);
 #pragma unroll 1
-          for (int c = 0; c < NCH; ++c)
+          for (int c = 0; c < NCH; ++c) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(row + c * C::CHUNK + 16 * i) = make_uint4(0, 0, 0, 0);
-        }
-        const bool open = t * TILE + TILE <= seen0;       // all rows see the whole tile
-        const float ls = log2f(s), rs = s == s ? 1.f / s : 1.f;   // (NaN reaches l through P)
-        float a[R], mine = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          a[r] = fmaf(join<NT>(z + r, R), sh.q_scale[r] * s, ls);
-          if (!open && pos >= sh.seen[r]) a[r] = -INFINITY;
-          const float mx = warp_max(a[r]);
-          if (lane == r) mine = mx;
-        }
-        if (lane < R) sh.red[k & 1][warp][lane] = mine;
-        failed = ptx::bar_red_or(1, 128, failed);
-        if (failed) break;
-        float alpha = 1.f;
-        bool grew = false;
-        if (lane < R) {
-          const float mx = fmaxf(fmaxf(sh.red[k & 1][0][lane], sh.red[k & 1][1][lane]),
-                                 fmaxf(sh.red[k & 1][2][lane], sh.red[k & 1][3][lane]));
-          if (mx > m_row + kSlack || (m_row == -INFINITY && mx > -INFINITY)) {
-            grew = m_row != -INFINITY;
-            alpha = ex2(m_row - mx);
-            m_row = mx;
+              *reinterpret_cast<uint4*>(sm + at * CHUNK + tt * 128 + 16 * i) = make_uint4(0, 0, 0, 0);
+            if (++at == ring) at = 0;
           }
         }
-        const float m_use = m_row == -INFINITY ? 0.f : m_row - kBias;
-        const bool rescale = __any_sync(0xffffffffu, grew);
-        // ---- P of tile k - 1 has been read, O holds it
-        if (k > 0 && !wait(&sh.o_done, (k - 1) & 1, ab)) failed = true;
-        if (rescale) {
-          ptx::tc_fence_after();
-          float al[R];
+        // ---- the maxima as the tile before left them
+        const bool first = t == seg.t0;
+        if (!first) {
+          if (!wait(&sh.m_full[par ^ 1], ((k - 1) >> 1) & 1, ab)) failed = true;
+          if (sh.changed[par ^ 1]) {
+            if (tt < R) {
+              const float m = sh.m[tt];
+              sh.alpha[par][tt] = ex2(sh.mb[par][tt] - m);
+              sh.mb[par][tt] = m;
+            }
+            bar_sync(1 + wg, 128);
+#pragma unroll
+            for (int r = 0; r < R; ++r) l[r] *= sh.alpha[par][r];
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; ++r) top = fmaxf(top, a[r] - sh.mb[par][r]);
+        const bool grew = ptx::bar_red_or(1 + wg, 128, failed || top > kBias + kSlack);
+        if (tt == 0) sh.changed[par] = grew;
+        if (grew) {
+          // a row outgrew P's range (or has its first position): new maxima, and O
+          // follows once the products so far are in it
+          if (*ab) failed = true;
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            al[r] = __shfl_sync(0xffffffffu, alpha, r);
-            l[r] *= al[r];
+            const float mx = warp_max(a[r]);
+            if (lane == 0) sh.red[warp][r] = mx;
           }
+          failed = ptx::bar_red_or(1 + wg, 128, failed);
+          if (failed) break;
+          if (tt < R) {
+            const float* red = &sh.red[4 * wg][tt];
+            const float mx = fmaxf(fmaxf(red[0], red[32]), fmaxf(red[64], red[96]));
+            const float old = sh.m[tt];
+            const bool up = mx - old > kBias + kSlack;
+            sh.alpha[par][tt] = up ? ex2(old - (mx - kBias)) : 1.f;
+            if (up) sh.m[tt] = sh.mb[par][tt] = mx - kBias;
+          }
+          bar_sync(1 + wg, 128);
+          if (!first) {
+            if (!o_done(k - 1)) failed = true;
+            ptx::tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < NCH * NT; ++c) {
-            float o[R];
-            ptx::tmem_ld<R>(tmem + c * R + lane_base, o);
-            ptx::tmem_wait_ld();
+            for (int c = 0; c < NCH * NO; c += 48) {
+              float o[48];
+              ptx::tmem_ld<48>(tmem + c + lane_base, o);
+              ptx::tmem_wait_ld();
 #pragma unroll
-            for (int r = 0; r < R; ++r) o[r] *= al[r];
-            ptx::tmem_st<R>(tmem + c * R + lane_base, o);
+              for (int i = 0; i < 48; ++i) o[i] *= sh.alpha[par][(c + i) % R];
+              ptx::tmem_st<48>(tmem + c + lane_base, o);
+            }
+            ptx::tmem_wait_st();
+            ptx::tc_fence_before();
           }
-          ptx::tmem_wait_st();
+#pragma unroll
+          for (int r = 0; r < R; ++r) l[r] *= sh.alpha[par][r];
         }
+        ptx::mbar_arrive(&sh.m_full[par]);
+        // ---- P, once the buffer's last products have read it
+        if (k > 1 && !o_done(k - 2)) failed = true;
+        uint8_t* pt = p_s + par * NO * 128 + tt * 16;
 #pragma unroll
-        for (int r = 0; r < R; r += 4) {
-          float e4[4];
+        for (int g = 0; g < R / 16; ++g) {
+          uint32_t term[NP][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e4[i] = ex2(a[r + i] - __shfl_sync(0xffffffffu, m_use, r + i));
-            l[r + i] = fmaf(e4[i], rs, l[r + i]);
+          for (int q = 0; q < 4; ++q) {
+            float e4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = 16 * g + 4 * q + i;
+              e4[i] = ex2(a[r] - sh.mb[par][r]);
+              l[r] = fmaf(e4[i], rs, l[r]);
+            }
+            uint32_t u[NP];
+            split4<NP>(e4, u);
+#pragma unroll
+            for (int j = 0; j < NP; ++j) term[j][q] = u[j];
           }
-          uint32_t tm[NT];
-          split4<NT>(e4, tm);
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              p_s[swz(j * R + r + i, tt)] = (uint8_t)(tm[j] >> (8 * i));
+          for (int j = 0; j < NP; ++j)
+            *reinterpret_cast<uint4*>(pt + (j * (R / 16) + g) * (TILE * 16)) =
+                make_uint4(term[j][0], term[j][1], term[j][2], term[j][3]);
         }
         ptx::fence_proxy_async_smem();
-        ptx::tc_fence_before();
-        ptx::mbar_arrive(&sh.p_full);
+        ptx::mbar_arrive(&sh.p_full[par]);
+        ls_next = log2f(s_next);
+        rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
       }
       // ---- the segment's result
-      if (!failed && !wait(&sh.o_done, (k - 1) & 1, ab)) failed = true;
+      if (!failed && !o_done(k - 1)) failed = true;
       ptx::tc_fence_after();
-      float mine = 0.f;
+      bar_sync(3, 256);                         // the maxima are final
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float x = l[r];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (lane == r) mine = x;
-      }
-      // (the other buffer than the last tile's: no warp still reads it)
-      if (lane < R) sh.red[k & 1][warp][lane] = mine;
-      failed = ptx::bar_red_or(1, 128, failed);
+      for (int r = 0; r < R; ++r) l[r] *= ex2(sh.mb[wg][r] - sh.m[r]);
+      const float mine = warp_sums<R>(l, lane);
+      if (lane < R) sh.red[warp][lane] = mine;
+      failed = ptx::bar_red_or(3, 256, failed);
       if (failed) break;
       float total = 0.f;
-      if (lane < R)
-        total = (sh.red[k & 1][0][lane] + sh.red[k & 1][1][lane]) +
-                (sh.red[k & 1][2][lane] + sh.red[k & 1][3][lane]);
+      if (lane < R) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) total += sh.red[i][lane];
+      }
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      const float lse2 = m_row == -INFINITY && total == 0.f ? -INFINITY
-                                                            : m_row - kBias + log2f(total);
       const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
       const int slot = 2 * blockIdx.x + (seg.t0 > 0 ? 0 : 1);
       if (warp == 0 && lane < rows) {
+        const float lse2 = total == 0.f ? -INFINITY : sh.m[lane] + log2f(total);
         if (!whole) w.lse2[slot * R + lane] = lse2;
-        else if (p.lse)
-          p.lse[(int64_t)(walk.s.first + (row0 + lane) / p.H) * p.lse_s + (row0 + lane) % p.H] =
-              lse2 * kLn2;
+        else if (p.lse) p.lse[sh.lse[lane]] = lse2 * kLn2;
       }
 #pragma unroll 1
-      for (int c = 0; c < NCH; ++c) {
-        float o[N];
-        ptx::tmem_ld<N>(tmem + c * N + lane_base, o);
-        ptx::tmem_wait_ld();
+      for (int i = wg; i < NCH * (R / 16); i += 2) {       // 128 channels of 16 rows
+        const int c = i / (R / 16), g = 16 * (i % (R / 16));
+        float o[NP * 16];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float f = __shfl_sync(0xffffffffu, inv, r);
-          const float x = f == 0.f ? 0.f : join<NT>(o + r, R) * f;
-          if (r < rows) {
-            const int ch = c * 128 + tt;
-            if (whole) {
-              T* dst = static_cast<T*>(p.out) + (int64_t)(walk.s.first + (row0 + r) / p.H) * p.o_s[0] +
-                       (int64_t)((row0 + r) % p.H) * p.o_s[1];
-              st(dst + ch, x);
-            } else {
-              w.part[((int64_t)slot * R + r) * p.KVL + ch] = x;
-            }
-          }
+        for (int j = 0; j < NP; ++j)
+          ptx::tmem_ld16(tmem + c * NO + j * R + g + lane_base, o + 16 * j);
+        ptx::tmem_wait_ld();
+        const int ch = c * 128 + tt;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float f = __shfl_sync(0xffffffffu, inv, g + r);
+          o[r] = f == 0.f ? 0.f : join<NP>(o + r, 16) * f;
+        }
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (g + r < rows) st(static_cast<T*>(p.out) + sh.out[g + r] + ch, o[r]);
+        } else {
+          float* part = w.part + ((int64_t)slot * R + g) * p.KVL + ch;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (g + r < rows) part[r * p.KVL] = o[r];
         }
       }
-      // the next segment's queries and row figures come after all warps are done here
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      ptx::tc_fence_before();
+      bar_sync(3, 256);                         // before the next segment's figures and products
     }
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  if (warp == 5) {
+  if (warp == 9) {
     ptx::tmem_relinquish();
     ptx::tmem_dealloc(tmem, 512);
   }
@@ -809,11 +944,10 @@ int device_sms() {
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Rows per group: 16 where the sequences of the call have no more rows than that
-// on average, or where 32 rows leave no room for the two stages that the order
-// of the products needs (fp16, KVL 512 with a rope part); else 32.
-int rows_per_group(const CacheParams& p, int terms) {
+// on average, or where 32 rows leave too small a ring; else 32.
+int rows_per_group(const CacheParams& p, int q_terms) {
   if (((int64_t)p.N * p.H + p.B - 1) / p.B <= 16) return 16;
-  return stages(p.KVL, p.DR, terms, 32) >= 2 ? 32 : 16;
+  return ring_chunks(p.KVL, q_terms, 32) >= ring_least(p.KVL, p.DR) ? 32 : 16;
 }
 
 template <typename T, int R, int NCH>
@@ -821,10 +955,10 @@ cudaError_t launch(const CacheParams& p, Work w, const CUtensorMap& mc, const CU
                    int ranges, cudaStream_t s) {
   using C = Cfg<T, R, NCH>;
   auto k = cache_attn_kernel<T, R, NCH>;
-  w.stages = stages(p.KVL, p.DR, C::NT, R);
+  w.ring = ring_chunks(p.KVL, C::NQ, R);
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
   if (e != cudaSuccess) return e;
-  const size_t smem = fixed_bytes(p.KVL, C::NT, R) + w.stages * stage_bytes(p.KVL, p.DR);
+  const size_t smem = fixed_bytes(p.KVL, C::NQ, R) + w.ring * CHUNK;
   e = launch_dependent(k, dim3(ranges), kThreads, smem, s, p, w, mc, mr);
   if (e != cudaSuccess) return e;
   return launch_dependent(cache_join_kernel<T, R>, dim3(ranges - 1, R), 128, 0, s, p, w);
@@ -867,7 +1001,7 @@ size_t attention_workspace_bytes(const CacheParams& p) {
 
 cudaError_t launch_attention(const CacheParams& p, int io_dtype, void* workspace, cudaStream_t s) {
   const int ranges = device_sms();
-  const int R = rows_per_group(p, io_dtype == KDA_DTYPE_F16 ? kTerms<__half> : kTerms<__nv_bfloat16>);
+  const int R = rows_per_group(p, io_dtype == KDA_DTYPE_F16 ? kQTerms<__half> : kQTerms<__nv_bfloat16>);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Work w{};
   w.part = reinterpret_cast<float*>(ws);
