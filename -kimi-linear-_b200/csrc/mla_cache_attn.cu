@@ -9,20 +9,18 @@
 // of both products, the rows are the N side.
 //   S^T [128 positions x rows]   = codes [128 x KVL] (K-major)       Q^T
 //   O^T [128 channels x rows] += codes^T [128 ch x 128 pos] (M-major) P^T, per 128 channels
-// What is not e4m3 is split into e4m3 terms that are exact or nearly so, each
-// 16 times finer than the one before: x = x0 + x1 / 16 (+ x2 / 256).  A query
-// (scaled by a power of two) in bf16 has 8 significant bits, two terms; fp16 has
-// 11, three.  The softmax's weights take as many terms: 2^-9 or 2^-13 of each
-// weight, and 2^-20 of the largest, less than the output's own rounding.  The
-// terms are more columns of N and are added in fp32 afterwards: at 16 rows the
-// products are bound by reading the codes from shared memory (4 KB per
-// instruction of 128 x N x 32), so the extra columns cost next to nothing.
+// What is not in 8 bits is split into 8-bit terms, each finer than the one before:
+// x = x0 + x1 / 16 + ... .  A query (scaled by a power of two) in bf16 has 8
+// significant bits, two e4m3 terms hold it; fp16 takes three.  A softmax weight takes
+// three terms, enough that the output's own rounding is the larger error.  The terms
+// are more columns of N and are added in fp32 afterwards: an instruction of 128 x N x
+// 32 spends its time on reading 4 KB of codes from shared memory, so the columns cost
+// little (41 cycles at N = 32, 49 at 64, 56 at 96).
 //
-// A position's scale is a power of two, so the weight that meets the codes is
+// A position's scale s_t is a power of two, so the weight that meets the codes is
 //   P_t = exp2(z_t log2e + log2 s_t - M),  M the running maximum of the exponents,
-// and the sum takes P_t / s_t: the largest P is 1 whatever the scales are.  M
-// moves (and O is rescaled in TMEM) only where a row's maximum grew by more than
-// 2^2: P carries a factor 2^6, so it stays below e4m3's largest 448 until then.
+// and the sum takes P_t / s_t: P stays in range whatever the scales are.  M moves
+// (and O is rescaled in TMEM) only where a row outgrows P's format.
 //
 // Work: a row group (R rows of a sequence) times its tiles; all the tiles of a
 // call, in order, are cut into equal ranges, one per SM, so a long sequence is
@@ -51,13 +49,37 @@ constexpr int kSmemMax = 232448;           // 227 KB per block
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kBias = 4.f;               // P carries 2^4 ...
-constexpr float kSlack = 4.f;              // ... and may outgrow the maximum by 2^4 (2^8 < 448)
 constexpr float kUnset = -1e30f;           // maximum of a row that has seen nothing
 
-// e4m3 terms of a query and of a softmax weight
+// e4m3 terms of a query, each 16 times finer: exact for bf16 (8 bits), 2^-12 for fp16
 template <typename T> constexpr int kQTerms = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
+// Terms of a softmax weight P.  bf16: e5m2, each 8 times finer (2^-9 of the weight).
+// Its range lets P carry 2^5 and outgrow the maximum by 2^10 (2^15 < 57344) before
+// the maximum moves, and weights of 2^-28 of the largest still count.  fp16: e4m3,
+// each 16 times finer (2^-12), 2^2, 2^6 (2^8 < 448) and 2^-20.
 constexpr int NP = 3;
+template <typename T> struct PFormat {
+  static constexpr uint32_t FMT = 0;
+  static constexpr float FINER = 16.f, BIAS = 2.f, SLACK = 6.f;
+  static __device__ __forceinline__ uint32_t to(float a, float b, float c, float d) {
+    return to_e4m3x4(a, b, c, d);
+  }
+  static __device__ __forceinline__ float2 from(uint32_t u) { return from_e4m3x2(u); }
+};
+template <> struct PFormat<__nv_bfloat16> {
+  static constexpr uint32_t FMT = 1;
+  static constexpr float FINER = 8.f, BIAS = 5.f, SLACK = 10.f;
+  static __device__ __forceinline__ uint32_t to(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E5M2);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E5M2);
+    return lo | (hi << 16);
+  }
+  static __device__ __forceinline__ float2 from(uint32_t u) {      // e5m2: the upper half of fp16
+    const uint32_t h = __byte_perm(u, 0, 0x1404);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+  }
+};
+struct QFormat : PFormat<__half> {};       // queries: e4m3
 
 template <typename T, int R, int NCH>
 struct Cfg {
@@ -236,9 +258,11 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
          (static_cast<uint64_t>(2) << 61);
 }
-// Instruction descriptors: fp32 accumulator; e4m3 operands, or `fmt` 0 = f16, 1 = bf16
-__host__ __device__ constexpr uint32_t idesc(int N, bool a_m_major, bool b_n_major, uint32_t fmt) {
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_m_major ? 1u : 0u) << 15) |
+// Instruction descriptors: fp32 accumulator; 8-bit formats 0 = e4m3, 1 = e5m2, 16-bit
+// ones 0 = f16, 1 = bf16
+__host__ __device__ constexpr uint32_t idesc(int N, bool a_m_major, bool b_n_major, uint32_t a_fmt,
+                                              uint32_t b_fmt) {
+  return (1u << 4) | (a_fmt << 7) | (b_fmt << 10) | ((a_m_major ? 1u : 0u) << 15) |
          ((b_n_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
 }
 // largest of the 32 lanes' values (NaN ignored)
@@ -277,27 +301,27 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   }
 }
 
-// x = t[0] + t[1] / 16 (+ t[2] / 256), for four values: four codes per term
-template <int NT>
+// x = t[0] + t[1] / FINER (+ t[2] / FINER^2), for four values: four codes per term
+template <typename F, int NT>
 __device__ __forceinline__ void split4(const float (&x)[4], uint32_t (&t)[NT]) {
   float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    t[j] = to_e4m3x4(r[0], r[1], r[2], r[3]);
+    t[j] = F::to(r[0], r[1], r[2], r[3]);
     if (j + 1 < NT) {
-      const float2 lo = from_e4m3x2(t[j]), hi = from_e4m3x2(t[j] >> 16);
-      r[0] = (r[0] - lo.x) * 16.f;
-      r[1] = (r[1] - lo.y) * 16.f;
-      r[2] = (r[2] - hi.x) * 16.f;
-      r[3] = (r[3] - hi.y) * 16.f;
+      const float2 lo = F::from(t[j]), hi = F::from(t[j] >> 16);
+      r[0] = (r[0] - lo.x) * F::FINER;
+      r[1] = (r[1] - lo.y) * F::FINER;
+      r[2] = (r[2] - hi.x) * F::FINER;
+      r[3] = (r[3] - hi.y) * F::FINER;
     }
   }
 }
-template <int NT>
-__device__ __forceinline__ float join(const float* t, int stride) {   // t[0] + t[1] / 16 (+ ...)
+template <typename F, int NT>
+__device__ __forceinline__ float join(const float* t, int stride) {
   float x = t[(NT - 1) * stride];
 #pragma unroll
-  for (int j = NT - 2; j >= 0; --j) x = fmaf(x, 1.f / 16.f, t[j * stride]);
+  for (int j = NT - 2; j >= 0; --j) x = fmaf(x, 1.f / F::FINER, t[j * stride]);
   return x;
 }
 
@@ -312,7 +336,7 @@ struct Shared {            // at the end of dynamic shared memory
   int b;
   // per row of the group
   float q_scale[32];       // 2^e scale log2e
-  float m[32];             // running maximum less kBias
+  float m[32];             // running maximum less BIAS
   float mb[2][32];         // the same as of each softmax group's last tile
   float alpha[2][32];      // what its sums (and O) are rescaled by
   int seen[32];            // positions that it sees
@@ -347,6 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUtensorMap map_codes,
                   const __grid_constant__ CUtensorMap map_rope) {
   using C = Cfg<T, R, NCH>;
+  using F = PFormat<T>;
   constexpr int NQ = C::NQ, NS = C::NS, NO = C::NO;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -488,8 +513,10 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   } else if (warp == 9) {
     // ======== MMA issue: S of tile k + 1 ahead of O of tile k
     {
-      constexpr uint32_t id_s = idesc(NS, false, false, 0), id_o = idesc(NO, true, true, 0);
-      constexpr uint32_t id_r = idesc(R, false, false, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+      constexpr uint32_t kHalf = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      constexpr uint32_t id_s = idesc(NS, false, false, 0, QFormat::FMT);
+      constexpr uint32_t id_o = idesc(NO, true, true, 0, F::FMT);
+      constexpr uint32_t id_r = idesc(R, false, false, kHalf, kHalf);
       const uint32_t sm0 = ptx::smem_u32(sm);
       const uint64_t dq = sdesc_sw128(ptx::smem_u32(q_s)), dqr = sdesc_sw128(ptx::smem_u32(qr_s));
       // P: 16 rows x 8 positions a core matrix, 128 bytes on along the positions,
@@ -669,7 +696,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[c][j] *= inv;
             uint32_t term[NQ];
-            split4<NQ>(x[c], term);
+            split4<QFormat, NQ>(x[c], term);
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
               *reinterpret_cast<uint32_t*>(q_s + c * NS * 128 + swz(j * R + r, 4 * lane)) = term[j];
@@ -720,7 +747,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           ptx::tmem_wait_ld();
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            a[g + r] = fmaf(join<NQ>(z + r, 16), sh.q_scale[g + r] * s, ls);
+            a[g + r] = fmaf(join<QFormat, NQ>(z + r, 16), sh.q_scale[g + r] * s, ls);
         }
         ptx::tc_fence_before();
         ptx::mbar_arrive(&sh.s_empty[par]);
@@ -759,7 +786,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         float top = -INFINITY;
 #pragma unroll
         for (int r = 0; r < R; ++r) top = fmaxf(top, a[r] - sh.mb[par][r]);
-        const bool grew = ptx::bar_red_or(1 + wg, 128, failed || top > kBias + kSlack);
+        const bool grew = ptx::bar_red_or(1 + wg, 128, failed || top > F::BIAS + F::SLACK);
         if (tt == 0) sh.changed[par] = grew;
         if (grew) {
           // a row outgrew P's range (or has its first position): new maxima, and O
@@ -776,22 +803,31 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
             const float* red = &sh.red[4 * wg][tt];
             const float mx = fmaxf(fmaxf(red[0], red[32]), fmaxf(red[64], red[96]));
             const float old = sh.m[tt];
-            const bool up = mx - old > kBias + kSlack;
-            sh.alpha[par][tt] = up ? ex2(old - (mx - kBias)) : 1.f;
-            if (up) sh.m[tt] = sh.mb[par][tt] = mx - kBias;
+            const bool up = mx - old > F::BIAS + F::SLACK;
+            sh.alpha[par][tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
+            if (up) sh.m[tt] = sh.mb[par][tt] = mx - F::BIAS;
           }
           bar_sync(1 + wg, 128);
           if (!first) {
             if (!o_done(k - 1)) failed = true;
             ptx::tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < NCH * NO; c += 48) {
-              float o[48];
-              ptx::tmem_ld<48>(tmem + c + lane_base, o);
-              ptx::tmem_wait_ld();
+            for (int g = 0; g < R; g += 16) {
+              float al[16];
 #pragma unroll
-              for (int i = 0; i < 48; ++i) o[i] *= sh.alpha[par][(c + i) % R];
-              ptx::tmem_st<48>(tmem + c + lane_base, o);
+              for (int r = 0; r < 16; ++r) al[r] = sh.alpha[par][g + r];
+#pragma unroll 1
+              for (int c = 0; c < NCH; ++c) {
+                const uint32_t at = tmem + c * NO + g + lane_base;
+                float o[NP * 16];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) ptx::tmem_ld16(at + j * R, o + 16 * j);
+                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < NP * 16; ++i) o[i] *= al[i % 16];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) ptx::tmem_st16(at + j * R, o + 16 * j);
+              }
             }
             ptx::tmem_wait_st();
             ptx::tc_fence_before();
@@ -816,7 +852,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
               l[r] = fmaf(e4[i], rs, l[r]);
             }
             uint32_t u[NP];
-            split4<NP>(e4, u);
+            split4<F, NP>(e4, u);
 #pragma unroll
             for (int j = 0; j < NP; ++j) term[j][q] = u[j];
           }
@@ -865,7 +901,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float f = __shfl_sync(0xffffffffu, inv, g + r);
-          o[r] = f == 0.f ? 0.f : join<NP>(o + r, 16) * f;
+          o[r] = f == 0.f ? 0.f : join<F, NP>(o + r, 16) * f;
         }
         if (whole) {
 #pragma unroll
