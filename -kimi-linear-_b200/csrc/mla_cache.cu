@@ -280,6 +280,9 @@ int mla_cache_attention(const MlaCacheArgs* a, void* stream) {
   p.vec = aligned16(a->q_lat) && a->q_lat_stride[0] % 8 == 0 && a->q_lat_stride[1] % 8 == 0 &&
           (!a->DR || (aligned16(a->q_rope) && a->q_rope_stride[0] % 8 == 0 &&
                       a->q_rope_stride[1] % 8 == 0));
+  p.h_mul = p.H == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / p.H);
+  p.out_vec = reinterpret_cast<uintptr_t>(a->out) % 4 == 0 && a->out_stride[0] % 2 == 0 &&
+              a->out_stride[1] % 2 == 0;
   const cudaError_t e =
       launch_attention(p, a->io_dtype, a->workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;

@@ -30,6 +30,8 @@ struct CacheParams {
   const void* q_rope; int64_t qr_s[2];
   void* out; int64_t o_s[2];
   float* lse; int64_t lse_s;
+  uint32_t h_mul;                   // 2^32 / H, rounded down (H = 1: 2^32 - 1)
+  bool out_vec;                     // out rows start on 4-byte boundaries
   bool vec;                         // c_kv / k_rope (append, read) or q_lat / q_rope (attention)
                                     // rows start on 16-byte boundaries
 };

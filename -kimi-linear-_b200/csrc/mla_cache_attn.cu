@@ -43,8 +43,12 @@ namespace {
 
 constexpr int TILE = 128;                  // positions per tile (MMA M)
 constexpr int CHUNK = TILE * 128;          // bytes of 128 positions x 128 bytes
-constexpr int kThreads = 320;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue
+constexpr int kThreads = 384;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue, 10 cuts
+// Registers: the block starts with 384 x 168; the softmax warps take 208 each, the
+// others keep 88 (256 x 208 + 128 x 88 = 384 x 168).
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr int kMaxRing = 14;
+constexpr int kMaxRanges = 256;            // blocks (SMs) that a call's tiles are cut over
 constexpr int kSmemMax = 232448;           // 227 KB per block
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -53,33 +57,60 @@ constexpr float kUnset = -1e30f;           // maximum of a row that has seen not
 
 // e4m3 terms of a query, each 16 times finer: exact for bf16 (8 bits), 2^-12 for fp16
 template <typename T> constexpr int kQTerms = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
-// Terms of a softmax weight P.  bf16: e5m2, each 8 times finer (2^-9 of the weight).
-// Its range lets P carry 2^5 and outgrow the maximum by 2^10 (2^15 < 57344) before
-// the maximum moves, and weights of 2^-28 of the largest still count.  fp16: e4m3,
-// each 16 times finer (2^-12), 2^2, 2^6 (2^8 < 448) and 2^-20.
+// Terms of a softmax weight P, cut out of its fp16 value (a code of either format is a
+// run of an fp16's bits), so that only one conversion is needed:
+//  * bf16: e5m2 = the upper byte of fp16.  P is rounded to 9 bits (2^-10 of itself) and
+//    cut into three terms, each 8 times finer.  It carries 2^5 and may outgrow the
+//    maximum by 2^10 (2^15 < 57344) before the maximum moves.
+//  * fp16: e4m3 = bits 13 .. 7 of fp16, for the value times 2^-8.  P in fp16 (11 bits,
+//    2^-12) is cut into three terms, each 16 times finer.  It carries 2^-6 and may
+//    outgrow the maximum by 2^6 (2^8 2^-8; 448 is the format's largest).
+// Weights down to 2^-27 (2^-18) of the largest still count.
 constexpr int NP = 3;
 template <typename T> struct PFormat {
   static constexpr uint32_t FMT = 0;
-  static constexpr float FINER = 16.f, BIAS = 2.f, SLACK = 6.f;
-  static __device__ __forceinline__ uint32_t to(float a, float b, float c, float d) {
-    return to_e4m3x4(a, b, c, d);
+  static constexpr float FINER = 16.f, BIAS = -6.f, SLACK = 6.f, GAIN = 256.f;   // code value / P
+  static __device__ __forceinline__ void split(const float (&x)[4], uint32_t (&t)[NP]) {
+    __half2 r[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
+    const __half2 finer = __float2half2_rn(FINER);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      uint32_t c[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        c[i] = *reinterpret_cast<const uint32_t*>(&r[i]) & 0x3f803f80u;
+        if (j + 1 < NP) r[i] = __hmul2(__hsub2(r[i], *reinterpret_cast<const __half2*>(&c[i])), finer);
+      }
+      t[j] = __byte_perm(c[0] >> 7, c[1] >> 7, 0x6420);
+    }
   }
-  static __device__ __forceinline__ float2 from(uint32_t u) { return from_e4m3x2(u); }
 };
 template <> struct PFormat<__nv_bfloat16> {
   static constexpr uint32_t FMT = 1;
-  static constexpr float FINER = 8.f, BIAS = 5.f, SLACK = 10.f;
-  static __device__ __forceinline__ uint32_t to(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E5M2);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E5M2);
-    return lo | (hi << 16);
-  }
-  static __device__ __forceinline__ float2 from(uint32_t u) {      // e5m2: the upper half of fp16
-    const uint32_t h = __byte_perm(u, 0, 0x1404);
-    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+  static constexpr float FINER = 8.f, BIAS = 5.f, SLACK = 10.f, GAIN = 1.f;
+  static __device__ __forceinline__ void split(const float (&x)[4], uint32_t (&t)[NP]) {
+    __half2 r[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
+    const __half2 finer = __float2half2_rn(FINER);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t u = *reinterpret_cast<const uint32_t*>(&r[i]);
+      u = (u + 0x00020002u) & 0xfffcfffcu;           // (a NaN is lost here; the sum keeps it)
+      r[i] = *reinterpret_cast<const __half2*>(&u);
+    }
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      uint32_t c[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        c[i] = *reinterpret_cast<const uint32_t*>(&r[i]) & 0xff00ff00u;
+        if (j + 1 < NP) r[i] = __hmul2(__hsub2(r[i], *reinterpret_cast<const __half2*>(&c[i])), finer);
+      }
+      t[j] = __byte_perm(c[0], c[1], 0x7531);
+    }
   }
 };
-struct QFormat : PFormat<__half> {};       // queries: e4m3
+constexpr uint32_t kE4M3 = 0;
+constexpr float kQFiner = 16.f;
 
 template <typename T, int R, int NCH>
 struct Cfg {
@@ -89,12 +120,12 @@ struct Cfg {
   static_assert(NCH * NO + SBUF * NS <= 512, "TMEM columns");
 };
 
-// Shared memory besides the ring (4 KB: barriers, rows; 1 KB: alignment), and the
+// Shared memory besides the ring (barriers and rows; 1 KB: alignment), and the
 // chunks that fit beside it.  The order of the products needs the codes of one
 // tile and all of the next at once.
-constexpr int kFixedBytes = 4096 + 1024;
+constexpr int kSharedBytes(int R) { return R == 16 ? 4096 : 5120; }
 int fixed_bytes(int kvl, int q_terms, int R) {
-  return kFixedBytes + q_terms * R * kvl + R * 128 + 2 * NP * R * 128;
+  return kSharedBytes(R) + 1024 + q_terms * R * kvl + R * 128 + 2 * NP * R * 128;
 }
 int ring_chunks(int kvl, int q_terms, int R) {
   const int n = (kSmemMax - fixed_bytes(kvl, q_terms, R)) / CHUNK;
@@ -119,22 +150,28 @@ struct Work {
 // ---------------------------------------------------------------------------
 // how the tiles of a call are counted and cut
 // ---------------------------------------------------------------------------
-// Sequence b as R-row groups.  Groups of one sequence see more and more
-// positions; they are counted in pairs (g, groups - 1 - g), which all have about
-// as many tiles, so that a place in the count is found by a division.
+// Sequence b as R-row groups.  A group counts for its tiles and kSetup more: what
+// its queries, its first tile's latency and its result cost (measured: about three
+// tiles).  Groups of one sequence see more and more positions; they are counted in
+// pairs (g, groups - 1 - g), which all count about the same, so that a place in the
+// count is found by a division.
+constexpr int kSetup = 3;
 struct Seq {
   int first, n, off;       // new tokens; token i sits at off + i
-  int groups, pair;        // row groups; tiles counted per pair
+  int groups, pair;        // row groups; count per pair
   int cap;                 // positions that the table holds
 };
 
-template <int R>
+__device__ __forceinline__ int div_heads(const CacheParams& p, int row) {
+  const uint32_t q = __umulhi((uint32_t)row, p.h_mul);      // h_mul = 2^32 / H: short by one at most
+  return (int)q + ((uint32_t)row - q * p.H >= (uint32_t)p.H);
+}
 __device__ __forceinline__ int seen_by(const CacheParams& p, const Seq& s, int row) {
-  return max(0, min(s.off + min(row / p.H, s.n - 1) + 1, s.cap));
+  return max(0, min(s.off + min(div_heads(p, row), s.n - 1) + 1, s.cap));
 }
 template <int R>
 __device__ __forceinline__ int group_tiles(const CacheParams& p, const Seq& s, int g) {
-  return max(1, (seen_by<R>(p, s, g * R + R - 1) + TILE - 1) / TILE);
+  return max(1, (seen_by(p, s, g * R + R - 1) + TILE - 1) / TILE);
 }
 template <int R>
 __device__ __forceinline__ Seq load_seq(const CacheParams& p, int b) {
@@ -144,17 +181,38 @@ __device__ __forceinline__ Seq load_seq(const CacheParams& p, int b) {
   s.cap = p.max_pages * p.page_size;
   s.groups = (int)(((int64_t)s.n * p.H + R - 1) / R);
   s.pair = 0;
-  if (s.groups == 1) s.pair = group_tiles<R>(p, s, 0);
+  if (s.groups == 1) s.pair = kSetup + group_tiles<R>(p, s, 0);
   // the first pair's sum, and up to two more: the last group may be short, and the
   // tiles are rounded up.  (Where the table ends before the sequence: all may be as long
   // as the last.)
   if (s.groups > 1)
-    s.pair = group_tiles<R>(p, s, s.off + s.n > s.cap ? s.groups - 1 : 0) +
-             group_tiles<R>(p, s, s.groups - 1) + 2;
+    s.pair = 2 * kSetup + 2 + group_tiles<R>(p, s, s.off + s.n > s.cap ? s.groups - 1 : 0) +
+             group_tiles<R>(p, s, s.groups - 1);
   return s;
 }
 __device__ __forceinline__ int64_t seq_tiles(const Seq& s) {
   return (int64_t)((s.groups + 1) / 2) * s.pair;
+}
+
+// What lies at count r of a sequence: place q of pair (g1, g2), which has n1 + n2
+// tiles (n2 = 0: the middle group, alone).  Group g1 takes the places up to kSetup +
+// n1, its tile i place kSetup + i; g2 follows in the same way.
+template <int R>
+__device__ __forceinline__ void place(const CacheParams& p, const Seq& s, int64_t r, int& g1, int& q,
+                                      int& g2, int& n1, int& n2) {
+  if (r < s.pair) {
+    g1 = 0;
+    q = (int)r;
+  } else if (r <= 0x7fffffff) {
+    g1 = (int)((uint32_t)r / (uint32_t)s.pair);
+    q = (int)r - g1 * s.pair;
+  } else {
+    g1 = (int)(r / s.pair);
+    q = (int)(r - (int64_t)g1 * s.pair);
+  }
+  g2 = s.groups - 1 - g1;
+  n1 = group_tiles<R>(p, s, g1);
+  n2 = g2 > g1 ? group_tiles<R>(p, s, g2) : 0;
 }
 
 struct Segment {
@@ -169,16 +227,13 @@ struct Walk {
   Seq s;
   int b;
   int64_t u, end, base;    // base: count at which sequence b starts
-  int second_t1;           // pending second group of a pair: its last tile (0: none)
-  int second_g, second_t0;
-  __device__ Walk(const CacheParams& p_, int b_, int64_t base_, int64_t u_, int64_t end_)
-      : p(p_), b(b_), u(u_), end(end_), base(base_), second_t1(0) {
-    if (u < end) s = load_seq<R>(p, b);
-  }
+  Segment second;          // of the pair under way, when there is one (t1 > t0)
+  __device__ Walk(const CacheParams& p_, const Seq& s_, int b_, int64_t base_, int64_t u_, int64_t end_)
+      : p(p_), s(s_), b(b_), u(u_), end(end_), base(base_), second{0, 0, 0, 0, 0} {}
   __device__ bool next(Segment& seg) {
-    if (second_t1 > 0) {
-      seg = Segment{b, second_g, second_t0, second_t1, group_tiles<R>(p, s, second_g)};
-      second_t1 = 0;
+    if (second.t1 > second.t0) {
+      seg = second;
+      second.t1 = second.t0;
       return true;
     }
     while (u < end) {
@@ -186,25 +241,19 @@ struct Walk {
         base += seq_tiles(s);
         s = load_seq<R>(p, ++b);
       }
-      const int64_t r = u - base;
-      const int pair = (int)(r / s.pair), q = (int)(r % s.pair);
-      const int g1 = pair, g2 = s.groups - 1 - pair;
-      const int n1 = group_tiles<R>(p, s, g1), n2 = g2 > g1 ? group_tiles<R>(p, s, g2) : 0;
-      const int stop = (int)min((int64_t)s.pair, q + (end - u));
-      // the last place of a pair takes whatever is left of it
-      const int last = stop == s.pair ? n1 + n2 : min(stop, n1 + n2);
+      int g1, q, g2, n1, n2;
+      place<R>(p, s, u - base, g1, q, g2, n1, n2);
+      const int end1 = kSetup + n1, all = end1 + (n2 > 0 ? kSetup + n2 : 0);
+      int stop = (int)min((int64_t)s.pair, q + (end - u));
       u += stop - q;
-      if (q < n1) {
-        seg = Segment{b, g1, q, min(last, n1), n1};
-        if (last > n1) {
-          second_g = g2;
-          second_t0 = 0;
-          second_t1 = last - n1;
-        }
-        return true;
-      }
-      if (q < last) {
-        seg = Segment{b, g2, q - n1, last - n1, n2};
+      // the last place of a pair takes whatever is left of it
+      stop = stop == s.pair ? all : min(stop, all);
+      second = Segment{b, g2, max(0, q - end1 - kSetup), stop - end1 - kSetup, n2};
+      seg = Segment{b, g1, max(0, q - kSetup), min(stop, end1) - kSetup, n1};
+      if (seg.t1 > seg.t0) return true;
+      if (second.t1 > second.t0) {
+        seg = second;
+        second.t1 = second.t0;
         return true;
       }
     }
@@ -301,49 +350,57 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   }
 }
 
-// x = t[0] + t[1] / FINER (+ t[2] / FINER^2), for four values: four codes per term
-template <typename F, int NT>
-__device__ __forceinline__ void split4(const float (&x)[4], uint32_t (&t)[NT]) {
+// A query's values as e4m3 terms: x = t[0] + t[1] / 16 (+ t[2] / 256), four at a time.
+template <int NT>
+__device__ __forceinline__ void split_query(const float (&x)[4], uint32_t (&t)[NT]) {
   float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    t[j] = F::to(r[0], r[1], r[2], r[3]);
+    t[j] = to_e4m3x4(r[0], r[1], r[2], r[3]);
     if (j + 1 < NT) {
-      const float2 lo = F::from(t[j]), hi = F::from(t[j] >> 16);
-      r[0] = (r[0] - lo.x) * F::FINER;
-      r[1] = (r[1] - lo.y) * F::FINER;
-      r[2] = (r[2] - hi.x) * F::FINER;
-      r[3] = (r[3] - hi.y) * F::FINER;
+      const float2 lo = from_e4m3x2(t[j]), hi = from_e4m3x2(t[j] >> 16);
+      r[0] = (r[0] - lo.x) * kQFiner;
+      r[1] = (r[1] - lo.y) * kQFiner;
+      r[2] = (r[2] - hi.x) * kQFiner;
+      r[3] = (r[3] - hi.y) * kQFiner;
     }
   }
 }
-template <typename F, int NT>
-__device__ __forceinline__ float join(const float* t, int stride) {
+// the sum of a value's terms, each `finer` times finer
+template <int NT>
+__device__ __forceinline__ float join(const float* t, int stride, float finer) {
   float x = t[(NT - 1) * stride];
 #pragma unroll
-  for (int j = NT - 2; j >= 0; --j) x = fmaf(x, 1.f / F::FINER, t[j * stride]);
+  for (int j = NT - 2; j >= 0; --j) x = fmaf(x, 1.f / finer, t[j * stride]);
   return x;
 }
 
+template <int R>
+struct Rows {              // per row of a group
+  float q_scale[R];        // 2^e scale log2e
+  float m[R];              // running maximum less BIAS
+  float mb[2][R];          // the same as of each softmax group's last tile
+  float alpha[2][R];       // what its sums (and O) are rescaled by
+  float inv[R];            // 1 / sum
+  int seen[R];             // positions that it sees
+  int64_t out[R], lse[R];  // where its results go
+};
+template <int R>
 struct Shared {            // at the end of dynamic shared memory
   uint64_t full[kMaxRing], empty[kMaxRing];
   uint64_t s_full[2], s_empty[2], p_full[2], o_done[4], m_full[2], q_ready, drain;
   uint32_t tmem;
   int abort_flag;
   int changed[2];          // the tile of this parity moved the maxima
-  int64_t scan[kThreads / 32];
+  int64_t scan[(kThreads + 31) / 32];
   int64_t base;            // where the range starts: count at which sequence b starts
   int b;
-  // per row of the group
-  float q_scale[32];       // 2^e scale log2e
-  float m[32];             // running maximum less BIAS
-  float mb[2][32];         // the same as of each softmax group's last tile
-  float alpha[2][32];      // what its sums (and O) are rescaled by
-  int seen[32];            // positions that it sees
-  int64_t out[32], lse[32];  // where its results go
-  float red[8][32];        // per warp and row: maxima, sums
+  Seq seq;                 // and that sequence
+  Rows<R> rows[2];         // of this segment and the next
+  float red[8][R];         // per warp and row: maxima, sums
 };
-static_assert(sizeof(Shared) <= kFixedBytes - 1024, "room for barriers and rows");
+static_assert(sizeof(Shared<16>) <= kSharedBytes(16) && sizeof(Shared<32>) <= kSharedBytes(32),
+              "room for barriers and rows");
 
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -378,7 +435,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   uint8_t* q_s = sm + w.ring * CHUNK;
   uint8_t* qr_s = q_s + NCH * NS * 128;
   uint8_t* p_s = qr_s + R * 128;                // two buffers
-  Shared& sh = *reinterpret_cast<Shared*>(p_s + 2 * NO * 128);
+  Shared<R>& sh = *reinterpret_cast<Shared<R>*>(p_s + 2 * NO * 128);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int ring = w.ring, tile_chunks = NCH + (p.DR ? 1 : 0);
 
@@ -405,12 +462,16 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   ptx::grid_dep_launch();
 
   // ---- this block's range of the call's tiles
-  int64_t u0, u1;
+  int64_t u0, u1, range_tiles;
   {
     const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += seq_tiles(load_seq<R>(p, b));
+    Seq s{};
+    for (int b = b0; b < b1; ++b) {
+      s = load_seq<R>(p, b);
+      mine += seq_tiles(s);
+    }
     int64_t x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -430,53 +491,54 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     u1 = min(total, u0 + range);
     if (u0 < u1 && u0 >= before && u0 < before + mine) {
       int b = b0;
-      for (;; ++b) {
-        const int64_t n = seq_tiles(load_seq<R>(p, b));
-        if (u0 < before + n) break;
-        before += n;
+      if (per > 1) {
+        for (;; ++b) {
+          s = load_seq<R>(p, b);
+          if (u0 < before + seq_tiles(s)) break;
+          before += seq_tiles(s);
+        }
       }
       sh.b = b;
       sh.base = before;
+      sh.seq = s;
     }
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
-    // the group that this range starts inside of, for cache_join_kernel
-    if (tid == 0) {
-      Cut cut{-1, 0, 0, 0};
-      if (u0 < u1 && blockIdx.x > 0) {
-        const Seq s = load_seq<R>(p, sh.b);
-        const int64_t r = u0 - sh.base;
-        const int pair = (int)(r / s.pair), q = (int)(r % s.pair);
-        const int g1 = pair, g2 = s.groups - 1 - pair;
-        const int n1 = group_tiles<R>(p, s, g1), n2 = g2 > g1 ? group_tiles<R>(p, s, g2) : 0;
-        int64_t start = u0 - q;              // of the group
-        int n = 0;
-        if (q > 0 && q < n1) {
-          cut.b = sh.b; cut.g = g1; n = n1;
-        } else if (q > n1 && q < n1 + n2) {
-          cut.b = sh.b; cut.g = g2; start += n1; n = n2;
-        }
-        if (cut.b >= 0 && start >= u0 - range)
-          cut.parts = (int)((start + n - 1) / range) - (int)(start / range) + 1;
-      }
-      w.cuts[blockIdx.x] = cut;
-    }
+    range_tiles = range;
   }
   const uint32_t tmem = sh.tmem;
   const uint32_t tm_s = tmem + NCH * NO;        // S buffers after the O chunks
   volatile int* ab = &sh.abort_flag;
-  Walk<R> walk(p, sh.b, sh.base, u0, u1);
-  Segment seg;
-
-  if (warp == 8) {
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1);
+    Segment seg;
+  if (warp == 10) {
+    // ======== the group that this range starts inside of, for cache_join_kernel
+    Cut cut{-1, 0, 0, 0};
+    if (u0 < u1 && blockIdx.x > 0) {
+      int g1, q, g2, n1, n2;
+      place<R>(p, walk.s, u0 - sh.base, g1, q, g2, n1, n2);
+      int64_t start = u0 - q + kSetup;         // where the group's first tile counts
+      int n = 0;
+      if (q > kSetup && q < kSetup + n1) {
+        cut.b = sh.b; cut.g = g1; n = n1;
+      } else if (n2 > 0 && q > 2 * kSetup + n1 && q < 2 * kSetup + n1 + n2) {
+        cut.b = sh.b; cut.g = g2; start += kSetup + n1; n = n2;
+      }
+      if (cut.b >= 0 && start >= u0 - range_tiles)
+        cut.parts = (int)((start + n - 1) / range_tiles) - (int)(start / range_tiles) + 1;
+    }
+    if (lane == 0) w.cuts[blockIdx.x] = cut;
+  } else if (warp == 8) {
     // ======== loads: boxes of one page (at most 128 positions) x 128 bytes into a
     // ring of 16 KB chunks; a tile is its rope chunk, then its code chunks
     int slot = 0, round = 0, issued = 0;
     const int box_rows = min(p.page_size, TILE), boxes = TILE / box_rows;
     bool ok = true;
     while (ok && walk.next(seg)) {
-      const int seen = seen_by<R>(p, walk.s, seg.g * R + R - 1);
+      const int seen = seen_by(p, walk.s, seg.g * R + R - 1);
       if (seen == 0) continue;
       for (int t = seg.t0; t < seg.t1 && ok; ++t) {
         const int pos = t * TILE;
@@ -514,8 +576,8 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     // ======== MMA issue: S of tile k + 1 ahead of O of tile k
     {
       constexpr uint32_t kHalf = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-      constexpr uint32_t id_s = idesc(NS, false, false, 0, QFormat::FMT);
-      constexpr uint32_t id_o = idesc(NO, true, true, 0, F::FMT);
+      constexpr uint32_t id_s = idesc(NS, false, false, kE4M3, kE4M3);
+      constexpr uint32_t id_o = idesc(NO, true, true, kE4M3, F::FMT);
       constexpr uint32_t id_r = idesc(R, false, false, kHalf, kHalf);
       const uint32_t sm0 = ptx::smem_u32(sm);
       const uint64_t dq = sdesc_sw128(ptx::smem_u32(q_s)), dqr = sdesc_sw128(ptx::smem_u32(qr_s));
@@ -551,7 +613,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         return true;
       };
       while (ok && walk.next(seg)) {
-        if (seen_by<R>(p, walk.s, seg.g * R + R - 1) == 0) continue;
+        if (seen_by(p, walk.s, seg.g * R + R - 1) == 0) continue;
         if (!wait(&sh.q_ready, segs & 1, ab)) break;
         ++segs;
         for (int t = seg.t0; t < seg.t1; ++t) {
@@ -595,9 +657,12 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       }
     }
     __syncwarp();
+  }
   } else {
     // ======== softmax: two groups of four warps take the tiles in turn; thread =
     // position of the tile = TMEM lane
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1);
     const int wg = warp >> 2;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int tt = tid & 127;
@@ -607,124 +672,157 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     // neighbours; each group waits for its own last tile's products, so with four
     // barriers the phase asked for is the one under way or the one just ended.
     auto o_done = [&](int i) { return wait(&sh.o_done[i & 3], (i >> 2) & 1, ab); };
-    while (!failed && walk.next(seg)) {
-      const int row0 = seg.g * R, rows = min(R, (int)((int64_t)walk.s.n * p.H - row0));
-      const int seen = seen_by<R>(p, walk.s, row0 + R - 1);
-      const int seen0 = seen_by<R>(p, walk.s, row0);
-      if (seen == 0) {                          // nobody sees anything
+
+    // ---- the next segment that sees anything
+    struct Info : Segment {
+      int row0, rows, first, off;               // its rows, its sequence's new tokens
+      int seen, seen0;                          // positions that its last and first row see
+    };
+    auto next_segment = [&](Info& sg) {
+      while (walk.next(sg)) {
+        const int row0 = sg.g * R, rows = (int)min((int64_t)R, (int64_t)walk.s.n * p.H - row0);
+        const int first = walk.s.first;
+        sg.row0 = row0;
+        sg.rows = rows;
+        sg.first = first;
+        sg.off = walk.s.off;
+        sg.seen = seen_by(p, walk.s, row0 + R - 1);
+        sg.seen0 = seen_by(p, walk.s, row0);
+        if (tid == 0 && sg.off + walk.s.n > walk.s.cap) atomicExch(&g_attn_device_error, kErrOutside);
+        if (sg.seen > 0) return true;
         for (int r = warp; r < rows; r += 8) {
-          const int64_t n = walk.s.first + (row0 + r) / p.H, h = (row0 + r) % p.H;
+          const int i = div_heads(p, row0 + r);
+          const int64_t n = first + i, h = row0 + r - i * p.H;
           T* o = static_cast<T*>(p.out) + n * p.o_s[0] + h * p.o_s[1];
           for (int c = lane; c < p.KVL; c += 32) st(o + c, 0.f);
           if (lane == 0 && p.lse) p.lse[n * p.lse_s + h] = -INFINITY;
         }
-        continue;
       }
-      if (tid == 0 && walk.s.off + walk.s.n > walk.s.cap) atomicExch(&g_attn_device_error, kErrOutside);
-      // ---- scale of this thread's position, its page a tile before that
-      const int t_mine = seg.t0 + ((k ^ wg) & 1);          // this group's first tile
-      auto page_at = [&](int t) {
-        const int pos = t * TILE + tt;
-        return t < seg.t1 && pos < seen ? page_of(p, seg.b, pos) : -2;
-      };
-      auto scale_at = [&](int t, int page) {
-        if (page == -2) return 1.f;
-        if (page < 0) {
-          atomicExch(&g_attn_device_error, kErrOutside);
-          return __uint_as_float(0x7fffffffu);
-        }
-        return p.scales[(int64_t)page * p.scales_s + ((t * TILE + tt) & (p.page_size - 1))];
-      };
-      const int page_first = page_at(t_mine);
-      int page_next = page_at(t_mine + 2);
-      // ---- queries: scaled by a power of two, split into e4m3 terms (rows past the end: zeros)
-      {
-        constexpr int RW = R / 8;               // rows of a warp: warp + 8 i
-        uint2 raw[RW][NCH];                     // channels 128 c + 4 lane + j
-        uint32_t raw_r[RW];                     // rope 2 lane + j
-        const T *ql[RW], *qr[RW];
+      return false;
+    };
+    // ---- its loads: the queries, the pages of this thread's first two positions
+    constexpr int RW = R / 8;                   // rows of a warp: warp + 8 i
+    uint2 raw[RW][NCH];                         // channels 128 c + 4 lane + j
+    uint32_t raw_r[RW];                         // rope 2 lane + j
+    auto page_at = [&](const Info& sg, int t) {
+      const int pos = t * TILE + tt;
+      return t < sg.t1 && pos < sg.seen ? page_of(p, sg.b, pos) : -2;
+    };
+    int page_first, page_second;
+    auto fetch = [&](const Info& sg, int k0) {             // k0: its first tile
+      const int t = sg.t0 + ((k0 ^ wg) & 1);
+      page_first = page_at(sg, t);
+      page_second = page_at(sg, t + 2);
+      const T *ql[RW], *qr[RW];
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {          // (rows past the end: the last one's)
-          const int row = row0 + min(warp + 8 * i, rows - 1);
-          const int64_t n = walk.s.first + row / p.H, h = row % p.H;
-          ql[i] = static_cast<const T*>(p.q_lat) + n * p.ql_s[0] + h * p.ql_s[1] + 4 * lane;
-          qr[i] = static_cast<const T*>(p.q_rope) + n * p.qr_s[0] + h * p.qr_s[1] + 2 * lane;
-          raw_r[i] = 0;
-        }
-        if (p.vec) {
-#pragma unroll
-          for (int i = 0; i < RW; ++i) {
-#pragma unroll
-            for (int c = 0; c < NCH; ++c) raw[i][c] = *reinterpret_cast<const uint2*>(ql[i] + c * 128);
-            if (p.DR) raw_r[i] = *reinterpret_cast<const uint32_t*>(qr[i]);
-          }
-        } else {
-          const auto bits = [](const T* q) { return (uint32_t)*reinterpret_cast<const uint16_t*>(q); };
-#pragma unroll
-          for (int i = 0; i < RW; ++i) {
-#pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-              const T* q = ql[i] + c * 128;
-              raw[i][c] = make_uint2(bits(q) | bits(q + 1) << 16, bits(q + 2) | bits(q + 3) << 16);
-            }
-            if (p.DR) raw_r[i] = bits(qr[i]) | bits(qr[i] + 1) << 16;
-          }
-        }
+      for (int i = 0; i < RW; ++i) {            // (rows past the end: the last one's)
+        const int row = sg.row0 + min(warp + 8 * i, sg.rows - 1), tok = div_heads(p, row);
+        const int64_t n = sg.first + tok, h = row - tok * p.H;
+        ql[i] = static_cast<const T*>(p.q_lat) + n * p.ql_s[0] + h * p.ql_s[1] + 4 * lane;
+        qr[i] = static_cast<const T*>(p.q_rope) + n * p.qr_s[0] + h * p.qr_s[1] + 2 * lane;
+        raw_r[i] = 0;
+      }
+      if (p.vec) {
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
-          const int r = warp + 8 * i;
-          const bool live = r < rows;
-          float x[NCH][4], y[2];
-          uint32_t amax = 0;
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) raw[i][c] = *reinterpret_cast<const uint2*>(ql[i] + c * 128);
+          if (p.DR) raw_r[i] = *reinterpret_cast<const uint32_t*>(qr[i]);
+        }
+      } else {
+        const auto bits = [](const T* q) { return (uint32_t)*reinterpret_cast<const uint16_t*>(q); };
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
 #pragma unroll
           for (int c = 0; c < NCH; ++c) {
-            const T* v = reinterpret_cast<const T*>(&raw[i][c]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[c][j] = live ? ld(v + j) : 0.f;
-              amax = max(amax, abs_bits(x[c][j]));
-            }
+            const T* q = ql[i] + c * 128;
+            raw[i][c] = make_uint2(bits(q) | bits(q + 1) << 16, bits(q + 2) | bits(q + 3) << 16);
           }
-          const T* v = reinterpret_cast<const T*>(&raw_r[i]);
-          y[0] = live ? ld(v) : 0.f;
-          y[1] = live ? ld(v + 1) : 0.f;
-          const uint32_t rmax = max(abs_bits(y[0]), abs_bits(y[1]));
-          const int e = scale_exp(warp_max_u32(amax), warp_max_u32(rmax));
-          const float inv = pow2i(-e);
+          if (p.DR) raw_r[i] = bits(qr[i]) | bits(qr[i] + 1) << 16;
+        }
+      }
+    };
+    // ---- its queries, scaled by a power of two and split into e4m3 terms (rows past
+    // the end: zeros), and its rows' figures
+    auto write_queries = [&](const Info& sg, Rows<R>& rw) {
 #pragma unroll
-          for (int c = 0; c < NCH; ++c) {
+      for (int i = 0; i < RW; ++i) {
+        const int r = warp + 8 * i;
+        const bool live = r < sg.rows;
+        float x[NCH][4], y[2];
+        uint32_t amax = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[c][j] *= inv;
-            uint32_t term[NQ];
-            split4<QFormat, NQ>(x[c], term);
+        for (int c = 0; c < NCH; ++c) {
+          const T* v = reinterpret_cast<const T*>(&raw[i][c]);
 #pragma unroll
-            for (int j = 0; j < NQ; ++j)
-              *reinterpret_cast<uint32_t*>(q_s + c * NS * 128 + swz(j * R + r, 4 * lane)) = term[j];
+          for (int j = 0; j < 4; ++j) {
+            x[c][j] = live ? ld(v + j) : 0.f;
+            amax = max(amax, abs_bits(x[c][j]));
           }
-          if (p.DR) {
-            T* d = reinterpret_cast<T*>(qr_s + swz(r, 4 * lane));
-            st(d, y[0] * inv);
-            st(d + 1, y[1] * inv);
-          }
-          if (lane == 0) {
-            const int row = row0 + r;
-            const int64_t n = walk.s.first + row / p.H, h = row % p.H;
-            sh.q_scale[r] = pow2i(e) * p.scale * kLog2e;
-            sh.seen[r] = r < rows ? seen_by<R>(p, walk.s, row) : seen;
-            sh.m[r] = sh.mb[0][r] = sh.mb[1][r] = kUnset;
-            sh.out[r] = n * p.o_s[0] + h * p.o_s[1];
-            sh.lse[r] = n * p.lse_s + h;
-          }
+        }
+        const T* v = reinterpret_cast<const T*>(&raw_r[i]);
+        y[0] = live ? ld(v) : 0.f;
+        y[1] = live ? ld(v + 1) : 0.f;
+        const uint32_t rmax = max(abs_bits(y[0]), abs_bits(y[1]));
+        const int e = scale_exp(warp_max_u32(amax), p.DR ? warp_max_u32(rmax) : 0);
+        const float inv = pow2i(-e);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[c][j] *= inv;
+          uint32_t term[NQ];
+          split_query<NQ>(x[c], term);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+            *reinterpret_cast<uint32_t*>(q_s + c * NS * 128 + swz(j * R + r, 4 * lane)) = term[j];
+        }
+        if (p.DR) {
+          T* d = reinterpret_cast<T*>(qr_s + swz(r, 4 * lane));
+          st(d, y[0] * inv);
+          st(d + 1, y[1] * inv);
+        }
+        if (lane == 0) {
+          const int row = sg.row0 + min(r, sg.rows - 1), tok = div_heads(p, row);
+          const int64_t n = sg.first + tok, h = row - tok * p.H;
+          rw.q_scale[r] = pow2i(e) * p.scale * kLog2e;
+          rw.seen[r] = live ? max(0, min(sg.off + tok + 1, sg.seen)) : sg.seen;
+          rw.m[r] = rw.mb[0][r] = rw.mb[1][r] = kUnset;
+          rw.out[r] = n * p.o_s[0] + h * p.o_s[1];
+          rw.lse[r] = n * p.lse_s + h;
         }
       }
       ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(&sh.q_ready);
-      float s_next = scale_at(t_mine, page_first);
+    };
+    auto scale_at = [&](int t, int page) {
+      if (page == -2) return 1.f;
+      if (page < 0) {
+        atomicExch(&g_attn_device_error, kErrOutside);
+        return __uint_as_float(0x7fffffffu);
+      }
+      return p.scales[(int64_t)page * p.scales_s + ((t * TILE + tt) & (p.page_size - 1))];
+    };
+
+    Info seg, nseg;
+    bool have = next_segment(seg);
+    float s_first = 1.f;
+    if (have) {
+      fetch(seg, 0);
+      write_queries(seg, sh.rows[0]);
+      s_first = scale_at(seg.t0 + wg, page_first);
+    }
+    for (int si = 0; have; ++si) {
+      Rows<R>& rw = sh.rows[si & 1];
+      const int k_end = k + seg.t1 - seg.t0;    // the next segment's first tile
+      bool have_next = false, fetched = false;
+      float s_next = s_first;
+      int page_next = page_second;
       float ls_next = log2f(s_next), rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
-      bar_sync(3, 256);                         // the rows' figures are written
       float l[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) l[r] = 0.f;
+      ptx::tc_fence_before();
+      bar_sync(3, 256);                         // the rows' figures are written, O has been read
       for (int t = seg.t0; t < seg.t1; ++t, ++k) {
         const int par = k & 1;
         if (par != wg) continue;
@@ -732,7 +830,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         // the sum through P, where the row sees the position)
         const float s = s_next, ls = ls_next, rs = rs_next;
         s_next = scale_at(t + 2, page_next);
-        page_next = page_at(t + 4);
+        page_next = page_at(seg, t + 4);
         const int buf = C::SBUF == 2 ? par : 0;
         const int pos = t * TILE + tt;
         if (!wait(&sh.s_full[par], (k >> 1) & 1, ab)) failed = true;
@@ -747,18 +845,18 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           ptx::tmem_wait_ld();
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            a[g + r] = fmaf(join<QFormat, NQ>(z + r, 16), sh.q_scale[g + r] * s, ls);
+            a[g + r] = fmaf(join<NQ>(z + r, 16, kQFiner), rw.q_scale[g + r] * s, ls);
         }
         ptx::tc_fence_before();
         ptx::mbar_arrive(&sh.s_empty[par]);
-        if (t * TILE + TILE > seen0) {          // some row does not see the whole tile
+        if (t * TILE + TILE > seg.seen0) {      // some row does not see the whole tile
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            if (pos >= sh.seen[r]) a[r] = -INFINITY;
+            if (pos >= rw.seen[r]) a[r] = -INFINITY;
         }
         // positions that nobody sees, or that are NaN as a whole, must not meet
         // a weight of zero: their codes become zeros
-        if (pos >= seen || s != s) {
+        if (pos >= seg.seen || s != s) {
           int at = (int)(((int64_t)k * tile_chunks + tile_chunks - NCH) % ring);
 #pragma unroll 1
           for (int c = 0; c < NCH; ++c) {
@@ -769,23 +867,23 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           }
         }
         // ---- the maxima as the tile before left them
-        const bool first = t == seg.t0;
-        if (!first) {
+        const bool start = t == seg.t0;
+        if (!start) {
           if (!wait(&sh.m_full[par ^ 1], ((k - 1) >> 1) & 1, ab)) failed = true;
           if (sh.changed[par ^ 1]) {
             if (tt < R) {
-              const float m = sh.m[tt];
-              sh.alpha[par][tt] = ex2(sh.mb[par][tt] - m);
-              sh.mb[par][tt] = m;
+              const float m = rw.m[tt];
+              rw.alpha[par][tt] = ex2(rw.mb[par][tt] - m);
+              rw.mb[par][tt] = m;
             }
             bar_sync(1 + wg, 128);
 #pragma unroll
-            for (int r = 0; r < R; ++r) l[r] *= sh.alpha[par][r];
+            for (int r = 0; r < R; ++r) l[r] *= rw.alpha[par][r];
           }
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < R; ++r) top = fmaxf(top, a[r] - sh.mb[par][r]);
+        for (int r = 0; r < R; ++r) top = fmaxf(top, a[r] - rw.mb[par][r]);
         const bool grew = ptx::bar_red_or(1 + wg, 128, failed || top > F::BIAS + F::SLACK);
         if (tt == 0) sh.changed[par] = grew;
         if (grew) {
@@ -801,21 +899,21 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           if (failed) break;
           if (tt < R) {
             const float* red = &sh.red[4 * wg][tt];
-            const float mx = fmaxf(fmaxf(red[0], red[32]), fmaxf(red[64], red[96]));
-            const float old = sh.m[tt];
+            const float mx = fmaxf(fmaxf(red[0], red[R]), fmaxf(red[2 * R], red[3 * R]));
+            const float old = rw.m[tt];
             const bool up = mx - old > F::BIAS + F::SLACK;
-            sh.alpha[par][tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
-            if (up) sh.m[tt] = sh.mb[par][tt] = mx - F::BIAS;
+            rw.alpha[par][tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
+            if (up) rw.m[tt] = rw.mb[par][tt] = mx - F::BIAS;
           }
           bar_sync(1 + wg, 128);
-          if (!first) {
+          if (!start) {
             if (!o_done(k - 1)) failed = true;
             ptx::tc_fence_after();
 #pragma unroll 1
             for (int g = 0; g < R; g += 16) {
               float al[16];
 #pragma unroll
-              for (int r = 0; r < 16; ++r) al[r] = sh.alpha[par][g + r];
+              for (int r = 0; r < 16; ++r) al[r] = rw.alpha[par][g + r];
 #pragma unroll 1
               for (int c = 0; c < NCH; ++c) {
                 const uint32_t at = tmem + c * NO + g + lane_base;
@@ -833,7 +931,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
             ptx::tc_fence_before();
           }
 #pragma unroll
-          for (int r = 0; r < R; ++r) l[r] *= sh.alpha[par][r];
+          for (int r = 0; r < R; ++r) l[r] *= rw.alpha[par][r];
         }
         ptx::mbar_arrive(&sh.m_full[par]);
         // ---- P, once the buffer's last products have read it
@@ -848,11 +946,11 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int r = 16 * g + 4 * q + i;
-              e4[i] = ex2(a[r] - sh.mb[par][r]);
+              e4[i] = ex2(a[r] - rw.mb[par][r]);
               l[r] = fmaf(e4[i], rs, l[r]);
             }
             uint32_t u[NP];
-            split4<F, NP>(e4, u);
+            F::split(e4, u);
 #pragma unroll
             for (int j = 0; j < NP; ++j) term[j][q] = u[j];
           }
@@ -865,29 +963,45 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         ptx::mbar_arrive(&sh.p_full[par]);
         ls_next = log2f(s_next);
         rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
+        if (!fetched) {                         // the next segment's loads, well ahead
+          have_next = next_segment(nseg);
+          if (have_next) fetch(nseg, k_end);
+          fetched = true;
+        }
+      }
+      if (!fetched) {
+        have_next = next_segment(nseg);
+        if (have_next) fetch(nseg, k_end);
+      }
+      // ---- the next segment's queries, so that its scores are under way while this
+      // one's result is written
+      bar_sync(3, 256);                         // the maxima are final, the scores all read
+      if (have_next && !failed) {
+        s_first = scale_at(nseg.t0 + ((k ^ wg) & 1), page_first);
+        write_queries(nseg, sh.rows[(si + 1) & 1]);
       }
       // ---- the segment's result
+#pragma unroll
+      for (int r = 0; r < R; ++r) l[r] *= ex2(rw.mb[wg][r] - rw.m[r]);
+      const float sum = warp_sums<R>(l, lane);
+      if (lane < R) sh.red[warp][lane] = sum;
       if (!failed && !o_done(k - 1)) failed = true;
       ptx::tc_fence_after();
-      bar_sync(3, 256);                         // the maxima are final
-#pragma unroll
-      for (int r = 0; r < R; ++r) l[r] *= ex2(sh.mb[wg][r] - sh.m[r]);
-      const float mine = warp_sums<R>(l, lane);
-      if (lane < R) sh.red[warp][lane] = mine;
       failed = ptx::bar_red_or(3, 256, failed);
       if (failed) break;
-      float total = 0.f;
-      if (lane < R) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) total += sh.red[i][lane];
-      }
-      const float inv = total == 0.f ? 0.f : 1.f / total;
       const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
       const int slot = 2 * blockIdx.x + (seg.t0 > 0 ? 0 : 1);
-      if (warp == 0 && lane < rows) {
-        const float lse2 = total == 0.f ? -INFINITY : sh.m[lane] + log2f(total);
-        if (!whole) w.lse2[slot * R + lane] = lse2;
-        else if (p.lse) p.lse[sh.lse[lane]] = lse2 * kLn2;
+      float inv = 0.f;                          // of row `lane`
+      if (lane < R) {
+        float total = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) total += sh.red[i][lane];
+        inv = total == 0.f ? 0.f : 1.f / (total * F::GAIN);
+        if (warp == 0 && lane < seg.rows) {
+          const float lse2 = total == 0.f ? -INFINITY : rw.m[lane] + log2f(total);
+          if (!whole) w.lse2[slot * R + lane] = lse2;
+          else if (p.lse) p.lse[rw.lse[lane]] = lse2 * kLn2;
+        }
       }
 #pragma unroll 1
       for (int i = wg; i < NCH * (R / 16); i += 2) {       // 128 channels of 16 rows
@@ -901,21 +1015,37 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float f = __shfl_sync(0xffffffffu, inv, g + r);
-          o[r] = f == 0.f ? 0.f : join<F, NP>(o + r, 16) * f;
+          o[r] = f == 0.f ? 0.f : join<NP>(o + r, 16, F::FINER) * f;
         }
         if (whole) {
+          // neighbouring lanes swap a row each: four bytes a store
+          const bool odd = lane & 1;
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (g + r < rows) st(static_cast<T*>(p.out) + sh.out[g + r] + ch, o[r]);
+          for (int r = 0; r < 16; r += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? o[r] : o[r + 1], 1);
+            const int row = g + r + odd;
+            if (row < seg.rows) {
+              T* dst = static_cast<T*>(p.out) + rw.out[row] + (ch & ~1);
+              T pair[2];
+              st(pair, odd ? other : o[r]);
+              st(pair + 1, odd ? o[r + 1] : other);
+              if (p.out_vec) {
+                *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(pair);
+              } else {
+                dst[0] = pair[0];
+                dst[1] = pair[1];
+              }
+            }
+          }
         } else {
           float* part = w.part + ((int64_t)slot * R + g) * p.KVL + ch;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (g + r < rows) part[r * p.KVL] = o[r];
+            if (g + r < seg.rows) part[r * p.KVL] = o[r];
         }
       }
-      ptx::tc_fence_before();
-      bar_sync(3, 256);                         // before the next segment's figures and products
+      seg = nseg;
+      have = have_next;
     }
   }
   ptx::tc_fence_before();
@@ -928,43 +1058,94 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 }
 
 // Joins the parts of a group that several ranges share, in order: one block per
-// (range that starts inside a group, row).
+// (range that starts inside a group, row).  Two halves of the block take every second
+// part each, eight loads in flight.
+constexpr int kJoinThreads = 256;
+
 template <typename T, int R>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinThreads)
 cache_join_kernel(const CacheParams p, const Work w) {
+  __shared__ float weight[kMaxRanges];
+  __shared__ float red[kJoinThreads / 32];
+  __shared__ float4 half[128];
   ptx::grid_dep_wait();
   const int c0 = blockIdx.x + 1;
   const Cut cut = w.cuts[c0];
   if (cut.b < 0 || cut.parts == 0) return;
-  const Seq s = load_seq<R>(p, cut.b);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = cut.parts;
   const int r = blockIdx.y, row = cut.g * R + r;
-  if (row >= (int64_t)s.n * p.H) return;
+  int first, count;
+  new_tokens(p, cut.b, first, count);
+  if (row >= (int64_t)count * p.H) return;
   // part 0: what range c0 - 1 left unfinished; part i: what range c0 + i - 1 begins with
-  auto slot = [&](int i) { return i == 0 ? 2 * (c0 - 1) + 1 : 2 * (c0 + i - 1); };
-  float mx = -INFINITY;
-  for (int i = 0; i < cut.parts; ++i) mx = fmaxf(mx, w.lse2[slot(i) * R + r]);
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (c0 - 1) + 1 : 2 * (c0 + i - 1)) * R + r; };
+  const int ch = 4 * (tid & 127), h0 = tid >> 7;
+  const bool live = ch < p.KVL;
+  float4 x[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (live && h0 + 2 * u < parts)
+      x[u] = *reinterpret_cast<const float4*>(w.part + slot(h0 + 2 * u) * p.KVL + ch);
+  float mine[2], mx = -INFINITY;
+  static_assert(kMaxRanges <= 2 * kJoinThreads, "two parts per thread");
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = tid + j * kJoinThreads;
+    mine[j] = i < parts ? w.lse2[slot(i)] : -INFINITY;
+    mx = fmaxf(mx, mine[j]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) red[warp] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[i]);
   const float m = mx == -INFINITY ? 0.f : mx;
-  const int ch = 4 * threadIdx.x;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, tot = 0.f;
-  for (int i = 0; i < cut.parts; ++i) {
-    const float f = exp2f(w.lse2[slot(i) * R + r] - m);
+  __syncthreads();
+  float tot = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = tid + j * kJoinThreads;
+    const float f = i < parts ? exp2f(mine[j] - m) : 0.f;
+    if (i < parts) weight[i] = f;
     tot += f;
-    if (ch < p.KVL) {
-      const float4 x = *reinterpret_cast<const float4*>(w.part + ((int64_t)slot(i) * R + r) * p.KVL + ch);
-      acc[0] = fmaf(f, x.x, acc[0]);
-      acc[1] = fmaf(f, x.y, acc[1]);
-      acc[2] = fmaf(f, x.z, acc[2]);
-      acc[3] = fmaf(f, x.w, acc[3]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+  if (lane == 0) red[warp] = tot;
+  __syncthreads();
+  tot = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) tot += red[i];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = h0; i < parts; i += 16) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = i + 2 * u;
+      if (live && j < parts) {
+        const float f = weight[j];
+        acc.x = fmaf(f, x[u].x, acc.x);
+        acc.y = fmaf(f, x[u].y, acc.y);
+        acc.z = fmaf(f, x[u].z, acc.z);
+        acc.w = fmaf(f, x[u].w, acc.w);
+        if (j + 16 < parts) x[u] = *reinterpret_cast<const float4*>(w.part + slot(j + 16) * p.KVL + ch);
+      }
     }
   }
-  const int64_t n = s.first + row / p.H, h = row % p.H;
+  if (h0 == 1) half[tid & 127] = acc;
+  __syncthreads();
+  const int tok = div_heads(p, row);
+  const int64_t n = first + tok, h = row - tok * p.H;
   const float inv = tot == 0.f ? 0.f : 1.f / tot;
-  if (ch < p.KVL) {
+  if (h0 == 0 && live) {
+    const float4 b = half[tid];
     T* o = static_cast<T*>(p.out) + n * p.o_s[0] + h * p.o_s[1] + ch;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) st(o + i, acc[i] * inv);
+    st(o, (acc.x + b.x) * inv);
+    st(o + 1, (acc.y + b.y) * inv);
+    st(o + 2, (acc.z + b.z) * inv);
+    st(o + 3, (acc.w + b.w) * inv);
   }
-  if (threadIdx.x == 0 && p.lse)
+  if (tid == 0 && p.lse)
     p.lse[n * p.lse_s + h] = tot == 0.f ? -INFINITY : (m + log2f(tot)) * kLn2;
 }
 
@@ -975,7 +1156,7 @@ int device_sms() {
   int dev = 0, n = 148;
   if (cudaGetDevice(&dev) == cudaSuccess)
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  return n > 1 ? min(n, kMaxRanges) : 2;
 }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -997,7 +1178,7 @@ cudaError_t launch(const CacheParams& p, Work w, const CUtensorMap& mc, const CU
   const size_t smem = fixed_bytes(p.KVL, C::NQ, R) + w.ring * CHUNK;
   e = launch_dependent(k, dim3(ranges), kThreads, smem, s, p, w, mc, mr);
   if (e != cudaSuccess) return e;
-  return launch_dependent(cache_join_kernel<T, R>, dim3(ranges - 1, R), 128, 0, s, p, w);
+  return launch_dependent(cache_join_kernel<T, R>, dim3(ranges - 1, R), kJoinThreads, 0, s, p, w);
 }
 
 template <typename T, int R>
