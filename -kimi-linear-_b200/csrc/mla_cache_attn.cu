@@ -43,10 +43,8 @@ namespace {
 
 constexpr int TILE = 128;                  // positions per tile (MMA M)
 constexpr int CHUNK = TILE * 128;          // bytes of 128 positions x 128 bytes
-constexpr int kThreads = 384;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue, 10 cuts
-// Registers: the block starts with 384 x 168; the softmax warps take 208 each, the
-// others keep 88 (256 x 208 + 128 x 88 = 384 x 168).
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr int kThreads = 352;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue, 10 cuts
+
 constexpr int kMaxRing = 14;
 constexpr int kMaxRanges = 256;            // blocks (SMs) that a call's tiles are cut over
 constexpr int kSmemMax = 232448;           // 227 KB per block
@@ -123,9 +121,9 @@ struct Cfg {
 // Shared memory besides the ring (barriers and rows; 1 KB: alignment), and the
 // chunks that fit beside it.  The order of the products needs the codes of one
 // tile and all of the next at once.
-constexpr int kSharedBytes(int R) { return R == 16 ? 4096 : 5120; }
+constexpr int kSharedBytes = 4096;
 int fixed_bytes(int kvl, int q_terms, int R) {
-  return kSharedBytes(R) + 1024 + q_terms * R * kvl + R * 128 + 2 * NP * R * 128;
+  return kSharedBytes + 1024 + q_terms * R * kvl + R * 128 + 2 * NP * R * 128;
 }
 int ring_chunks(int kvl, int q_terms, int R) {
   const int n = (kSmemMax - fixed_bytes(kvl, q_terms, R)) / CHUNK;
@@ -379,38 +377,35 @@ template <int R>
 struct Rows {              // per row of a group
   float q_scale[R];        // 2^e scale log2e
   float m[R];              // running maximum less BIAS
-  float mb[2][R];          // the same as of each softmax group's last tile
-  float alpha[2][R];       // what its sums (and O) are rescaled by
-  float inv[R];            // 1 / sum
+  float alpha[R];          // what its sums and O are rescaled by
   int seen[R];             // positions that it sees
   int64_t out[R], lse[R];  // where its results go
 };
 template <int R>
 struct Shared {            // at the end of dynamic shared memory
   uint64_t full[kMaxRing], empty[kMaxRing];
-  uint64_t s_full[2], s_empty[2], p_full[2], o_done[4], m_full[2], q_ready, drain;
+  uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], q_ready, drain;
   uint32_t tmem;
   int abort_flag;
-  int changed[2];          // the tile of this parity moved the maxima
   int64_t scan[(kThreads + 31) / 32];
   int64_t base;            // where the range starts: count at which sequence b starts
   int b;
   Seq seq;                 // and that sequence
   Rows<R> rows[2];         // of this segment and the next
-  float red[8][R];         // per warp and row: maxima, sums
+  float red[8][R / 2];     // per warp and row: maxima, sums
 };
-static_assert(sizeof(Shared<16>) <= kSharedBytes(16) && sizeof(Shared<32>) <= kSharedBytes(32),
+static_assert(sizeof(Shared<32>) <= kSharedBytes,
               "room for barriers and rows");
 
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// sums of v[0 .. R - 1] over the warp: lane i < R (and i + R) gets the sum of v[i]
-template <int R>
-__device__ __forceinline__ float warp_sums(float (&v)[R], int lane) {
+// sums of v[0 .. N - 1] over the warp: lanes i, i + N, ... get the sum of v[i]
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N], int lane) {
 #pragma unroll
-  for (int n = R / 2; n >= 1; n /= 2) {
+  for (int n = N / 2; n >= 1; n /= 2) {
     const bool up = lane & n;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
@@ -419,8 +414,32 @@ __device__ __forceinline__ float warp_sums(float (&v)[R], int lane) {
     }
   }
 #pragma unroll
-  for (int o = R; o < 32; o <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  for (int o = N; o < 32; o <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
   return v[0];
+}
+// 8 or 16 consecutive TMEM columns of this warp's lanes
+template <int N>
+__device__ __forceinline__ void tmem_get(uint32_t at, float* v) {
+  if constexpr (N == 16) {
+    ptx::tmem_ld16(at, v);
+  } else {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(at));
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_put(uint32_t at, const float* v) {
+  if constexpr (N == 16) {
+    ptx::tmem_st16(at, v);
+  } else {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  }
 }
 
 template <typename T, int R, int NCH>
@@ -446,11 +465,9 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&sh.s_full[i], 1);
-      ptx::mbar_init(&sh.s_empty[i], 128);
-      ptx::mbar_init(&sh.p_full[i], 128);
+      ptx::mbar_init(&sh.s_empty[i], 256);
+      ptx::mbar_init(&sh.p_full[i], 256);
       ptx::mbar_init(&sh.o_done[i], 1);
-      ptx::mbar_init(&sh.o_done[i + 2], 1);
-      ptx::mbar_init(&sh.m_full[i], 128);
     }
     ptx::mbar_init(&sh.q_ready, 256);
     ptx::mbar_init(&sh.drain, 1);
@@ -511,7 +528,6 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   const uint32_t tm_s = tmem + NCH * NO;        // S buffers after the O chunks
   volatile int* ab = &sh.abort_flag;
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1);
     Segment seg;
   if (warp == 10) {
@@ -609,7 +625,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
                       dp + ((par * NO * 128 + kk * 512) >> 4), id_o, !(first && kk == 0));
 #pragma unroll
         for (int c = 0; c < NCH; ++c) commit(&sh.empty[at[c]]);
-        commit(&sh.o_done[i & 3]);
+        commit(&sh.o_done[par]);
         return true;
       };
       while (ok && walk.next(seg)) {
@@ -659,19 +675,16 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     __syncwarp();
   }
   } else {
-    // ======== softmax: two groups of four warps take the tiles in turn; thread =
+    // ======== softmax: two groups of four warps have half of the rows each; thread =
     // position of the tile = TMEM lane
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1);
-    const int wg = warp >> 2;
+    constexpr int HR = R / 2;                   // rows of a group
+    const int wg = warp >> 2, rb = wg * HR;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int tt = tid & 127;
     int k = 0;
     bool failed = false;
-    // The products of tile i are in O.  A wait tells a barrier's phase only from its
-    // neighbours; each group waits for its own last tile's products, so with four
-    // barriers the phase asked for is the one under way or the one just ended.
-    auto o_done = [&](int i) { return wait(&sh.o_done[i & 3], (i >> 2) & 1, ab); };
+    auto o_done = [&](int i) { return wait(&sh.o_done[i & 1], (i >> 1) & 1, ab); };   // products of tile i
 
     // ---- the next segment that sees anything
     struct Info : Segment {
@@ -709,10 +722,9 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       return t < sg.t1 && pos < sg.seen ? page_of(p, sg.b, pos) : -2;
     };
     int page_first, page_second;
-    auto fetch = [&](const Info& sg, int k0) {             // k0: its first tile
-      const int t = sg.t0 + ((k0 ^ wg) & 1);
-      page_first = page_at(sg, t);
-      page_second = page_at(sg, t + 2);
+    auto fetch = [&](const Info& sg) {
+      page_first = page_at(sg, sg.t0);
+      page_second = page_at(sg, sg.t0 + 1);
       const T *ql[RW], *qr[RW];
 #pragma unroll
       for (int i = 0; i < RW; ++i) {            // (rows past the end: the last one's)
@@ -786,7 +798,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           const int64_t n = sg.first + tok, h = row - tok * p.H;
           rw.q_scale[r] = pow2i(e) * p.scale * kLog2e;
           rw.seen[r] = live ? max(0, min(sg.off + tok + 1, sg.seen)) : sg.seen;
-          rw.m[r] = rw.mb[0][r] = rw.mb[1][r] = kUnset;
+          rw.m[r] = kUnset;
           rw.out[r] = n * p.o_s[0] + h * p.o_s[1];
           rw.lse[r] = n * p.lse_s + h;
         }
@@ -807,56 +819,54 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     bool have = next_segment(seg);
     float s_first = 1.f;
     if (have) {
-      fetch(seg, 0);
+      fetch(seg);
       write_queries(seg, sh.rows[0]);
-      s_first = scale_at(seg.t0 + wg, page_first);
+      s_first = scale_at(seg.t0, page_first);
     }
     for (int si = 0; have; ++si) {
       Rows<R>& rw = sh.rows[si & 1];
-      const int k_end = k + seg.t1 - seg.t0;    // the next segment's first tile
-      bool have_next = false, fetched = false;
+      const float *q_scale = rw.q_scale + rb, *m = rw.m + rb, *alpha = rw.alpha + rb;
+      const int* sees = rw.seen + rb;
+      bool have_next = false;
       float s_next = s_first;
       int page_next = page_second;
       float ls_next = log2f(s_next), rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
-      float l[R];
+      float l[HR];
 #pragma unroll
-      for (int r = 0; r < R; ++r) l[r] = 0.f;
+      for (int r = 0; r < HR; ++r) l[r] = 0.f;
       ptx::tc_fence_before();
       bar_sync(3, 256);                         // the rows' figures are written, O has been read
       for (int t = seg.t0; t < seg.t1; ++t, ++k) {
         const int par = k & 1;
-        if (par != wg) continue;
+        const bool start = t == seg.t0;
         // log2 of the position's scale and its reciprocal (a NaN scale: NaN reaches
         // the sum through P, where the row sees the position)
         const float s = s_next, ls = ls_next, rs = rs_next;
-        s_next = scale_at(t + 2, page_next);
-        page_next = page_at(seg, t + 4);
-        const int buf = C::SBUF == 2 ? par : 0;
+        s_next = scale_at(t + 1, page_next);
+        page_next = page_at(seg, t + 2);
         const int pos = t * TILE + tt;
         if (!wait(&sh.s_full[par], (k >> 1) & 1, ab)) failed = true;
         ptx::tc_fence_after();
-        float a[R];
+        float a[HR];
+        {
+          float z[NQ * HR];
+          const uint32_t at = tm_s + (C::SBUF == 2 ? par * NS : 0) + rb + lane_base;
 #pragma unroll
-        for (int g = 0; g < R; g += 16) {       // 16 rows at a time: registers
-          float z[NQ * 16];
-#pragma unroll
-          for (int j = 0; j < NQ; ++j)
-            ptx::tmem_ld16(tm_s + buf * NS + j * R + g + lane_base, z + 16 * j);
+          for (int j = 0; j < NQ; ++j) tmem_get<HR>(at + j * R, z + HR * j);
           ptx::tmem_wait_ld();
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(&sh.s_empty[par]);
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            a[g + r] = fmaf(join<NQ>(z + r, 16, kQFiner), rw.q_scale[g + r] * s, ls);
+          for (int r = 0; r < HR; ++r) a[r] = fmaf(join<NQ>(z + r, HR, kQFiner), q_scale[r] * s, ls);
         }
-        ptx::tc_fence_before();
-        ptx::mbar_arrive(&sh.s_empty[par]);
         if (t * TILE + TILE > seg.seen0) {      // some row does not see the whole tile
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (pos >= rw.seen[r]) a[r] = -INFINITY;
+          for (int r = 0; r < HR; ++r)
+            if (pos >= sees[r]) a[r] = -INFINITY;
         }
         // positions that nobody sees, or that are NaN as a whole, must not meet
         // a weight of zero: their codes become zeros
-        if (pos >= seg.seen || s != s) {
+        if (wg == 0 && (pos >= seg.seen || s != s)) {
           int at = (int)(((int64_t)k * tile_chunks + tile_chunks - NCH) % ring);
 #pragma unroll 1
           for (int c = 0; c < NCH; ++c) {
@@ -866,164 +876,141 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
             if (++at == ring) at = 0;
           }
         }
-        // ---- the maxima as the tile before left them
-        const bool start = t == seg.t0;
-        if (!start) {
-          if (!wait(&sh.m_full[par ^ 1], ((k - 1) >> 1) & 1, ab)) failed = true;
-          if (sh.changed[par ^ 1]) {
-            if (tt < R) {
-              const float m = rw.m[tt];
-              rw.alpha[par][tt] = ex2(rw.mb[par][tt] - m);
-              rw.mb[par][tt] = m;
-            }
-            bar_sync(1 + wg, 128);
-#pragma unroll
-            for (int r = 0; r < R; ++r) l[r] *= rw.alpha[par][r];
-          }
-        }
         float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < R; ++r) top = fmaxf(top, a[r] - rw.mb[par][r]);
-        const bool grew = ptx::bar_red_or(1 + wg, 128, failed || top > F::BIAS + F::SLACK);
-        if (tt == 0) sh.changed[par] = grew;
-        if (grew) {
+        for (int r = 0; r < HR; ++r) top = fmaxf(top, a[r] - m[r]);
+        if (ptx::bar_red_or(1 + wg, 128, failed || top > F::BIAS + F::SLACK)) {
           // a row outgrew P's range (or has its first position): new maxima, and O
           // follows once the products so far are in it
           if (*ab) failed = true;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
+          for (int r = 0; r < HR; ++r) {
             const float mx = warp_max(a[r]);
             if (lane == 0) sh.red[warp][r] = mx;
           }
           failed = ptx::bar_red_or(1 + wg, 128, failed);
           if (failed) break;
-          if (tt < R) {
+          if (tt < HR) {
             const float* red = &sh.red[4 * wg][tt];
-            const float mx = fmaxf(fmaxf(red[0], red[R]), fmaxf(red[2 * R], red[3 * R]));
-            const float old = rw.m[tt];
+            const float mx = fmaxf(fmaxf(red[0], red[HR]), fmaxf(red[2 * HR], red[3 * HR]));
+            const float old = m[tt];
             const bool up = mx - old > F::BIAS + F::SLACK;
-            rw.alpha[par][tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
-            if (up) rw.m[tt] = rw.mb[par][tt] = mx - F::BIAS;
+            rw.alpha[rb + tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
+            if (up) rw.m[rb + tt] = mx - F::BIAS;
           }
           bar_sync(1 + wg, 128);
           if (!start) {
             if (!o_done(k - 1)) failed = true;
             ptx::tc_fence_after();
+            float al[HR];
+#pragma unroll
+            for (int r = 0; r < HR; ++r) {
+              al[r] = alpha[r];
+              l[r] *= al[r];
+            }
 #pragma unroll 1
-            for (int g = 0; g < R; g += 16) {
-              float al[16];
+            for (int c = 0; c < NCH; ++c) {
+              const uint32_t at = tmem + c * NO + rb + lane_base;
+              float o[NP * HR];
 #pragma unroll
-              for (int r = 0; r < 16; ++r) al[r] = rw.alpha[par][g + r];
-#pragma unroll 1
-              for (int c = 0; c < NCH; ++c) {
-                const uint32_t at = tmem + c * NO + g + lane_base;
-                float o[NP * 16];
+              for (int j = 0; j < NP; ++j) tmem_get<HR>(at + j * R, o + HR * j);
+              ptx::tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < NP; ++j) ptx::tmem_ld16(at + j * R, o + 16 * j);
-                ptx::tmem_wait_ld();
+              for (int i = 0; i < NP * HR; ++i) o[i] *= al[i % HR];
 #pragma unroll
-                for (int i = 0; i < NP * 16; ++i) o[i] *= al[i % 16];
-#pragma unroll
-                for (int j = 0; j < NP; ++j) ptx::tmem_st16(at + j * R, o + 16 * j);
-              }
+              for (int j = 0; j < NP; ++j) tmem_put<HR>(at + j * R, o + HR * j);
             }
             ptx::tmem_wait_st();
             ptx::tc_fence_before();
           }
-#pragma unroll
-          for (int r = 0; r < R; ++r) l[r] *= rw.alpha[par][r];
         }
-        ptx::mbar_arrive(&sh.m_full[par]);
         // ---- P, once the buffer's last products have read it
         if (k > 1 && !o_done(k - 2)) failed = true;
-        uint8_t* pt = p_s + par * NO * 128 + tt * 16;
+        // (16 rows of a position are 16 bytes, 8 rows one half of them)
+        uint8_t* pt = p_s + par * NO * 128 + tt * 16 + (HR == 8 ? wg * 8 : wg * (TILE * 16));
+        uint32_t term[NP][HR / 4];
 #pragma unroll
-        for (int g = 0; g < R / 16; ++g) {
-          uint32_t term[NP][4];
+        for (int q = 0; q < HR / 4; ++q) {
+          float e4[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float e4[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 16 * g + 4 * q + i;
-              e4[i] = ex2(a[r] - rw.mb[par][r]);
-              l[r] = fmaf(e4[i], rs, l[r]);
-            }
-            uint32_t u[NP];
-            F::split(e4, u);
-#pragma unroll
-            for (int j = 0; j < NP; ++j) term[j][q] = u[j];
+          for (int i = 0; i < 4; ++i) {
+            e4[i] = ex2(a[4 * q + i] - m[4 * q + i]);
+            l[4 * q + i] = fmaf(e4[i], rs, l[4 * q + i]);
           }
+          uint32_t u[NP];
+          F::split(e4, u);
 #pragma unroll
-          for (int j = 0; j < NP; ++j)
-            *reinterpret_cast<uint4*>(pt + (j * (R / 16) + g) * (TILE * 16)) =
-                make_uint4(term[j][0], term[j][1], term[j][2], term[j][3]);
+          for (int j = 0; j < NP; ++j) term[j][q] = u[j];
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          uint8_t* d = pt + j * (R / 16) * (TILE * 16);
+          if constexpr (HR == 16)
+            *reinterpret_cast<uint4*>(d) = make_uint4(term[j][0], term[j][1], term[j][2], term[j][3]);
+          else
+            *reinterpret_cast<uint2*>(d) = make_uint2(term[j][0], term[j][1]);
         }
         ptx::fence_proxy_async_smem();
         ptx::mbar_arrive(&sh.p_full[par]);
         ls_next = log2f(s_next);
         rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
-        if (!fetched) {                         // the next segment's loads, well ahead
+        // the next segment's loads, well ahead (with 32 rows there are no registers to
+        // hold them meanwhile)
+        if (R == 16 && start) {
           have_next = next_segment(nseg);
-          if (have_next) fetch(nseg, k_end);
-          fetched = true;
+          if (have_next) fetch(nseg);
         }
       }
-      if (!fetched) {
+      if (R != 16) {
         have_next = next_segment(nseg);
-        if (have_next) fetch(nseg, k_end);
+        if (have_next) fetch(nseg);
       }
       // ---- the next segment's queries, so that its scores are under way while this
       // one's result is written
-      bar_sync(3, 256);                         // the maxima are final, the scores all read
+      bar_sync(3, 256);                         // the scores have all been read
       if (have_next && !failed) {
-        s_first = scale_at(nseg.t0 + ((k ^ wg) & 1), page_first);
+        s_first = scale_at(nseg.t0, page_first);
         write_queries(nseg, sh.rows[(si + 1) & 1]);
       }
       // ---- the segment's result
-#pragma unroll
-      for (int r = 0; r < R; ++r) l[r] *= ex2(rw.mb[wg][r] - rw.m[r]);
-      const float sum = warp_sums<R>(l, lane);
-      if (lane < R) sh.red[warp][lane] = sum;
+      const float sum = warp_sums<HR>(l, lane);
+      if (lane < HR) sh.red[warp][lane] = sum;
       if (!failed && !o_done(k - 1)) failed = true;
       ptx::tc_fence_after();
       failed = ptx::bar_red_or(3, 256, failed);
       if (failed) break;
       const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
       const int slot = 2 * blockIdx.x + (seg.t0 > 0 ? 0 : 1);
-      float inv = 0.f;                          // of row `lane`
-      if (lane < R) {
-        float total = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) total += sh.red[i][lane];
+      float inv = 0.f;                          // of row rb + lane
+      if (lane < HR) {
+        const float* red = &sh.red[4 * wg][lane];
+        const float total = (red[0] + red[HR]) + (red[2 * HR] + red[3 * HR]);
         inv = total == 0.f ? 0.f : 1.f / (total * F::GAIN);
-        if (warp == 0 && lane < seg.rows) {
-          const float lse2 = total == 0.f ? -INFINITY : rw.m[lane] + log2f(total);
-          if (!whole) w.lse2[slot * R + lane] = lse2;
-          else if (p.lse) p.lse[rw.lse[lane]] = lse2 * kLn2;
+        if ((warp & 3) == 0 && rb + lane < seg.rows) {
+          const float lse2 = total == 0.f ? -INFINITY : m[lane] + log2f(total);
+          if (!whole) w.lse2[slot * R + rb + lane] = lse2;
+          else if (p.lse) p.lse[rw.lse[rb + lane]] = lse2 * kLn2;
         }
       }
-#pragma unroll 1
-      for (int i = wg; i < NCH * (R / 16); i += 2) {       // 128 channels of 16 rows
-        const int c = i / (R / 16), g = 16 * (i % (R / 16));
-        float o[NP * 16];
+      float f[HR];
 #pragma unroll
-        for (int j = 0; j < NP; ++j)
-          ptx::tmem_ld16(tmem + c * NO + j * R + g + lane_base, o + 16 * j);
+      for (int r = 0; r < HR; ++r) f[r] = __shfl_sync(0xffffffffu, inv, r);
+#pragma unroll 1
+      for (int c = 0; c < NCH; ++c) {           // 128 channels of this group's rows
+        float o[NP * HR];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) tmem_get<HR>(tmem + c * NO + j * R + rb + lane_base, o + HR * j);
         ptx::tmem_wait_ld();
         const int ch = c * 128 + tt;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float f = __shfl_sync(0xffffffffu, inv, g + r);
-          o[r] = f == 0.f ? 0.f : join<NP>(o + r, 16, F::FINER) * f;
-        }
+        for (int r = 0; r < HR; ++r) o[r] = f[r] == 0.f ? 0.f : join<NP>(o + r, HR, F::FINER) * f[r];
         if (whole) {
           // neighbouring lanes swap a row each: four bytes a store
           const bool odd = lane & 1;
 #pragma unroll
-          for (int r = 0; r < 16; r += 2) {
+          for (int r = 0; r < HR; r += 2) {
             const float other = __shfl_xor_sync(0xffffffffu, odd ? o[r] : o[r + 1], 1);
-            const int row = g + r + odd;
+            const int row = rb + r + odd;
             if (row < seg.rows) {
               T* dst = static_cast<T*>(p.out) + rw.out[row] + (ch & ~1);
               T pair[2];
@@ -1038,10 +1025,10 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
             }
           }
         } else {
-          float* part = w.part + ((int64_t)slot * R + g) * p.KVL + ch;
+          float* part = w.part + ((int64_t)slot * R + rb) * p.KVL + ch;
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (g + r < seg.rows) part[r * p.KVL] = o[r];
+          for (int r = 0; r < HR; ++r)
+            if (rb + r < seg.rows) part[r * p.KVL] = o[r];
         }
       }
       seg = nseg;
