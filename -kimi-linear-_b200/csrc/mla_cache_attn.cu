@@ -43,9 +43,13 @@ namespace {
 
 constexpr int TILE = 128;                  // positions per tile (MMA M)
 constexpr int CHUNK = TILE * 128;          // bytes of 128 positions x 128 bytes
-constexpr int kThreads = 352;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue, 10 cuts
+constexpr int kThreads = 384;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue, 10 cuts
+// Registers: the block starts with 384 x 168; the softmax warps take 192 each, the
+// others keep 120 (256 x 192 + 128 x 120 = 384 x 168).
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 120;
 
 constexpr int kMaxRing = 14;
+constexpr int kWholeTiles = 4;             // contexts of at most so many tiles are not split
 constexpr int kMaxRanges = 256;            // blocks (SMs) that a call's tiles are cut over
 constexpr int kSmemMax = 232448;           // 227 KB per block
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -62,7 +66,7 @@ template <typename T> constexpr int kQTerms = std::is_same<T, __nv_bfloat16>::va
 //    maximum by 2^10 (2^15 < 57344) before the maximum moves.
 //  * fp16: e4m3 = bits 13 .. 7 of fp16, for the value times 2^-8.  P in fp16 (11 bits,
 //    2^-12) is cut into three terms, each 16 times finer.  It carries 2^-6 and may
-//    outgrow the maximum by 2^6 (2^8 2^-8; 448 is the format's largest).
+//    outgrow the maximum by 2^6 (to 1, so that no term reaches 1.875, the code of NaN).
 // Weights down to 2^-27 (2^-18) of the largest still count.
 constexpr int NP = 3;
 template <typename T> struct PFormat {
@@ -143,6 +147,7 @@ struct Work {
   float* lse2;     // [2 ranges][R] log2 of the sum of a part
   Cut* cuts;       // [ranges]
   int ring;        // chunks of the ring
+  bool whole;      // a group belongs to the range that it starts in: no parts, no join
 };
 
 // ---------------------------------------------------------------------------
@@ -225,9 +230,11 @@ struct Walk {
   Seq s;
   int b;
   int64_t u, end, base;    // base: count at which sequence b starts
+  bool whole;              // groups that start in the range, to their end
   Segment second;          // of the pair under way, when there is one (t1 > t0)
-  __device__ Walk(const CacheParams& p_, const Seq& s_, int b_, int64_t base_, int64_t u_, int64_t end_)
-      : p(p_), s(s_), b(b_), u(u_), end(end_), base(base_), second{0, 0, 0, 0, 0} {}
+  __device__ Walk(const CacheParams& p_, const Seq& s_, int b_, int64_t base_, int64_t u_, int64_t end_,
+                  bool whole_)
+      : p(p_), s(s_), b(b_), u(u_), end(end_), base(base_), whole(whole_), second{0, 0, 0, 0, 0} {}
   __device__ bool next(Segment& seg) {
     if (second.t1 > second.t0) {
       seg = second;
@@ -244,6 +251,17 @@ struct Walk {
       const int end1 = kSetup + n1, all = end1 + (n2 > 0 ? kSetup + n2 : 0);
       int stop = (int)min((int64_t)s.pair, q + (end - u));
       u += stop - q;
+      if (whole) {
+        second = Segment{b, g2, 0, q <= end1 && end1 < stop ? n2 : 0, n2};
+        seg = Segment{b, g1, 0, q == 0 ? n1 : 0, n1};
+        if (seg.t1 > 0) return true;
+        if (second.t1 > 0) {
+          seg = second;
+          second.t1 = 0;
+          return true;
+        }
+        continue;
+      }
       // the last place of a pair takes whatever is left of it
       stop = stop == s.pair ? all : min(stop, all);
       second = Segment{b, g2, max(0, q - end1 - kSetup), stop - end1 - kSetup, n2};
@@ -348,20 +366,23 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   }
 }
 
-// A query's values as e4m3 terms: x = t[0] + t[1] / 16 (+ t[2] / 256), four at a time.
+// A query's values (times 2^-8; at most 1, so that no term reaches 1.875, the code of
+// NaN) as e4m3 terms, x = t[0] + t[1] / 16 (+ t[2] / 256), four at a time: like
+// PFormat<__half>, with signs.
 template <int NT>
 __device__ __forceinline__ void split_query(const float (&x)[4], uint32_t (&t)[NT]) {
-  float r[4] = {x[0], x[1], x[2], x[3]};
+  __half2 r[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
+  const __half2 finer = __float2half2_rn(kQFiner);
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    t[j] = to_e4m3x4(r[0], r[1], r[2], r[3]);
-    if (j + 1 < NT) {
-      const float2 lo = from_e4m3x2(t[j]), hi = from_e4m3x2(t[j] >> 16);
-      r[0] = (r[0] - lo.x) * kQFiner;
-      r[1] = (r[1] - lo.y) * kQFiner;
-      r[2] = (r[2] - hi.x) * kQFiner;
-      r[3] = (r[3] - hi.y) * kQFiner;
+    uint32_t c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(&r[i]) & 0xbf80bf80u;
+      if (j + 1 < NT) r[i] = __hmul2(__hsub2(r[i], *reinterpret_cast<const __half2*>(&u)), finer);
+      c[i] = ((u >> 7) & 0x007f007fu) | ((u >> 8) & 0x00800080u);
     }
+    t[j] = __byte_perm(c[0], c[1], 0x6420);
   }
 }
 // the sum of a value's terms, each `finer` times finer
@@ -528,12 +549,13 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   const uint32_t tm_s = tmem + NCH * NO;        // S buffers after the O chunks
   volatile int* ab = &sh.abort_flag;
   if (warp >= 8) {
-    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1, w.whole);
     Segment seg;
   if (warp == 10) {
     // ======== the group that this range starts inside of, for cache_join_kernel
     Cut cut{-1, 0, 0, 0};
-    if (u0 < u1 && blockIdx.x > 0) {
+    if (u0 < u1 && blockIdx.x > 0 && !w.whole) {
       int g1, q, g2, n1, n2;
       place<R>(p, walk.s, u0 - sh.base, g1, q, g2, n1, n2);
       int64_t start = u0 - q + kSetup;         // where the group's first tile counts
@@ -677,7 +699,8 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   } else {
     // ======== softmax: two groups of four warps have half of the rows each; thread =
     // position of the tile = TMEM lane
-    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1, w.whole);
     constexpr int HR = R / 2;                   // rows of a group
     const int wg = warp >> 2, rb = wg * HR;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -777,11 +800,12 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         y[1] = live ? ld(v + 1) : 0.f;
         const uint32_t rmax = max(abs_bits(y[0]), abs_bits(y[1]));
         const int e = scale_exp(warp_max_u32(amax), p.DR ? warp_max_u32(rmax) : 0);
-        const float inv = pow2i(-e);
+        // half of what scale_exp allows: at most 224
+        const float inv = 0.5f * pow2i(-e), inv8 = inv * (1.f / 256.f);
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[c][j] *= inv;
+          for (int j = 0; j < 4; ++j) x[c][j] *= inv8;
           uint32_t term[NQ];
           split_query<NQ>(x[c], term);
 #pragma unroll
@@ -796,7 +820,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         if (lane == 0) {
           const int row = sg.row0 + min(r, sg.rows - 1), tok = div_heads(p, row);
           const int64_t n = sg.first + tok, h = row - tok * p.H;
-          rw.q_scale[r] = pow2i(e) * p.scale * kLog2e;
+          rw.q_scale[r] = 2.f * pow2i(e) * p.scale * kLog2e;
           rw.seen[r] = live ? max(0, min(sg.off + tok + 1, sg.seen)) : sg.seen;
           rw.m[r] = kUnset;
           rw.out[r] = n * p.o_s[0] + h * p.o_s[1];
@@ -954,8 +978,6 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         ptx::mbar_arrive(&sh.p_full[par]);
         ls_next = log2f(s_next);
         rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
-        // the next segment's loads, well ahead (with 32 rows there are no registers to
-        // hold them meanwhile)
         if (R == 16 && start) {
           have_next = next_segment(nseg);
           if (have_next) fetch(nseg);
@@ -992,40 +1014,41 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           else if (p.lse) p.lse[rw.lse[rb + lane]] = lse2 * kLn2;
         }
       }
+      const bool odd = lane & 1;
       float f[HR];
+      T* dst[HR / 2];                           // neighbouring lanes swap a row each: four bytes a store
 #pragma unroll
       for (int r = 0; r < HR; ++r) f[r] = __shfl_sync(0xffffffffu, inv, r);
+#pragma unroll
+      for (int r = 0; r < HR; r += 2)
+        dst[r / 2] = static_cast<T*>(p.out) + rw.out[rb + r + odd] + (tt & ~1);
 #pragma unroll 1
       for (int c = 0; c < NCH; ++c) {           // 128 channels of this group's rows
         float o[NP * HR];
 #pragma unroll
         for (int j = 0; j < NP; ++j) tmem_get<HR>(tmem + c * NO + j * R + rb + lane_base, o + HR * j);
         ptx::tmem_wait_ld();
-        const int ch = c * 128 + tt;
 #pragma unroll
-        for (int r = 0; r < HR; ++r) o[r] = f[r] == 0.f ? 0.f : join<NP>(o + r, HR, F::FINER) * f[r];
+        for (int r = 0; r < HR; ++r) o[r] = join<NP>(o + r, HR, F::FINER) * f[r];
         if (whole) {
-          // neighbouring lanes swap a row each: four bytes a store
-          const bool odd = lane & 1;
 #pragma unroll
           for (int r = 0; r < HR; r += 2) {
             const float other = __shfl_xor_sync(0xffffffffu, odd ? o[r] : o[r + 1], 1);
-            const int row = rb + r + odd;
-            if (row < seg.rows) {
-              T* dst = static_cast<T*>(p.out) + rw.out[row] + (ch & ~1);
-              T pair[2];
-              st(pair, odd ? other : o[r]);
-              st(pair + 1, odd ? o[r + 1] : other);
+            T pair[2];
+            st(pair, odd ? other : o[r]);
+            st(pair + 1, odd ? o[r + 1] : other);
+            if (rb + r + odd < seg.rows) {
+              T* d = dst[r / 2] + c * 128;
               if (p.out_vec) {
-                *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(pair);
+                *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(pair);
               } else {
-                dst[0] = pair[0];
-                dst[1] = pair[1];
+                d[0] = pair[0];
+                d[1] = pair[1];
               }
             }
           }
         } else {
-          float* part = w.part + ((int64_t)slot * R + rb) * p.KVL + ch;
+          float* part = w.part + ((int64_t)slot * R + rb) * p.KVL + c * 128 + tt;
 #pragma unroll
           for (int r = 0; r < HR; ++r)
             if (rb + r < seg.rows) part[r * p.KVL] = o[r];
@@ -1163,8 +1186,11 @@ cudaError_t launch(const CacheParams& p, Work w, const CUtensorMap& mc, const CU
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
   if (e != cudaSuccess) return e;
   const size_t smem = fixed_bytes(p.KVL, C::NQ, R) + w.ring * CHUNK;
+  // Contexts that a block goes through about as fast as it would join parts of them
+  // stay whole, and the second launch goes.
+  w.whole = (int64_t)p.max_pages * p.page_size <= kWholeTiles * TILE;
   e = launch_dependent(k, dim3(ranges), kThreads, smem, s, p, w, mc, mr);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || w.whole) return e;
   return launch_dependent(cache_join_kernel<T, R>, dim3(ranges - 1, R), kJoinThreads, 0, s, p, w);
 }
 

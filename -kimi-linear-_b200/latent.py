@@ -36,7 +36,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DT, _call
+from .ops import _DT, KdaError, _call
 
 _HALF = (torch.float16, torch.bfloat16)
 _I64x2 = ctypes.c_int64 * 2
@@ -117,52 +117,78 @@ class LatentCache:
         self._args = bytes(a)
 
 
-def _check(fn, cache, tensors):
-    """16-bit operands of the cache's type on its device, unit innermost stride."""
-    dev, dt, grad = cache.device, cache.dtype, torch.is_grad_enabled()
-    if dev.type != "cuda":
-        raise RuntimeError(f"{fn}: the cache is on {dev}; the B200 kernels need CUDA tensors "
-                           f"(there is no CPU path)")
-    for name, t in tensors:
-        if t is None:
+def _refuse(fn, cache, name, t):
+    """Why operand ``t`` is not a 16-bit tensor of the cache's type on its device."""
+    dev, dt = cache.device, cache.dtype
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{fn}: {name} must be a torch.Tensor")
+    if dev.type != "cuda" or t.device != dev:
+        raise RuntimeError(f"{fn}: {name} is on {t.device}, the cache on {dev}; the B200 kernels "
+                           f"need CUDA tensors on one device (there is no CPU path)")
+    if t.dtype is not dt:
+        raise TypeError(f"{fn}: {name} is {t.dtype}, the cache's type is {dt}")
+    raise RuntimeError(f"{fn}: the latent cache is forward-only; call under torch.no_grad() or "
+                       f"detach the inputs")
+
+
+def _operand(fn, cache, name, t):
+    if not isinstance(t, torch.Tensor) or t.dtype is not cache.dtype or \
+            t.device != cache.device or not t.is_cuda or \
+            (t.requires_grad and torch.is_grad_enabled()):
+        _refuse(fn, cache, name, t)
+
+
+def _refuse_index(fn, cache, block_table, lens, q_start):
+    if cache.device.type != "cuda":
+        raise RuntimeError(f"{fn}: the cache is on {cache.device}; the B200 kernels need CUDA "
+                           f"tensors (there is no CPU path)")
+    for name, t, dims in (("block_table", block_table, 2), ("lens", lens, 1),
+                          ("q_start", q_start, 1)):
+        if t is None and name == "q_start":
             continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{fn}: {name} must be a torch.Tensor")
-        if t.device != dev:
-            raise RuntimeError(f"{fn}: {name} is on {t.device}, expected {dev} (the B200 kernels "
-                               f"need CUDA tensors)")
-        if t.dtype is not dt:
-            raise TypeError(f"{fn}: {name} is {t.dtype}, the cache's type is {dt}")
-        if grad and t.requires_grad:
-            raise RuntimeError(f"{fn}: the latent cache is forward-only; call under "
-                               f"torch.no_grad() or detach the inputs")
+        if not _is_index(t, dims, cache.device):
+            raise RuntimeError(f"{fn}: {name} must be an int32 tensor of {dims} dimension(s) with "
+                               f"a unit innermost stride on {cache.device}")
+    raise RuntimeError(
+        f"{fn}: block_table {tuple(block_table.shape)}, lens {tuple(lens.shape)} and q_start "
+        f"{None if q_start is None else tuple(q_start.shape)} do not describe one batch")
+
+
+def _is_index(t, dims, dev):
+    return isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == dev and \
+        t.dim() == dims and (t.stride(-1) == 1 or t.numel() <= 1)
 
 
 def _args(fn, cache, block_table, lens, q_start, N):
     """The argument block with the pool, the table and the lengths filled in."""
     dev = cache.device
-    for name, t, dims in (("block_table", block_table, 2), ("lens", lens, 1),
-                          ("q_start", q_start, 1)):
-        if t is None and name == "q_start":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != dev or \
-                t.dim() != dims or (t.stride(-1) != 1 and t.numel() > 1):
-            raise RuntimeError(f"{fn}: {name} must be an int32 tensor of {dims} dimension(s) with "
-                               f"a unit innermost stride on {dev}")
+    if dev.type != "cuda" or not _is_index(block_table, 2, dev) or not _is_index(lens, 1, dev) or \
+            (q_start is not None and not _is_index(q_start, 1, dev)):
+        _refuse_index(fn, cache, block_table, lens, q_start)
     B = lens.shape[0]
-    if block_table.shape[0] != B or (q_start is not None and q_start.shape[0] != B + 1):
-        raise RuntimeError(
-            f"{fn}: block_table {tuple(block_table.shape)}, lens {tuple(lens.shape)} and q_start "
-            f"{None if q_start is None else tuple(q_start.shape)} do not describe one batch")
+    rows, width = block_table.shape
+    if rows != B or (q_start is not None and q_start.shape[0] != B + 1):
+        _refuse_index(fn, cache, block_table, lens, q_start)
     if q_start is None and (N % B if B else N):
         raise RuntimeError(f"{fn}: {N} new tokens do not divide over {B} sequences; pass q_start")
     a = _lib.MlaCacheArgs.from_buffer_copy(cache._args)
-    a.B, a.N, a.max_pages = B, N, block_table.shape[1]
+    a.B, a.N, a.max_pages = B, N, width
     a.block_table, a.table_stride = block_table.data_ptr(), block_table.stride(0)
     a.lens = lens.data_ptr()
     if q_start is not None:
         a.q_start = q_start.data_ptr()
     return a
+
+
+def _launch(fn, entry, a, dev):
+    """Call a C entry point on the current stream of ``dev`` (:func:`ops._call`
+    with less host work: these calls can be a few microseconds long)."""
+    index = dev.index
+    if torch.cuda.current_device() != index:
+        return _call(fn, entry, a, dev)
+    st = entry(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
+    if st != _lib.KDA_OK:
+        raise KdaError(fn, st)
 
 
 def _rows(fn, name, t, N, width):
@@ -182,19 +208,20 @@ def latent_append(cache, c_kv, block_table, lens, q_start=None, k_rope=None):
     NaN.  Tokens whose position is negative (``lens[b]`` below the number of new
     tokens) are skipped.  Two tokens of one call must not share a slot."""
     fn = "latent_append"
-    _check(fn, cache, (("c_kv", c_kv), ("k_rope", k_rope)))
+    _operand(fn, cache, "c_kv", c_kv)
     N = c_kv.shape[0]
     c_kv = _rows(fn, "c_kv", c_kv, N, cache.kv_lora_rank)
-    if (k_rope is None) != (cache.rope_dim == 0):
+    if (k_rope is None) != (cache.rope is None):
         raise RuntimeError(f"{fn}: k_rope must be given exactly when the cache has a rope part")
     a = _args(fn, cache, block_table, lens, q_start, N)
     if N == 0:
         return
     a.c_kv, a.c_kv_stride = c_kv.data_ptr(), c_kv.stride(0)
     if k_rope is not None:
+        _operand(fn, cache, "k_rope", k_rope)
         k_rope = _rows(fn, "k_rope", k_rope, N, cache.rope_dim)
         a.k_rope, a.k_rope_stride = k_rope.data_ptr(), k_rope.stride(0)
-    _call(fn, _lib.load().mla_cache_append, a, cache.device)
+    _launch(fn, _lib.load().mla_cache_append, a, cache.device)
 
 
 def latent_read(cache, block_table, lens, num_tokens, q_start=None):
@@ -203,19 +230,18 @@ def latent_read(cache, block_table, lens, num_tokens, q_start=None):
     ``q_start``, or ``N / B`` each): what :func:`latent_append` of the same
     arguments wrote, as values.  Zeros for tokens whose position is negative."""
     fn = "latent_read"
-    _check(fn, cache, ())
     N, dev = int(num_tokens), cache.device
     if N < 0:
         raise RuntimeError(f"{fn}: num_tokens {N} is negative")
     a = _args(fn, cache, block_table, lens, q_start, N)
-    c_kv = torch.empty(N, cache.kv_lora_rank, dtype=cache.dtype, device=dev)
+    c_kv = torch.empty((N, cache.kv_lora_rank), dtype=cache.dtype, device=dev)
     k_rope = None
     a.c_kv, a.c_kv_stride = c_kv.data_ptr(), cache.kv_lora_rank
-    if cache.rope_dim:
-        k_rope = torch.empty(N, cache.rope_dim, dtype=cache.dtype, device=dev)
+    if cache.rope is not None:
+        k_rope = torch.empty((N, cache.rope_dim), dtype=cache.dtype, device=dev)
         a.k_rope, a.k_rope_stride = k_rope.data_ptr(), cache.rope_dim
     if N:
-        _call(fn, _lib.load().mla_cache_read, a, dev)
+        _launch(fn, _lib.load().mla_cache_read, a, dev)
     return c_kv, k_rope
 
 
@@ -234,41 +260,45 @@ def latent_attention(q_lat, cache, block_table, lens, scale, q_start=None, q_rop
 
     The new tokens' own latents must be in the cache (:func:`latent_append`
     first).  Scores and sums are fp32; queries enter the products exactly
-    (bf16) or to 2^-12 (fp16), the softmax's weights to 2^-8 (bf16) or 2^-12
+    (bf16) or to 2^-12 (fp16), the softmax's weights to 2^-9 (bf16) or 2^-12
     (fp16) relative, below the outputs' own rounding."""
     fn = "latent_attention"
-    _check(fn, cache, (("q_lat", q_lat), ("q_rope", q_rope)))
-    if q_lat.dim() != 3 or q_lat.shape[2] != cache.kv_lora_rank:
-        raise RuntimeError(f"{fn}: q_lat shape {tuple(q_lat.shape)} is not "
-                           f"[N, H, {cache.kv_lora_rank}]")
-    N, H = q_lat.shape[:2]
-    if (q_rope is None) != (cache.rope_dim == 0):
+    _operand(fn, cache, "q_lat", q_lat)
+    kvl = cache.kv_lora_rank
+    if q_lat.dim() != 3 or q_lat.shape[2] != kvl:
+        raise RuntimeError(f"{fn}: q_lat shape {tuple(q_lat.shape)} is not [N, H, {kvl}]")
+    N, H, _ = q_lat.shape
+    if (q_rope is None) != (cache.rope is None):
         raise RuntimeError(f"{fn}: q_rope must be given exactly when the cache has a rope part")
     a = _args(fn, cache, block_table, lens, q_start, N)
     dev = cache.device
-    out = torch.empty(N, H, cache.kv_lora_rank, dtype=cache.dtype, device=dev)
-    lse = torch.empty(N, H, dtype=torch.float32, device=dev) if return_lse else None
+    out = torch.empty((N, H, kvl), dtype=cache.dtype, device=dev)
+    lse = torch.empty((N, H), dtype=torch.float32, device=dev) if return_lse else None
     if N and H:
         if q_lat.stride(2) != 1:
             q_lat = q_lat.contiguous()
         a.H, a.scale = H, float(scale)
-        a.q_lat, a.q_lat_stride = q_lat.data_ptr(), _I64x2(*q_lat.stride()[:2])
+        a.q_lat = q_lat.data_ptr()
+        a.q_lat_stride[0], a.q_lat_stride[1] = q_lat.stride(0), q_lat.stride(1)
         if q_rope is not None:
+            _operand(fn, cache, "q_rope", q_rope)
             if tuple(q_rope.shape) != (N, H, cache.rope_dim):
                 raise RuntimeError(f"{fn}: q_rope shape {tuple(q_rope.shape)} != "
                                    f"{(N, H, cache.rope_dim)}")
             if q_rope.stride(2) != 1:
                 q_rope = q_rope.contiguous()
-            a.q_rope, a.q_rope_stride = q_rope.data_ptr(), _I64x2(*q_rope.stride()[:2])
-        a.out, a.out_stride = out.data_ptr(), _I64x2(H * cache.kv_lora_rank, cache.kv_lora_rank)
+            a.q_rope = q_rope.data_ptr()
+            a.q_rope_stride[0], a.q_rope_stride[1] = q_rope.stride(0), q_rope.stride(1)
+        a.out = out.data_ptr()
+        a.out_stride[0], a.out_stride[1] = H * kvl, kvl
         if lse is not None:
             a.lse, a.lse_stride = lse.data_ptr(), H
         lib = _lib.load()
         need = lib.mla_cache_workspace_bytes(ctypes.byref(a))
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = torch.empty((need,), dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        _call(fn, lib.mla_cache_attention, a, dev)
+        _launch(fn, lib.mla_cache_attention, a, dev)
     return (out, lse) if return_lse else out
 
 
