@@ -19,8 +19,33 @@ __device__ int g_cache_device_error = 0;
 namespace {
 
 constexpr int kLanes = 16;                 // lanes per token
-constexpr int kTokens = 16;                // tokens per block
+constexpr int kTokens = 8;                 // tokens per block: small blocks, so that the
+                                           // last ones leave no SM idle for long
 constexpr int kThreads = kLanes * kTokens;
+
+// eight 16-bit elements as they are; `vec`: the address is 16-byte aligned
+template <typename T>
+__device__ __forceinline__ uint4 raw8(const T* p, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(p);
+  const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// largest magnitude of the halves of `m` and the eight elements, as 16-bit patterns (in
+// which infinities and NaN are the largest)
+__device__ __forceinline__ uint32_t max8(uint32_t m, const uint4& u) {
+  m = __vmaxu2(m, u.x & 0x7fff7fffu);
+  m = __vmaxu2(m, u.y & 0x7fff7fffu);
+  m = __vmaxu2(m, u.z & 0x7fff7fffu);
+  return __vmaxu2(m, u.w & 0x7fff7fffu);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t to_float_bits(uint32_t pattern) {
+  const uint16_t h = (uint16_t)pattern;
+  return abs_bits(ld(reinterpret_cast<const T*>(&h)));
+}
 
 template <typename T, int STEPS>
 __global__ void __launch_bounds__(kThreads)
@@ -28,51 +53,54 @@ cache_append_kernel(const CacheParams p) {
   const int lane = threadIdx.x % kLanes;
   const int n = blockIdx.x * kTokens + threadIdx.x / kLanes;
   const bool live = n < p.N;
-  float x[STEPS][8], y[8];
-  uint32_t amax = 0, rmax = 0;
+  uint4 x[STEPS], y = make_uint4(0, 0, 0, 0);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = 0.f;
+  for (int s = 0; s < STEPS; ++s) x[s] = y;
   if (live) {
     const T* c = static_cast<const T*>(p.c_kv) + (int64_t)n * p.c_s + 8 * lane;
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) ld8(c + 128 * s, p.vec, x[s]);
+    for (int s = 0; s < STEPS; ++s) x[s] = raw8(c + 128 * s, p.vec);
     if (p.DR && lane < 8)
-      ld8(static_cast<const T*>(p.k_rope) + (int64_t)n * p.k_s + 8 * lane, p.vec, y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) amax = max(amax, abs_bits(x[s][i]));
-      rmax = max(rmax, abs_bits(y[i]));
-    }
+      y = raw8(static_cast<const T*>(p.k_rope) + (int64_t)n * p.k_s + 8 * lane, p.vec);
   }
+  // where it goes, while its values are on their way
+  int b, pos, page = -1;
+  locate(p, min(n, p.N - 1), b, pos);
+  if (live && pos >= 0) page = page_of(p, b, pos);
+  uint32_t amax = 0, rmax = max8(0, y);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) amax = max8(amax, x[s]);
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) {
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    rmax = max(rmax, __shfl_xor_sync(0xffffffffu, rmax, o));
+    amax = __vmaxu2(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    rmax = __vmaxu2(rmax, __shfl_xor_sync(0xffffffffu, rmax, o));
   }
-  if (!live) return;
-  int b, pos;
-  locate(p, n, b, pos);
-  if (pos < 0) return;
-  const int page = page_of(p, b, pos);
+  if (!live || pos < 0) return;
   if (page < 0) {
     if (lane == 0) atomicExch(&g_cache_device_error, kErrOutside);
     return;
   }
   const int off = pos & (p.page_size - 1);
-  const int e = scale_exp(amax, rmax);
+  const int e = scale_exp(to_float_bits<T>(max(amax & 0xffffu, amax >> 16)),
+                          to_float_bits<T>(max(rmax & 0xffffu, rmax >> 16)));
   const float inv = pow2i(-e);
   uint8_t* q = p.codes + (int64_t)page * p.codes_s[0] + (int64_t)off * p.codes_s[1] + 8 * lane;
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-    *reinterpret_cast<uint2*>(q + 128 * s) =
-        make_uint2(to_e4m3x4(x[s][0] * inv, x[s][1] * inv, x[s][2] * inv, x[s][3] * inv),
-                   to_e4m3x4(x[s][4] * inv, x[s][5] * inv, x[s][6] * inv, x[s][7] * inv));
-  if (p.DR && lane < 8) {
+  for (int s = 0; s < STEPS; ++s) {
+    const T* v = reinterpret_cast<const T*>(&x[s]);
+    float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= inv;
+    for (int i = 0; i < 8; ++i) f[i] = ld(v + i) * inv;
+    *reinterpret_cast<uint2*>(q + 128 * s) =
+        make_uint2(to_e4m3x4(f[0], f[1], f[2], f[3]), to_e4m3x4(f[4], f[5], f[6], f[7]));
+  }
+  if (p.DR && lane < 8) {
+    const T* v = reinterpret_cast<const T*>(&y);
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = ld(v + i) * inv;
     st8(static_cast<T*>(p.rope) + (int64_t)page * p.rope_s[0] + (int64_t)off * p.rope_s[1] +
-            8 * lane, true, y);
+            8 * lane, true, f);
   }
   if (lane == 0) p.scales[(int64_t)page * p.scales_s + off] = pow2i(e);
 }
@@ -82,9 +110,9 @@ __global__ void __launch_bounds__(kThreads)
 cache_read_kernel(const CacheParams p) {
   const int lane = threadIdx.x % kLanes;
   const int n = blockIdx.x * kTokens + threadIdx.x / kLanes;
-  if (n >= p.N) return;
   int b, pos;
-  locate(p, n, b, pos);
+  locate(p, min(n, p.N - 1), b, pos);
+  if (n >= p.N) return;
   int page = -1;
   if (pos >= 0) {
     page = page_of(p, b, pos);

@@ -47,7 +47,9 @@ __device__ __forceinline__ void new_tokens(const CacheParams& p, int b, int& fir
   }
 }
 
-// Sequence and position of new token n (position < 0: it has none).
+// Sequence and position of new token n (position < 0: it has none), for all lanes of
+// a warp at once; lanes of one half have one n.  The sequences' starts are counted 32
+// at a time: one load's latency, where a search by halves has one for each step.
 __device__ __forceinline__ void locate(const CacheParams& p, int n, int& b, int& pos) {
   int first, count;
   if (p.q_start == nullptr) {
@@ -55,15 +57,19 @@ __device__ __forceinline__ void locate(const CacheParams& p, int n, int& b, int&
     b = n / count;
     first = b * count;
   } else {
-    int lo = 0, hi = p.B;            // q_start[lo] <= n < q_start[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.q_start[mid] <= n) lo = mid; else hi = mid;
+    const int lane = threadIdx.x & 31;
+    const int n0 = __shfl_sync(0xffffffffu, n, 0), n1 = __shfl_sync(0xffffffffu, n, 16);
+    int c0 = 0, c1 = 0;              // starts 1 .. B - 1 that are <= n
+    for (int i = 1; i < p.B; i += 32) {
+      const int x = i + lane < p.B ? p.q_start[i + lane] : 0x7fffffff;
+      c0 += __popc(__ballot_sync(0xffffffffu, x <= n0));
+      c1 += __popc(__ballot_sync(0xffffffffu, x <= n1));
     }
-    b = lo;
+    b = lane < 16 ? c0 : c1;
     new_tokens(p, b, first, count);
   }
-  pos = n - first < count ? max(p.lens[b], 0) - count + (n - first) : -1;
+  const int i = n - first;
+  pos = i >= 0 && i < count ? max(p.lens[b], 0) - count + i : -1;
 }
 
 // Page of position pos of sequence b, or -1 where the table or the pool ends.

@@ -43,7 +43,7 @@ namespace {
 
 constexpr int TILE = 128;                  // positions per tile (MMA M)
 constexpr int CHUNK = TILE * 128;          // bytes of 128 positions x 128 bytes
-constexpr int kThreads = 384;              // warps 0-3 and 4-7 softmax, 8 loads, 9 MMA issue, 10 cuts
+constexpr int kThreads = 384;              // warps 0-7 softmax, 8 loads, 9 S, 10 segments, 11 O
 // Registers: the block starts with 384 x 168; the softmax warps take 192 each, the
 // others keep 120 (256 x 192 + 128 x 120 = 384 x 168).
 constexpr int kSoftmaxRegs = 192, kOtherRegs = 120;
@@ -52,7 +52,6 @@ constexpr int kMaxRing = 14;
 constexpr int kWholeTiles = 4;             // contexts of at most so many tiles are not split
 constexpr int kMaxRanges = 256;            // blocks (SMs) that a call's tiles are cut over
 constexpr int kSmemMax = 232448;           // 227 KB per block
-constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kUnset = -1e30f;           // maximum of a row that has seen nothing
@@ -223,7 +222,7 @@ struct Segment {
   int tiles;               // of the whole group
 };
 
-// Walks the segments of the range [u, end): every role runs its own copy.
+// Walks the segments of the range [u, end).
 template <int R>
 struct Walk {
   const CacheParams& p;
@@ -284,26 +283,31 @@ struct Walk {
 // lane itself: the operands then stay in uniform registers.  One instruction of 128 x
 // 32 x 32 takes 41 cycles this way (49 with N = 64: reading its operands from shared
 // memory), 80 or 143 from a branch that one lane takes.
+// A shared-memory descriptor is its low word (address and leading offset) and a high
+// word that the layout fixes; consecutive operands differ in the low word alone.
 // D[tmem] = A[smem] B[smem] (+ D): 8-bit operands, fp32 accumulation
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                       uint32_t idesc, uint32_t accumulate) {
+template <uint32_t A_HI, uint32_t B_HI>
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+                                       uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 x;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %6};\n\t"
       "elect.sync x|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(A_HI), "n"(B_HI)
       : "memory");
 }
 // D += A B, 16-bit operands of one type
-__device__ __forceinline__ void mma_half(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                         uint32_t idesc) {
+template <uint32_t A_HI, uint32_t B_HI>
+__device__ __forceinline__ void mma_half(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 x;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %5};\n\t"
       "elect.sync x|e, 0xffffffff;\n\t"
       "setp.eq.b32 p, 0, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc)
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(A_HI), "n"(B_HI)
       : "memory");
 }
 // arrive on `bar` once the warp's products so far have completed
@@ -315,14 +319,14 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
           ptx::smem_u32(bar))
       : "memory");
 }
-// Shared-memory descriptor of 128-byte rows with the 128-byte swizzle (eight
-// rows = 1024 bytes, consecutive).  K-major operands: rows are M or N; M-major
-// ones: rows are K, and the 128 bytes of a row are all of M.
-__device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
-         (static_cast<uint64_t>(2) << 61);
-}
+// 128-byte rows with the 128-byte swizzle (eight rows = 1024 bytes, consecutive).
+// K-major operands: rows are M or N; M-major ones: rows are K, and the 128 bytes of a
+// row are all of M.  (High word: stride 1024, version 1, swizzle code 2.)
+constexpr uint32_t kSw128Hi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+// no swizzle: core matrices of 8 x 16 bytes, 128 bytes on along K, 2048 along N
+constexpr uint32_t kPHi = (TILE * 16 >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t p_lo(uint32_t saddr) { return (saddr >> 4) | ((128 >> 4) << 16); }
 // Instruction descriptors: fp32 accumulator; 8-bit formats 0 = e4m3, 1 = e5m2, 16-bit
 // ones 0 = f16, 1 = bf16
 __host__ __device__ constexpr uint32_t idesc(int N, bool a_m_major, bool b_n_major, uint32_t a_fmt,
@@ -349,20 +353,34 @@ __device__ __forceinline__ uint32_t swz(int row, int byte) {
   return (uint32_t)(row * 128 + ((((byte >> 4) ^ row) & 7) << 4) + (byte & 15));
 }
 
-// Bounded wait: false once the block gave up (the caller then leaves its loop).
+// Bounded wait: false once the block gave up (the caller then leaves its loop).  A
+// try sleeps for at most about a microsecond, so that the limit is some seconds.
+constexpr int kTries = 1 << 21;
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(ptx::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (ptx::mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = ptx::globaltimer_ns();
-  for (;;) {
 #pragma unroll 1
-    for (int i = 0; i < 32; ++i)
-      if (ptx::mbar_try_wait(bar, parity)) return true;
+  for (int i = 0; i < kTries; ++i) {
+    if (try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (ptx::globaltimer_ns() - t0 > kWaitNs) {
-      *abort_flag = 1;
-      atomicExch(&g_attn_device_error, kErrWait);
-      return false;
-    }
+  }
+  *abort_flag = 1;
+  atomicExch(&g_attn_device_error, kErrWait);
+  return false;
+}
+// the same for what is in flight when the block has given up already
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < kTries && !try_wait(bar, parity); ++i) {
   }
 }
 
@@ -402,16 +420,26 @@ struct Rows {              // per row of a group
   int seen[R];             // positions that it sees
   int64_t out[R], lse[R];  // where its results go
 };
+// A segment as the other warps get it (t1 = t0: there are no more).
+struct Info {
+  int b, t0, t1, tiles;    // tiles t0 .. t1 - 1 of a group that has `tiles`
+  int row0, rows;          // its rows
+  int first, off;          // its sequence's new tokens
+  int seen, seen0;         // positions that its last and its first row see
+};
+constexpr int kQueue = 4;  // segments that are known ahead
+
 template <int R>
 struct Shared {            // at the end of dynamic shared memory
-  uint64_t full[kMaxRing], empty[kMaxRing];
-  uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], q_ready, drain;
+  uint64_t full[kMaxRing], empty[kMaxRing], seg_full[kQueue], seg_empty[kQueue];
+  uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], q_ready, drain[2];
   uint32_t tmem;
   int abort_flag;
   int64_t scan[(kThreads + 31) / 32];
   int64_t base;            // where the range starts: count at which sequence b starts
   int b;
   Seq seq;                 // and that sequence
+  Info queue[kQueue];
   Rows<R> rows[2];         // of this segment and the next
   float red[8][R / 2];     // per warp and row: maxima, sums
 };
@@ -490,8 +518,13 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       ptx::mbar_init(&sh.p_full[i], 256);
       ptx::mbar_init(&sh.o_done[i], 1);
     }
+    for (int i = 0; i < kQueue; ++i) {
+      ptx::mbar_init(&sh.seg_full[i], 1);
+      ptx::mbar_init(&sh.seg_empty[i], 3 + 256);
+    }
     ptx::mbar_init(&sh.q_ready, 256);
-    ptx::mbar_init(&sh.drain, 1);
+    ptx::mbar_init(&sh.drain[0], 1);
+    ptx::mbar_init(&sh.drain[1], 1);
     sh.abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -548,39 +581,88 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   const uint32_t tmem = sh.tmem;
   const uint32_t tm_s = tmem + NCH * NO;        // S buffers after the O chunks
   volatile int* ab = &sh.abort_flag;
+  // the next segment from the queue, copied out; 0: there are no more, -1: given up
+  int taken = 0;
+  auto take = [&](Info& sg, bool one_arrives) {
+    const int i = taken % kQueue;
+    if (!wait(&sh.seg_full[i], (taken / kQueue) & 1, ab)) return -1;
+    sg = sh.queue[i];
+    if (one_arrives) {
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.seg_empty[i]);
+    } else {
+      ptx::mbar_arrive(&sh.seg_empty[i]);
+    }
+    ++taken;
+    return sg.t1 > sg.t0 ? 1 : 0;
+  };
+
+  const auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1, w.whole);
-    Segment seg;
-  if (warp == 10) {
-    // ======== the group that this range starts inside of, for cache_join_kernel
-    Cut cut{-1, 0, 0, 0};
-    if (u0 < u1 && blockIdx.x > 0 && !w.whole) {
-      int g1, q, g2, n1, n2;
-      place<R>(p, walk.s, u0 - sh.base, g1, q, g2, n1, n2);
-      int64_t start = u0 - q + kSetup;         // where the group's first tile counts
-      int n = 0;
-      if (q > kSetup && q < kSetup + n1) {
-        cut.b = sh.b; cut.g = g1; n = n1;
-      } else if (n2 > 0 && q > 2 * kSetup + n1 && q < 2 * kSetup + n1 + n2) {
-        cut.b = sh.b; cut.g = g2; start += kSetup + n1; n = n2;
+    if (warp == 10) {
+      // ======== segments: a queue of them for the other warps; groups that see nothing
+      // get their zeros here
+      Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1, w.whole);
+      for (int i = 0;;) {
+        Segment seg;
+        const bool have = walk.next(seg);
+        Info info{};
+        if (have) {
+          const int row0 = seg.g * R;
+          info = Info{seg.b, seg.t0, seg.t1, seg.tiles, row0,
+                      (int)min((int64_t)R, (int64_t)walk.s.n * p.H - row0), walk.s.first, walk.s.off,
+                      seen_by(p, walk.s, row0 + R - 1), seen_by(p, walk.s, row0)};
+          if (lane == 0 && walk.s.off + walk.s.n > walk.s.cap)
+            atomicExch(&g_attn_device_error, kErrOutside);
+          if (info.seen == 0) {
+            for (int r = 0; r < info.rows; ++r) {
+              const int tok = div_heads(p, row0 + r);
+              const int64_t n = info.first + tok, h = row0 + r - tok * p.H;
+              T* o = static_cast<T*>(p.out) + n * p.o_s[0] + h * p.o_s[1];
+              for (int c = lane; c < p.KVL; c += 32) st(o + c, 0.f);
+              if (lane == 0 && p.lse) p.lse[n * p.lse_s + h] = -INFINITY;
+            }
+            continue;
+          }
+        }
+        if (i >= kQueue && !wait(&sh.seg_empty[i % kQueue], (i / kQueue - 1) & 1, ab)) break;
+        if (lane == 0) {
+          sh.queue[i % kQueue] = info;
+          ptx::mbar_arrive(&sh.seg_full[i % kQueue]);
+        }
+        if (!have) break;
+        ++i;
       }
-      if (cut.b >= 0 && start >= u0 - range_tiles)
-        cut.parts = (int)((start + n - 1) / range_tiles) - (int)(start / range_tiles) + 1;
-    }
-    if (lane == 0) w.cuts[blockIdx.x] = cut;
-  } else if (warp == 8) {
+      // ---- the group that this range starts inside of, for cache_join_kernel
+      Cut cut{-1, 0, 0, 0};
+      if (u0 < u1 && blockIdx.x > 0 && !w.whole) {
+        int g1, q, g2, n1, n2;
+        place<R>(p, sh.seq, u0 - sh.base, g1, q, g2, n1, n2);
+        int64_t start = u0 - q + kSetup;         // where the group's first tile counts
+        int n = 0;
+        if (q > kSetup && q < kSetup + n1) {
+          cut.b = sh.b; cut.g = g1; n = n1;
+        } else if (n2 > 0 && q > 2 * kSetup + n1 && q < 2 * kSetup + n1 + n2) {
+          cut.b = sh.b; cut.g = g2; start += kSetup + n1; n = n2;
+        }
+        if (cut.b >= 0 && start >= u0 - range_tiles)
+          cut.parts = (int)((start + n - 1) / range_tiles) - (int)(start / range_tiles) + 1;
+      }
+      if (lane == 0 && !w.whole) w.cuts[blockIdx.x] = cut;
+      __syncwarp();
+    } else if (warp == 8) {
     // ======== loads: boxes of one page (at most 128 positions) x 128 bytes into a
     // ring of 16 KB chunks; a tile is its rope chunk, then its code chunks
     int slot = 0, round = 0, issued = 0;
     const int box_rows = min(p.page_size, TILE), boxes = TILE / box_rows;
     bool ok = true;
-    while (ok && walk.next(seg)) {
-      const int seen = seen_by(p, walk.s, seg.g * R + R - 1);
-      if (seen == 0) continue;
+    Info seg;
+    while (ok && take(seg, true) > 0) {
       for (int t = seg.t0; t < seg.t1 && ok; ++t) {
         const int pos = t * TILE;
-        const int nbox = min(boxes, (seen - pos + box_rows - 1) / box_rows);
+        const int nbox = min(boxes, (seg.seen - pos + box_rows - 1) / box_rows);
         int page = p.num_pages;                 // outside: the copy fills in zeros
         if (lane < nbox) {
           const int x = page_of(p, seg.b, pos + lane * box_rows);
@@ -603,96 +685,98 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     }
     if (*ab) {                                  // copies in flight land before the block ends
       for (int i = max(0, issued - ring); i < issued; ++i) {
-        const uint64_t t0 = ptx::globaltimer_ns();
-        while (!ptx::mbar_try_wait(&sh.full[i % ring], (i / ring) & 1) &&
-               ptx::globaltimer_ns() - t0 < kWaitNs) {
-        }
+        drain(&sh.full[i % ring], (i / ring) & 1);
       }
     }
     __syncwarp();
   } else if (warp == 9) {
-    // ======== MMA issue: S of tile k + 1 ahead of O of tile k
-    {
-      constexpr uint32_t kHalf = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-      constexpr uint32_t id_s = idesc(NS, false, false, kE4M3, kE4M3);
-      constexpr uint32_t id_o = idesc(NO, true, true, kE4M3, F::FMT);
-      constexpr uint32_t id_r = idesc(R, false, false, kHalf, kHalf);
-      const uint32_t sm0 = ptx::smem_u32(sm);
-      const uint64_t dq = sdesc_sw128(ptx::smem_u32(q_s)), dqr = sdesc_sw128(ptx::smem_u32(qr_s));
-      // P: 16 rows x 8 positions a core matrix, 128 bytes on along the positions,
-      // 2048 along the rows
-      const uint64_t dp = ptx::sdesc(ptx::smem_u32(p_s), 128, TILE * 16);
-      int k = 0, segs = 0;
-      int slot = 0, round = 0;                  // of the next chunk that S reads
-      int oslot = 0;                            // of the next chunk that O reads
-      bool ok = true;
-      auto issue_o = [&](int i, bool first) {   // O += codes^T P of tile i
-        const int par = i & 1;
-        if (!wait(&sh.p_full[par], (i >> 1) & 1, ab)) return false;
+    // ======== S^T = codes Q^T, a tile or two ahead of the softmax.  (Two warps issue the
+    // two products: one warp issues more slowly than the products execute, and would
+    // hold back the scores of a tile behind the wait for another's weights.)
+    constexpr uint32_t kHalf = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    constexpr uint32_t id_s = idesc(NS, false, false, kE4M3, kE4M3);
+    constexpr uint32_t id_r = idesc(R, false, false, kHalf, kHalf);
+    const uint32_t dq = sw128_lo(ptx::smem_u32(q_s)), dqr = sw128_lo(ptx::smem_u32(qr_s));
+    const uint32_t dk0 = sw128_lo(ptx::smem_u32(sm)), ts = (uint32_t)uniform((int)tm_s);
+    int k = 0, segs = 0, slot = 0, round = 0;
+    bool ok = true;
+    Info seg;
+    while (ok && uniform(take(seg, true)) > 0) {
+      const int tiles = uniform(seg.t1 - seg.t0);
+      if (!wait(&sh.q_ready, segs & 1, ab)) break;
+      ++segs;
+      for (int t = 0; t < tiles; ++t, ++k) {
+        const int before = k - C::SBUF;         // the tile whose scores were here
+        if (before >= 0 && !wait(&sh.s_empty[before & 1], (before >> 1) & 1, ab)) { ok = false; break; }
+        const uint32_t d = ts + (C::SBUF == 2 ? (k & 1) * NS : 0);
+        const int rope_slot = slot;
+        if (p.DR) {
+          if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
+          if (++slot == ring) { slot = 0; ++round; }
+        }
+        for (int c = 0; c < NCH; ++c) {
+          if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
+          ptx::tc_fence_after();
+          const uint32_t dk = dk0 + slot * (CHUNK >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dq + ((c * NS * 128 + kk * 32) >> 4), id_s,
+                                       c + kk > 0);
+          if (++slot == ring) { slot = 0; ++round; }
+        }
+        if (!ok) break;
+        if (p.DR) {
+          const uint32_t dk = dk0 + rope_slot * (CHUNK >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_half<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dqr + ((kk * 32) >> 4), id_r);
+          commit(&sh.empty[rope_slot]);
+        }
+        commit(&sh.s_full[k & 1]);
+      }
+    }
+    if (*ab) {                                  // products in flight end before TMEM is freed
+      commit(&sh.drain[0]);
+      drain(&sh.drain[0], 0);
+    }
+    __syncwarp();
+  } else if (warp == 11) {
+    // ======== O^T += codes^T P^T
+    constexpr uint32_t id_o = idesc(NO, true, true, kE4M3, F::FMT);
+    const uint32_t dp = p_lo(ptx::smem_u32(p_s)), dk0 = sw128_lo(ptx::smem_u32(sm));
+    const uint32_t to = (uint32_t)uniform((int)tmem);
+    int k = 0, slot = 0;
+    bool ok = true;
+    Info seg;
+    while (ok && uniform(take(seg, true)) > 0) {
+      const int tiles = uniform(seg.t1 - seg.t0);
+      for (int t = 0; t < tiles; ++t, ++k) {
+        const int par = k & 1;
+        if (!wait(&sh.p_full[par], (k >> 1) & 1, ab)) { ok = false; break; }
         ptx::tc_fence_after();
-        if (p.DR && ++oslot == ring) oslot = 0;
-        uint64_t dv[NCH];
+        if (p.DR && ++slot == ring) slot = 0;
+        uint32_t dv[NCH];
         int at[NCH];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-          at[c] = oslot;
-          dv[c] = sdesc_sw128(sm0 + oslot * CHUNK);
-          if (++oslot == ring) oslot = 0;
+          at[c] = slot;
+          dv[c] = dk0 + slot * (CHUNK >> 4);
+          if (++slot == ring) slot = 0;
         }
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+        for (int c = 0; c < NCH; ++c) {
 #pragma unroll
-          for (int c = 0; c < NCH; ++c)
-            mma_f8(tmem + c * NO, dv[c] + ((kk * 4096) >> 4),
-                      dp + ((par * NO * 128 + kk * 512) >> 4), id_o, !(first && kk == 0));
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) commit(&sh.empty[at[c]]);
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8<kSw128Hi, kPHi>(to + c * NO, dv[c] + ((kk * 4096) >> 4),
+                                   dp + ((par * NO * 128 + kk * 512) >> 4), id_o, t > 0 || kk > 0);
+          commit(&sh.empty[at[c]]);
+        }
         commit(&sh.o_done[par]);
-        return true;
-      };
-      while (ok && walk.next(seg)) {
-        if (seen_by(p, walk.s, seg.g * R + R - 1) == 0) continue;
-        if (!wait(&sh.q_ready, segs & 1, ab)) break;
-        ++segs;
-        for (int t = seg.t0; t < seg.t1; ++t) {
-          const int before = k - C::SBUF;       // the tile whose scores were here
-          if (before >= 0 && !wait(&sh.s_empty[before & 1], (before >> 1) & 1, ab)) { ok = false; break; }
-          const uint32_t d = tm_s + (C::SBUF == 2 ? (k & 1) * NS : 0);
-          const int rope_slot = slot;
-          if (p.DR) {
-            if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
-            if (++slot == ring) { slot = 0; ++round; }
-          }
-          for (int c = 0; c < NCH; ++c) {
-            if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
-            ptx::tc_fence_after();
-            const uint64_t dk = sdesc_sw128(sm0 + slot * CHUNK);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_f8(d, dk + ((kk * 32) >> 4), dq + ((c * NS * 128 + kk * 32) >> 4), id_s,
-                        c + kk > 0);
-            if (++slot == ring) { slot = 0; ++round; }
-          }
-          if (!ok) break;
-          if (p.DR) {
-            const uint64_t dk = sdesc_sw128(sm0 + rope_slot * CHUNK);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_half(d, dk + ((kk * 32) >> 4), dqr + ((kk * 32) >> 4), id_r);
-            commit(&sh.empty[rope_slot]);
-          }
-          commit(&sh.s_full[k & 1]);
-          if (t > seg.t0 && !issue_o(k - 1, t - 1 == seg.t0)) { ok = false; break; }
-          ++k;
-        }
-        if (ok) ok = issue_o(k - 1, seg.t1 - 1 == seg.t0);
       }
-      if (*ab) {                                // products in flight end before TMEM is freed
-        commit(&sh.drain);
-        const uint64_t t0 = ptx::globaltimer_ns();
-        while (!ptx::mbar_try_wait(&sh.drain, 0) && ptx::globaltimer_ns() - t0 < kWaitNs) {
-        }
-      }
+    }
+    if (*ab) {
+      commit(&sh.drain[1]);
+      drain(&sh.drain[1], 0);
     }
     __syncwarp();
   }
@@ -700,7 +784,6 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     // ======== softmax: two groups of four warps have half of the rows each; thread =
     // position of the tile = TMEM lane
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1, w.whole);
     constexpr int HR = R / 2;                   // rows of a group
     const int wg = warp >> 2, rb = wg * HR;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -709,34 +792,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     bool failed = false;
     auto o_done = [&](int i) { return wait(&sh.o_done[i & 1], (i >> 1) & 1, ab); };   // products of tile i
 
-    // ---- the next segment that sees anything
-    struct Info : Segment {
-      int row0, rows, first, off;               // its rows, its sequence's new tokens
-      int seen, seen0;                          // positions that its last and first row see
-    };
-    auto next_segment = [&](Info& sg) {
-      while (walk.next(sg)) {
-        const int row0 = sg.g * R, rows = (int)min((int64_t)R, (int64_t)walk.s.n * p.H - row0);
-        const int first = walk.s.first;
-        sg.row0 = row0;
-        sg.rows = rows;
-        sg.first = first;
-        sg.off = walk.s.off;
-        sg.seen = seen_by(p, walk.s, row0 + R - 1);
-        sg.seen0 = seen_by(p, walk.s, row0);
-        if (tid == 0 && sg.off + walk.s.n > walk.s.cap) atomicExch(&g_attn_device_error, kErrOutside);
-        if (sg.seen > 0) return true;
-        for (int r = warp; r < rows; r += 8) {
-          const int i = div_heads(p, row0 + r);
-          const int64_t n = first + i, h = row0 + r - i * p.H;
-          T* o = static_cast<T*>(p.out) + n * p.o_s[0] + h * p.o_s[1];
-          for (int c = lane; c < p.KVL; c += 32) st(o + c, 0.f);
-          if (lane == 0 && p.lse) p.lse[n * p.lse_s + h] = -INFINITY;
-        }
-      }
-      return false;
-    };
-    // ---- its loads: the queries, the pages of this thread's first two positions
+    // ---- a segment's loads: the queries, the pages of this thread's first two positions
     constexpr int RW = R / 8;                   // rows of a warp: warp + 8 i
     uint2 raw[RW][NCH];                         // channels 128 c + 4 lane + j
     uint32_t raw_r[RW];                         // rope 2 lane + j
@@ -744,7 +800,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       const int pos = t * TILE + tt;
       return t < sg.t1 && pos < sg.seen ? page_of(p, sg.b, pos) : -2;
     };
-    int page_first, page_second;
+    int page_first = -2, page_second = -2;
     auto fetch = [&](const Info& sg) {
       page_first = page_at(sg, sg.t0);
       page_second = page_at(sg, sg.t0 + 1);
@@ -839,23 +895,24 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       return p.scales[(int64_t)page * p.scales_s + ((t * TILE + tt) & (p.page_size - 1))];
     };
 
+    // Each round: the next segment's loads, this segment's tiles, the next one's queries
+    // (so that its scores are under way meanwhile), this one's result.
     Info seg, nseg;
-    bool have = next_segment(seg);
+    bool have = false;
     float s_first = 1.f;
-    if (have) {
-      fetch(seg);
-      write_queries(seg, sh.rows[0]);
-      s_first = scale_at(seg.t0, page_first);
-    }
-    for (int si = 0; have; ++si) {
+    for (int si = 1;; ++si) {
+      const int took = take(nseg, false);
+      const bool have_next = took > 0;
+      if (took < 0) failed = true;
+      float s_next = s_first;
+      int page_next = page_second;
+      if (have_next) fetch(nseg);
       Rows<R>& rw = sh.rows[si & 1];
       const float *q_scale = rw.q_scale + rb, *m = rw.m + rb, *alpha = rw.alpha + rb;
       const int* sees = rw.seen + rb;
-      bool have_next = false;
-      float s_next = s_first;
-      int page_next = page_second;
-      float ls_next = log2f(s_next), rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
       float l[HR];
+      if (have) {
+      float ls_next = log2f(s_next), rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
 #pragma unroll
       for (int r = 0; r < HR; ++r) l[r] = 0.f;
       ptx::tc_fence_before();
@@ -978,22 +1035,15 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         ptx::mbar_arrive(&sh.p_full[par]);
         ls_next = log2f(s_next);
         rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
-        if (R == 16 && start) {
-          have_next = next_segment(nseg);
-          if (have_next) fetch(nseg);
-        }
       }
-      if (R != 16) {
-        have_next = next_segment(nseg);
-        if (have_next) fetch(nseg);
       }
-      // ---- the next segment's queries, so that its scores are under way while this
-      // one's result is written
-      bar_sync(3, 256);                         // the scores have all been read
-      if (have_next && !failed) {
+      failed = ptx::bar_red_or(3, 256, failed);  // the scores have all been read
+      if (failed) break;
+      if (have_next) {
         s_first = scale_at(nseg.t0, page_first);
         write_queries(nseg, sh.rows[(si + 1) & 1]);
       }
+      if (have) {
       // ---- the segment's result
       const float sum = warp_sums<HR>(l, lane);
       if (lane < HR) sh.red[warp][lane] = sum;
@@ -1054,8 +1104,10 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
             if (rb + r < seg.rows) part[r * p.KVL] = o[r];
         }
       }
+      }
+      if (!have_next) break;
       seg = nseg;
-      have = have_next;
+      have = true;
     }
   }
   ptx::tc_fence_before();
@@ -1170,6 +1222,12 @@ int device_sms() {
 }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Contexts that a block goes through about as fast as it would join parts of them
+// stay whole: no workspace and no second launch.
+bool whole_groups(const CacheParams& p) {
+  return (int64_t)p.max_pages * p.page_size <= kWholeTiles * TILE;
+}
+
 // Rows per group: 16 where the sequences of the call have no more rows than that
 // on average, or where 32 rows leave too small a ring; else 32.
 int rows_per_group(const CacheParams& p, int q_terms) {
@@ -1186,9 +1244,6 @@ cudaError_t launch(const CacheParams& p, Work w, const CUtensorMap& mc, const CU
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
   if (e != cudaSuccess) return e;
   const size_t smem = fixed_bytes(p.KVL, C::NQ, R) + w.ring * CHUNK;
-  // Contexts that a block goes through about as fast as it would join parts of them
-  // stay whole, and the second launch goes.
-  w.whole = (int64_t)p.max_pages * p.page_size <= kWholeTiles * TILE;
   e = launch_dependent(k, dim3(ranges), kThreads, smem, s, p, w, mc, mr);
   if (e != cudaSuccess || w.whole) return e;
   return launch_dependent(cache_join_kernel<T, R>, dim3(ranges - 1, R), kJoinThreads, 0, s, p, w);
@@ -1224,6 +1279,7 @@ bool encode(CUtensorMap* m, CUtensorMapDataType dt, int elt, void* base, int wid
 
 // partials | their log sums | cuts
 size_t attention_workspace_bytes(const CacheParams& p) {
+  if (whole_groups(p)) return 0;
   const size_t ranges = device_sms(), R = 32;
   return align256(2 * ranges * R * p.KVL * 4) + align256(2 * ranges * R * 4) +
          align256(ranges * sizeof(Cut));
@@ -1234,6 +1290,7 @@ cudaError_t launch_attention(const CacheParams& p, int io_dtype, void* workspace
   const int R = rows_per_group(p, io_dtype == KDA_DTYPE_F16 ? kQTerms<__half> : kQTerms<__nv_bfloat16>);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Work w{};
+  w.whole = whole_groups(p);
   w.part = reinterpret_cast<float*>(ws);
   ws += align256((size_t)2 * ranges * R * p.KVL * 4);
   w.lse2 = reinterpret_cast<float*>(ws);

@@ -104,7 +104,7 @@ class LatentCache:
             raise RuntimeError(f"{fn}: {pages} pages of {page} tokens not supported (page_size a "
                                f"power of two from 16 to 1024, fewer than 2^31 tokens)")
         self.codes, self.scales, self.rope = codes, scales, rope
-        self.dtype, self.device = dtype, codes.device
+        self.dtype, self.device, self.on_gpu = dtype, codes.device, codes.is_cuda
         self.num_pages, self.page_size, self.kv_lora_rank, self.rope_dim = pages, page, kvl, dr
         a = _lib.MlaCacheArgs()
         a.abi_version = _lib.ABI_VERSION
@@ -162,7 +162,7 @@ def _is_index(t, dims, dev):
 def _args(fn, cache, block_table, lens, q_start, N):
     """The argument block with the pool, the table and the lengths filled in."""
     dev = cache.device
-    if dev.type != "cuda" or not _is_index(block_table, 2, dev) or not _is_index(lens, 1, dev) or \
+    if not cache.on_gpu or not _is_index(block_table, 2, dev) or not _is_index(lens, 1, dev) or \
             (q_start is not None and not _is_index(q_start, 1, dev)):
         _refuse_index(fn, cache, block_table, lens, q_start)
     B = lens.shape[0]
@@ -238,7 +238,7 @@ def latent_read(cache, block_table, lens, num_tokens, q_start=None):
     k_rope = None
     a.c_kv, a.c_kv_stride = c_kv.data_ptr(), cache.kv_lora_rank
     if cache.rope is not None:
-        k_rope = torch.empty((N, cache.rope_dim), dtype=cache.dtype, device=dev)
+        k_rope = cache.rope.new_empty((N, cache.rope_dim))
         a.k_rope, a.k_rope_stride = k_rope.data_ptr(), cache.rope_dim
     if N:
         _launch(fn, _lib.load().mla_cache_read, a, dev)
@@ -272,8 +272,8 @@ def latent_attention(q_lat, cache, block_table, lens, scale, q_start=None, q_rop
         raise RuntimeError(f"{fn}: q_rope must be given exactly when the cache has a rope part")
     a = _args(fn, cache, block_table, lens, q_start, N)
     dev = cache.device
-    out = torch.empty((N, H, kvl), dtype=cache.dtype, device=dev)
-    lse = torch.empty((N, H), dtype=torch.float32, device=dev) if return_lse else None
+    out = q_lat.new_empty((N, H, kvl))
+    lse = cache.scales.new_empty((N, H)) if return_lse else None
     if N and H:
         if q_lat.stride(2) != 1:
             q_lat = q_lat.contiguous()
@@ -296,7 +296,7 @@ def latent_attention(q_lat, cache, block_table, lens, scale, q_start=None, q_rop
         lib = _lib.load()
         need = lib.mla_cache_workspace_bytes(ctypes.byref(a))
         if need:
-            ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+            ws = lens.new_empty((-(-need // 4),))
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         _launch(fn, lib.mla_cache_attention, a, dev)
     return (out, lse) if return_lse else out
