@@ -48,7 +48,6 @@ constexpr int kThreads = 384;              // warps 0-7 softmax, 8 loads, 9 S, 1
 // others keep 120 (256 x 192 + 128 x 120 = 384 x 168).
 constexpr int kSoftmaxRegs = 192, kOtherRegs = 120;
 
-constexpr int kMaxRing = 14;
 constexpr int kWholeTiles = 4;             // contexts of at most so many tiles are not split
 constexpr int kMaxRanges = 256;            // blocks (SMs) that a call's tiles are cut over
 constexpr int kSmemMax = 232448;           // 227 KB per block
@@ -122,17 +121,17 @@ struct Cfg {
 };
 
 // Shared memory besides the ring (barriers and rows; 1 KB: alignment), and the
-// chunks that fit beside it.  The order of the products needs the codes of one
-// tile and all of the next at once.
+// chunks that fit beside it, four tiles of them at most.  The order of the products
+// needs the chunks of two tiles at once.
 constexpr int kSharedBytes = 4096;
 int fixed_bytes(int kvl, int q_terms, int R) {
   return kSharedBytes + 1024 + q_terms * R * kvl + R * 128 + 2 * NP * R * 128;
 }
-int ring_chunks(int kvl, int q_terms, int R) {
+int tile_chunks(int kvl, int dr) { return kvl / 128 + (dr ? 1 : 0); }
+int ring_chunks(int kvl, int dr, int q_terms, int R) {
   const int n = (kSmemMax - fixed_bytes(kvl, q_terms, R)) / CHUNK;
-  return n < kMaxRing ? n : kMaxRing;
+  return min(n, 4 * tile_chunks(kvl, dr));
 }
-int ring_least(int kvl, int dr) { return 2 * (kvl / 128) + (dr ? 1 : 0); }
 
 // Where a range of tiles starts inside a group; what cache_join_kernel reads.
 struct Cut {
@@ -327,6 +326,25 @@ __device__ __forceinline__ uint32_t sw128_lo(uint32_t saddr) { return (saddr >> 
 // no swizzle: core matrices of 8 x 16 bytes, 128 bytes on along K, 2048 along N
 constexpr uint32_t kPHi = (TILE * 16 >> 4) | (1u << 14);
 __device__ __forceinline__ uint32_t p_lo(uint32_t saddr) { return (saddr >> 4) | ((128 >> 4) << 16); }
+// One lane of the warp: bytes to expect on a barrier, and a box of a tensor map.
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 x;\n\t"
+      "elect.sync x|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                         uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 x;\n\t"
+      "elect.sync x|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
 // Instruction descriptors: fp32 accumulator; 8-bit formats 0 = e4m3, 1 = e5m2, 16-bit
 // ones 0 = f16, 1 = bf16
 __host__ __device__ constexpr uint32_t idesc(int N, bool a_m_major, bool b_n_major, uint32_t a_fmt,
@@ -431,8 +449,8 @@ constexpr int kQueue = 4;  // segments that are known ahead
 
 template <int R>
 struct Shared {            // at the end of dynamic shared memory
-  uint64_t full[kMaxRing], empty[kMaxRing], seg_full[kQueue], seg_empty[kQueue];
-  uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], q_ready, drain[2];
+  uint64_t full[8], freed[8], seg_full[kQueue], seg_empty[kQueue];   // full, freed: half tile % 8
+  uint64_t s_full[2], s_empty[2], p_full[2], q_ready, drain[2];      // tile % 2
   uint32_t tmem;
   int abort_flag;
   int64_t scan[(kThreads + 31) / 32];
@@ -506,17 +524,18 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   Shared<R>& sh = *reinterpret_cast<Shared<R>*>(p_s + 2 * NO * 128);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int ring = w.ring, tile_chunks = NCH + (p.DR ? 1 : 0);
+  constexpr int HC = (NCH + 1) / 2;             // code chunks of a tile's first half
+  const int half = tile_chunks - NCH + HC;      // chunks of it
 
   if (tid == 0) {
-    for (int i = 0; i < ring; ++i) {
+    for (int i = 0; i < 8; ++i) {
       ptx::mbar_init(&sh.full[i], 1);
-      ptx::mbar_init(&sh.empty[i], 1);
+      ptx::mbar_init(&sh.freed[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&sh.s_full[i], 1);
       ptx::mbar_init(&sh.s_empty[i], 256);
       ptx::mbar_init(&sh.p_full[i], 256);
-      ptx::mbar_init(&sh.o_done[i], 1);
     }
     for (int i = 0; i < kQueue; ++i) {
       ptx::mbar_init(&sh.seg_full[i], 1);
@@ -654,39 +673,55 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       __syncwarp();
     } else if (warp == 8) {
     // ======== loads: boxes of one page (at most 128 positions) x 128 bytes into a
-    // ring of 16 KB chunks; a tile is its rope chunk, then its code chunks
-    int slot = 0, round = 0, issued = 0;
+    // ring of 16 KB chunks; a tile is its rope chunk, then its code chunks, in two halves
+    // that land and are freed apart.  (A look at a barrier takes some 300 cycles while
+    // the products read shared memory: one for each chunk was too many, one for a whole
+    // tile keeps the chunks waiting for one another.)
+    const int ahead = ring / tile_chunks, spare = ring % tile_chunks;
     const int box_rows = min(p.page_size, TILE), boxes = TILE / box_rows;
+    const uint32_t sm0 = ptx::smem_u32(sm);
+    int k = 0, slot = 0, freed = -1;            // freed: half tiles known to be
     bool ok = true;
     Info seg;
-    while (ok && take(seg, true) > 0) {
-      for (int t = seg.t0; t < seg.t1 && ok; ++t) {
-        const int pos = t * TILE;
-        const int nbox = min(boxes, (seg.seen - pos + box_rows - 1) / box_rows);
-        int page = p.num_pages;                 // outside: the copy fills in zeros
-        if (lane < nbox) {
-          const int x = page_of(p, seg.b, pos + lane * box_rows);
-          if (x >= 0) page = x;
-        }
+    while (ok && uniform(take(seg, true)) > 0) {
+      const int t1 = uniform(seg.t1), seen = uniform(seg.seen);
+      // lane i: page of box i of a tile
+      auto page_of_box = [&](int t) {
+        const int pos = t * TILE + lane * box_rows, i = pos >> p.page_shift;
+        int x = -1;
+        if (lane < boxes && t < t1 && pos < seen && i < p.max_pages)
+          x = p.table[(int64_t)seg.b * p.table_s + i];
+        return x;
+      };
+      int page_next = page_of_box(seg.t0);
+      for (int t = uniform(seg.t0); t < t1 && ok; ++t, ++k) {
+        // outside the pool: the copy fills in zeros
+        const int page = (uint32_t)page_next < (uint32_t)p.num_pages ? page_next : p.num_pages;
+        page_next = page_of_box(t + 1);
+        const int pos = t * TILE, nbox = min(boxes, (seen - pos + box_rows - 1) / box_rows);
         const int at = p.page_size > TILE ? pos & (p.page_size - 1) : 0;
-        for (int c = p.DR ? -1 : 0; c < NCH; ++c) {
-          if (round > 0 && !wait(&sh.empty[slot], (round - 1) & 1, ab)) { ok = false; break; }
-          if (lane == 0) ptx::mbar_arrive_expect_tx(&sh.full[slot], nbox * box_rows * 128);
-          __syncwarp();
-          uint8_t* dst = sm + slot * CHUNK + lane * box_rows * 128;
-          if (lane < nbox) {
-            if (c < 0) ptx::tma_load_3d(dst, &map_rope, 0, at, page, &sh.full[slot]);
-            else ptx::tma_load_3d(dst, &map_codes, c * 128, at, page, &sh.full[slot]);
+        const uint32_t bar = ptx::smem_u32(&sh.full[2 * (k & 3)]);
+        expect_bytes(bar, nbox * box_rows * 128 * half);
+        expect_bytes(bar + 8, nbox * box_rows * 128 * (tile_chunks - half));
+        for (int c = 0; c < tile_chunks; ++c) {
+          // whose place this chunk takes: chunk `old` of tile j
+          const int j = k - ahead - (c < spare), old = c - spare + (c < spare ? tile_chunks : 0);
+          const int need = 2 * j + (old >= half);
+          if (j >= 0 && need > freed) {
+            if (!wait(&sh.freed[need & 7], (need >> 3) & 1, ab)) { ok = false; break; }
+            freed = need;
           }
-          ++issued;
-          if (++slot == ring) { slot = 0; ++round; }
+          const int code = c - (tile_chunks - NCH);
+          const CUtensorMap* map = code < 0 ? &map_rope : &map_codes;
+          for (int i = 0; i < nbox; ++i)
+            load_box(sm0 + slot * CHUNK + i * box_rows * 128, map, max(code, 0) * 128, at,
+                     __shfl_sync(0xffffffffu, page, i), bar + 8 * (c >= half));
+          if (++slot == ring) slot = 0;
         }
       }
     }
     if (*ab) {                                  // copies in flight land before the block ends
-      for (int i = max(0, issued - ring); i < issued; ++i) {
-        drain(&sh.full[i % ring], (i / ring) & 1);
-      }
+      for (int i = max(0, 2 * k - 6); i <= 2 * k + 1; ++i) drain(&sh.full[i & 7], (i >> 3) & 1);
     }
     __syncwarp();
   } else if (warp == 9) {
@@ -698,7 +733,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     constexpr uint32_t id_r = idesc(R, false, false, kHalf, kHalf);
     const uint32_t dq = sw128_lo(ptx::smem_u32(q_s)), dqr = sw128_lo(ptx::smem_u32(qr_s));
     const uint32_t dk0 = sw128_lo(ptx::smem_u32(sm)), ts = (uint32_t)uniform((int)tm_s);
-    int k = 0, segs = 0, slot = 0, round = 0;
+    int k = 0, segs = 0, slot = 0;
     bool ok = true;
     Info seg;
     while (ok && uniform(take(seg, true)) > 0) {
@@ -710,19 +745,19 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         if (before >= 0 && !wait(&sh.s_empty[before & 1], (before >> 1) & 1, ab)) { ok = false; break; }
         const uint32_t d = ts + (C::SBUF == 2 ? (k & 1) * NS : 0);
         const int rope_slot = slot;
-        if (p.DR) {
-          if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
-          if (++slot == ring) { slot = 0; ++round; }
-        }
+        if (p.DR && ++slot == ring) slot = 0;
+#pragma unroll
         for (int c = 0; c < NCH; ++c) {
-          if (!wait(&sh.full[slot], round & 1, ab)) { ok = false; break; }
-          ptx::tc_fence_after();
+          if (c == 0 || c == HC) {
+            if (!wait(&sh.full[2 * (k & 3) + (c == HC)], (k >> 2) & 1, ab)) { ok = false; break; }
+            ptx::tc_fence_after();
+          }
           const uint32_t dk = dk0 + slot * (CHUNK >> 4);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             mma_f8<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dq + ((c * NS * 128 + kk * 32) >> 4), id_s,
                                        c + kk > 0);
-          if (++slot == ring) { slot = 0; ++round; }
+          if (++slot == ring) slot = 0;
         }
         if (!ok) break;
         if (p.DR) {
@@ -730,7 +765,6 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             mma_half<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dqr + ((kk * 32) >> 4), id_r);
-          commit(&sh.empty[rope_slot]);
         }
         commit(&sh.s_full[k & 1]);
       }
@@ -755,23 +789,17 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         if (!wait(&sh.p_full[par], (k >> 1) & 1, ab)) { ok = false; break; }
         ptx::tc_fence_after();
         if (p.DR && ++slot == ring) slot = 0;
-        uint32_t dv[NCH];
-        int at[NCH];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-          at[c] = slot;
-          dv[c] = dk0 + slot * (CHUNK >> 4);
-          if (++slot == ring) slot = 0;
-        }
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
+          const uint32_t dv = dk0 + slot * (CHUNK >> 4);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_f8<kSw128Hi, kPHi>(to + c * NO, dv[c] + ((kk * 4096) >> 4),
+            mma_f8<kSw128Hi, kPHi>(to + c * NO, dv + ((kk * 4096) >> 4),
                                    dp + ((par * NO * 128 + kk * 512) >> 4), id_o, t > 0 || kk > 0);
-          commit(&sh.empty[at[c]]);
+          if (++slot == ring) slot = 0;
+          if (c == HC - 1) commit(&sh.freed[2 * (k & 3)]);
         }
-        commit(&sh.o_done[par]);
+        commit(&sh.freed[2 * (k & 3) + 1]);
       }
     }
     if (*ab) {
@@ -790,7 +818,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     const int tt = tid & 127;
     int k = 0;
     bool failed = false;
-    auto o_done = [&](int i) { return wait(&sh.o_done[i & 1], (i >> 1) & 1, ab); };   // products of tile i
+    auto o_done = [&](int i) { return wait(&sh.freed[2 * (i & 3) + 1], (i >> 2) & 1, ab); };   // of tile i
 
     // ---- a segment's loads: the queries, the pages of this thread's first two positions
     constexpr int RW = R / 8;                   // rows of a warp: warp + 8 i
@@ -1232,7 +1260,7 @@ bool whole_groups(const CacheParams& p) {
 // on average, or where 32 rows leave too small a ring; else 32.
 int rows_per_group(const CacheParams& p, int q_terms) {
   if (((int64_t)p.N * p.H + p.B - 1) / p.B <= 16) return 16;
-  return ring_chunks(p.KVL, q_terms, 32) >= ring_least(p.KVL, p.DR) ? 32 : 16;
+  return ring_chunks(p.KVL, p.DR, q_terms, 32) >= 2 * tile_chunks(p.KVL, p.DR) ? 32 : 16;
 }
 
 template <typename T, int R, int NCH>
@@ -1240,7 +1268,7 @@ cudaError_t launch(const CacheParams& p, Work w, const CUtensorMap& mc, const CU
                    int ranges, cudaStream_t s) {
   using C = Cfg<T, R, NCH>;
   auto k = cache_attn_kernel<T, R, NCH>;
-  w.ring = ring_chunks(p.KVL, C::NQ, R);
+  w.ring = ring_chunks(p.KVL, p.DR, C::NQ, R);
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
   if (e != cudaSuccess) return e;
   const size_t smem = fixed_bytes(p.KVL, C::NQ, R) + w.ring * CHUNK;
