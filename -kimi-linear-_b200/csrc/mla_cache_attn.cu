@@ -135,9 +135,10 @@ int ring_chunks(int kvl, int dr, int q_terms, int R) {
 
 // Where a range of tiles starts inside a group; what cache_join_kernel reads.
 struct Cut {
-  int b, g;        // the group that the range starts in the middle of (b < 0: none)
-  int parts;       // ranges that share the group; 0: an earlier cut joins it
-  int pad;
+  int parts;       // ranges that share the group that the range starts in the middle of
+                   // (0: none, or an earlier cut joins it)
+  int row0, rows;  // the group's rows
+  int first;       // its sequence's first new token
 };
 
 struct Work {
@@ -655,19 +656,22 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         ++i;
       }
       // ---- the group that this range starts inside of, for cache_join_kernel
-      Cut cut{-1, 0, 0, 0};
+      Cut cut{0, 0, 0, 0};
+      int cut_g = -1;
       if (u0 < u1 && blockIdx.x > 0 && !w.whole) {
         int g1, q, g2, n1, n2;
         place<R>(p, sh.seq, u0 - sh.base, g1, q, g2, n1, n2);
         int64_t start = u0 - q + kSetup;         // where the group's first tile counts
         int n = 0;
         if (q > kSetup && q < kSetup + n1) {
-          cut.b = sh.b; cut.g = g1; n = n1;
+          cut_g = g1; n = n1;
         } else if (n2 > 0 && q > 2 * kSetup + n1 && q < 2 * kSetup + n1 + n2) {
-          cut.b = sh.b; cut.g = g2; start += kSetup + n1; n = n2;
+          cut_g = g2; start += kSetup + n1; n = n2;
         }
-        if (cut.b >= 0 && start >= u0 - range_tiles)
-          cut.parts = (int)((start + n - 1) / range_tiles) - (int)(start / range_tiles) + 1;
+        if (cut_g >= 0 && start >= u0 - range_tiles) {
+          cut = Cut{(int)((start + n - 1) / range_tiles) - (int)(start / range_tiles) + 1, cut_g * R,
+                    (int)min((int64_t)R, (int64_t)sh.seq.n * p.H - cut_g * R), sh.seq.first};
+        }
       }
       if (lane == 0 && !w.whole) w.cuts[blockIdx.x] = cut;
       __syncwarp();
@@ -824,14 +828,16 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     constexpr int RW = R / 8;                   // rows of a warp: warp + 8 i
     uint2 raw[RW][NCH];                         // channels 128 c + 4 lane + j
     uint32_t raw_r[RW];                         // rope 2 lane + j
+    // (a table entry as it is, so that nothing waits for it here; kNoPage: not needed)
+    constexpr int kNoPage = -0x7fffffff;
     auto page_at = [&](const Info& sg, int t) {
-      const int pos = t * TILE + tt;
-      return t < sg.t1 && pos < sg.seen ? page_of(p, sg.b, pos) : -2;
+      const int pos = t * TILE + tt, i = pos >> p.page_shift;
+      int x = kNoPage;
+      if (t < sg.t1 && pos < sg.seen) x = i < p.max_pages ? p.table[(int64_t)sg.b * p.table_s + i] : -1;
+      return x;
     };
-    int page_first = -2, page_second = -2;
+    int page_first = kNoPage, page_second = kNoPage;
     auto fetch = [&](const Info& sg) {
-      page_first = page_at(sg, sg.t0);
-      page_second = page_at(sg, sg.t0 + 1);
       const T *ql[RW], *qr[RW];
 #pragma unroll
       for (int i = 0; i < RW; ++i) {            // (rows past the end: the last one's)
@@ -860,6 +866,8 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           if (p.DR) raw_r[i] = bits(qr[i]) | bits(qr[i] + 1) << 16;
         }
       }
+      page_first = page_at(sg, sg.t0);
+      page_second = page_at(sg, sg.t0 + 1);
     };
     // ---- its queries, scaled by a power of two and split into e4m3 terms (rows past
     // the end: zeros), and its rows' figures
@@ -915,8 +923,8 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       ptx::mbar_arrive(&sh.q_ready);
     };
     auto scale_at = [&](int t, int page) {
-      if (page == -2) return 1.f;
-      if (page < 0) {
+      if (page == kNoPage) return 1.f;
+      if ((uint32_t)page >= (uint32_t)p.num_pages) {
         atomicExch(&g_attn_device_error, kErrOutside);
         return __uint_as_float(0x7fffffffu);
       }
@@ -1149,24 +1157,19 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 
 // Joins the parts of a group that several ranges share, in order: one block per
 // (range that starts inside a group, row).  Two halves of the block take every second
-// part each, eight loads in flight.
+// part each, eight loads in flight; every warp works the weights out for itself.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int R>
 __global__ void __launch_bounds__(kJoinThreads)
 cache_join_kernel(const CacheParams p, const Work w) {
-  __shared__ float weight[kMaxRanges];
-  __shared__ float red[kJoinThreads / 32];
   __shared__ float4 half[128];
   ptx::grid_dep_wait();
-  const int c0 = blockIdx.x + 1;
+  const int c0 = blockIdx.x + 1, r = blockIdx.y;
   const Cut cut = w.cuts[c0];
-  if (cut.b < 0 || cut.parts == 0) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = cut.parts;
-  const int r = blockIdx.y, row = cut.g * R + r;
-  int first, count;
-  new_tokens(p, cut.b, first, count);
-  if (row >= (int64_t)count * p.H) return;
+  const int parts = cut.parts;
+  if (parts == 0 || r >= cut.rows) return;
+  const int tid = threadIdx.x, lane = tid & 31;
   // part 0: what range c0 - 1 left unfinished; part i: what range c0 + i - 1 begins with
   auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (c0 - 1) + 1 : 2 * (c0 + i - 1)) * R + r; };
   const int ch = 4 * (tid & 127), h0 = tid >> 7;
@@ -1176,56 +1179,38 @@ cache_join_kernel(const CacheParams p, const Work w) {
   for (int u = 0; u < 8; ++u)
     if (live && h0 + 2 * u < parts)
       x[u] = *reinterpret_cast<const float4*>(w.part + slot(h0 + 2 * u) * p.KVL + ch);
-  float mine[2], mx = -INFINITY;
-  static_assert(kMaxRanges <= 2 * kJoinThreads, "two parts per thread");
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = tid + j * kJoinThreads;
-    mine[j] = i < parts ? w.lse2[slot(i)] : -INFINITY;
-    mx = fmaxf(mx, mine[j]);
-  }
+  float mx = -INFINITY;
+  for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, w.lse2[slot(i)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if (lane == 0) red[warp] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[i]);
   const float m = mx == -INFINITY ? 0.f : mx;
-  __syncthreads();
   float tot = 0.f;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = tid + j * kJoinThreads;
-    const float f = i < parts ? exp2f(mine[j] - m) : 0.f;
-    if (i < parts) weight[i] = f;
-    tot += f;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
-  if (lane == 0) red[warp] = tot;
-  __syncthreads();
-  tot = 0.f;
-#pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) tot += red[i];
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = h0; i < parts; i += 16) {
+  for (int i0 = 0; i0 < parts; i0 += 32) {     // lane i: the weight of part i0 + i
+    const float weight = i0 + lane < parts ? exp2f(w.lse2[slot(i0 + lane)] - m) : 0.f;
+    tot += weight;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int j = i + 2 * u;
-      if (live && j < parts) {
-        const float f = weight[j];
-        acc.x = fmaf(f, x[u].x, acc.x);
-        acc.y = fmaf(f, x[u].y, acc.y);
-        acc.z = fmaf(f, x[u].z, acc.z);
-        acc.w = fmaf(f, x[u].w, acc.w);
-        if (j + 16 < parts) x[u] = *reinterpret_cast<const float4*>(w.part + slot(j + 16) * p.KVL + ch);
+    for (int j0 = 0; j0 < 32; j0 += 16) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int j = i0 + j0 + h0 + 2 * u;
+        const float f = __shfl_sync(0xffffffffu, weight, j0 + h0 + 2 * u);
+        if (live && j < parts) {
+          acc.x = fmaf(f, x[u].x, acc.x);
+          acc.y = fmaf(f, x[u].y, acc.y);
+          acc.z = fmaf(f, x[u].z, acc.z);
+          acc.w = fmaf(f, x[u].w, acc.w);
+          if (j + 16 < parts) x[u] = *reinterpret_cast<const float4*>(w.part + slot(j + 16) * p.KVL + ch);
+        }
       }
     }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
   if (h0 == 1) half[tid & 127] = acc;
   __syncthreads();
-  const int tok = div_heads(p, row);
-  const int64_t n = first + tok, h = row - tok * p.H;
+  const int row = cut.row0 + r, tok = div_heads(p, row);
+  const int64_t n = cut.first + tok, h = row - tok * p.H;
   const float inv = tot == 0.f ? 0.f : 1.f / tot;
   if (h0 == 0 && live) {
     const float4 b = half[tid];
