@@ -292,7 +292,7 @@ int mla_cache_read(const MlaCacheArgs* a, void* stream) {
 size_t mla_cache_workspace_bytes(const MlaCacheArgs* a) {
   using namespace kda::cache;
   if (validate_attention(a) != KDA_OK || a->B == 0 || a->N == 0 || a->H == 0) return 0;
-  return attention_workspace_bytes(to_params(a));
+  return attention_workspace_bytes(to_params(a), a->io_dtype);
 }
 
 int mla_cache_attention(const MlaCacheArgs* a, void* stream) {
@@ -301,7 +301,7 @@ int mla_cache_attention(const MlaCacheArgs* a, void* stream) {
   if (st != KDA_OK) return st;
   if (a->B == 0 || a->N == 0 || a->H == 0) return KDA_OK;
   CacheParams p = to_params(a);
-  const size_t need = attention_workspace_bytes(p);
+  const size_t need = attention_workspace_bytes(p, a->io_dtype);
   if (need && (a->workspace == nullptr || a->workspace_bytes < need)) return KDA_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return KDA_ERR_ALIGNMENT;
   if ((st = check_device()) != KDA_OK) return st;

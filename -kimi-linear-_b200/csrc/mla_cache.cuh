@@ -138,7 +138,7 @@ __device__ __forceinline__ void st8(T* p, bool vec, const float (&x)[8]) {
   }
 }
 
-size_t attention_workspace_bytes(const CacheParams& p);
+size_t attention_workspace_bytes(const CacheParams& p, int io_dtype);
 cudaError_t launch_attention(const CacheParams& p, int io_dtype, void* workspace, cudaStream_t s);
 
 }  // namespace cache

@@ -48,7 +48,6 @@ constexpr int kThreads = 384;              // warps 0-7 softmax, 8 loads, 9 S, 1
 // others keep 120 (256 x 192 + 128 x 120 = 384 x 168).
 constexpr int kSoftmaxRegs = 192, kOtherRegs = 120;
 
-constexpr int kWholeTiles = 4;             // contexts of at most so many tiles are not split
 constexpr int kMaxRanges = 256;            // blocks (SMs) that a call's tiles are cut over
 constexpr int kSmemMax = 232448;           // 227 KB per block
 constexpr float kLog2e = 1.4426950408889634f;
@@ -157,7 +156,7 @@ struct Work {
 // tiles).  Groups of one sequence see more and more positions; they are counted in
 // pairs (g, groups - 1 - g), which all count about the same, so that a place in the
 // count is found by a division.
-constexpr int kSetup = 3;
+constexpr int kSetup = 4;
 struct Seq {
   int first, n, off;       // new tokens; token i sits at off + i
   int groups, pair;        // row groups; count per pair
@@ -202,6 +201,12 @@ __device__ __forceinline__ int64_t seq_tiles(const Seq& s) {
 template <int R>
 __device__ __forceinline__ void place(const CacheParams& p, const Seq& s, int64_t r, int& g1, int& q,
                                       int& g2, int& n1, int& n2) {
+  if (s.groups == 1) {
+    g1 = g2 = n2 = 0;
+    q = (int)r;
+    n1 = s.pair - kSetup;
+    return;
+  }
   if (r < s.pair) {
     g1 = 0;
     q = (int)r;
@@ -577,7 +582,9 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       if (i < warp) before += sh.scan[i];
       total += sh.scan[i];
     }
-    const int64_t range = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t range = total <= 0x7fffffff
+                              ? ((uint32_t)total + gridDim.x - 1) / gridDim.x
+                              : (total + gridDim.x - 1) / gridDim.x;
     u0 = min(total, range * blockIdx.x);
     u1 = min(total, u0 + range);
     if (u0 < u1 && u0 >= before && u0 < before + mine) {
@@ -1235,14 +1242,24 @@ int device_sms() {
 }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Contexts that a block goes through about as fast as it would join parts of them
-// stay whole: no workspace and no second launch.
-bool whole_groups(const CacheParams& p) {
-  return (int64_t)p.max_pages * p.page_size <= kWholeTiles * TILE;
+int q_terms(int io_dtype) {
+  return io_dtype == KDA_DTYPE_F16 ? kQTerms<__half> : kQTerms<__nv_bfloat16>;
 }
 
-// Rows per group: 16 where the sequences of the call have no more rows than that
-// on average, or where 32 rows leave too small a ring; else 32.
+// Contexts that a block goes through about as fast as it would join parts of them stay
+// whole: no workspace and no second launch.  Up to 4 tiles (one token for each of B
+// sequences of 512, 16 heads, KVL 512; whole and split, us): B = 1 11.7 and 11.8, B = 16
+// 12.3 and 13.7; at 768 14.5 and 11.9, 15.1 and 14.8.  Up to 8 tiles where 64 groups or
+// more occupy the SMs anyhow: B = 64 at 1024 19.0 and 23.5, at 2048 30.6 and 28.5.
+bool whole_groups(const CacheParams& p, int R) {
+  const int64_t groups = max((int64_t)min(p.B, p.N), (int64_t)p.N * p.H / R);
+  return (int64_t)p.max_pages * p.page_size <= (groups >= 64 ? 8 : 4) * TILE;
+}
+
+// Rows per group: 16 where the sequences of the call have no more rows than that on
+// average, or where 32 rows leave too small a ring; else 32.  (16 sequences of 4096, 16
+// and 32 rows a group, us: 16 rows a sequence 18.5 and 22.9, 32 rows 25.0 and 25.6, 48
+// rows 37.0 and 32.9; 128 tokens of one prompt 64.9 and 50.0.)
 int rows_per_group(const CacheParams& p, int q_terms) {
   if (((int64_t)p.N * p.H + p.B - 1) / p.B <= 16) return 16;
   return ring_chunks(p.KVL, p.DR, q_terms, 32) >= 2 * tile_chunks(p.KVL, p.DR) ? 32 : 16;
@@ -1291,19 +1308,19 @@ bool encode(CUtensorMap* m, CUtensorMapDataType dt, int elt, void* base, int wid
 }  // namespace
 
 // partials | their log sums | cuts
-size_t attention_workspace_bytes(const CacheParams& p) {
-  if (whole_groups(p)) return 0;
-  const size_t ranges = device_sms(), R = 32;
+size_t attention_workspace_bytes(const CacheParams& p, int io_dtype) {
+  const size_t ranges = device_sms(), R = rows_per_group(p, q_terms(io_dtype));
+  if (whole_groups(p, (int)R)) return 0;
   return align256(2 * ranges * R * p.KVL * 4) + align256(2 * ranges * R * 4) +
          align256(ranges * sizeof(Cut));
 }
 
 cudaError_t launch_attention(const CacheParams& p, int io_dtype, void* workspace, cudaStream_t s) {
   const int ranges = device_sms();
-  const int R = rows_per_group(p, io_dtype == KDA_DTYPE_F16 ? kQTerms<__half> : kQTerms<__nv_bfloat16>);
+  const int R = rows_per_group(p, q_terms(io_dtype));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Work w{};
-  w.whole = whole_groups(p);
+  w.whole = whole_groups(p, R);
   w.part = reinterpret_cast<float*>(ws);
   ws += align256((size_t)2 * ranges * R * p.KVL * 4);
   w.lse2 = reinterpret_cast<float*>(ws);
