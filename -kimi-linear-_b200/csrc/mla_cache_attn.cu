@@ -27,6 +27,24 @@
 // split over many SMs and short ones share one.  A group cut by a range's end
 // leaves fp32 partials and cache_join_kernel adds them in order: the result does
 // not depend on timing.
+//
+// Roles: warp 10 walks the block's range and queues its segments (a group's tiles in
+// the range); warp 8 loads by TMA into a ring of 16 KB chunks; warps 9 and 11 issue the
+// two products, a warp each, because a product that waits for a barrier would hold the
+// other one's instructions back (issued from one warp: slower than they execute);
+// warps 0-7 do the softmax, half of the rows each four, a position a thread.
+//
+// Measured (B200, 16 heads, KVL 512, inputs that rotate past L2, join included):
+//   one token each for 8 sequences of 32768, bf16     35.3 us, 3.8 TB/s of the cache
+//   one token each for 64 sequences of 300 to 8192    36.0 us, 3.3 TB/s
+//   512 tokens of one prompt against 8192 positions   212.6 us, 666 TFLOP/s as counted
+//     (4 KVL for a row and key), 2.5 times that as executed on the terms
+// What bounds it: at 16 rows a tile takes the time of its 64 KB from HBM (1.5 us for
+// each SM), and around the tiles stand 7.5 us until the first scores (lengths, page
+// numbers, queries, the first tile), 1 to 2 us for a result and 4 us until the join's
+// end.  At 32 rows the ring holds 2.5 tiles, less than the chain load -> S -> softmax ->
+// O spans (about two tiles' time, 2800 cycles each), and the products' reads of shared
+// memory alone take 2200 of them.
 #include <cuda.h>
 
 #include <type_traits>
@@ -152,8 +170,9 @@ struct Work {
 // how the tiles of a call are counted and cut
 // ---------------------------------------------------------------------------
 // Sequence b as R-row groups.  A group counts for its tiles and kSetup more: what
-// its queries, its first tile's latency and its result cost (measured: about three
-// tiles).  Groups of one sequence see more and more positions; they are counted in
+// its queries, its first tile's latency and its result cost (3, 4 and 5, us: 64
+// sequences of 300 to 8192 tokens 36.9, 36.0, 38.1; prompts of 1 to 1500 tokens 226,
+// 225, 221; 4 sequences of 8192 20.3, 19.9, 20.2).  Groups of one sequence see more and more positions; they are counted in
 // pairs (g, groups - 1 - g), which all count about the same, so that a place in the
 // count is found by a division.
 constexpr int kSetup = 4;
@@ -683,142 +702,142 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       if (lane == 0 && !w.whole) w.cuts[blockIdx.x] = cut;
       __syncwarp();
     } else if (warp == 8) {
-    // ======== loads: boxes of one page (at most 128 positions) x 128 bytes into a
-    // ring of 16 KB chunks; a tile is its rope chunk, then its code chunks, in two halves
-    // that land and are freed apart.  (A look at a barrier takes some 300 cycles while
-    // the products read shared memory: one for each chunk was too many, one for a whole
-    // tile keeps the chunks waiting for one another.)
-    const int ahead = ring / tile_chunks, spare = ring % tile_chunks;
-    const int box_rows = min(p.page_size, TILE), boxes = TILE / box_rows;
-    const uint32_t sm0 = ptx::smem_u32(sm);
-    int k = 0, slot = 0, freed = -1;            // freed: half tiles known to be
-    bool ok = true;
-    Info seg;
-    while (ok && uniform(take(seg, true)) > 0) {
-      const int t1 = uniform(seg.t1), seen = uniform(seg.seen);
-      // lane i: page of box i of a tile
-      auto page_of_box = [&](int t) {
-        const int pos = t * TILE + lane * box_rows, i = pos >> p.page_shift;
-        int x = -1;
-        if (lane < boxes && t < t1 && pos < seen && i < p.max_pages)
-          x = p.table[(int64_t)seg.b * p.table_s + i];
-        return x;
-      };
-      int page_next = page_of_box(seg.t0);
-      for (int t = uniform(seg.t0); t < t1 && ok; ++t, ++k) {
-        // outside the pool: the copy fills in zeros
-        const int page = (uint32_t)page_next < (uint32_t)p.num_pages ? page_next : p.num_pages;
-        page_next = page_of_box(t + 1);
-        const int pos = t * TILE, nbox = min(boxes, (seen - pos + box_rows - 1) / box_rows);
-        const int at = p.page_size > TILE ? pos & (p.page_size - 1) : 0;
-        const uint32_t bar = ptx::smem_u32(&sh.full[2 * (k & 3)]);
-        expect_bytes(bar, nbox * box_rows * 128 * half);
-        expect_bytes(bar + 8, nbox * box_rows * 128 * (tile_chunks - half));
-        for (int c = 0; c < tile_chunks; ++c) {
-          // whose place this chunk takes: chunk `old` of tile j
-          const int j = k - ahead - (c < spare), old = c - spare + (c < spare ? tile_chunks : 0);
-          const int need = 2 * j + (old >= half);
-          if (j >= 0 && need > freed) {
-            if (!wait(&sh.freed[need & 7], (need >> 3) & 1, ab)) { ok = false; break; }
-            freed = need;
+      // ======== loads: boxes of one page (at most 128 positions) x 128 bytes into a
+      // ring of 16 KB chunks; a tile is its rope chunk, then its code chunks, in two halves
+      // that land and are freed apart.  (A look at a barrier takes some 300 cycles while
+      // the products read shared memory: one for each chunk was too many, one for a whole
+      // tile keeps the chunks waiting for one another.)
+      const int ahead = ring / tile_chunks, spare = ring % tile_chunks;
+      const int box_rows = min(p.page_size, TILE), boxes = TILE / box_rows;
+      const uint32_t sm0 = ptx::smem_u32(sm);
+      int k = 0, slot = 0, freed = -1;            // freed: half tiles known to be
+      bool ok = true;
+      Info seg;
+      while (ok && uniform(take(seg, true)) > 0) {
+        const int t1 = uniform(seg.t1), seen = uniform(seg.seen);
+        // lane i: page of box i of a tile
+        auto page_of_box = [&](int t) {
+          const int pos = t * TILE + lane * box_rows, i = pos >> p.page_shift;
+          int x = -1;
+          if (lane < boxes && t < t1 && pos < seen && i < p.max_pages)
+            x = p.table[(int64_t)seg.b * p.table_s + i];
+          return x;
+        };
+        int page_next = page_of_box(seg.t0);
+        for (int t = uniform(seg.t0); t < t1 && ok; ++t, ++k) {
+          // outside the pool: the copy fills in zeros
+          const int page = (uint32_t)page_next < (uint32_t)p.num_pages ? page_next : p.num_pages;
+          page_next = page_of_box(t + 1);
+          const int pos = t * TILE, nbox = min(boxes, (seen - pos + box_rows - 1) / box_rows);
+          const int at = p.page_size > TILE ? pos & (p.page_size - 1) : 0;
+          const uint32_t bar = ptx::smem_u32(&sh.full[2 * (k & 3)]);
+          expect_bytes(bar, nbox * box_rows * 128 * half);
+          expect_bytes(bar + 8, nbox * box_rows * 128 * (tile_chunks - half));
+          for (int c = 0; c < tile_chunks; ++c) {
+            // whose place this chunk takes: chunk `old` of tile j
+            const int j = k - ahead - (c < spare), old = c - spare + (c < spare ? tile_chunks : 0);
+            const int need = 2 * j + (old >= half);
+            if (j >= 0 && need > freed) {
+              if (!wait(&sh.freed[need & 7], (need >> 3) & 1, ab)) { ok = false; break; }
+              freed = need;
+            }
+            const int code = c - (tile_chunks - NCH);
+            const CUtensorMap* map = code < 0 ? &map_rope : &map_codes;
+            for (int i = 0; i < nbox; ++i)
+              load_box(sm0 + slot * CHUNK + i * box_rows * 128, map, max(code, 0) * 128, at,
+                       __shfl_sync(0xffffffffu, page, i), bar + 8 * (c >= half));
+            if (++slot == ring) slot = 0;
           }
-          const int code = c - (tile_chunks - NCH);
-          const CUtensorMap* map = code < 0 ? &map_rope : &map_codes;
-          for (int i = 0; i < nbox; ++i)
-            load_box(sm0 + slot * CHUNK + i * box_rows * 128, map, max(code, 0) * 128, at,
-                     __shfl_sync(0xffffffffu, page, i), bar + 8 * (c >= half));
-          if (++slot == ring) slot = 0;
         }
       }
-    }
-    if (*ab) {                                  // copies in flight land before the block ends
-      for (int i = max(0, 2 * k - 6); i <= 2 * k + 1; ++i) drain(&sh.full[i & 7], (i >> 3) & 1);
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    // ======== S^T = codes Q^T, a tile or two ahead of the softmax.  (Two warps issue the
-    // two products: one warp issues more slowly than the products execute, and would
-    // hold back the scores of a tile behind the wait for another's weights.)
-    constexpr uint32_t kHalf = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-    constexpr uint32_t id_s = idesc(NS, false, false, kE4M3, kE4M3);
-    constexpr uint32_t id_r = idesc(R, false, false, kHalf, kHalf);
-    const uint32_t dq = sw128_lo(ptx::smem_u32(q_s)), dqr = sw128_lo(ptx::smem_u32(qr_s));
-    const uint32_t dk0 = sw128_lo(ptx::smem_u32(sm)), ts = (uint32_t)uniform((int)tm_s);
-    int k = 0, segs = 0, slot = 0;
-    bool ok = true;
-    Info seg;
-    while (ok && uniform(take(seg, true)) > 0) {
-      const int tiles = uniform(seg.t1 - seg.t0);
-      if (!wait(&sh.q_ready, segs & 1, ab)) break;
-      ++segs;
-      for (int t = 0; t < tiles; ++t, ++k) {
-        const int before = k - C::SBUF;         // the tile whose scores were here
-        if (before >= 0 && !wait(&sh.s_empty[before & 1], (before >> 1) & 1, ab)) { ok = false; break; }
-        const uint32_t d = ts + (C::SBUF == 2 ? (k & 1) * NS : 0);
-        const int rope_slot = slot;
-        if (p.DR && ++slot == ring) slot = 0;
+      if (*ab) {                                  // copies in flight land before the block ends
+        for (int i = max(0, 2 * k - 6); i <= 2 * k + 1; ++i) drain(&sh.full[i & 7], (i >> 3) & 1);
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // ======== S^T = codes Q^T, a tile or two ahead of the softmax.  (Two warps issue the
+      // two products: one warp issues more slowly than the products execute, and would
+      // hold back the scores of a tile behind the wait for another's weights.)
+      constexpr uint32_t kHalf = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      constexpr uint32_t id_s = idesc(NS, false, false, kE4M3, kE4M3);
+      constexpr uint32_t id_r = idesc(R, false, false, kHalf, kHalf);
+      const uint32_t dq = sw128_lo(ptx::smem_u32(q_s)), dqr = sw128_lo(ptx::smem_u32(qr_s));
+      const uint32_t dk0 = sw128_lo(ptx::smem_u32(sm)), ts = (uint32_t)uniform((int)tm_s);
+      int k = 0, segs = 0, slot = 0;
+      bool ok = true;
+      Info seg;
+      while (ok && uniform(take(seg, true)) > 0) {
+        const int tiles = uniform(seg.t1 - seg.t0);
+        if (!wait(&sh.q_ready, segs & 1, ab)) break;
+        ++segs;
+        for (int t = 0; t < tiles; ++t, ++k) {
+          const int before = k - C::SBUF;         // the tile whose scores were here
+          if (before >= 0 && !wait(&sh.s_empty[before & 1], (before >> 1) & 1, ab)) { ok = false; break; }
+          const uint32_t d = ts + (C::SBUF == 2 ? (k & 1) * NS : 0);
+          const int rope_slot = slot;
+          if (p.DR && ++slot == ring) slot = 0;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-          if (c == 0 || c == HC) {
-            if (!wait(&sh.full[2 * (k & 3) + (c == HC)], (k >> 2) & 1, ab)) { ok = false; break; }
-            ptx::tc_fence_after();
+          for (int c = 0; c < NCH; ++c) {
+            if (c == 0 || c == HC) {
+              if (!wait(&sh.full[2 * (k & 3) + (c == HC)], (k >> 2) & 1, ab)) { ok = false; break; }
+              ptx::tc_fence_after();
+            }
+            const uint32_t dk = dk0 + slot * (CHUNK >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f8<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dq + ((c * NS * 128 + kk * 32) >> 4), id_s,
+                                         c + kk > 0);
+            if (++slot == ring) slot = 0;
           }
-          const uint32_t dk = dk0 + slot * (CHUNK >> 4);
+          if (!ok) break;
+          if (p.DR) {
+            const uint32_t dk = dk0 + rope_slot * (CHUNK >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dq + ((c * NS * 128 + kk * 32) >> 4), id_s,
-                                       c + kk > 0);
-          if (++slot == ring) slot = 0;
+            for (int kk = 0; kk < 4; ++kk)
+              mma_half<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dqr + ((kk * 32) >> 4), id_r);
+          }
+          commit(&sh.s_full[k & 1]);
         }
-        if (!ok) break;
-        if (p.DR) {
-          const uint32_t dk = dk0 + rope_slot * (CHUNK >> 4);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_half<kSw128Hi, kSw128Hi>(d, dk + ((kk * 32) >> 4), dqr + ((kk * 32) >> 4), id_r);
-        }
-        commit(&sh.s_full[k & 1]);
       }
-    }
-    if (*ab) {                                  // products in flight end before TMEM is freed
-      commit(&sh.drain[0]);
-      drain(&sh.drain[0], 0);
-    }
-    __syncwarp();
-  } else if (warp == 11) {
-    // ======== O^T += codes^T P^T
-    constexpr uint32_t id_o = idesc(NO, true, true, kE4M3, F::FMT);
-    const uint32_t dp = p_lo(ptx::smem_u32(p_s)), dk0 = sw128_lo(ptx::smem_u32(sm));
-    const uint32_t to = (uint32_t)uniform((int)tmem);
-    int k = 0, slot = 0;
-    bool ok = true;
-    Info seg;
-    while (ok && uniform(take(seg, true)) > 0) {
-      const int tiles = uniform(seg.t1 - seg.t0);
-      for (int t = 0; t < tiles; ++t, ++k) {
-        const int par = k & 1;
-        if (!wait(&sh.p_full[par], (k >> 1) & 1, ab)) { ok = false; break; }
-        ptx::tc_fence_after();
-        if (p.DR && ++slot == ring) slot = 0;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-          const uint32_t dv = dk0 + slot * (CHUNK >> 4);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8<kSw128Hi, kPHi>(to + c * NO, dv + ((kk * 4096) >> 4),
-                                   dp + ((par * NO * 128 + kk * 512) >> 4), id_o, t > 0 || kk > 0);
-          if (++slot == ring) slot = 0;
-          if (c == HC - 1) commit(&sh.freed[2 * (k & 3)]);
-        }
-        commit(&sh.freed[2 * (k & 3) + 1]);
+      if (*ab) {                                  // products in flight end before TMEM is freed
+        commit(&sh.drain[0]);
+        drain(&sh.drain[0], 0);
       }
+      __syncwarp();
+    } else if (warp == 11) {
+      // ======== O^T += codes^T P^T
+      constexpr uint32_t id_o = idesc(NO, true, true, kE4M3, F::FMT);
+      const uint32_t dp = p_lo(ptx::smem_u32(p_s)), dk0 = sw128_lo(ptx::smem_u32(sm));
+      const uint32_t to = (uint32_t)uniform((int)tmem);
+      int k = 0, slot = 0;
+      bool ok = true;
+      Info seg;
+      while (ok && uniform(take(seg, true)) > 0) {
+        const int tiles = uniform(seg.t1 - seg.t0);
+        for (int t = 0; t < tiles; ++t, ++k) {
+          const int par = k & 1;
+          if (!wait(&sh.p_full[par], (k >> 1) & 1, ab)) { ok = false; break; }
+          ptx::tc_fence_after();
+          if (p.DR && ++slot == ring) slot = 0;
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            const uint32_t dv = dk0 + slot * (CHUNK >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f8<kSw128Hi, kPHi>(to + c * NO, dv + ((kk * 4096) >> 4),
+                                     dp + ((par * NO * 128 + kk * 512) >> 4), id_o, t > 0 || kk > 0);
+            if (++slot == ring) slot = 0;
+            if (c == HC - 1) commit(&sh.freed[2 * (k & 3)]);
+          }
+          commit(&sh.freed[2 * (k & 3) + 1]);
+        }
+      }
+      if (*ab) {
+        commit(&sh.drain[1]);
+        drain(&sh.drain[1], 0);
+      }
+      __syncwarp();
     }
-    if (*ab) {
-      commit(&sh.drain[1]);
-      drain(&sh.drain[1], 0);
-    }
-    __syncwarp();
-  }
   } else {
     // ======== softmax: two groups of four warps have half of the rows each; thread =
     // position of the tile = TMEM lane
@@ -955,130 +974,130 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       const int* sees = rw.seen + rb;
       float l[HR];
       if (have) {
-      float ls_next = log2f(s_next), rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
+        float ls_next = log2f(s_next), rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
 #pragma unroll
-      for (int r = 0; r < HR; ++r) l[r] = 0.f;
-      ptx::tc_fence_before();
-      bar_sync(3, 256);                         // the rows' figures are written, O has been read
-      for (int t = seg.t0; t < seg.t1; ++t, ++k) {
-        const int par = k & 1;
-        const bool start = t == seg.t0;
-        // log2 of the position's scale and its reciprocal (a NaN scale: NaN reaches
-        // the sum through P, where the row sees the position)
-        const float s = s_next, ls = ls_next, rs = rs_next;
-        s_next = scale_at(t + 1, page_next);
-        page_next = page_at(seg, t + 2);
-        const int pos = t * TILE + tt;
-        if (!wait(&sh.s_full[par], (k >> 1) & 1, ab)) failed = true;
-        ptx::tc_fence_after();
-        float a[HR];
-        {
-          float z[NQ * HR];
-          const uint32_t at = tm_s + (C::SBUF == 2 ? par * NS : 0) + rb + lane_base;
+        for (int r = 0; r < HR; ++r) l[r] = 0.f;
+        ptx::tc_fence_before();
+        bar_sync(3, 256);                         // the rows' figures are written, O has been read
+        for (int t = seg.t0; t < seg.t1; ++t, ++k) {
+          const int par = k & 1;
+          const bool start = t == seg.t0;
+          // log2 of the position's scale and its reciprocal (a NaN scale: NaN reaches
+          // the sum through P, where the row sees the position)
+          const float s = s_next, ls = ls_next, rs = rs_next;
+          s_next = scale_at(t + 1, page_next);
+          page_next = page_at(seg, t + 2);
+          const int pos = t * TILE + tt;
+          if (!wait(&sh.s_full[par], (k >> 1) & 1, ab)) failed = true;
+          ptx::tc_fence_after();
+          float a[HR];
+          {
+            float z[NQ * HR];
+            const uint32_t at = tm_s + (C::SBUF == 2 ? par * NS : 0) + rb + lane_base;
 #pragma unroll
-          for (int j = 0; j < NQ; ++j) tmem_get<HR>(at + j * R, z + HR * j);
-          ptx::tmem_wait_ld();
-          ptx::tc_fence_before();
-          ptx::mbar_arrive(&sh.s_empty[par]);
+            for (int j = 0; j < NQ; ++j) tmem_get<HR>(at + j * R, z + HR * j);
+            ptx::tmem_wait_ld();
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(&sh.s_empty[par]);
 #pragma unroll
-          for (int r = 0; r < HR; ++r) a[r] = fmaf(join<NQ>(z + r, HR, kQFiner), q_scale[r] * s, ls);
-        }
-        if (t * TILE + TILE > seg.seen0) {      // some row does not see the whole tile
-#pragma unroll
-          for (int r = 0; r < HR; ++r)
-            if (pos >= sees[r]) a[r] = -INFINITY;
-        }
-        // positions that nobody sees, or that are NaN as a whole, must not meet
-        // a weight of zero: their codes become zeros
-        if (wg == 0 && (pos >= seg.seen || s != s)) {
-          int at = (int)(((int64_t)k * tile_chunks + tile_chunks - NCH) % ring);
-#pragma unroll 1
-          for (int c = 0; c < NCH; ++c) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(sm + at * CHUNK + tt * 128 + 16 * i) = make_uint4(0, 0, 0, 0);
-            if (++at == ring) at = 0;
+            for (int r = 0; r < HR; ++r) a[r] = fmaf(join<NQ>(z + r, HR, kQFiner), q_scale[r] * s, ls);
           }
-        }
-        float top = -INFINITY;
+          if (t * TILE + TILE > seg.seen0) {      // some row does not see the whole tile
 #pragma unroll
-        for (int r = 0; r < HR; ++r) top = fmaxf(top, a[r] - m[r]);
-        if (ptx::bar_red_or(1 + wg, 128, failed || top > F::BIAS + F::SLACK)) {
-          // a row outgrew P's range (or has its first position): new maxima, and O
-          // follows once the products so far are in it
-          if (*ab) failed = true;
-#pragma unroll
-          for (int r = 0; r < HR; ++r) {
-            const float mx = warp_max(a[r]);
-            if (lane == 0) sh.red[warp][r] = mx;
+            for (int r = 0; r < HR; ++r)
+              if (pos >= sees[r]) a[r] = -INFINITY;
           }
-          failed = ptx::bar_red_or(1 + wg, 128, failed);
-          if (failed) break;
-          if (tt < HR) {
-            const float* red = &sh.red[4 * wg][tt];
-            const float mx = fmaxf(fmaxf(red[0], red[HR]), fmaxf(red[2 * HR], red[3 * HR]));
-            const float old = m[tt];
-            const bool up = mx - old > F::BIAS + F::SLACK;
-            rw.alpha[rb + tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
-            if (up) rw.m[rb + tt] = mx - F::BIAS;
-          }
-          bar_sync(1 + wg, 128);
-          if (!start) {
-            if (!o_done(k - 1)) failed = true;
-            ptx::tc_fence_after();
-            float al[HR];
-#pragma unroll
-            for (int r = 0; r < HR; ++r) {
-              al[r] = alpha[r];
-              l[r] *= al[r];
-            }
+          // positions that nobody sees, or that are NaN as a whole, must not meet
+          // a weight of zero: their codes become zeros
+          if (wg == 0 && (pos >= seg.seen || s != s)) {
+            int at = (int)(((int64_t)k * tile_chunks + tile_chunks - NCH) % ring);
 #pragma unroll 1
             for (int c = 0; c < NCH; ++c) {
-              const uint32_t at = tmem + c * NO + rb + lane_base;
-              float o[NP * HR];
 #pragma unroll
-              for (int j = 0; j < NP; ++j) tmem_get<HR>(at + j * R, o + HR * j);
-              ptx::tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < NP * HR; ++i) o[i] *= al[i % HR];
-#pragma unroll
-              for (int j = 0; j < NP; ++j) tmem_put<HR>(at + j * R, o + HR * j);
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint4*>(sm + at * CHUNK + tt * 128 + 16 * i) = make_uint4(0, 0, 0, 0);
+              if (++at == ring) at = 0;
             }
-            ptx::tmem_wait_st();
-            ptx::tc_fence_before();
           }
-        }
-        // ---- P, once the buffer's last products have read it
-        if (k > 1 && !o_done(k - 2)) failed = true;
-        // (16 rows of a position are 16 bytes, 8 rows one half of them)
-        uint8_t* pt = p_s + par * NO * 128 + tt * 16 + (HR == 8 ? wg * 8 : wg * (TILE * 16));
-        uint32_t term[NP][HR / 4];
+          float top = -INFINITY;
 #pragma unroll
-        for (int q = 0; q < HR / 4; ++q) {
-          float e4[4];
+          for (int r = 0; r < HR; ++r) top = fmaxf(top, a[r] - m[r]);
+          if (ptx::bar_red_or(1 + wg, 128, failed || top > F::BIAS + F::SLACK)) {
+            // a row outgrew P's range (or has its first position): new maxima, and O
+            // follows once the products so far are in it
+            if (*ab) failed = true;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e4[i] = ex2(a[4 * q + i] - m[4 * q + i]);
-            l[4 * q + i] = fmaf(e4[i], rs, l[4 * q + i]);
+            for (int r = 0; r < HR; ++r) {
+              const float mx = warp_max(a[r]);
+              if (lane == 0) sh.red[warp][r] = mx;
+            }
+            failed = ptx::bar_red_or(1 + wg, 128, failed);
+            if (failed) break;
+            if (tt < HR) {
+              const float* red = &sh.red[4 * wg][tt];
+              const float mx = fmaxf(fmaxf(red[0], red[HR]), fmaxf(red[2 * HR], red[3 * HR]));
+              const float old = m[tt];
+              const bool up = mx - old > F::BIAS + F::SLACK;
+              rw.alpha[rb + tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
+              if (up) rw.m[rb + tt] = mx - F::BIAS;
+            }
+            bar_sync(1 + wg, 128);
+            if (!start) {
+              if (!o_done(k - 1)) failed = true;
+              ptx::tc_fence_after();
+              float al[HR];
+#pragma unroll
+              for (int r = 0; r < HR; ++r) {
+                al[r] = alpha[r];
+                l[r] *= al[r];
+              }
+#pragma unroll 1
+              for (int c = 0; c < NCH; ++c) {
+                const uint32_t at = tmem + c * NO + rb + lane_base;
+                float o[NP * HR];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) tmem_get<HR>(at + j * R, o + HR * j);
+                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < NP * HR; ++i) o[i] *= al[i % HR];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) tmem_put<HR>(at + j * R, o + HR * j);
+              }
+              ptx::tmem_wait_st();
+              ptx::tc_fence_before();
+            }
           }
-          uint32_t u[NP];
-          F::split(e4, u);
+          // ---- P, once the buffer's last products have read it
+          if (k > 1 && !o_done(k - 2)) failed = true;
+          // (16 rows of a position are 16 bytes, 8 rows one half of them)
+          uint8_t* pt = p_s + par * NO * 128 + tt * 16 + (HR == 8 ? wg * 8 : wg * (TILE * 16));
+          uint32_t term[NP][HR / 4];
 #pragma unroll
-          for (int j = 0; j < NP; ++j) term[j][q] = u[j];
-        }
+          for (int q = 0; q < HR / 4; ++q) {
+            float e4[4];
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          uint8_t* d = pt + j * (R / 16) * (TILE * 16);
-          if constexpr (HR == 16)
-            *reinterpret_cast<uint4*>(d) = make_uint4(term[j][0], term[j][1], term[j][2], term[j][3]);
-          else
-            *reinterpret_cast<uint2*>(d) = make_uint2(term[j][0], term[j][1]);
+            for (int i = 0; i < 4; ++i) {
+              e4[i] = ex2(a[4 * q + i] - m[4 * q + i]);
+              l[4 * q + i] = fmaf(e4[i], rs, l[4 * q + i]);
+            }
+            uint32_t u[NP];
+            F::split(e4, u);
+#pragma unroll
+            for (int j = 0; j < NP; ++j) term[j][q] = u[j];
+          }
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            uint8_t* d = pt + j * (R / 16) * (TILE * 16);
+            if constexpr (HR == 16)
+              *reinterpret_cast<uint4*>(d) = make_uint4(term[j][0], term[j][1], term[j][2], term[j][3]);
+            else
+              *reinterpret_cast<uint2*>(d) = make_uint2(term[j][0], term[j][1]);
+          }
+          ptx::fence_proxy_async_smem();
+          ptx::mbar_arrive(&sh.p_full[par]);
+          ls_next = log2f(s_next);
+          rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
         }
-        ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(&sh.p_full[par]);
-        ls_next = log2f(s_next);
-        rs_next = s_next == s_next ? __frcp_rn(s_next) : 1.f;
-      }
       }
       failed = ptx::bar_red_or(3, 256, failed);  // the scores have all been read
       if (failed) break;
@@ -1087,66 +1106,66 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         write_queries(nseg, sh.rows[(si + 1) & 1]);
       }
       if (have) {
-      // ---- the segment's result
-      const float sum = warp_sums<HR>(l, lane);
-      if (lane < HR) sh.red[warp][lane] = sum;
-      if (!failed && !o_done(k - 1)) failed = true;
-      ptx::tc_fence_after();
-      failed = ptx::bar_red_or(3, 256, failed);
-      if (failed) break;
-      const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
-      const int slot = 2 * blockIdx.x + (seg.t0 > 0 ? 0 : 1);
-      float inv = 0.f;                          // of row rb + lane
-      if (lane < HR) {
-        const float* red = &sh.red[4 * wg][lane];
-        const float total = (red[0] + red[HR]) + (red[2 * HR] + red[3 * HR]);
-        inv = total == 0.f ? 0.f : 1.f / (total * F::GAIN);
-        if ((warp & 3) == 0 && rb + lane < seg.rows) {
-          const float lse2 = total == 0.f ? -INFINITY : m[lane] + log2f(total);
-          if (!whole) w.lse2[slot * R + rb + lane] = lse2;
-          else if (p.lse) p.lse[rw.lse[rb + lane]] = lse2 * kLn2;
+        // ---- the segment's result
+        const float sum = warp_sums<HR>(l, lane);
+        if (lane < HR) sh.red[warp][lane] = sum;
+        if (!failed && !o_done(k - 1)) failed = true;
+        ptx::tc_fence_after();
+        failed = ptx::bar_red_or(3, 256, failed);
+        if (failed) break;
+        const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
+        const int slot = 2 * blockIdx.x + (seg.t0 > 0 ? 0 : 1);
+        float inv = 0.f;                          // of row rb + lane
+        if (lane < HR) {
+          const float* red = &sh.red[4 * wg][lane];
+          const float total = (red[0] + red[HR]) + (red[2 * HR] + red[3 * HR]);
+          inv = total == 0.f ? 0.f : 1.f / (total * F::GAIN);
+          if ((warp & 3) == 0 && rb + lane < seg.rows) {
+            const float lse2 = total == 0.f ? -INFINITY : m[lane] + log2f(total);
+            if (!whole) w.lse2[slot * R + rb + lane] = lse2;
+            else if (p.lse) p.lse[rw.lse[rb + lane]] = lse2 * kLn2;
+          }
         }
-      }
-      const bool odd = lane & 1;
-      float f[HR];
-      T* dst[HR / 2];                           // neighbouring lanes swap a row each: four bytes a store
+        const bool odd = lane & 1;
+        float f[HR];
+        T* dst[HR / 2];                           // neighbouring lanes swap a row each: four bytes a store
 #pragma unroll
-      for (int r = 0; r < HR; ++r) f[r] = __shfl_sync(0xffffffffu, inv, r);
+        for (int r = 0; r < HR; ++r) f[r] = __shfl_sync(0xffffffffu, inv, r);
 #pragma unroll
-      for (int r = 0; r < HR; r += 2)
-        dst[r / 2] = static_cast<T*>(p.out) + rw.out[rb + r + odd] + (tt & ~1);
+        for (int r = 0; r < HR; r += 2)
+          dst[r / 2] = static_cast<T*>(p.out) + rw.out[rb + r + odd] + (tt & ~1);
 #pragma unroll 1
-      for (int c = 0; c < NCH; ++c) {           // 128 channels of this group's rows
-        float o[NP * HR];
+        for (int c = 0; c < NCH; ++c) {           // 128 channels of this group's rows
+          float o[NP * HR];
 #pragma unroll
-        for (int j = 0; j < NP; ++j) tmem_get<HR>(tmem + c * NO + j * R + rb + lane_base, o + HR * j);
-        ptx::tmem_wait_ld();
+          for (int j = 0; j < NP; ++j) tmem_get<HR>(tmem + c * NO + j * R + rb + lane_base, o + HR * j);
+          ptx::tmem_wait_ld();
 #pragma unroll
-        for (int r = 0; r < HR; ++r) o[r] = join<NP>(o + r, HR, F::FINER) * f[r];
-        if (whole) {
+          for (int r = 0; r < HR; ++r) o[r] = join<NP>(o + r, HR, F::FINER) * f[r];
+          if (whole) {
 #pragma unroll
-          for (int r = 0; r < HR; r += 2) {
-            const float other = __shfl_xor_sync(0xffffffffu, odd ? o[r] : o[r + 1], 1);
-            T pair[2];
-            st(pair, odd ? other : o[r]);
-            st(pair + 1, odd ? o[r + 1] : other);
-            if (rb + r + odd < seg.rows) {
-              T* d = dst[r / 2] + c * 128;
-              if (p.out_vec) {
-                *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(pair);
-              } else {
-                d[0] = pair[0];
-                d[1] = pair[1];
+            for (int r = 0; r < HR; r += 2) {
+              const float other = __shfl_xor_sync(0xffffffffu, odd ? o[r] : o[r + 1], 1);
+              T pair[2];
+              st(pair, odd ? other : o[r]);
+              st(pair + 1, odd ? o[r + 1] : other);
+              if (rb + r + odd < seg.rows) {
+                T* d = dst[r / 2] + c * 128;
+                if (p.out_vec) {
+                  *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(pair);
+                } else {
+                  d[0] = pair[0];
+                  d[1] = pair[1];
+                }
               }
             }
-          }
-        } else {
-          float* part = w.part + ((int64_t)slot * R + rb) * p.KVL + c * 128 + tt;
+          } else {
+            float* part = w.part + ((int64_t)slot * R + rb) * p.KVL + c * 128 + tt;
 #pragma unroll
-          for (int r = 0; r < HR; ++r)
-            if (rb + r < seg.rows) part[r * p.KVL] = o[r];
+            for (int r = 0; r < HR; ++r)
+              if (rb + r < seg.rows) part[r * p.KVL] = o[r];
+          }
         }
-      }
       }
       if (!have_next) break;
       seg = nseg;
@@ -1164,7 +1183,9 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 
 // Joins the parts of a group that several ranges share, in order: one block per
 // (range that starts inside a group, row).  Two halves of the block take every second
-// part each, eight loads in flight; every warp works the weights out for itself.
+// part each, eight loads in flight; every warp works the weights out for itself.  Bound
+// by latency: the launch, a cut, the parts' sums, then the parts, one after the other;
+// 3 us with 19 parts of 16 rows of 512.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int R>

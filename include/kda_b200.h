@@ -364,7 +364,8 @@ size_t mla_decode_args_size(void);
  * A position past the table's max_pages or a page outside the pool sets the
  * device error word (6) where it is met: append skips the token, read gives
  * zeros, attention ignores positions past the table and gives NaN for a
- * sequence with a visible page outside the pool.
+ * sequence with a visible page outside the pool.  7: a wait inside attention ran out
+ * (its outputs are not valid).
  *
  * Requires 16-bit io_dtype, KVL in {128, 256, 384, 512}, DR in {0, 64},
  * page_size a power of two from 16 to 1024, num_pages * page_size < 2^31, max_pages *
