@@ -172,9 +172,9 @@ struct Work {
 // Sequence b as R-row groups.  A group counts for its tiles and kSetup more: what
 // its queries, its first tile's latency and its result cost (3, 4 and 5, us: 64
 // sequences of 300 to 8192 tokens 36.9, 36.0, 38.1; prompts of 1 to 1500 tokens 226,
-// 225, 221; 4 sequences of 8192 20.3, 19.9, 20.2).  Groups of one sequence see more and more positions; they are counted in
-// pairs (g, groups - 1 - g), which all count about the same, so that a place in the
-// count is found by a division.
+// 225, 221; 4 sequences of 8192 20.3, 19.9, 20.2).  Groups of one sequence see more and
+// more positions; they are counted in pairs (g, groups - 1 - g), which all count about
+// the same, so that a place in the count is found by a division.
 constexpr int kSetup = 4;
 struct Seq {
   int first, n, off;       // new tokens; token i sits at off + i
