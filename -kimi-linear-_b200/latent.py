@@ -260,7 +260,7 @@ def latent_attention(q_lat, cache, block_table, lens, scale, q_start=None, q_rop
 
     The new tokens' own latents must be in the cache (:func:`latent_append`
     first).  Scores and sums are fp32; queries enter the products exactly
-    (bf16) or to 2^-12 (fp16), the softmax's weights to 2^-9 (bf16) or 2^-12
+    (bf16) or to 2^-12 (fp16), the softmax's weights to 2^-10 (bf16) or 2^-12
     (fp16) relative, below the outputs' own rounding."""
     fn = "latent_attention"
     _operand(fn, cache, "q_lat", q_lat)
