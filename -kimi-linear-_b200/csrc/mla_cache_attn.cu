@@ -50,6 +50,7 @@
 #include <type_traits>
 
 #include "mla_cache.cuh"
+#include "mla_cache_ring.cuh"
 #include "tc_ptx.cuh"
 
 namespace kda {
@@ -138,7 +139,7 @@ struct Cfg {
 };
 
 // Shared memory besides the ring (barriers and rows; 1 KB: alignment), and the
-// chunks that fit beside it, four tiles of them at most.  The order of the products
+// chunks that fit beside it, kRingTiles tiles of them at most.  The order of the products
 // needs the chunks of two tiles at once.
 constexpr int kSharedBytes = 4096;
 int fixed_bytes(int kvl, int q_terms, int R) {
@@ -147,7 +148,7 @@ int fixed_bytes(int kvl, int q_terms, int R) {
 int tile_chunks(int kvl, int dr) { return kvl / 128 + (dr ? 1 : 0); }
 int ring_chunks(int kvl, int dr, int q_terms, int R) {
   const int n = (kSmemMax - fixed_bytes(kvl, q_terms, R)) / CHUNK;
-  return min(n, 4 * tile_chunks(kvl, dr));
+  return min(n, kRingTiles * tile_chunks(kvl, dr));
 }
 
 // Where a range of tiles starts inside a group; what cache_join_kernel reads.
@@ -474,7 +475,8 @@ constexpr int kQueue = 4;  // segments that are known ahead
 
 template <int R>
 struct Shared {            // at the end of dynamic shared memory
-  uint64_t full[8], freed[8], seg_full[kQueue], seg_empty[kQueue];   // full, freed: half tile % 8
+  uint64_t full[2 * kStages], freed[2 * kStages];                    // by half tiles
+  uint64_t seg_full[kQueue], seg_empty[kQueue];
   uint64_t s_full[2], s_empty[2], p_full[2], q_ready, drain[2];      // tile % 2
   uint32_t tmem;
   int abort_flag;
@@ -553,7 +555,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
   const int half = tile_chunks - NCH + HC;      // chunks of it
 
   if (tid == 0) {
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 2 * kStages; ++i) {
       ptx::mbar_init(&sh.full[i], 1);
       ptx::mbar_init(&sh.freed[i], 1);
     }
@@ -707,7 +709,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       // that land and are freed apart.  (A look at a barrier takes some 300 cycles while
       // the products read shared memory: one for each chunk was too many, one for a whole
       // tile keeps the chunks waiting for one another.)
-      const int ahead = ring / tile_chunks, spare = ring % tile_chunks;
+      const Ring places(ring, tile_chunks, half);
       const int box_rows = min(p.page_size, TILE), boxes = TILE / box_rows;
       const uint32_t sm0 = ptx::smem_u32(sm);
       int k = 0, slot = 0, freed = -1;            // freed: half tiles known to be
@@ -730,15 +732,13 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           page_next = page_of_box(t + 1);
           const int pos = t * TILE, nbox = min(boxes, (seen - pos + box_rows - 1) / box_rows);
           const int at = p.page_size > TILE ? pos & (p.page_size - 1) : 0;
-          const uint32_t bar = ptx::smem_u32(&sh.full[2 * (k & 3)]);
+          const uint32_t bar = ptx::smem_u32(&sh.full[half_barrier(2 * k)]);
           expect_bytes(bar, nbox * box_rows * 128 * half);
           expect_bytes(bar + 8, nbox * box_rows * 128 * (tile_chunks - half));
           for (int c = 0; c < tile_chunks; ++c) {
-            // whose place this chunk takes: chunk `old` of tile j
-            const int j = k - ahead - (c < spare), old = c - spare + (c < spare ? tile_chunks : 0);
-            const int need = 2 * j + (old >= half);
-            if (j >= 0 && need > freed) {
-              if (!wait(&sh.freed[need & 7], (need >> 3) & 1, ab)) { ok = false; break; }
+            const int need = places.held_by(k, c);
+            if (need > freed) {
+              if (!wait(&sh.freed[half_barrier(need)], half_parity(need), ab)) { ok = false; break; }
               freed = need;
             }
             const int code = c - (tile_chunks - NCH);
@@ -751,7 +751,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         }
       }
       if (*ab) {                                  // copies in flight land before the block ends
-        for (int i = max(0, 2 * k - 6); i <= 2 * k + 1; ++i) drain(&sh.full[i & 7], (i >> 3) & 1);
+        for (int i = max(0, 2 * k - 6); i <= 2 * k + 1; ++i) drain(&sh.full[half_barrier(i)], half_parity(i));
       }
       __syncwarp();
     } else if (warp == 9) {
@@ -779,7 +779,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
 #pragma unroll
           for (int c = 0; c < NCH; ++c) {
             if (c == 0 || c == HC) {
-              if (!wait(&sh.full[2 * (k & 3) + (c == HC)], (k >> 2) & 1, ab)) { ok = false; break; }
+              if (!wait(&sh.full[half_barrier(2 * k) + (c == HC)], half_parity(2 * k), ab)) { ok = false; break; }
               ptx::tc_fence_after();
             }
             const uint32_t dk = dk0 + slot * (CHUNK >> 4);
@@ -827,9 +827,9 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
               mma_f8<kSw128Hi, kPHi>(to + c * NO, dv + ((kk * 4096) >> 4),
                                      dp + ((par * NO * 128 + kk * 512) >> 4), id_o, t > 0 || kk > 0);
             if (++slot == ring) slot = 0;
-            if (c == HC - 1) commit(&sh.freed[2 * (k & 3)]);
+            if (c == HC - 1) commit(&sh.freed[half_barrier(2 * k)]);
           }
-          commit(&sh.freed[2 * (k & 3) + 1]);
+          commit(&sh.freed[half_barrier(2 * k + 1)]);
         }
       }
       if (*ab) {
@@ -848,7 +848,9 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     const int tt = tid & 127;
     int k = 0;
     bool failed = false;
-    auto o_done = [&](int i) { return wait(&sh.freed[2 * (i & 3) + 1], (i >> 2) & 1, ab); };   // of tile i
+    auto o_done = [&](int i) {                  // the products have read tile i
+      return wait(&sh.freed[half_barrier(2 * i + 1)], half_parity(2 * i + 1), ab);
+    };
 
     // ---- a segment's loads: the queries, the pages of this thread's first two positions
     constexpr int RW = R / 8;                   // rows of a warp: warp + 8 i
