@@ -11,8 +11,8 @@
 //   O^T [128 channels x rows] += codes^T [128 ch x 128 pos] (M-major) P^T, per 128 channels
 // What is not in 8 bits is split into 8-bit terms, each finer than the one before:
 // x = x0 + x1 / 16 + ... .  A query (scaled by a power of two) in bf16 has 8
-// significant bits, two e4m3 terms hold it; fp16 takes three.  A softmax weight takes
-// three terms, enough that the output's own rounding is the larger error.  The terms
+// significant bits, two e4m3 terms hold it; fp16 takes three.  A softmax weight is
+// rounded to 11 bits and takes three e5m2 terms, which keep it when it is small.  The terms
 // are more columns of N and are added in fp32 afterwards: an instruction of 128 x N x
 // 32 spends its time on reading 4 KB of codes from shared memory, so the columns cost
 // little (41 cycles at N = 32, 49 at 64, 56 at 96).
@@ -73,60 +73,45 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kUnset = -1e30f;           // maximum of a row that has seen nothing
 
-// e4m3 terms of a query, each 16 times finer: exact for bf16 (8 bits), 2^-12 for fp16
+// e4m3 terms of a query, each 16 times finer: two hold bf16's 8 bits, three fp16's 11.
+// (Values below 2^-12 of the row's largest are off by at most 2^-19 (2^-23) of it: the
+// terms' last steps.)
 template <typename T> constexpr int kQTerms = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
-// Terms of a softmax weight P, cut out of its fp16 value (a code of either format is a
-// run of an fp16's bits), so that only one conversion is needed:
-//  * bf16: e5m2 = the upper byte of fp16.  P is rounded to 9 bits (2^-10 of itself) and
-//    cut into three terms, each 8 times finer.  It carries 2^5 and may outgrow the
-//    maximum by 2^10 (2^15 < 57344) before the maximum moves.
-//  * fp16: e4m3 = bits 13 .. 7 of fp16, for the value times 2^-8.  P in fp16 (11 bits,
-//    2^-12) is cut into three terms, each 16 times finer.  It carries 2^-6 and may
-//    outgrow the maximum by 2^6 (to 1, so that no term reaches 1.875, the code of NaN).
-// Weights down to 2^-27 (2^-18) of the largest still count.
+// A softmax weight P is rounded to fp16 (11 bits: 2^-11 of itself) and cut into three
+// e5m2 terms, each 16 times finer than the one before.  An e5m2 code is an fp16's upper
+// byte, so a term is the byte nearest to what is left, and its remainder, of either sign,
+// comes next: of 11 bits at most 8 remain, then 4, which three bits hold (they fit whole:
+// up to 8 steps).  Nothing of the fp16 value is lost, subnormals included, and no term
+// exceeds 2^15.
+// P carries 2^BIAS of the row's maximum and may outgrow it by 2^SLACK, to 2^15, before
+// the maximum moves.  So a weight holds 11 bits down to 2^-(14 + BIAS) of the largest one,
+// and is off by at most 2^-(25 + BIAS) of it below that, while the sum takes it unrounded:
+// a crowd of n small weights may lose n 2^-(25 + BIAS) of the largest.  More BIAS costs
+// rescales.  (bf16, BIAS 5, 7 and 9, us: 512 tokens on 8192 211, 215, 222; 8 x 32768 34.9,
+// 35.4, 36.0.  With 7 a weight of 2^-20 of the largest has all its 11 bits, so that a long
+// crowd's part holds to bf16's rounding.)
 constexpr int NP = 3;
-template <typename T> struct PFormat {
-  static constexpr uint32_t FMT = 0;
-  static constexpr float FINER = 16.f, BIAS = -6.f, SLACK = 6.f, GAIN = 256.f;   // code value / P
-  static __device__ __forceinline__ void split(const float (&x)[4], uint32_t (&t)[NP]) {
-    __half2 r[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
-    const __half2 finer = __float2half2_rn(FINER);
+constexpr uint32_t kE5M2 = 1;
+constexpr float kPFiner = 16.f;
+template <typename T> constexpr float kBias = std::is_same<T, __nv_bfloat16>::value ? 7.f : 9.f;
+constexpr float kPTop = 15.f;             // BIAS + SLACK
+__device__ __forceinline__ void split_weights(const float (&x)[4], uint32_t (&t)[NP]) {
+  __half2 r[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
+  const __half2 finer = __float2half2_rn(kPFiner);
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      uint32_t c[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        c[i] = *reinterpret_cast<const uint32_t*>(&r[i]) & 0x3f803f80u;
-        if (j + 1 < NP) r[i] = __hmul2(__hsub2(r[i], *reinterpret_cast<const __half2*>(&c[i])), finer);
-      }
-      t[j] = __byte_perm(c[0] >> 7, c[1] >> 7, 0x6420);
-    }
-  }
-};
-template <> struct PFormat<__nv_bfloat16> {
-  static constexpr uint32_t FMT = 1;
-  static constexpr float FINER = 8.f, BIAS = 5.f, SLACK = 10.f, GAIN = 1.f;
-  static __device__ __forceinline__ void split(const float (&x)[4], uint32_t (&t)[NP]) {
-    __half2 r[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
-    const __half2 finer = __float2half2_rn(FINER);
+  for (int j = 0; j < NP; ++j) {
+    uint32_t c[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      uint32_t u = *reinterpret_cast<const uint32_t*>(&r[i]);
-      u = (u + 0x00020002u) & 0xfffcfffcu;           // (a NaN is lost here; the sum keeps it)
-      r[i] = *reinterpret_cast<const __half2*>(&u);
-    }
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      uint32_t c[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        c[i] = *reinterpret_cast<const uint32_t*>(&r[i]) & 0xff00ff00u;
-        if (j + 1 < NP) r[i] = __hmul2(__hsub2(r[i], *reinterpret_cast<const __half2*>(&c[i])), finer);
+      c[i] = *reinterpret_cast<const uint32_t*>(&r[i]);
+      if (j + 1 < NP) {                   // (a NaN may be lost here; the sum keeps it)
+        c[i] = (c[i] + 0x00800080u) & 0xff00ff00u;
+        r[i] = __hmul2(__hsub2(r[i], *reinterpret_cast<const __half2*>(&c[i])), finer);
       }
-      t[j] = __byte_perm(c[0], c[1], 0x7531);
     }
+    t[j] = __byte_perm(c[0], c[1], 0x7531);
   }
-};
+}
 constexpr uint32_t kE4M3 = 0;
 constexpr float kQFiner = 16.f;
 
@@ -429,8 +414,8 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
 }
 
 // A query's values (times 2^-8; at most 1, so that no term reaches 1.875, the code of
-// NaN) as e4m3 terms, x = t[0] + t[1] / 16 (+ t[2] / 256), four at a time: like
-// PFormat<__half>, with signs.
+// NaN) as e4m3 terms, x = t[0] + t[1] / 16 (+ t[2] / 256), four at a time.  An e4m3 code
+// is the sign and bits 13 .. 7 of the fp16 of the value times 2^-8.
 template <int NT>
 __device__ __forceinline__ void split_query(const float (&x)[4], uint32_t (&t)[NT]) {
   __half2 r[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
@@ -541,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUtensorMap map_codes,
                   const __grid_constant__ CUtensorMap map_rope) {
   using C = Cfg<T, R, NCH>;
-  using F = PFormat<T>;
+  constexpr float BIAS = kBias<T>;
   constexpr int NQ = C::NQ, NS = C::NS, NO = C::NO;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -806,7 +791,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
       __syncwarp();
     } else if (warp == 11) {
       // ======== O^T += codes^T P^T
-      constexpr uint32_t id_o = idesc(NO, true, true, kE4M3, F::FMT);
+      constexpr uint32_t id_o = idesc(NO, true, true, kE4M3, kE5M2);
       const uint32_t dp = p_lo(ptx::smem_u32(p_s)), dk0 = sw128_lo(ptx::smem_u32(sm));
       const uint32_t to = (uint32_t)uniform((int)tmem);
       int k = 0, slot = 0;
@@ -1024,7 +1009,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           float top = -INFINITY;
 #pragma unroll
           for (int r = 0; r < HR; ++r) top = fmaxf(top, a[r] - m[r]);
-          if (ptx::bar_red_or(1 + wg, 128, failed || top > F::BIAS + F::SLACK)) {
+          if (ptx::bar_red_or(1 + wg, 128, failed || top > kPTop)) {
             // a row outgrew P's range (or has its first position): new maxima, and O
             // follows once the products so far are in it
             if (*ab) failed = true;
@@ -1039,9 +1024,9 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
               const float* red = &sh.red[4 * wg][tt];
               const float mx = fmaxf(fmaxf(red[0], red[HR]), fmaxf(red[2 * HR], red[3 * HR]));
               const float old = m[tt];
-              const bool up = mx - old > F::BIAS + F::SLACK;
-              rw.alpha[rb + tt] = up ? ex2(old - (mx - F::BIAS)) : 1.f;
-              if (up) rw.m[rb + tt] = mx - F::BIAS;
+              const bool up = mx - old > kPTop;
+              rw.alpha[rb + tt] = up ? ex2(old - (mx - BIAS)) : 1.f;
+              if (up) rw.m[rb + tt] = mx - BIAS;
             }
             bar_sync(1 + wg, 128);
             if (!start) {
@@ -1083,7 +1068,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
               l[4 * q + i] = fmaf(e4[i], rs, l[4 * q + i]);
             }
             uint32_t u[NP];
-            F::split(e4, u);
+            split_weights(e4, u);
 #pragma unroll
             for (int j = 0; j < NP; ++j) term[j][q] = u[j];
           }
@@ -1121,7 +1106,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         if (lane < HR) {
           const float* red = &sh.red[4 * wg][lane];
           const float total = (red[0] + red[HR]) + (red[2 * HR] + red[3 * HR]);
-          inv = total == 0.f ? 0.f : 1.f / (total * F::GAIN);
+          inv = total == 0.f ? 0.f : 1.f / total;
           if ((warp & 3) == 0 && rb + lane < seg.rows) {
             const float lse2 = total == 0.f ? -INFINITY : m[lane] + log2f(total);
             if (!whole) w.lse2[slot * R + rb + lane] = lse2;
@@ -1143,7 +1128,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           for (int j = 0; j < NP; ++j) tmem_get<HR>(tmem + c * NO + j * R + rb + lane_base, o + HR * j);
           ptx::tmem_wait_ld();
 #pragma unroll
-          for (int r = 0; r < HR; ++r) o[r] = join<NP>(o + r, HR, F::FINER) * f[r];
+          for (int r = 0; r < HR; ++r) o[r] = join<NP>(o + r, HR, kPFiner) * f[r];
           if (whole) {
 #pragma unroll
             for (int r = 0; r < HR; r += 2) {

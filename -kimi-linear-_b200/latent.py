@@ -259,9 +259,11 @@ def latent_attention(q_lat, cache, block_table, lens, scale, q_start=None, q_rop
     by it).  A row that sees nothing gives zeros and ``-inf``.
 
     The new tokens' own latents must be in the cache (:func:`latent_append`
-    first).  Scores and sums are fp32; queries enter the products exactly
-    (bf16) or to 2^-12 (fp16), the softmax's weights to 2^-10 (bf16) or 2^-12
-    (fp16) relative, below the outputs' own rounding."""
+    first).  Scores and sums are fp32.  Queries enter the products exactly, but
+    for values below 2^-12 of the row's largest, which are off by at most 2^-19
+    (bf16) or 2^-23 (fp16) of it.  A softmax weight (times its token's scale) is
+    rounded to 11 bits down to 2^-21 (bf16) or 2^-23 (fp16) of the row's largest,
+    and is off by at most 2^-32 or 2^-34 of it below that."""
     fn = "latent_attention"
     _operand(fn, cache, "q_lat", q_lat)
     kvl = cache.kv_lora_rank
