@@ -188,10 +188,10 @@ int validate(const MlaCacheArgs* a) {
   if (a->num_pages < 1 || (int64_t)a->num_pages * a->page_size >= (1ll << 31)) return KDA_ERR_SHAPE;
   if (a->B < 0 || a->N < 0 || a->max_pages < 0 || a->max_pages > (1 << 24)) return KDA_ERR_SHAPE;
   if ((int64_t)a->max_pages * a->page_size > (1ll << 30)) return KDA_ERR_SHAPE;
-  if (a->B == 0 || a->N == 0) return KDA_OK;               // nothing to do
-  if (a->q_start == nullptr && a->N % a->B != 0) return KDA_ERR_SHAPE;
-  if (!a->codes || !a->scales || (a->DR && !a->rope) || !a->lens ||
-      (a->max_pages > 0 && !a->block_table))
+  if (a->N == 0) return KDA_OK;                            // nothing to do
+  if (a->B > 0 && a->q_start == nullptr && a->N % a->B != 0) return KDA_ERR_SHAPE;
+  if (!a->codes || !a->scales || (a->DR && !a->rope) ||
+      (a->B > 0 && (!a->lens || (a->max_pages > 0 && !a->block_table))))
     return KDA_ERR_NULL_POINTER;
   if (!aligned16(a->codes) || a->codes_stride[0] % 16 || a->codes_stride[1] % 16 ||
       reinterpret_cast<uintptr_t>(a->scales) % 4)
@@ -240,7 +240,7 @@ int check_device() {
 int run_tokens(const MlaCacheArgs* a, bool append, void* stream) {
   int st = validate(a);
   if (st != KDA_OK) return st;
-  if (a->B == 0 || a->N == 0) return KDA_OK;
+  if (a->N == 0 || (append && a->B == 0)) return KDA_OK;
   if (!a->c_kv || (a->DR && !a->k_rope)) return KDA_ERR_NULL_POINTER;
   if (reinterpret_cast<uintptr_t>(a->c_kv) % 2 || reinterpret_cast<uintptr_t>(a->k_rope) % 2)
     return KDA_ERR_ALIGNMENT;
@@ -258,7 +258,7 @@ int validate_attention(const MlaCacheArgs* a) {
   const int st = validate(a);
   if (st != KDA_OK) return st;
   if (a->H < 0 || a->H > 1024 || (int64_t)a->N * a->H > (1ll << 30)) return KDA_ERR_SHAPE;
-  if (a->B == 0 || a->N == 0 || a->H == 0) return KDA_OK;
+  if (a->N == 0 || a->H == 0) return KDA_OK;
   if (!a->q_lat || !a->out || (a->DR && !a->q_rope)) return KDA_ERR_NULL_POINTER;
   if (reinterpret_cast<uintptr_t>(a->q_lat) % 2 || reinterpret_cast<uintptr_t>(a->q_rope) % 2 ||
       reinterpret_cast<uintptr_t>(a->out) % 2 || reinterpret_cast<uintptr_t>(a->lse) % 4)
@@ -295,7 +295,7 @@ int mla_cache_read(const MlaCacheArgs* a, void* stream) {
 
 size_t mla_cache_workspace_bytes(const MlaCacheArgs* a) {
   using namespace kda::cache;
-  if (validate_attention(a) != KDA_OK || a->B == 0 || a->N == 0 || a->H == 0) return 0;
+  if (validate_attention(a) != KDA_OK || a->N == 0 || a->H == 0) return 0;
   return attention_workspace_bytes(to_params(a), a->io_dtype);
 }
 
@@ -303,7 +303,7 @@ int mla_cache_attention(const MlaCacheArgs* a, void* stream) {
   using namespace kda::cache;
   int st = validate_attention(a);
   if (st != KDA_OK) return st;
-  if (a->B == 0 || a->N == 0 || a->H == 0) return KDA_OK;
+  if (a->N == 0 || a->H == 0) return KDA_OK;
   CacheParams p = to_params(a);
   const size_t need = attention_workspace_bytes(p, a->io_dtype);
   if (need && (a->workspace == nullptr || a->workspace_bytes < need)) return KDA_ERR_WORKSPACE;

@@ -48,10 +48,15 @@ __device__ __forceinline__ void new_tokens(const CacheParams& p, int b, int& fir
 }
 
 // Sequence and position of new token n (position < 0: it has none), for all lanes of
-// a warp at once; lanes of one half have one n.  The sequences' starts are counted 32
+// a warp at once; lanes of one half have one n.  (No sequence has it: -1.)  The sequences' starts are counted 32
 // at a time: one load's latency, where a search by halves has one for each step.
 __device__ __forceinline__ void locate(const CacheParams& p, int n, int& b, int& pos) {
   int first, count;
+  if (p.B == 0) {
+    b = 0;
+    pos = -1;
+    return;
+  }
   if (p.q_start == nullptr) {
     count = p.N / p.B;
     b = n / count;

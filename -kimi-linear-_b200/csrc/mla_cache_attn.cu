@@ -636,7 +636,12 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 10) {
       // ======== segments: a queue of them for the other warps; groups that see nothing
-      // get their zeros here
+      // get their zeros here, and so do the rows of no sequence
+      const auto empty_row = [&](int64_t n, int64_t h) {
+        T* o = static_cast<T*>(p.out) + n * p.o_s[0] + h * p.o_s[1];
+        for (int c = lane; c < p.KVL; c += 32) st(o + c, 0.f);
+        if (lane == 0 && p.lse) p.lse[n * p.lse_s + h] = -INFINITY;
+      };
       Walk<R> walk(p, sh.seq, sh.b, sh.base, u0, u1, w.whole);
       for (int i = 0;;) {
         Segment seg;
@@ -652,10 +657,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           if (info.seen == 0) {
             for (int r = 0; r < info.rows; ++r) {
               const int tok = div_heads(p, row0 + r);
-              const int64_t n = info.first + tok, h = row0 + r - tok * p.H;
-              T* o = static_cast<T*>(p.out) + n * p.o_s[0] + h * p.o_s[1];
-              for (int c = lane; c < p.KVL; c += 32) st(o + c, 0.f);
-              if (lane == 0 && p.lse) p.lse[n * p.lse_s + h] = -INFINITY;
+              empty_row(info.first + tok, row0 + r - tok * p.H);
             }
             continue;
           }
@@ -687,6 +689,16 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         }
       }
       if (lane == 0 && !w.whole) w.cuts[blockIdx.x] = cut;
+      // ---- new tokens before the first sequence's and after the last one's (a batch that
+      // is padded to a fixed N)
+      if (p.q_start != nullptr || p.B == 0) {
+        const int lo = p.B > 0 ? min(max(p.q_start[0], 0), p.N) : 0;
+        const int hi = p.B > 0 ? max(min(p.q_start[p.B], p.N), lo) : 0;
+        for (int r = blockIdx.x; r < (lo + p.N - hi) * p.H; r += gridDim.x) {
+          const int tok = div_heads(p, r);
+          empty_row(tok < lo ? tok : hi + tok - lo, r - tok * p.H);
+        }
+      }
       __syncwarp();
     } else if (warp == 8) {
       // ======== loads: boxes of one page (at most 128 positions) x 128 bytes into a
@@ -1269,7 +1281,7 @@ bool whole_groups(const CacheParams& p, int R) {
 // and 32 rows a group, us: 16 rows a sequence 18.5 and 22.9, 32 rows 25.0 and 25.6, 48
 // rows 37.0 and 32.9; 128 tokens of one prompt 64.9 and 50.0.)
 int rows_per_group(const CacheParams& p, int q_terms) {
-  if (((int64_t)p.N * p.H + p.B - 1) / p.B <= 16) return 16;
+  if ((int64_t)p.N * p.H <= (int64_t)p.B * 16) return 16;
   return ring_chunks(p.KVL, p.DR, q_terms, 32) >= 2 * tile_chunks(p.KVL, p.DR) ? 32 : 16;
 }
 

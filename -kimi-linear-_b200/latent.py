@@ -13,7 +13,9 @@ Three operators share the cache.  Each takes ``block_table`` int32
 new ones included) and ``q_start`` int32 ``[B + 1]`` (sequence ``b`` owns rows
 ``q_start[b] .. q_start[b + 1] - 1`` of the new tokens; None: ``N / B`` each).
 New token ``i`` of the ``n`` of sequence ``b`` sits at position
-``lens[b] - n + i``:
+``lens[b] - n + i``.  Rows before ``q_start[0]`` and from ``q_start[B]`` on (a
+batch padded to a fixed ``N``) belong to no sequence: append skips them, read
+gives zeros, attention zeros and ``-inf``:
 
 * :func:`latent_append` quantises new tokens into their slots;
 * :func:`latent_read` gives tokens back in the 16-bit type;

@@ -351,6 +351,8 @@ size_t mla_decode_args_size(void);
  * Sequence b holds lens[b] tokens, its last n_b new: n_b = q_start[b + 1] -
  * q_start[b], or N / B when q_start is NULL.  New token i of b sits at position
  * p = lens[b] - n_b + i: slot p % page_size of page block_table[b, p / page_size].
+ * q_start ascends; tokens before q_start[0] and from q_start[B] on (all, with B = 0)
+ * belong to no sequence and count as tokens with p < 0.
  *
  * mla_cache_append: writes codes, scale and rope of c_kv [N, KVL], k_rope
  *   [N, DR] into their slots.  Tokens with p < 0 are skipped.

@@ -78,3 +78,91 @@ def test_a_heavy_token_over_a_long_context(share, n, cuda_dev):
     tol = 2.0 ** -24 * 576 * 20 + 2.0 ** -20 * (1 + wlse.abs())
     assert bool(((lse.double().cpu().view(B, n, H) - wlse).abs() <= tol).all())
     assert pkg().device_error() == 0
+
+
+def _dirty(dev):
+    """What the allocator hands out next reads as NaN."""
+    blocks = [torch.full((size,), math.nan, device=dev) for size in [1 << k for k in range(7, 20)] * 3]
+    del blocks
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("lens,counts", [([700, 90], [1, 1]), ([130, 5, 700], [9, 5, 40])])
+def test_rows_of_no_sequence(lens, counts, dt, cuda_dev):
+    """Rows before q_start[0] and from q_start[B] on: zeros and -inf from attention, zeros
+    from read, skipped by append; the others as without them."""
+    kb = pkg()
+    m = make(lens, counts, H=5, KVL=128, DR=64, page=64, dt=dt, seed=len(lens))
+    N, before, after = sum(counts), 3, 150
+    want, wl = attend(m)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(before + N + after, 5, 128, generator=g).to(dt).to(m.dev)
+    qr = torch.randn(before + N + after, 5, 64, generator=g).to(dt).to(m.dev)
+    q[before:before + N], qr[before:before + N] = m.q.to(m.dev), m.qr.to(m.dev)
+    q_start = m.q_start + before
+    own = torch.zeros(before + N + after, dtype=torch.bool, device=m.dev)
+    own[before:before + N] = True
+    for wide in (m.table, torch.cat([m.table] * 20, 1)):        # whole contexts, and split ones
+        _dirty(m.dev)
+        out, lse = kb.latent_attention(q, m.cache, wide.contiguous(), m.lens, m.scale, q_start=q_start,
+                                       q_rope=qr, return_lse=True)
+        assert bool((out[~own] == 0).all()) and bool(torch.isneginf(lse[~own]).all())
+        assert torch.equal(torch.isneginf(lse[own]), torch.isneginf(wl))
+        assert float((out[own].float() - want.float()).abs().max()) <= 2.0 ** -6 * float(want.abs().max())
+    c0, _ = kb.latent_read(m.cache, m.table, m.lens, N, q_start=m.q_start)
+    _dirty(m.dev)
+    c, k = kb.latent_read(m.cache, m.table, m.lens, before + N + after, q_start=q_start)
+    assert torch.equal(c[own], c0) and bool((c[~own] == 0).all()) and bool((k[~own] == 0).all())
+    codes = m.cache.codes.view(torch.uint8).clone()
+    slots = [w[2] for w in lo.slots(m.table.cpu(), lens, counts, 64) if w[2] is not None]
+    kb.latent_append(m.cache, q[:, 0].contiguous(), m.table, m.lens, q_start=q_start,
+                     k_rope=qr[:, 0].contiguous())
+    same = (codes == m.cache.codes.view(torch.uint8)).all(-1).view(-1).cpu()
+    same[slots] = True
+    assert bool(same.all())
+    assert kb.device_error() == 0
+
+
+def test_no_sequence_at_all(cuda_dev):
+    """B = 0 with a q_start of one entry."""
+    kb = pkg()
+    cache = kb.LatentCache(2, 16, 128, device=cuda_dev)
+    i32 = dict(dtype=torch.int32, device=cuda_dev)
+    table, lens, q_start = torch.zeros(0, 1, **i32), torch.zeros(0, **i32), torch.zeros(1, **i32)
+    x = torch.ones(7, 4, 128, dtype=BF16, device=cuda_dev)
+    for t in (table, torch.zeros(0, 4096, **i32)):
+        _dirty(cuda_dev)
+        out, lse = kb.latent_attention(x, cache, t, lens, 1.0, q_start=q_start, return_lse=True)
+        c, _ = kb.latent_read(cache, t, lens, 7, q_start=q_start)
+        assert bool((out == 0).all()) and bool(torch.isneginf(lse).all()) and bool((c == 0).all())
+    before = cache.codes.view(torch.uint8).clone()
+    kb.latent_append(cache, x[:, 0].contiguous(), table, lens, q_start=q_start)
+    assert torch.equal(before, cache.codes.view(torch.uint8)) and kb.device_error() == 0
+
+
+def test_a_padded_batch_in_a_graph(cuda_dev):
+    """One captured call of eight rows, replayed with fewer and fewer of them owned."""
+    kb = pkg()
+    m = make([900, 333], [4, 4], H=16, KVL=128, page=64, seed=5)
+    q, q_start = m.q.to(m.dev), m.q_start.clone()
+    args = (q, m.cache, m.table, m.lens, m.scale)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kb.latent_attention(*args, q_start=q_start, return_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = kb.latent_attention(*args, q_start=q_start, return_lse=True)
+    for starts in ([0, 4, 8], [0, 4, 5], [0, 1, 2], [2, 4, 4], [0, 0, 0]):
+        q_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        out.fill_(math.nan)
+        lse.fill_(math.nan)
+        graph.replay()
+        want, wl = kb.latent_attention(*args, q_start=q_start, return_lse=True)
+        own = torch.zeros(8, dtype=torch.bool)
+        own[starts[0]:starts[2]] = True
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+        assert bool((out[~own] == 0).all()) and bool(torch.isneginf(lse[~own]).all())
+        assert bool(torch.isfinite(lse[own]).all())
+    del graph
