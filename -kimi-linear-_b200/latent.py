@@ -315,10 +315,11 @@ def mla_step(module, x, q_nope, q_rope, c_kv, k_rope, state, use_cache):
     ``[B, T, DR]`` (rotated; None without a rope part), ``c_kv`` ``[B, T, KVL]``.
     ``state``: ``cache`` (a :class:`LatentCache`), ``block_table`` and ``lens``;
     the pages for ``lens + T`` tokens must be in the table.  ``lens`` is advanced
-    by ``T`` on the device, the tokens are appended, the queries folded into the
-    latent space by the module's own ``kv_b_proj`` weight, attended, and brought
-    out by its value half and ``o_proj``.  The folded queries and the mixed
-    latents are in the 16-bit type."""
+    by ``T`` on the device (a step that raises takes that back), the tokens are
+    appended, the queries folded into the latent space by the module's own
+    ``kv_b_proj`` weight (cast on every step unless it is in the cache's type),
+    attended, and brought out by its value half and ``o_proj``.  The folded queries
+    and the mixed latents are in the 16-bit type."""
     B, T = x.shape[:2]
     cache, lens, table = state["cache"], state["lens"], state["block_table"]
     H, DN, DV, KVL = (module.num_heads, module.qk_nope_head_dim, module.v_head_dim,
@@ -329,17 +330,21 @@ def mla_step(module, x, q_nope, q_rope, c_kv, k_rope, state, use_cache):
     dt = cache.dtype
     w = module.kv_b_proj.weight.detach().to(dt).view(H, DN + DV, KVL)
     lens.add_(T)
-    if cache.rope_dim:
-        k_rope = k_rope.reshape(B * T, cache.rope_dim).to(dt)
-        q_rope = q_rope.reshape(B * T, H, cache.rope_dim).to(dt)
-    else:
-        k_rope = q_rope = None
-    latent_append(cache, c_kv.reshape(B * T, KVL).to(dt), table, lens, k_rope=k_rope)
-    qn = q_nope.reshape(B * T, H, DN).to(dt)
-    q_lat = torch.bmm(qn.transpose(0, 1), w[:, :DN]).transpose(0, 1)           # [N, H, KVL]
-    mixed = latent_attention(q_lat, cache, table, lens, module.scale, q_rope=q_rope)
-    out = torch.bmm(mixed.transpose(0, 1), w[:, DN:].transpose(1, 2))          # [H, N, DV]
-    out = module.o_proj(out.transpose(0, 1).reshape(B, T, H * DV).to(x.dtype))
+    try:
+        if cache.rope_dim:
+            k_rope = k_rope.reshape(B * T, cache.rope_dim).to(dt)
+            q_rope = q_rope.reshape(B * T, H, cache.rope_dim).to(dt)
+        else:
+            k_rope = q_rope = None
+        latent_append(cache, c_kv.reshape(B * T, KVL).to(dt), table, lens, k_rope=k_rope)
+        qn = q_nope.reshape(B * T, H, DN).to(dt)
+        q_lat = torch.bmm(qn.transpose(0, 1), w[:, :DN]).transpose(0, 1)           # [N, H, KVL]
+        mixed = latent_attention(q_lat, cache, table, lens, module.scale, q_rope=q_rope)
+        out = torch.bmm(mixed.transpose(0, 1), w[:, DN:].transpose(1, 2))          # [H, N, DV]
+        out = module.o_proj(out.transpose(0, 1).reshape(B, T, H * DV).to(x.dtype))
+    except BaseException:
+        lens.sub_(T)             # refused: the sequences are as long as they were
+        raise
     if use_cache:
         return out, state
     return out

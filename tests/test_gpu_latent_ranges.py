@@ -11,7 +11,7 @@ import torch
 
 from conftest import pkg
 from oracle import latent_oracle as lo
-from test_gpu_latent import BF16, F16, attend, check, make
+from test_gpu_latent import BF16, F16, _module, attend, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -166,3 +166,34 @@ def test_a_padded_batch_in_a_graph(cuda_dev):
         assert bool((out[~own] == 0).all()) and bool(torch.isneginf(lse[~own]).all())
         assert bool(torch.isfinite(lse[own]).all())
     del graph
+
+
+@pytest.mark.parametrize("spoil", ["grad", "heads", "table"])
+def test_a_refused_layer_step_changes_nothing(spoil, cuda_dev):
+    """A step that is refused, before or after its tokens were written, leaves the lengths;
+    the next one gives what it would have given without it."""
+    kb, dev = pkg(), cuda_dev
+    mod = _module(4, 16, 16, 128, 0, 32, dev, BF16)
+    cache = kb.LatentCache(4, 16, 128, device=dev)
+    state = {"cache": cache, "block_table": torch.arange(4, dtype=torch.int32, device=dev).view(2, 2),
+             "lens": torch.zeros(2, dtype=torch.int32, device=dev)}
+    g = torch.Generator(device=dev).manual_seed(2)
+    x, q, c = (torch.randn(*s, generator=g, device=dev).to(BF16)
+               for s in ((2, 3, 32), (2, 3, 4, 16), (2, 3, 128)))
+    with torch.no_grad():
+        want = kb.latent.mla_step(mod, x, q, None, c, None, dict(state, lens=state["lens"].clone()), False)
+    bad = dict(state)
+    args = [mod, x, q, None, c, None]
+    if spoil == "grad":
+        args[4] = c.clone().requires_grad_(True)
+    elif spoil == "heads":
+        args[2] = torch.cat([q, q], 2)                # found after the tokens are written
+    else:
+        bad["block_table"] = state["block_table"][:1]
+    with pytest.raises(RuntimeError):
+        with torch.set_grad_enabled(spoil == "grad"):
+            kb.latent.mla_step(*args, bad, True)
+    assert state["lens"].tolist() == [0, 0]
+    with torch.no_grad():
+        out = kb.latent.mla_step(mod, x, q, None, c, None, state, False)
+    assert torch.equal(out, want) and state["lens"].tolist() == [3, 3]
