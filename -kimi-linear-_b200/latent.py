@@ -52,7 +52,11 @@ class LatentCache:
     ``page_size``: a power of two from 16 to 1024; ``kv_lora_rank`` 128, 256,
     384 or 512; ``rope_dim`` 0 or 64; ``dtype`` (of the latents, queries and
     outputs) fp16 or bf16.  Slots are written before they are read, so the
-    memory starts uninitialised."""
+    memory starts uninitialised.
+
+    The attributes are read-only (the tensors' values are not): calls pass the
+    addresses that the cache was made with.  A pool that moves or grows is
+    another cache (:meth:`from_tensors`)."""
 
     def __init__(self, num_pages, page_size, kv_lora_rank, rope_dim=0, dtype=torch.bfloat16,
                  device="cuda"):
@@ -105,9 +109,6 @@ class LatentCache:
         if pages < 1 or page < 16 or page > 1024 or page & (page - 1) or pages * page >= 2 ** 31:
             raise RuntimeError(f"{fn}: {pages} pages of {page} tokens not supported (page_size a "
                                f"power of two from 16 to 1024, fewer than 2^31 tokens)")
-        self.codes, self.scales, self.rope = codes, scales, rope
-        self.dtype, self.device, self.on_gpu = dtype, codes.device, codes.is_cuda
-        self.num_pages, self.page_size, self.kv_lora_rank, self.rope_dim = pages, page, kvl, dr
         a = _lib.MlaCacheArgs()
         a.abi_version = _lib.ABI_VERSION
         a.io_dtype = _DT[dtype]
@@ -116,7 +117,20 @@ class LatentCache:
         a.scales, a.scales_stride = scales.data_ptr(), scales.stride(0)
         if rope is not None:
             a.rope, a.rope_stride = rope.data_ptr(), _I64x2(*rope.stride()[:2])
-        self._args = bytes(a)
+        self.__dict__.update(
+            codes=codes, scales=scales, rope=rope, dtype=dtype, device=codes.device,
+            on_gpu=codes.is_cuda, num_pages=pages, page_size=page, kv_lora_rank=kvl, rope_dim=dr,
+            _args=bytes(a))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"LatentCache.{name} is read-only; make another cache of other "
+                             f"tensors with LatentCache.from_tensors")
+
+    def __delattr__(self, name):
+        self.__setattr__(name, None)
+
+    def __reduce__(self):        # a copy has the addresses of its own tensors
+        return LatentCache.from_tensors, (self.codes, self.scales, self.rope, self.dtype)
 
 
 def _refuse(fn, cache, name, t):

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import copy
 import types
 
 import pytest
@@ -34,3 +35,30 @@ def test_a_refused_step_leaves_the_lengths_alone(spoil):
         with pytest.raises((RuntimeError, TypeError)):
             pkg().latent.mla_step(*args, True)
         assert args[6]["lens"].tolist() == [3, 5]
+
+
+def test_the_pool_of_a_cache_is_fixed():
+    """The kernels' argument block holds the pool's addresses and sizes, so none of them can
+    be replaced behind it; a larger pool is another cache."""
+    kb = pkg()
+    c = kb.LatentCache(2, 16, 128, 64, device="cpu")
+    other = kb.LatentCache(4, 16, 128, 64, device="cpu")
+    for name in ("codes", "scales", "rope", "dtype", "device", "num_pages", "page_size",
+                 "kv_lora_rank", "rope_dim"):
+        before = getattr(c, name)
+        with pytest.raises(AttributeError, match="from_tensors"):
+            setattr(c, name, getattr(other, name))
+        with pytest.raises(AttributeError, match="from_tensors"):
+            delattr(c, name)
+        assert getattr(c, name) is before
+    grown = kb.LatentCache.from_tensors(other.codes, other.scales, other.rope)
+    assert grown.num_pages == 4 and grown.codes is other.codes
+
+
+def test_a_copied_cache_has_its_own_addresses():
+    kb = pkg()
+    c = kb.LatentCache(2, 16, 128, 64, device="cpu")
+    for other, own in ((copy.deepcopy(c), True), (copy.copy(c), False)):
+        a = kb._lib.MlaCacheArgs.from_buffer_copy(other._args)
+        assert (a.codes, a.scales, a.rope) == tuple(t.data_ptr() for t in (other.codes, other.scales, other.rope))
+        assert (other.codes.data_ptr() != c.codes.data_ptr()) == own and other.dtype is c.dtype
