@@ -346,6 +346,15 @@ __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
       "r"(bytes)
       : "memory");
 }
+// bytes that a barrier expects and that will not come
+__device__ __forceinline__ void give_back(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 x;\n\t"
+      "elect.sync x|e, 0xffffffff;\n\t"
+      "@e mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
                                          uint32_t bar) {
   asm volatile(
@@ -735,7 +744,11 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
           for (int c = 0; c < tile_chunks; ++c) {
             const int need = places.held_by(k, c);
             if (need > freed) {
-              if (!wait(&sh.freed[half_barrier(need)], half_parity(need), ab)) { ok = false; break; }
+              if (!wait(&sh.freed[half_barrier(need)], half_parity(need), ab)) {
+                for (int h = 0; h < 2; ++h) give_back(bar + 8 * h, nbox * box_rows * 128 * places.missing(c, h));
+                ok = false;
+                break;
+              }
               freed = need;
             }
             const int code = c - (tile_chunks - NCH);
@@ -748,7 +761,7 @@ cache_attn_kernel(const CacheParams p, const Work w, const __grid_constant__ CUt
         }
       }
       if (*ab) {                                  // copies in flight land before the block ends
-        for (int i = max(0, 2 * k - 6); i <= 2 * k + 1; ++i) drain(&sh.full[half_barrier(i)], half_parity(i));
+        for (int i = first_in_flight(k); i < 2 * k; ++i) drain(&sh.full[half_barrier(i)], half_parity(i));
       }
       __syncwarp();
     } else if (warp == 9) {

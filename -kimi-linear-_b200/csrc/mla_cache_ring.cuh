@@ -30,6 +30,13 @@ KDA_RING_FN constexpr unsigned half_parity(int half_tile) {
   return static_cast<unsigned>(half_tile) / (2 * kStages) & 1;
 }
 
+// Copies may be in flight for the half tiles from this one up to 2 tiles - 1, when `tiles`
+// tiles have been armed: a ring's worth and the last one, which may have found no place;
+// each has a barrier of its own.
+KDA_RING_FN constexpr int first_in_flight(int tiles) {
+  return tiles <= kRingTiles ? 0 : 2 * (tiles - kRingTiles - 1);
+}
+
 struct Ring {
   int tile_chunks, half;
   int ahead, spare;              // the ring in tiles, and the chunks over
@@ -39,6 +46,12 @@ struct Ring {
   KDA_RING_FN int held_by(int k, int c) const {
     const int j = k - ahead - (c < spare), old = c - spare + (c < spare ? tile_chunks : 0);
     return 2 * j + (old >= half);
+  }
+  // A loader that gives up before chunk c of a tile has armed the whole tile: how many
+  // chunks of half h it has not asked for.  With their bytes given back, what is armed
+  // completes once the copies in flight have landed.
+  KDA_RING_FN int missing(int c, int h) const {
+    return h == 0 ? (c < half ? half - c : 0) : tile_chunks - (c < half ? half : c);
   }
 };
 
