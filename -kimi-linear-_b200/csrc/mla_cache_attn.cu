@@ -71,7 +71,7 @@ constexpr int kMaxRanges = 256;            // blocks (SMs) that a call's tiles a
 constexpr int kSmemMax = 232448;           // 227 KB per block
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kUnset = -1e30f;           // maximum of a row that has seen nothing
+constexpr float kUnset = -3.4e38f;         // maximum of a row that has seen nothing: below any score
 
 // e4m3 terms of a query, each 16 times finer: two hold bf16's 8 bits, three fp16's 11.
 // (Values below 2^-12 of the row's largest are off by at most 2^-19 (2^-23) of it: the

@@ -197,3 +197,25 @@ def test_a_refused_layer_step_changes_nothing(spoil, cuda_dev):
     with torch.no_grad():
         out = kb.latent.mla_step(mod, x, q, None, c, None, state, False)
     assert torch.equal(out, want) and state["lens"].tolist() == [3, 3]
+
+
+@pytest.mark.parametrize("lens", [[40], [4000]])
+def test_scores_far_below_zero(lens, cuda_dev):
+    """Scores of -1e31 and less: a row has seen something, however low its maximum."""
+    m = make(lens, [1], H=3, KVL=128, dt=BF16, seed=23)
+    L = lens[0]
+    slot = (m.table[0].long().cpu()[torch.arange(L) // 64] * 64 + torch.arange(L) % 64)
+    c = torch.zeros(L, 128)
+    c[:, 0] = 2.0 ** 41
+    c[L // 2, 0] = 2.0 ** 40                          # the least low: all of the weight
+    c[:, 1] = torch.arange(L) % 15 * 2.0 ** 38
+    s = 2.0 ** 33
+    m.cache.codes.view(torch.uint8).view(-1, 128)[slot.to(m.dev)] = \
+        (c / s).to(torch.float8_e4m3fn).view(torch.uint8).to(m.dev)
+    m.cache.scales.view(-1)[slot.to(m.dev)] = s
+    m.c = [c.double()]
+    m.q.zero_()
+    m.q[..., 0] = -2.0 ** 68
+    out, lse = attend(m)
+    assert bool((lse < -1e30).all()) and bool(torch.isfinite(lse).all())
+    check(m, out, lse)
