@@ -35,9 +35,9 @@
 // warps 0-7 do the softmax, half of the rows each four, a position a thread.
 //
 // Measured (B200, 16 heads, KVL 512, inputs that rotate past L2, join included):
-//   one token each for 8 sequences of 32768, bf16     35.3 us, 3.8 TB/s of the cache
-//   one token each for 64 sequences of 300 to 8192    36.0 us, 3.3 TB/s
-//   512 tokens of one prompt against 8192 positions   212.6 us, 666 TFLOP/s as counted
+//   one token each for 8 sequences of 32768, bf16     35.6 us, 3.8 TB/s of the cache
+//   one token each for 64 sequences of 300 to 8192    36.2 us, 3.3 TB/s
+//   512 tokens of one prompt against 8192 positions   215.7 us, 656 TFLOP/s as counted
 //     (4 KVL for a row and key), 2.5 times that as executed on the terms
 // What bounds it: at 16 rows a tile takes the time of its 64 KB from HBM (1.5 us for
 // each SM), and around the tiles stand 7.5 us until the first scores (lengths, page
@@ -158,7 +158,8 @@ struct Work {
 // Sequence b as R-row groups.  A group counts for its tiles and kSetup more: what
 // its queries, its first tile's latency and its result cost (3, 4 and 5, us: 64
 // sequences of 300 to 8192 tokens 36.9, 36.0, 38.1; prompts of 1 to 1500 tokens 226,
-// 225, 221; 4 sequences of 8192 20.3, 19.9, 20.2).  Groups of one sequence see more and
+// 225, 221; 4 sequences of 8192 20.3, 19.9, 20.2; all at KVL 512 and 16 heads, the count is
+// the same for other widths).  Groups of one sequence see more and
 // more positions; they are counted in pairs (g, groups - 1 - g), which all count about
 // the same, so that a place in the count is found by a division.
 constexpr int kSetup = 4;
@@ -1283,7 +1284,8 @@ int q_terms(int io_dtype) {
 // whole: no workspace and no second launch.  Up to 4 tiles (one token for each of B
 // sequences of 512, 16 heads, KVL 512; whole and split, us): B = 1 11.7 and 11.8, B = 16
 // 12.3 and 13.7; at 768 14.5 and 11.9, 15.1 and 14.8.  Up to 8 tiles where 64 groups or
-// more occupy the SMs anyhow: B = 64 at 1024 19.0 and 23.5, at 2048 30.6 and 28.5.
+// more occupy the SMs anyhow: B = 64 at 1024 19.0 and 23.5, at 2048 30.6 and 28.5.  (Not
+// swept at other widths.)
 bool whole_groups(const CacheParams& p, int R) {
   const int64_t groups = max((int64_t)min(p.B, p.N), (int64_t)p.N * p.H / R);
   return (int64_t)p.max_pages * p.page_size <= (groups >= 64 ? 8 : 4) * TILE;
@@ -1292,7 +1294,8 @@ bool whole_groups(const CacheParams& p, int R) {
 // Rows per group: 16 where the sequences of the call have no more rows than that on
 // average, or where 32 rows leave too small a ring; else 32.  (16 sequences of 4096, 16
 // and 32 rows a group, us: 16 rows a sequence 18.5 and 22.9, 32 rows 25.0 and 25.6, 48
-// rows 37.0 and 32.9; 128 tokens of one prompt 64.9 and 50.0.)
+// rows 37.0 and 32.9; 128 tokens of one prompt 64.9 and 50.0; KVL 512, other widths were not
+// swept.)
 int rows_per_group(const CacheParams& p, int q_terms) {
   if ((int64_t)p.N * p.H <= (int64_t)p.B * 16) return 16;
   return ring_chunks(p.KVL, p.DR, q_terms, 32) >= 2 * tile_chunks(p.KVL, p.DR) ? 32 : 16;

@@ -244,7 +244,8 @@ def latent_read(cache, block_table, lens, num_tokens, q_start=None):
     """``(c_kv [N, kv_lora_rank], k_rope [N, rope_dim] or None)`` of the last
     ``n`` tokens of every sequence, ``N = num_tokens`` in all (``n`` from
     ``q_start``, or ``N / B`` each): what :func:`latent_append` of the same
-    arguments wrote, as values.  Zeros for tokens whose position is negative."""
+    arguments wrote, as values (an fp16 latent of 63488 or more may have gone up to
+    65536, which reads as infinity).  Zeros for tokens whose position is negative."""
     fn = "latent_read"
     N, dev = int(num_tokens), cache.device
     if N < 0:
