@@ -18,6 +18,7 @@ ABI_VERSION = 2
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 FLAG_FORCE_SIMT = 1
+NORM_NONE, NORM_RMS, NORM_L2 = 0, 1, 2
 
 # kda_status_t
 KDA_OK = 0
@@ -57,6 +58,15 @@ EXPORTED = (
     "mla_cache_attention",
     "mla_cache_workspace_bytes",
     "mla_cache_args_size",
+    "kda_scan_fwd",
+    "kda_scan_bwd",
+    "kda_scan_step",
+    "kda_scan_ckpt_floats",
+    "kda_scan_args_size",
+    "kda_qk_fwd",
+    "kda_qk_bwd",
+    "kda_qk_partial_floats",
+    "kda_qk_args_size",
     "kda_args_size",
     "kda_abi_version",
 )
@@ -227,6 +237,60 @@ class MlaCacheArgs(ctypes.Structure):
     ]
 
 
+class KdaScanArgs(ctypes.Structure):
+    """Mirror of ``struct KdaScanArgs``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32), ("g_dtype", ctypes.c_int32),
+        ("complement", ctypes.c_int32),
+        ("num_states", ctypes.c_int32), ("scatter", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("x_stride", _I64x2),
+        ("g", ctypes.c_void_p), ("g_stride", _I64x2),
+        ("state_in", ctypes.c_void_p), ("state_in_stride", ctypes.c_int64),
+        ("q_start", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("h", ctypes.c_void_p), ("h_stride", _I64x2),
+        ("state_out", ctypes.c_void_p), ("state_out_stride", ctypes.c_int64),
+        ("ckpt", ctypes.c_void_p),
+        ("dh", ctypes.c_void_p), ("dh_stride", _I64x2),
+        ("dstate_out", ctypes.c_void_p), ("dstate_out_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p), ("dx_stride", _I64x2),
+        ("dg", ctypes.c_void_p), ("dg_stride", _I64x2),
+        ("dstate_in", ctypes.c_void_p), ("dstate_in_stride", ctypes.c_int64),
+    ]
+
+
+_I64x3x2 = _I64x3 * 2
+_P2 = ctypes.c_void_p * 2
+
+
+class KdaQkArgs(ctypes.Structure):
+    """Mirror of ``struct KdaQkArgs``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("R", ctypes.c_int32),
+        ("heads", ctypes.c_int32 * 2),
+        ("io_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("w_heads", ctypes.c_int32),
+        ("pos_64", ctypes.c_int32), ("pos_step", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("x", _P2), ("x_stride", _I64x3x2),
+        ("w", _P2),
+        ("positions", ctypes.c_void_p), ("pos_stride", _I64x2),
+        ("inv_freq", ctypes.c_void_p),
+        ("y", _P2), ("y_stride", _I64x3x2),
+        ("dy", _P2), ("dy_stride", _I64x3x2),
+        ("dx", _P2), ("dx_stride", _I64x3x2),
+        ("dw", _P2),
+        ("partial", ctypes.c_void_p), ("partial_floats", ctypes.c_size_t),
+    ]
+
+
 class KdaLibraryError(RuntimeError):
     """The CUDA library is missing or unusable (there is no fallback path)."""
 
@@ -271,6 +335,22 @@ def _declare(lib):
     lib.mla_cache_workspace_bytes.restype = ctypes.c_size_t
     lib.mla_cache_args_size.argtypes = []
     lib.mla_cache_args_size.restype = ctypes.c_size_t
+    S = ctypes.POINTER(KdaScanArgs)
+    for fn in ("kda_scan_fwd", "kda_scan_bwd", "kda_scan_step"):
+        getattr(lib, fn).argtypes = [S, ctypes.c_void_p]
+        getattr(lib, fn).restype = ctypes.c_int
+    lib.kda_scan_ckpt_floats.argtypes = [S]
+    lib.kda_scan_ckpt_floats.restype = ctypes.c_size_t
+    lib.kda_scan_args_size.argtypes = []
+    lib.kda_scan_args_size.restype = ctypes.c_size_t
+    Q = ctypes.POINTER(KdaQkArgs)
+    for fn in ("kda_qk_fwd", "kda_qk_bwd"):
+        getattr(lib, fn).argtypes = [Q, ctypes.c_void_p]
+        getattr(lib, fn).restype = ctypes.c_int
+    lib.kda_qk_partial_floats.argtypes = [Q]
+    lib.kda_qk_partial_floats.restype = ctypes.c_size_t
+    lib.kda_qk_args_size.argtypes = []
+    lib.kda_qk_args_size.restype = ctypes.c_size_t
     lib.kda_backward.argtypes = [ctypes.POINTER(KdaBackwardArgs), ctypes.c_void_p]
     lib.kda_backward.restype = ctypes.c_int
     lib.kda_backward_ckpt_floats.argtypes = [ctypes.c_int] * 5
@@ -312,7 +392,9 @@ def load(path: str | None = None):
                        ("kda_epilogue_args_size", KdaEpilogueArgs),
                        ("kda_backward_args_size", KdaBackwardArgs),
                        ("mla_decode_args_size", MlaDecodeArgs),
-                       ("mla_cache_args_size", MlaCacheArgs)):
+                       ("mla_cache_args_size", MlaCacheArgs),
+                       ("kda_scan_args_size", KdaScanArgs),
+                       ("kda_qk_args_size", KdaQkArgs)):
             if getattr(lib, fn)() != ctypes.sizeof(st):
                 raise KdaLibraryError(f"{p}: {fn}() != ctypes sizeof {ctypes.sizeof(st)}")
         if lib.kda_args_size() != ctypes.sizeof(KdaArgs):

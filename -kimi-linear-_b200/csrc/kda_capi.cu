@@ -374,8 +374,9 @@ int kda_device_error(int clear) {
   const int b = kda::mla::read_device_error(clear != 0);
   const int c = kda::cache::read_device_error(clear != 0);
   const int d = kda::cache::read_attn_device_error(clear != 0);
-  if (a < 0 || b < 0 || c < 0 || d < 0) return -1;
-  return a ? a : b ? b : c ? c : d;
+  const int e = kda::scan::read_device_error(clear != 0);
+  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0) return -1;
+  return a ? a : b ? b : c ? c : d ? d : e;
 }
 
 int kda_prologue_fwd(const KdaPrologueArgs* args, void* stream) {

@@ -45,6 +45,9 @@ namespace cache {
 int read_device_error(bool clear);        // latent cache append / read (mla_cache.cu)
 int read_attn_device_error(bool clear);   // latent cache attention (mla_cache_attn.cu)
 }
+namespace scan {
+int read_device_error(bool clear);   // gated recurrence (kda_scan.cu)
+}
 
 constexpr int kRecMaxK = 256;    // recurrent kernel: K <= 256, any V
 constexpr int kSimtMaxK = 256;   // SIMT chunkwise kernel: K <= 256, any V

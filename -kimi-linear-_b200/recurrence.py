@@ -1,0 +1,252 @@
+"""Gated linear recurrence, channel by channel (``csrc/kda_scan.cu``).
+
+Beside the delta-rule recurrence of :mod:`ops` (a K x V state per head), the
+elementwise one of gated linear RNN layers, with the same kind of gate::
+
+    h_t = a_t h_{t-1} + w_t x_t,    a_t = exp(g_t),    w_t = 1  or, complement=True,  1 - a_t
+
+``g`` is a log decay (``<= 0``; ``-inf`` forgets everything before the token), fp32 or
+in ``x``'s type, as ``kda_prologue`` leaves it for KDA.  States are fp32 throughout.
+
+* :func:`gated_scan`: whole sequences (prompts, training), a batch ``[B, T, D]``
+  or sequences packed one behind the other;
+* :func:`gated_step`: one token for each row of a serving batch;
+* :func:`gated_scan_backward`: the gradient, which autograd calls.
+
+As elsewhere in the package: CUDA tensors only (no fallback), the current
+stream of the inputs' device, nothing synchronises or is read on the host, so calls
+can be captured in CUDA graphs.  Nothing is kept between calls.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import _DT, _call, _check_tensors, _needs_grad
+
+_I64x2 = ctypes.c_int64 * 2
+
+
+def _unit(t):
+    """``t`` with a unit innermost stride."""
+    return t if t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
+
+
+def _bt(t, packed):
+    """(batch, token) strides."""
+    return _I64x2(0, t.stride(0)) if packed else _I64x2(t.stride(0), t.stride(1))
+
+
+def _check(fn, x, g, state, rows, others=()):
+    """Device of the operands, after checks of types and shapes."""
+    dev = _check_tensors(fn, [("x", x), ("g", g), ("state", state), *others])
+    if g is None or x.shape != g.shape:
+        raise RuntimeError(f"{fn}: x {tuple(x.shape)} and g "
+                           f"{None if g is None else tuple(g.shape)} differ in shape")
+    if g.dtype not in (torch.float32, x.dtype):
+        raise TypeError(f"{fn}: g must be float32 or {x.dtype} (got {g.dtype})")
+    if state is not None and tuple(state.shape) != (rows, x.shape[-1]):
+        raise RuntimeError(f"{fn}: state shape {tuple(state.shape)} != {(rows, x.shape[-1])}")
+    return dev
+
+
+def _batch(fn, x, q_start):
+    """Number of sequences of ``x``, after checks of what says so."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{fn}: x must be a torch.Tensor")
+    if q_start is None:
+        if x.dim() != 3:
+            raise RuntimeError(f"{fn}: expected x, g [B, T, D] (or [N, D] with q_start); got "
+                               f"{tuple(x.shape)}")
+        return x.shape[0]
+    if x.dim() != 2:
+        raise RuntimeError(f"{fn}: expected x, g [N, D] with q_start; got {tuple(x.shape)}")
+    if not isinstance(q_start, torch.Tensor) or q_start.dtype != torch.int32 or q_start.dim() != 1 \
+            or q_start.device != x.device or q_start.shape[0] < 1 \
+            or (q_start.shape[0] > 1 and q_start.stride(0) != 1):
+        raise RuntimeError(f"{fn}: q_start must be an int32 tensor [sequences + 1] with a unit stride "
+                           f"on {x.device}")
+    return q_start.shape[0] - 1
+
+
+def _fill(x, g, state, q_start, complement):
+    packed = q_start is not None
+    a = _lib.KdaScanArgs()
+    a.abi_version = _lib.ABI_VERSION
+    a.B = q_start.shape[0] - 1 if packed else x.shape[0]
+    a.T, a.D = x.shape[-2], x.shape[-1]
+    a.x_dtype, a.g_dtype = _DT[x.dtype], _DT[g.dtype]
+    a.complement = 1 if complement else 0
+    a.x, a.x_stride = x.data_ptr(), _bt(x, packed)
+    a.g, a.g_stride = g.data_ptr(), _bt(g, packed)
+    if state is not None:
+        a.state_in, a.state_in_stride = state.data_ptr(), state.stride(0)
+    if packed:
+        a.q_start = q_start.data_ptr()
+    return a
+
+
+def _forward(x, g, state, q_start, complement, keep):
+    """``(h, S, checkpoints)`` for operands that :func:`_check` has passed;
+    ``keep``: checkpoints for the backward pass are wanted."""
+    x, g = _unit(x), _unit(g)
+    state = None if state is None else _unit(state.float())
+    a = _fill(x, g, state, q_start, complement)
+    h = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    S = torch.empty((a.B, a.D), device=x.device, dtype=torch.float32)
+    a.h, a.h_stride = h.data_ptr(), _bt(h, q_start is not None)
+    a.state_out, a.state_out_stride = S.data_ptr(), a.D
+    lib = _lib.load()
+    ckpt = None
+    if keep:
+        ckpt = torch.empty(int(lib.kda_scan_ckpt_floats(ctypes.byref(a))), device=x.device,
+                           dtype=torch.float32)
+        a.ckpt = ckpt.data_ptr()
+    _call("gated_scan", lib.kda_scan_fwd, a, x.device)
+    return h, S, ckpt
+
+
+def gated_scan(x, g, initial_state=None, q_start=None, *, complement=False):
+    """``(h, S)``: every ``h_t``, in ``x``'s type, and every sequence's last one, fp32.
+
+    ``x`` and ``g`` ``[B, T, D]`` with ``initial_state`` ``[B, D]`` (None: zeros), or
+    packed: ``x`` and ``g`` ``[N, D]``, ``q_start`` int32 ``[B + 1]`` on the device, ascending:
+    sequence ``b`` owns rows ``q_start[b] .. q_start[b + 1] - 1`` and starts from
+    ``initial_state[b]``.  Rows before ``q_start[0]`` and from ``q_start[B]`` on belong to
+    no sequence and give zeros; a sequence without rows gives its initial state.
+
+    Differentiable in ``x``, ``g`` and ``initial_state``.  ``x`` f32, f16 or bf16,
+    ``g`` fp32 or ``x``'s type.  A state of any type is read as fp32."""
+    fn = "gated_scan"
+    B = _batch(fn, x, q_start)
+    if _needs_grad(x, g, initial_state):
+        with torch.no_grad():
+            _check(fn, x, g, initial_state, B)
+        return _GatedScan.apply(x, g, initial_state, q_start, bool(complement))
+    _check(fn, x, g, initial_state, B)
+    return _forward(x, g, initial_state, q_start, complement, False)[:2]
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, g, state, q_start, complement):
+        h, S, ckpt = _forward(x, g, state, q_start, complement, True)
+        ctx.save_for_backward(x, g, state, q_start, ckpt)
+        ctx.complement = complement
+        ctx.set_materialize_grads(False)
+        return h, S
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dS):
+        x, g, state, q_start, ckpt = ctx.saved_tensors
+        grads = _backward(x, g, state, q_start, ctx.complement, ckpt, dh, dS,
+                          ctx.needs_input_grad[:3])
+        return (*grads, None, None)
+
+
+def _backward(x, g, state, q_start, complement, ckpt, dh, dS, need):
+    packed = q_start is not None
+    x, g = _unit(x), _unit(g)
+    state32 = None if state is None else _unit(state.float())
+    a = _fill(x, g, state32, q_start, complement)
+    a.ckpt = ckpt.data_ptr()
+    if dh is not None:
+        dh = _unit(dh.to(x.dtype))
+        a.dh, a.dh_stride = dh.data_ptr(), _bt(dh, packed)
+    if dS is not None:
+        dS = _unit(dS.float())
+        a.dstate_out, a.dstate_out_stride = dS.data_ptr(), dS.stride(0)
+    dx = dg = dstate = None
+    if need[0]:
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        a.dx, a.dx_stride = dx.data_ptr(), _bt(dx, packed)
+    if need[1]:
+        dg = torch.empty(g.shape, device=x.device, dtype=g.dtype)
+        a.dg, a.dg_stride = dg.data_ptr(), _bt(dg, packed)
+    if need[2] and state is not None:
+        dstate = torch.empty(state.shape, device=x.device, dtype=torch.float32)
+        a.dstate_in, a.dstate_in_stride = dstate.data_ptr(), a.D
+    _call("gated_scan_backward", _lib.load().kda_scan_bwd, a, x.device)
+    return dx, dg, None if dstate is None else dstate.to(state.dtype)
+
+
+def gated_scan_backward(x, g, initial_state, dh, dS, q_start=None, *, complement=False):
+    """Gradients ``(dx, dg, dinitial_state)`` of :func:`gated_scan` for output
+    gradients ``dh`` (of ``h``, or None) and ``dS`` (of ``S``, or None).
+
+    Runs the forward pass again for its checkpoints; autograd keeps those of
+    the call that it differentiates."""
+    fn = "gated_scan_backward"
+    B = _batch(fn, x, q_start)
+    _check(fn, x, g, initial_state, B, [("dh", dh), ("dS", dS)])
+    if dh is not None and dh.shape != x.shape:
+        raise RuntimeError(f"{fn}: dh shape {tuple(dh.shape)} != {tuple(x.shape)}")
+    if dS is not None and tuple(dS.shape) != (B, x.shape[-1]):
+        raise RuntimeError(f"{fn}: dS shape {tuple(dS.shape)} != {(B, x.shape[-1])}")
+    ckpt = _forward(x, g, initial_state, q_start, complement, True)[2]
+    return _backward(x, g, initial_state, q_start, bool(complement), ckpt, dh, dS, (True, True, True))
+
+
+def gated_step(x, g, state=None, slots=None, *, complement=False, inplace=False):
+    """One token: ``(h, S)`` for ``x`` and ``g`` ``[B, D]`` (or ``[B, 1, D]``, then ``h`` is too).
+
+    ``state`` fp32 ``[B, D]`` (None: zeros).  With ``slots`` int32 ``[B]``, row ``b``'s
+    state is row ``slots[b]`` of a pool ``state`` ``[num_states, D]``; a negative slot marks an
+    idle row, whose ``h`` and ``S`` are zeros.  (A slot past the pool counts as idle and
+    sets the device error word: :func:`ops.device_error` returns 8.)  ``S`` ``[B, D]`` is a
+    new tensor; ``inplace=True`` writes the new states where the old ones were and
+    returns ``state`` itself (idle rows leave it alone; no slot twice in a call).
+    Forward only: :func:`gated_scan` with ``T = 1`` is the differentiable form."""
+    fn = "gated_step"
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{fn}: x must be a torch.Tensor")
+    if x.dim() not in (2, 3) or (x.dim() == 3 and x.shape[1] != 1):
+        raise RuntimeError(f"{fn}: expected x, g [B, D] or [B, 1, D]; got {tuple(x.shape)}")
+    shape = x.shape
+    if not isinstance(g, torch.Tensor) or g.shape != shape:
+        raise RuntimeError(f"{fn}: g must be a tensor of x's shape {tuple(shape)}")
+    if x.dim() == 3:
+        x, g = x[:, 0], g[:, 0]
+    B, D = x.shape
+    rows = B
+    if slots is not None:
+        if not isinstance(state, torch.Tensor) or state.dim() != 2:
+            raise RuntimeError(f"{fn}: slots need a state [num_states, {D}]")
+        if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int32 or \
+                tuple(slots.shape) != (B,) or slots.device != x.device or (B > 1 and slots.stride(0) != 1):
+            raise RuntimeError(f"{fn}: slots must be an int32 tensor [{B}] with a unit stride on {x.device}")
+        rows = state.shape[0]
+    dev = _check(fn, x, g, state, rows)
+    if state is not None and state.dtype != torch.float32:
+        raise TypeError(f"{fn}: state must be float32 (got {state.dtype})")
+    if inplace:
+        if state is None:
+            raise RuntimeError(f"{fn}: inplace needs a state")
+        if (D > 1 and state.stride(1) != 1) or (rows > 1 and state.stride(0) < D):
+            raise RuntimeError(f"{fn}: inplace needs states with a unit innermost stride that do not "
+                               f"overlap")
+    elif state is not None:
+        state = _unit(state)
+    x, g = _unit(x), _unit(g)
+    h = torch.empty(shape, device=dev, dtype=x.dtype)
+    S = state if inplace else torch.empty((B, D), device=dev, dtype=torch.float32)
+    a = _lib.KdaScanArgs()
+    a.abi_version = _lib.ABI_VERSION
+    a.B, a.T, a.D = B, 1, D
+    a.x_dtype, a.g_dtype = _DT[x.dtype], _DT[g.dtype]
+    a.complement = 1 if complement else 0
+    a.scatter = 1 if inplace else 0
+    a.x, a.x_stride[0] = x.data_ptr(), x.stride(0)
+    a.g, a.g_stride[0] = g.data_ptr(), g.stride(0)
+    a.h, a.h_stride[0] = h.data_ptr(), D
+    if state is not None:
+        a.state_in, a.state_in_stride = state.data_ptr(), state.stride(0)
+    a.state_out, a.state_out_stride = S.data_ptr(), S.stride(0)
+    if slots is not None:
+        a.slots, a.num_states = slots.data_ptr(), rows
+    _call(fn, _lib.load().kda_scan_step, a, dev)
+    return h, S

@@ -11,7 +11,10 @@
  * (kda_backward) and the static-buffer MLA decode step of the full-attention
  * layers (mla_decode_fwd, kimi_linear/mla.py:117-181); and, for serving those
  * layers, a paged latent cache in 8 bits with the attention over it
- * (mla_cache_append, mla_cache_read, mla_cache_attention).
+ * (mla_cache_append, mla_cache_read, mla_cache_attention).  Beside the core: a
+ * gated linear recurrence with its gradient and single-token step (kda_scan_fwd,
+ * kda_scan_bwd, kda_scan_step), and the norm and rotation of queries and keys
+ * with its gradient (kda_qk_fwd, kda_qk_bwd).
  *
  * Plain pointers, sizes and element strides only.  The Python host layer
  * (-kimi-linear-_b200/ops.py) keeps the reference's Python signatures and
@@ -152,8 +155,8 @@ int kda_device_supported(int device);
 
 /*
  * Error word written by a kernel that abandoned its work after a bounded wait
- * on the GPU ran out, or (MLA decode) found pos outside the buffer (0 = none);
- * clear != 0 resets it.  Synchronises with the device.  <0 on a CUDA error.
+ * on the GPU ran out, or found an index outside its buffer (MLA decode: pos; the
+ * latent cache: 6; the recurrence's step: 8) (0 = none); clear != 0 resets it.  Synchronises with the device.  <0 on a CUDA error.
  * No reference counterpart (diagnostic).
  */
 int kda_device_error(int clear);
@@ -408,6 +411,110 @@ size_t mla_cache_workspace_bytes(const MlaCacheArgs* args);
 
 /* sizeof(MlaCacheArgs) as compiled. */
 size_t mla_cache_args_size(void);
+
+/*
+ * Gated linear recurrence, channel by channel (no counterpart in the reference,
+ * whose recurrence is the delta rule with a K x V state):
+ *   h_t = a_t h_{t-1} + w_t x_t,  a_t = exp(g_t),  w_t = 1 (complement: 1 - a_t)
+ * over B sequences of T tokens, x, g, h [B, T, D], or, with q_start, over B
+ * sequences packed into T rows, x, g, h [T, D] (batch strides unused): sequence b owns
+ * rows q_start[b] .. q_start[b + 1] - 1; q_start ascends, rows outside
+ * q_start[0] .. q_start[B] - 1 get zeros.  h_{-1} is state_in [B, D] or zero,
+ * state_out [B, D] each sequence's last h (state_in where it has no token).
+ * g is a log decay (<= 0).  States are fp32.
+ *
+ * kda_scan_fwd: h, state_out, and (ckpt not NULL) what kda_scan_bwd needs:
+ *   kda_scan_ckpt_floats() values, the state that enters every 64th token.
+ * kda_scan_bwd: gradients dx, dg (types of x, g) and dstate_in (fp32), any of them
+ *   may be NULL, from dh (type of x) and dstate_out (either may be NULL: zero).
+ * kda_scan_step: one token for each of B rows: x, g, h [B, D] (T = 1, token strides
+ *   unused).  Row b's old state is row b of state_in, or row slots[b] of num_states;
+ *   state_out gets the new one: row b (dense), or row slots[b] (scatter = 1: a pool
+ *   updated in place, state_in == state_out; no slot twice in a call).  A row whose slot is
+ *   negative gives zeros (scatter: writes no state); one with a slot past num_states does the
+ *   same and sets the device error word (8).
+ */
+typedef struct KdaScanArgs {
+  int32_t abi_version;
+  int32_t B, T, D;
+  int32_t x_dtype, g_dtype;    /* g: fp32 or x's type */
+  int32_t complement;
+  int32_t num_states, scatter; /* step only */
+  int32_t reserved;
+  /* strides in elements (batch, token), unit channel stride */
+  const void* x;  int64_t x_stride[2];
+  const void* g;  int64_t g_stride[2];
+  const float* state_in; int64_t state_in_stride;
+  const int32_t* q_start;      /* [B + 1] or NULL */
+  const int32_t* slots;        /* [B] or NULL (step) */
+  void* h;        int64_t h_stride[2];
+  float* state_out; int64_t state_out_stride;
+  float* ckpt;
+  /* backward */
+  const void* dh; int64_t dh_stride[2];
+  const float* dstate_out; int64_t dstate_out_stride;
+  void* dx;       int64_t dx_stride[2];
+  void* dg;       int64_t dg_stride[2];
+  float* dstate_in; int64_t dstate_in_stride;
+} KdaScanArgs;
+
+int kda_scan_fwd(const KdaScanArgs* args, void* stream);
+int kda_scan_bwd(const KdaScanArgs* args, void* stream);
+int kda_scan_step(const KdaScanArgs* args, void* stream);
+
+/* fp32 values of KdaScanArgs.ckpt for these B, T, D (q_start set or not). */
+size_t kda_scan_ckpt_floats(const KdaScanArgs* args);
+
+/* sizeof(KdaScanArgs) as compiled. */
+size_t kda_scan_args_size(void);
+
+/*
+ * Queries and keys normalised per head and rotated by their token's position, in
+ * one pass (the norm: kimi_linear/kda.py:313-325 for KDA_NORM_L2, and with a weight
+ * :258-279 for KDA_NORM_RMS; the reference's layers have no rotation).
+ * Tensor 0 (queries) and 1 (keys; heads[1] = 0: none), each [B, T, heads, D]:
+ *   n = x r,  r = (mean x^2 + eps)^-1/2 (RMS), min(1 / |x|, 1 / eps) (L2) or 1 (NONE)
+ *   z = n w   (w [D] or, with w_heads, [heads, D]; NULL: 1)
+ *   y = z with channels 0 .. R - 1 rotated: pair i, channels (i, i + R / 2) or, with
+ *       interleaved, (2 i, 2 i + 1), by angle p inv_freq[i], computed in 64 bits
+ * Token t of sequence b sits at p = positions[b stride[0] + t stride[1]] + t pos_step
+ * (positions NULL: t pos_step).
+ * kda_qk_bwd: dx and dw (w's type; NULL: not wanted) from x and dy.  It needs
+ * kda_qk_partial_floats() fp32 values of scratch where a dw is wanted, and adds in a
+ * fixed order.
+ * Requires D <= 512, R even and <= D, eps >= 1e-12.
+ */
+enum { KDA_NORM_NONE = 0, KDA_NORM_RMS = 1, KDA_NORM_L2 = 2 };
+typedef struct KdaQkArgs {
+  int32_t abi_version;
+  int32_t B, T, D, R;
+  int32_t heads[2];
+  int32_t io_dtype, w_dtype;
+  int32_t norm, interleaved, w_heads;
+  int32_t pos_64, pos_step;    /* positions are int64 (else int32) */
+  float eps;
+  int32_t reserved;
+  /* strides in elements (batch, token, head), unit channel stride */
+  const void* x[2];  int64_t x_stride[2][3];
+  const void* w[2];            /* contiguous */
+  const void* positions; int64_t pos_stride[2];
+  const float* inv_freq;       /* [R / 2] */
+  void* y[2];        int64_t y_stride[2][3];
+  /* backward */
+  const void* dy[2]; int64_t dy_stride[2][3];
+  void* dx[2];       int64_t dx_stride[2][3];
+  void* dw[2];                 /* contiguous */
+  float* partial; size_t partial_floats;
+} KdaQkArgs;
+
+int kda_qk_fwd(const KdaQkArgs* args, void* stream);
+int kda_qk_bwd(const KdaQkArgs* args, void* stream);
+
+/* fp32 scratch of kda_qk_bwd for these sizes (0: none). */
+size_t kda_qk_partial_floats(const KdaQkArgs* args);
+
+/* sizeof(KdaQkArgs) as compiled. */
+size_t kda_qk_args_size(void);
 
 /* sizeof(KdaArgs) as compiled, for FFI layout checks. */
 size_t kda_args_size(void);
