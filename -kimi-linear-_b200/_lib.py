@@ -61,6 +61,7 @@ EXPORTED = (
     "kda_scan_fwd",
     "kda_scan_bwd",
     "kda_scan_step",
+    "kda_scan_workspace_bytes",
     "kda_scan_ckpt_floats",
     "kda_scan_args_size",
     "kda_qk_fwd",
@@ -260,6 +261,7 @@ class KdaScanArgs(ctypes.Structure):
         ("dx", ctypes.c_void_p), ("dx_stride", _I64x2),
         ("dg", ctypes.c_void_p), ("dg_stride", _I64x2),
         ("dstate_in", ctypes.c_void_p), ("dstate_in_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -339,8 +341,9 @@ def _declare(lib):
     for fn in ("kda_scan_fwd", "kda_scan_bwd", "kda_scan_step"):
         getattr(lib, fn).argtypes = [S, ctypes.c_void_p]
         getattr(lib, fn).restype = ctypes.c_int
-    lib.kda_scan_ckpt_floats.argtypes = [S]
-    lib.kda_scan_ckpt_floats.restype = ctypes.c_size_t
+    for fn in ("kda_scan_workspace_bytes", "kda_scan_ckpt_floats"):
+        getattr(lib, fn).argtypes = [S]
+        getattr(lib, fn).restype = ctypes.c_size_t
     lib.kda_scan_args_size.argtypes = []
     lib.kda_scan_args_size.restype = ctypes.c_size_t
     Q = ctypes.POINTER(KdaQkArgs)

@@ -89,6 +89,16 @@ def _fill(x, g, state, q_start, complement):
     return a
 
 
+def _workspace(a, q_start):
+    """Scratch for a packed batch, set in ``a``; the caller holds it through the call."""
+    if q_start is None:
+        return None
+    need = int(_lib.load().kda_scan_workspace_bytes(ctypes.byref(a)))
+    ws = torch.empty((need + 7) // 8, device=q_start.device, dtype=torch.int64)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    return ws
+
+
 def _forward(x, g, state, q_start, complement, keep):
     """``(h, S, checkpoints)`` for operands that :func:`_check` has passed;
     ``keep``: checkpoints for the backward pass are wanted."""
@@ -105,6 +115,7 @@ def _forward(x, g, state, q_start, complement, keep):
         ckpt = torch.empty(int(lib.kda_scan_ckpt_floats(ctypes.byref(a))), device=x.device,
                            dtype=torch.float32)
         a.ckpt = ckpt.data_ptr()
+    ws = _workspace(a, q_start)  # noqa: F841
     _call("gated_scan", lib.kda_scan_fwd, a, x.device)
     return h, S, ckpt
 
@@ -170,6 +181,7 @@ def _backward(x, g, state, q_start, complement, ckpt, dh, dS, need):
     if need[2] and state is not None:
         dstate = torch.empty(state.shape, device=x.device, dtype=torch.float32)
         a.dstate_in, a.dstate_in_stride = dstate.data_ptr(), a.D
+    ws = _workspace(a, q_start)  # noqa: F841
     _call("gated_scan_backward", _lib.load().kda_scan_bwd, a, x.device)
     return dx, dg, None if dstate is None else dstate.to(state.dtype)
 

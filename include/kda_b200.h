@@ -156,7 +156,9 @@ int kda_device_supported(int device);
 /*
  * Error word written by a kernel that abandoned its work after a bounded wait
  * on the GPU ran out, or found an index outside its buffer (MLA decode: pos; the
- * latent cache: 6; the recurrence's step: 8) (0 = none); clear != 0 resets it.  Synchronises with the device.  <0 on a CUDA error.
+ * latent cache: 6; the recurrence's step: 8) (0 = none); 9: a wait between the blocks of
+ * kda_scan_fwd or kda_scan_bwd ran out (its outputs are not valid); clear != 0
+ * resets it.  Synchronises with the device.  <0 on a CUDA error.
  * No reference counterpart (diagnostic).
  */
 int kda_device_error(int clear);
@@ -456,11 +458,15 @@ typedef struct KdaScanArgs {
   void* dx;       int64_t dx_stride[2];
   void* dg;       int64_t dg_stride[2];
   float* dstate_in; int64_t dstate_in_stride;
+  void* workspace; size_t workspace_bytes;   /* kda_scan_workspace_bytes(), 8-byte aligned */
 } KdaScanArgs;
 
 int kda_scan_fwd(const KdaScanArgs* args, void* stream);
 int kda_scan_bwd(const KdaScanArgs* args, void* stream);
 int kda_scan_step(const KdaScanArgs* args, void* stream);
+
+/* device scratch of kda_scan_fwd and kda_scan_bwd (0: none; packed batches have some). */
+size_t kda_scan_workspace_bytes(const KdaScanArgs* args);
 
 /* fp32 values of KdaScanArgs.ckpt for these B, T, D (q_start set or not). */
 size_t kda_scan_ckpt_floats(const KdaScanArgs* args);

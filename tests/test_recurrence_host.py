@@ -91,7 +91,8 @@ def test_scan_entry_points_refuse():
         for kw, want in ((dict(x_dtype=3), L.KDA_ERR_DTYPE), (dict(g_dtype=L.DTYPE_F16), L.KDA_ERR_DTYPE),
                          (dict(x=None), L.KDA_ERR_NULL_POINTER), (dict(g=None), L.KDA_ERR_NULL_POINTER),
                          (dict(x=FAKE + 1), L.KDA_ERR_ALIGNMENT), (dict(g=FAKE + 2), L.KDA_ERR_ALIGNMENT),
-                         (dict(q_start=FAKE + 2), L.KDA_ERR_ALIGNMENT), (dict(B=1 << 20), L.KDA_ERR_SHAPE)):
+                         (dict(q_start=FAKE + 2), L.KDA_ERR_ALIGNMENT), (dict(B=1 << 25), L.KDA_ERR_SHAPE),
+                         (dict(T=(1 << 30) + 1), L.KDA_ERR_SHAPE), (dict(q_start=FAKE), L.KDA_ERR_WORKSPACE)):
             assert fn(P(_scan_args(**kw)), None) == want, kw
         assert fn(P(_scan_args(D=0)), None) == L.KDA_OK
         assert fn(P(_scan_args(B=0)), None) == L.KDA_OK
@@ -103,6 +104,8 @@ def test_scan_entry_points_refuse():
     assert lib.kda_scan_step(P(_scan_args(**step, slots=FAKE, num_states=-1)), None) == L.KDA_ERR_SHAPE
     assert lib.kda_scan_step(P(_scan_args(**{**step, "state_in": FAKE + 64}, scatter=1)), None) == L.KDA_ERR_STRIDE
     assert lib.kda_scan_step(P(_scan_args(**{**step, "B": 0})), None) == L.KDA_OK
+    assert lib.kda_scan_workspace_bytes(P(_scan_args())) == 0
+    assert lib.kda_scan_workspace_bytes(P(_scan_args(T=65, q_start=FAKE))) == 2 * 24
     n = lib.kda_scan_ckpt_floats
     assert n(P(_scan_args(T=64))) == 2 * 16 and n(P(_scan_args(T=65))) == 2 * 2 * 16
     assert n(P(_scan_args(T=65, q_start=FAKE))) == 2 * 16 and n(P(_scan_args(T=0))) == 0
