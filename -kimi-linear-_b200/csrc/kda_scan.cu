@@ -24,12 +24,12 @@ namespace {
 // ---------------------------------------------------------------------------
 // packed batches: what each row is
 // ---------------------------------------------------------------------------
-// Blocks 0 .. tiles - 1: a tile each.  The others: a sequence without rows each, whose
+// Blocks below `marked`: kMarked rows each.  The others: a sequence without rows each, whose
 // state (gradient) goes through.
-__global__ void __launch_bounds__(kTile) mark_kernel(const ScanParams p, Marks* marks, const float* from,
-                                                     int64_t from_s, float* to, int64_t to_s) {
-  if ((int)blockIdx.x < p.tiles) {
-    const int t = blockIdx.x * kTile + threadIdx.x;
+__global__ void __launch_bounds__(kMarked) mark_kernel(const ScanParams p, int marked, Marks* marks,
+                                                       const float* from, int64_t from_s, float* to, int64_t to_s) {
+  if ((int)blockIdx.x < marked) {
+    const int t = blockIdx.x * kMarked + threadIdx.x;
     const int b = sequence_at(p.q_start, p.B, t);
     const int end = b >= 0 ? min(p.q_start[b + 1], p.T) : 0;
     const bool owned = end > t;
@@ -44,149 +44,204 @@ __global__ void __launch_bounds__(kTile) mark_kernel(const ScanParams p, Marks* 
     }
     return;
   }
-  const int b = blockIdx.x - p.tiles;
+  const int b = blockIdx.x - marked;
   const int lo = min(max(p.q_start[b], 0), p.T), hi = min(p.q_start[b + 1], p.T);
   if (to == nullptr || hi > lo) return;
-  for (int c = threadIdx.x; c < p.D; c += kTile) to[b * to_s + c] = from ? from[b * from_s + c] : 0.f;
+  for (int c = threadIdx.x; c < p.D; c += kMarked) to[b * to_s + c] = from ? from[b * from_s + c] : 0.f;
 }
 
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-constexpr int kStages = 2;
+constexpr int kWarps = 8;
+constexpr int kXSlots = 4, kGSlots = 2;
+using Fwd = Shape<kWarps>;
 
-template <typename TX, typename TG, bool WIDE, bool PACKED>
-__global__ void __launch_bounds__(kThreads, 3) scan_kernel(const ScanParams p) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ uint64_t full[2];
-  __shared__ __align__(16) float warps[2][kWarps * kPieceFloats];
-  using XRing = Ring<TX, WIDE, kStages>;
-  using GRing = Ring<TG, WIDE, kStages>;
-  const XRing xs(smem);
-  const GRing gs(smem + XRing::kBytes);
+struct Shared {
+  Parts<Fwd::kParts> parts[2];       // of two turns
+  uint64_t x_full[kXSlots], g_full[kGSlots], exchange[2];
+  uint8_t starts[2][Fwd::kParts];    // packed: a sequence starts in the part
+};
+
+template <typename TX, typename TG, bool WIDE, bool PACKED, bool COMPLEMENT>
+__global__ void __launch_bounds__(Fwd::kThreads, 2)
+scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap g_map) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  using XRing = Ring<TX, Fwd::kTile, kXSlots>;
+  using GRing = Ring<TG, Fwd::kTile, kGSlots>;
+  const XRing xs{smem};
+  const GRing gs{smem + XRing::kBytes};
+  Shared& sh = *reinterpret_cast<Shared*>(smem + XRing::kBytes + GRing::kBytes);
   const Place w = my_place<WIDE>(p);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % kLanes;
-  const bool upper = threadIdx.x % 32 >= kLanes;
+  const Exchange exchange(sh.exchange, reinterpret_cast<float*>(&sh + 1), p, w.rank);
+  Patience patience(&g_scan_device_error);
   const int turns = (p.tiles + p.cluster - 1) / p.cluster;
-  const int t_first = w.rank * kTile + w.run, t_step = p.cluster * kTile;
-  const TX* x = static_cast<const TX*>(p.x) + w.b * p.x_s[0] + (int64_t)t_first * p.x_s[1] + w.c;
-  const TG* g = static_cast<const TG*>(p.g) + w.b * p.g_s[0] + (int64_t)t_first * p.g_s[1] + w.c;
-  TX* out = static_cast<TX*>(p.h) + w.b * p.h_s[0] + (int64_t)t_first * p.h_s[1] + w.c;
-  float* ckpt = p.ckpt ? p.ckpt + ((int64_t)w.b * p.tiles + w.rank) * p.D + w.c : nullptr;
-  if constexpr (PACKED) ptx::grid_dep_wait();
-  float2 carry[kPairs];              // the state that enters the cluster's next tiles
-  load_state<WIDE>(PACKED || !p.state_in ? nullptr : p.state_in + w.b * p.si_s + w.c, w.on, carry);
-  const auto load = [&](int stage, int tile) {
-    const uint32_t there = row_mask<PACKED>(p, w, tile).there;
-    xs.load(stage, x, p.x_s[1], there, w.on);
-    gs.load(stage, g, p.g_s[1], there, w.on);
-    copy_commit();
-    x += t_step * p.x_s[1];
-    g += t_step * p.g_s[1];
-  };
-#pragma unroll
-  for (int k = 0; k < kStages - 1; ++k) load(k, k * p.cluster + w.rank);
-  Exchange exchange(full, reinterpret_cast<float*>(smem + XRing::kBytes + GRing::kBytes), p, w.rank,
-                    &g_scan_device_error);
-  int stage = 0;
-  for (int k = 0; k < turns; ++k) {
-    const int tile = k * p.cluster + w.rank, t0 = tile * kTile + w.run, buf = k & 1;
-    load(stage ? stage - 1 : kStages - 1, tile + (kStages - 1) * p.cluster);
-    const RowMask m = row_mask<PACKED>(p, w, tile);
-    copy_wait<kStages - 1>();
-    // the thread's piece
-    Decay a[kRun][kPairs];
-    float2 v[kRun][kPairs], sum[kPairs];
-    Piece q;
-#pragma unroll
-    for (int j = 0; j < kPairs; ++j) sum[j] = q.h[j] = both(0.f);
-#pragma unroll
-    for (int t = 0; t < kRun; ++t) {
-      float2 gt[kPairs];
-      gs.read(stage, t, gt);
-      xs.read(stage, t, v[t]);
-      if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, q.h);
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        a[t][j] = decay(gt[j]);
-        sum[j] = __fadd2_rn(sum[j], gt[j]);
-        if (p.complement) v[t][j] = __fmul2_rn(v[t][j], rest(a[t][j]));
-        q.h[j] = apply(a[t][j], q.h[j], v[t][j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kPairs; ++j) q.a[j] = PACKED && m.first ? cut() : decay(sum[j]);
-    const Piece low = shuffle(q, lane);            // the lower half warp's
-    if (upper) {
-      Piece both_halves = low;
-      append<PACKED>(both_halves, q);
-      put(warps[buf] + warp * kPieceFloats, lane, both_halves);
-    }
-    __syncthreads();
-    // the state that enters the block's tile, and the next turn's
-    float2 cur[kPairs], mine[kPairs];
-    if (p.cluster > 1) {
-      exchange.send<PACKED>(k, warps[buf], false);
-      exchange.wait(k);
-#pragma unroll 1
-      for (int i = 0; i < p.cluster; ++i) {
-        if (i == w.rank) {
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j) cur[j] = carry[j];
-        }
-        pass_on<PACKED>(take(exchange.row(k, i), lane), carry);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) cur[j] = carry[j];
-    }
-    if (ckpt) {
-      if (tile < p.tiles && threadIdx.x < kLanes) store_state<WIDE>(ckpt, w.on, cur);
-      ckpt += (int64_t)p.cluster * p.D;
-    }
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      if (i == warp) {
-#pragma unroll
-        for (int j = 0; j < kPairs; ++j) mine[j] = cur[j];
-      }
-      pass_on<PACKED>(take(warps[buf] + i * kPieceFloats, lane), cur);
-    }
-    if (p.cluster == 1) {
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) carry[j] = cur[j];
-    }
-    if (upper) pass_on<PACKED>(low, mine);
-    // and the thread's tokens again, from the state that enters them
-    TX* row = out;
-#pragma unroll
-    for (int t = 0; t < kRun; ++t) {
-      if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, mine);
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) mine[j] = apply(a[t][j], mine[j], v[t][j]);
-      if (m.there >> t & 1) {
-        write<WIDE>(row, w.on, mine);
-      } else if (PACKED && t0 + t < p.T) {
-        const float2 zero[kPairs] = {};
-        write<WIDE>(row, w.on, zero);
-      }
-      if (PACKED && (m.last >> t & 1))
-        store_state<WIDE>(const_cast<float*>(state_of(p, p.state_out, p.so_s, t0 + t, w.c)), w.on, mine);
-      row += p.h_s[1];
-    }
-    out += t_step * p.h_s[1];
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kXSlots; ++i) ptx::mbar_init(sh.x_full + i, 1);
+    for (int i = 0; i < kGSlots; ++i) ptx::mbar_init(sh.g_full + i, 1);
+    exchange.init();
+    ptx::fence_mbar_init();
   }
-  if (!PACKED && w.rank == 0 && threadIdx.x < kLanes)
-    store_state<WIDE>(p.state_out + w.b * p.so_s + w.c, w.on, carry);
-  exchange.leave();
+  __syncthreads();
+  exchange.barrier();
+  if (threadIdx.x >= Fwd::kWork) {
+    // a channel's state from turn to turn, and the copies
+    const int i_ch = threadIdx.x - Fwd::kWork, ch = w.block_c + shared_channel<WIDE>(i_ch);
+    const bool kept = ch < p.D, copies = WIDE && i_ch == 0;
+    const auto copy = [&](int k) {
+      const int tile = k * p.cluster + w.rank;
+      if (tile >= p.tiles) return;
+      xs.copy(&x_map, k, w.block_c, tile * Fwd::kTile, w.b, sh.x_full + k % kXSlots);
+      gs.copy(&g_map, k, w.block_c, tile * Fwd::kTile, w.b, sh.g_full + k % kGSlots);
+    };
+    if (copies)
+      for (int k = 0; k < 2; ++k) copy(k);
+    if constexpr (PACKED) ptx::grid_dep_wait();
+    float carry = !PACKED && kept && p.state_in ? p.state_in[w.b * p.si_s + ch] : 0.f;
+    float* ckpt = p.ckpt && kept ? p.ckpt + (int64_t)w.b * p.steps * p.D + ch : nullptr;
+    for (int k = 0; k < turns; ++k) {
+      const int buf = k & 1;
+      pieces_wait(buf, Fwd::kThreads);
+      // the workers are done with the gates of turn k and with the inputs of turn k - 2
+      if (copies && patience.limit) copy(k + 2);
+      uint32_t cuts = 0;
+      if constexpr (PACKED) {
+#pragma unroll
+        for (int i = 0; i < Fwd::kParts; ++i) cuts |= (uint32_t)sh.starts[buf][i] << i;
+      }
+      enter_parts<PACKED, false>(exchange, patience, k, sh.parts[buf], sh.parts[buf].h, cuts, carry, i_ch);
+      float kept_state[Fwd::kTile / kStep];
+#pragma unroll
+      for (int i = 0; i < Fwd::kTile / kStep; ++i) kept_state[i] = sh.parts[buf].h[i * (kStep / kRun)][i_ch];
+      states_done(buf, Fwd::kThreads);
+      if (ckpt) {
+#pragma unroll
+        for (int i = 0; i < Fwd::kTile / kStep; ++i) {
+          const int step = (k * p.cluster + w.rank) * (Fwd::kTile / kStep) + i;
+          if (step < p.steps) ckpt[(int64_t)step * p.D] = kept_state[i];
+        }
+      }
+    }
+    if (!PACKED && w.rank == 0 && kept) p.state_out[w.b * p.so_s + ch] = carry;
+    if (copies) {                    // (a worker may have given up)
+      Patience landed(&g_scan_device_error);
+      for (int k = max(turns - 2, 0); k < turns; ++k) {
+        if (k * p.cluster + w.rank >= p.tiles) continue;
+        landed.wait(sh.x_full + k % kXSlots, k / kXSlots & 1);
+        landed.wait(sh.g_full + k % kGSlots, k / kGSlots & 1);
+      }
+    }
+  } else {
+    if constexpr (PACKED) ptx::grid_dep_wait();
+    const int part = threadIdx.x / kLanes, row0 = part * kRun;
+    const TX* x = static_cast<const TX*>(p.x) + w.b * p.x_s[0] + w.c;
+    const TG* g = static_cast<const TG*>(p.g) + w.b * p.g_s[0] + w.c;
+    TX* const out = static_cast<TX*>(p.h) + w.b * p.h_s[0] + w.c;
+    const auto first_row = [&](int k) { return (k * p.cluster + w.rank) * Fwd::kTile + row0; };
+    // turn k's pieces
+    const auto pieces = [&](int k, int buf, Decays<COMPLEMENT>& a) {
+      const int t0 = first_row(k);
+      const RowMask m = row_mask<PACKED>(p, t0);
+      const bool tile_there = t0 - row0 < p.T;
+      if constexpr (WIDE) {
+        if (tile_there) {
+          patience.wait(sh.x_full + k % kXSlots, k / kXSlots & 1);
+          patience.wait(sh.g_full + k % kGSlots, k / kGSlots & 1);
+        }
+      } else {
+        xs.copy_own(x + (int64_t)t0 * p.x_s[1], p.x_s[1], k, row0, m.there, w.on);
+        gs.copy_own(g + (int64_t)t0 * p.g_s[1], p.g_s[1], k, row0, m.there, w.on);
+      }
+      float2 gt[kRun][kPairs], all_c[kPairs], all_r[kPairs], h[kPairs];
+#pragma unroll
+      for (int t = 0; t < kRun; ++t) {
+        gs.read(k, row0 + t, gt[t]);
+        // (rows past T are zeros already where their tile has any)
+        if (PACKED ? !(m.there >> t & 1) : !tile_there) gt[t][0] = gt[t][1] = both(0.f);
+      }
+      set_decays(a, gt, all_c, all_r);
+      h[0] = h[1] = both(0.f);
+#pragma unroll
+      for (int t = 0; t < kRun; ++t) {
+        float2 v[kPairs];
+        xs.read(k, row0 + t, v);
+        if (PACKED ? !(m.there >> t & 1) : !tile_there) v[0] = v[1] = both(0.f);
+        if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          if (COMPLEMENT) v[j] = __fmul2_rn(v[j], rest(a.c(t, j), a.r[t][j]));
+          h[j] = apply(a.c(t, j), a.r[t][j], h[j], v[j]);
+        }
+      }
+      put(sh.parts[buf].c[part], all_c);
+      put(sh.parts[buf].r[part], all_r);
+      put(sh.parts[buf].h[part], h);
+      if (PACKED && threadIdx.x % kLanes == 0) sh.starts[buf][part] = m.first != 0;
+      pieces_done(buf, Fwd::kThreads);
+    };
+    // turn k's tokens again, from the state that enters them
+    const auto states = [&](int k, int buf, const Decays<COMPLEMENT>& a) {
+      const int t0 = first_row(k);
+      const RowMask m = row_mask<PACKED>(p, t0);
+      states_wait(buf, Fwd::kThreads);
+      float2 h[kPairs];
+      get(sh.parts[buf].h[part], h);
+      TX* row = out + (int64_t)t0 * p.h_s[1];
+      if (WIDE && !w.on) return;
+#pragma unroll
+      for (int t = 0; t < kRun; ++t) {
+        float2 v[kPairs];
+        xs.read(k, row0 + t, v);
+        if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          if (COMPLEMENT) v[j] = __fmul2_rn(v[j], rest(a.c(t, j), a.r[t][j]));
+          h[j] = apply(a.c(t, j), a.r[t][j], h[j], v[j]);
+        }
+        if (m.there >> t & 1) {
+          write<WIDE>(row + t * p.h_s[1], w.on, h);
+        } else if (PACKED && t0 + t < p.T) {
+          const float2 zero[kPairs] = {};
+          write<WIDE>(row + t * p.h_s[1], w.on, zero);
+        }
+        if (PACKED && (m.last >> t & 1)) store_state<WIDE>(state_of(p, p.state_out, p.so_s, t0 + t, w.c), w.on, h);
+      }
+    };
+    // a turn's pieces before the turn before's states: those come meanwhile
+    Decays<COMPLEMENT> a, b;
+    for (int k = 0; k <= turns; k += 2) {
+      if (k < turns) pieces(k, 0, a);
+      if (k > 0) states(k - 1, 1, b);
+      if (k + 1 < turns) pieces(k + 1, 1, b);
+      if (k < turns) states(k, 0, a);
+    }
+  }
+  exchange.barrier();                // no block leaves while another may still send to it
 }
+
+cudaError_t launch_forward(ScanParams p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
+  choose_cluster(p, Fwd::kTile, 2 * 148);
+  return by_types(x_dtype, g_dtype, [&](auto x, auto g) {
+    using TX = decltype(x);
+    using TG = decltype(g);
+    CUtensorMap mx, mg;
+    const bool tma = wide && encode<TX>(&mx, p.x, p.x_s, p, Fwd::kTile) && encode<TG>(&mg, p.g, p.g_s, p, Fwd::kTile);
+    const size_t smem = Ring<TX, Fwd::kTile, kXSlots>::kBytes + Ring<TG, Fwd::kTile, kGSlots>::kBytes +
+                        sizeof(Shared) + cluster_bytes(p.cluster);
+    return by_flags(tma, p.q_start != nullptr, p.complement, [&](auto wide_, auto packed, auto complement) {
+      return launch_tiles(scan_kernel<TX, TG, wide_.value, packed.value, complement.value>, p, Fwd::kThreads, smem, s,
+                          mx, mg);
+    });
+  });
+}
+
+constexpr int kStepThreads = 128;
 
 // One token: a thread has VEC channels of a row.
 template <typename TX, typename TG, int VEC>
-__global__ void __launch_bounds__(kThreads) step_kernel(const ScanParams p, int blocks_per_row) {
+__global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, int blocks_per_row) {
   const int b = blockIdx.x / blocks_per_row;
-  const int c = ((blockIdx.x - b * blocks_per_row) * kThreads + threadIdx.x) * VEC;
+  const int c = ((blockIdx.x - b * blocks_per_row) * kStepThreads + threadIdx.x) * VEC;
   if (c >= p.D) return;
   int64_t row = b;
   bool live = true;
@@ -213,10 +268,11 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const ScanParams p, int 
     }
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const Decay a = decay(make_float2(g[i], g[i + 1]));
+      const bool nx = fabsf(g[i]) < kNear, ny = fabsf(g[i + 1]) < kNear;
+      const float2 r = decay(make_float2(g[i], g[i + 1]), nx, ny), c2 = one_if(nx, ny);
       float2 v = make_float2(x[i], x[i + 1]);
-      if (p.complement) v = __fmul2_rn(v, rest(a));
-      v = apply(a, make_float2(h[i], h[i + 1]), v);
+      if (p.complement) v = __fmul2_rn(v, rest(c2, r));
+      v = apply(c2, r, make_float2(h[i], h[i + 1]), v);
       h[i] = v.x;
       h[i + 1] = v.y;
     }
@@ -232,23 +288,10 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const ScanParams p, int 
   }
 }
 
-cudaError_t launch_forward(const ScanParams& p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
-  return by_types(x_dtype, g_dtype, [&](auto x, auto g) {
-    using TX = decltype(x);
-    using TG = decltype(g);
-    const size_t smem = Ring<TX, true, kStages>::kBytes + Ring<TG, true, kStages>::kBytes + cluster_bytes(p.cluster);
-    if (p.q_start)
-      return launch_tiles(wide ? scan_kernel<TX, TG, true, true> : scan_kernel<TX, TG, false, true>, p, smem, s);
-    return launch_tiles(wide ? scan_kernel<TX, TG, true, false> : scan_kernel<TX, TG, false, false>, p, smem, s);
-  });
-}
-
-constexpr int kWantBlocks = 512;   // clusters grow until a call has so many blocks
-
 int size_of(int dt) { return dt == KDA_DTYPE_F32 ? 4 : 2; }
 bool misaligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
 
-enum Pass { kForward, kBackward, kStep };
+enum class Pass { kForward, kBackward, kToken };
 
 int validate_sizes(const KdaScanArgs* a) {
   if (a == nullptr) return KDA_ERR_NULL_POINTER;
@@ -261,21 +304,21 @@ int validate_sizes(const KdaScanArgs* a) {
 int validate(const KdaScanArgs* a, Pass pass) {
   const int st = validate_sizes(a);
   if (st != KDA_OK) return st;
-  if (pass == kStep && a->T != 1) return KDA_ERR_SHAPE;
+  if (pass == Pass::kToken && a->T != 1) return KDA_ERR_SHAPE;
   if (a->x_dtype < KDA_DTYPE_F32 || a->x_dtype > KDA_DTYPE_BF16) return KDA_ERR_DTYPE;
   if (a->g_dtype != KDA_DTYPE_F32 && a->g_dtype != a->x_dtype) return KDA_ERR_DTYPE;
   if (a->D == 0) return KDA_OK;
   const int xs = size_of(a->x_dtype), gs = size_of(a->g_dtype);
   const bool tokens = a->T > 0 && (a->B > 0 || a->q_start != nullptr);
-  if (tokens && (!a->x || !a->g || (pass != kBackward && !a->h))) return KDA_ERR_NULL_POINTER;
-  if (a->B > 0 && pass != kBackward && !a->state_out) return KDA_ERR_NULL_POINTER;
-  if (tokens && pass == kBackward && a->B > 0 && !a->ckpt) return KDA_ERR_NULL_POINTER;
+  if (tokens && (!a->x || !a->g || (pass != Pass::kBackward && !a->h))) return KDA_ERR_NULL_POINTER;
+  if (a->B > 0 && pass != Pass::kBackward && !a->state_out) return KDA_ERR_NULL_POINTER;
+  if (tokens && pass == Pass::kBackward && a->B > 0 && !a->ckpt) return KDA_ERR_NULL_POINTER;
   if (misaligned(a->x, xs) || misaligned(a->h, xs) || misaligned(a->dh, xs) || misaligned(a->dx, xs) ||
       misaligned(a->g, gs) || misaligned(a->dg, gs) || misaligned(a->state_in, 4) ||
       misaligned(a->state_out, 4) || misaligned(a->dstate_out, 4) || misaligned(a->dstate_in, 4) ||
       misaligned(a->ckpt, 4) || misaligned(a->q_start, 4) || misaligned(a->slots, 4))
     return KDA_ERR_ALIGNMENT;
-  if (pass == kStep) {
+  if (pass == Pass::kToken) {
     if (a->slots && a->num_states < 0) return KDA_ERR_SHAPE;
     if (a->scatter && a->B > 0 && (a->state_in != a->state_out || a->state_in_stride != a->state_out_stride))
       return KDA_ERR_STRIDE;
@@ -286,7 +329,7 @@ int validate(const KdaScanArgs* a, Pass pass) {
 ScanParams to_params(const KdaScanArgs* a) {
   ScanParams p{};
   p.B = a->B; p.T = a->T; p.D = a->D;
-  p.tiles = (a->T + kTile - 1) / kTile;
+  p.steps = (a->T + kStep - 1) / kStep;
   p.complement = a->complement != 0;
   p.x = a->x; std::memcpy(p.x_s, a->x_stride, sizeof(p.x_s));
   p.g = a->g; std::memcpy(p.g_s, a->g_stride, sizeof(p.g_s));
@@ -314,7 +357,7 @@ int check_device() {
 }
 
 size_t workspace_bytes(const KdaScanArgs* a) {
-  return a->q_start ? ((size_t)a->T + kTile - 1) / kTile * sizeof(Marks) : 0;
+  return a->q_start ? ((size_t)a->T + kMarked - 1) / kMarked * sizeof(Marks) : 0;
 }
 
 // Rows start on kVec values' boundaries.
@@ -334,31 +377,31 @@ int run_scan(const KdaScanArgs* a, Pass pass, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int xs = size_of(a->x_dtype), gs = size_of(a->g_dtype);
   const bool wide = p.D % kVec == 0 && aligned_rows(p.x, p.x_s, xs) && aligned_rows(p.g, p.g_s, gs) &&
-                    (pass == kForward ? aligned_rows(p.h, p.h_s, xs)
+                    (pass == Pass::kForward ? aligned_rows(p.h, p.h_s, xs)
                                       : aligned_rows(p.dh, p.dh_s, xs) && aligned_rows(p.dx, p.dx_s, xs) &&
                                             aligned_rows(p.dg, p.dg_s, gs));
-  const int64_t blocks = (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels);
-  if (blocks * kMaxCluster > 0x7fffffff) return KDA_ERR_SHAPE;
-  while (p.cluster < kMaxCluster && p.cluster < p.tiles && blocks * p.cluster < kWantBlocks) p.cluster *= 2;
+  if ((int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels) * kMaxCluster > 0x7fffffff)
+    return KDA_ERR_SHAPE;
   cudaError_t e = cudaSuccess;
   if (p.q_start) {
     Marks* marks = static_cast<Marks*>(a->workspace);
     p.marks = marks;
-    const bool fwd = pass == kForward;
-    mark_kernel<<<p.tiles + p.B, kTile, 0, s>>>(p, marks, fwd ? p.state_in : p.dstate_out,
-                                                fwd ? p.si_s : p.dso_s, fwd ? p.state_out : p.dstate_in,
-                                                fwd ? p.so_s : p.dsi_s);
+    const bool fwd = pass == Pass::kForward;
+    const int marked = (p.T + kMarked - 1) / kMarked;
+    mark_kernel<<<marked + p.B, kMarked, 0, s>>>(p, marked, marks, fwd ? p.state_in : p.dstate_out,
+                                                 fwd ? p.si_s : p.dso_s, fwd ? p.state_out : p.dstate_in,
+                                                 fwd ? p.so_s : p.dsi_s);
     e = cudaGetLastError();
-    if (p.tiles == 0) return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+    if (p.T == 0) return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
   }
   if (e == cudaSuccess)
-    e = pass == kForward ? launch_forward(p, a->x_dtype, a->g_dtype, wide, s)
+    e = pass == Pass::kForward ? launch_forward(p, a->x_dtype, a->g_dtype, wide, s)
                          : launch_grad(p, a->x_dtype, a->g_dtype, wide, s);
   return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 
 int run_step(const KdaScanArgs* a, void* stream) {
-  int st = validate(a, kStep);
+  int st = validate(a, Pass::kToken);
   if (st != KDA_OK) return st;
   if (a->D == 0 || a->B == 0) return KDA_OK;
   if ((st = check_device()) != KDA_OK) return st;
@@ -368,22 +411,28 @@ int run_step(const KdaScanArgs* a, void* stream) {
                    !misaligned(p.g, 4 * gs) && !misaligned(p.state_in, 16) &&
                    !misaligned(p.state_out, 16) && p.x_s[0] % 4 == 0 && p.h_s[0] % 4 == 0 &&
                    p.g_s[0] % 4 == 0 && p.si_s % 4 == 0 && p.so_s % 4 == 0;
-  const int per_row = (p.D + kThreads * (vec ? 4 : 1) - 1) / (kThreads * (vec ? 4 : 1));
+  const int per_row = (p.D + kStepThreads * (vec ? 4 : 1) - 1) / (kStepThreads * (vec ? 4 : 1));
   if ((int64_t)per_row * p.B > 0x7fffffff) return KDA_ERR_SHAPE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = by_types(a->x_dtype, a->g_dtype, [&](auto x, auto g) {
     using TX = decltype(x);
     using TG = decltype(g);
     if (vec)
-      step_kernel<TX, TG, 4><<<per_row * p.B, kThreads, 0, s>>>(p, per_row);
+      step_kernel<TX, TG, 4><<<per_row * p.B, kStepThreads, 0, s>>>(p, per_row);
     else
-      step_kernel<TX, TG, 1><<<per_row * p.B, kThreads, 0, s>>>(p, per_row);
+      step_kernel<TX, TG, 1><<<per_row * p.B, kStepThreads, 0, s>>>(p, per_row);
     return cudaGetLastError();
   });
   return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 
 }  // namespace
+
+void choose_cluster(ScanParams& p, int tile, int slots) {
+  p.tiles = (p.T + tile - 1) / tile;
+  const int64_t blocks = (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels);
+  p.cluster = (int)max((int64_t)1, min((int64_t)min(kMaxCluster, p.tiles), slots / blocks));
+}
 
 int read_device_error(bool clear) {
   const int grad = read_grad_device_error(clear);
@@ -406,8 +455,8 @@ size_t kda_scan_args_size(void) { return sizeof(KdaScanArgs); }
 
 size_t kda_scan_ckpt_floats(const KdaScanArgs* a) {
   if (kda::scan::validate_sizes(a) != KDA_OK) return 0;
-  const size_t tiles = ((size_t)a->T + kda::scan::kTile - 1) / kda::scan::kTile;
-  return (a->q_start ? 1 : (size_t)a->B) * tiles * (size_t)a->D;
+  const size_t steps = ((size_t)a->T + kda::scan::kStep - 1) / kda::scan::kStep;
+  return (a->q_start ? 1 : (size_t)a->B) * steps * (size_t)a->D;
 }
 
 size_t kda_scan_workspace_bytes(const KdaScanArgs* a) {
@@ -416,11 +465,11 @@ size_t kda_scan_workspace_bytes(const KdaScanArgs* a) {
 }
 
 int kda_scan_fwd(const KdaScanArgs* a, void* stream) {
-  return kda::scan::run_scan(a, kda::scan::kForward, stream);
+  return kda::scan::run_scan(a, kda::scan::Pass::kForward, stream);
 }
 
 int kda_scan_bwd(const KdaScanArgs* a, void* stream) {
-  return kda::scan::run_scan(a, kda::scan::kBackward, stream);
+  return kda::scan::run_scan(a, kda::scan::Pass::kBackward, stream);
 }
 
 int kda_scan_step(const KdaScanArgs* a, void* stream) { return kda::scan::run_step(a, stream); }

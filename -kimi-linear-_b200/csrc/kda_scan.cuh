@@ -1,11 +1,12 @@
 // kda_scan.cuh -- gated linear recurrence: parameters, the arithmetic of its decays, and
 // what the scan and its gradient share.
 //
-// A decay a = exp(g) is held as c + r with c = 1, r = a - 1 where |g| < 1/4 and c = 0, r = a
-// elsewhere: rounding a itself to 24 bits is off by up to 2^-25 per token, always to the
-// same side for a steady g, which a state that remembers n tokens adds up to n 2^-25.
-// c h + r h is one instruction more than a product, and two channels share each
-// (fma.f32x2), so a thread works on pairs of channels.
+// A decay a = exp(g) is held as c + r, with c = 1, r = a - 1 for a channel's run of kRun tokens
+// that all have |g| < 1/4, and c = 0, r = a for the others: rounding a itself to 24 bits is
+// off by up to 2^-25 per token, always to the same side for a steady g, which a state that
+// remembers n tokens adds up to n 2^-25.  (A run with a larger |g| forgets a fifth, so that there
+// n stays below twenty.)  c h + r h is one instruction more than a product, and two channels
+// share each (fma.f32x2), so a thread works on pairs of channels.
 #pragma once
 
 #include "kda_internal.cuh"
@@ -16,9 +17,10 @@ namespace scan {
 
 constexpr int kErrSlot = 8;       // device error word: a step's slot past the pool
 constexpr int kErrWait = 9;       // device error word: a wait for a cluster's piece ran out
-constexpr int kTile = 64;         // tokens between two checkpoints of the state
+constexpr int kStep = 32;         // tokens between two checkpoints of the state
+constexpr int kMarked = 64;       // rows of a packed batch that one Marks describes
 
-// What the rows of a tile of a packed batch are, a bit a row.
+// What kMarked rows of a packed batch are, a bit a row.
 struct Marks {
   uint64_t first, last, owned;      // of a sequence; by any sequence
 };
@@ -26,7 +28,8 @@ struct Marks {
 // Device-side view of KdaScanArgs (strides in elements).
 struct ScanParams {
   int B, T, D;
-  int tiles;                        // checkpoints of a sequence (packed: of all rows)
+  int tiles;                        // the kernel's tiles of a sequence (packed: of all rows)
+  int steps;                        // checkpoints of the same
   bool complement;
   const void* x; int64_t x_s[2];
   const void* g; int64_t g_s[2];
@@ -34,13 +37,13 @@ struct ScanParams {
   const int* q_start;               // or null: a batch
   void* h; int64_t h_s[2];
   float* state_out; int64_t so_s;
-  float* ckpt;                      // [B][tiles][D], packed [tiles][D]
+  float* ckpt;                      // [B][steps][D], packed [steps][D]
   const void* dh; int64_t dh_s[2];
   const float* dstate_out; int64_t dso_s;
   void* dx; int64_t dx_s[2];
   void* dg; int64_t dg_s[2];
   float* dstate_in; int64_t dsi_s;
-  const Marks* marks;               // packed: [tiles], made by mark_kernel
+  const Marks* marks;               // packed: of all rows, made by mark_kernel
   int cluster;                      // blocks that share a sequence's tiles
   // step
   const int* slots; int num_states; bool scatter;
@@ -48,19 +51,16 @@ struct ScanParams {
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-struct Decay {                      // of a pair of channels
-  float2 c, r;
-};
-
-// exp(g).  Near zero the series of exp(g) - 1 up to g^6/6!, of which the first term left out
-// is 2^-24 of the sum at |g| = 1/4; elsewhere 2^(g log2 e) by the hardware's instruction
-// (2^-22 of itself, and 2^-24 |g| from the rounded exponent).  What is below 2^-126 is zero.
+// exp(g): near zero, less one, the series up to g^6/6!, of which the first term left out is 2^-24 of
+// the sum at |g| = 1/4; elsewhere 2^(g log2 e) by the hardware's instruction (2^-22 of itself, and
+// 2^-24 |g| from the rounded exponent).  What is below 2^-126 is zero.
+constexpr float kNear = 0.25f;
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ Decay decay(float2 g) {
+__device__ __forceinline__ float2 decay(float2 g, bool near_x, bool near_y) {
   float2 p = __ffma2_rn(g, both(1.f / 720.f), both(1.f / 120.f));
   p = __ffma2_rn(p, g, both(1.f / 24.f));
   p = __ffma2_rn(p, g, both(1.f / 6.f));
@@ -68,49 +68,18 @@ __device__ __forceinline__ Decay decay(float2 g) {
   p = __ffma2_rn(p, g, both(1.f));
   p = __fmul2_rn(p, g);
   const float2 e = __fmul2_rn(g, both(1.4426950408889634f));
-  const bool x = fabsf(g.x) < 0.25f, y = fabsf(g.y) < 0.25f;
-  return {make_float2(x ? 1.f : 0.f, y ? 1.f : 0.f),
-          make_float2(x ? p.x : exp2_fast(e.x), y ? p.y : exp2_fast(e.y))};
+  return make_float2(near_x ? p.x : exp2_fast(e.x), near_y ? p.y : exp2_fast(e.y));
 }
+__device__ __forceinline__ float2 one_if(bool x, bool y) { return make_float2(x ? 1.f : 0.f, y ? 1.f : 0.f); }
 // a h + b
-__device__ __forceinline__ float2 apply(const Decay& a, float2 h, float2 b) {
-  return __ffma2_rn(a.r, h, __ffma2_rn(a.c, h, b));
+__device__ __forceinline__ float2 apply(float2 c, float2 r, float2 h, float2 b) {
+  return __ffma2_rn(r, h, __ffma2_rn(c, h, b));
 }
 // a v
-__device__ __forceinline__ float2 times(const Decay& a, float2 v) {
-  return __ffma2_rn(a.r, v, __fmul2_rn(a.c, v));
-}
+__device__ __forceinline__ float2 times(float2 c, float2 r, float2 v) { return __ffma2_rn(r, v, __fmul2_rn(c, v)); }
 // 1 - a
-__device__ __forceinline__ float2 rest(const Decay& a) {
-  return __ffma2_rn(a.r, both(-1.f), __ffma2_rn(a.c, both(-1.f), both(1.f)));
-}
-// Decay over two pieces: (c1 + r1) (c2 + r2).
-__device__ __forceinline__ void renew(float& c, float& r) {
-  if (c == 1.f && r < -0.5f) {
-    c = 0.f;
-    r += 1.f;
-  }
-}
-__device__ __forceinline__ Decay join(const Decay& a, const Decay& b) {
-  Decay d{__fmul2_rn(a.c, b.c),
-          __ffma2_rn(a.c, b.r, __ffma2_rn(b.c, a.r, __fmul2_rn(a.r, b.r)))};
-  renew(d.c.x, d.r.x);
-  renew(d.c.y, d.r.y);
-  return d;
-}
-
-// A piece inside which a packed sequence starts passes nothing on of what came before it,
-// not even a NaN: c = 0, r = -infinity in both channels.
-__device__ __forceinline__ Decay cut() { return {both(0.f), both(__int_as_float((int)0xff800000))}; }
-__device__ __forceinline__ bool is_cut(const Decay& a) { return __float_as_int(a.r.x) == (int)0xff800000; }
-template <bool PACKED>
-__device__ __forceinline__ float2 pass_on(const Decay& a, float2 h, float2 b) {
-  const float2 n = apply(a, h, b);
-  return PACKED && is_cut(a) ? b : n;
-}
-template <bool PACKED>
-__device__ __forceinline__ Decay join_pieces(const Decay& a, const Decay& b) {
-  return PACKED && (is_cut(a) || is_cut(b)) ? cut() : join(a, b);
+__device__ __forceinline__ float2 rest(float2 c, float2 r) {
+  return __ffma2_rn(r, both(-1.f), __ffma2_rn(c, both(-1.f), both(1.f)));
 }
 
 // The last sequence of a packed batch that starts at row t or before it (-1: none).  Of those
@@ -125,46 +94,90 @@ __device__ __forceinline__ int sequence_at(const int* q_start, int B, int t) {
   return lo - 1;
 }
 
-constexpr int kThreads = 128;                 // of every kernel here
-constexpr int kWarps = kThreads / 32;
 constexpr int kLanes = 16;                    // threads that share a row
 constexpr int kVec = 4;                       // channels of a thread
 constexpr int kPairs = kVec / 2;
 constexpr int kChannels = kLanes * kVec;      // of a block
-constexpr int kRun = kTile / (kWarps * 2);    // tokens of a thread
+constexpr int kRun = 4;                       // tokens of a thread in a tile
+constexpr int kCarry = kChannels;             // threads that carry a channel's state each
 constexpr int kMaxCluster = 8;
+constexpr uint64_t kWaitNs = 2000000000;      // a wait that takes longer gives up (device error word 9)
+
+// A block's working warps and what follows from their number.
+template <int WARPS>
+struct Shape {
+  static constexpr int kWork = WARPS * 32;
+  static constexpr int kThreads = kWork + kCarry;
+  static constexpr int kParts = kWork / kLanes;        // half warps, each with kRun tokens of a tile
+  static constexpr int kTile = kParts * kRun;
+};
 
 // ---------------------------------------------------------------------------
-// rows into a thread's own places in shared memory
+// waits
 // ---------------------------------------------------------------------------
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src, bool ok) {
-  const int n = ok ? BYTES : 0;               // 0: the place is filled with zeros
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src),
-                 "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src),
-                 "r"(n), "n"(BYTES) : "memory");
+__device__ __forceinline__ bool here(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(ptx::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// A thread whose wait runs out goes on, so that the block's other barriers stay matched, and
+// waits no more.
+struct Patience {
+  int* error;
+  uint64_t limit;
+  __device__ explicit Patience(int* error_) : error(error_), limit(kWaitNs) {}
+  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
+    if (here(bar, parity)) return;
+    const uint64_t start = ptx::globaltimer_ns();
+    while (!here(bar, parity)) {
+      if (ptx::globaltimer_ns() - start >= limit) {
+        *error = kErrWait;
+        limit = 0;
+        return;
+      }
+    }
+  }
+};
+// The block's named barriers, two of each kind (buf 0 and 1): the workers' pieces are there (the
+// workers go on, the carrying threads wait); the states that enter the parts are there (the
+// other way round).
+template <int ID>
+__device__ __forceinline__ void bar_arrive(int count) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"n"(ID), "r"(count) : "memory");
 }
+template <int ID>
+__device__ __forceinline__ void bar_sync(int count) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"n"(ID), "r"(count) : "memory");
+}
+__device__ __forceinline__ void pieces_done(int buf, int count) { buf ? bar_arrive<2>(count) : bar_arrive<1>(count); }
+__device__ __forceinline__ void pieces_wait(int buf, int count) { buf ? bar_sync<2>(count) : bar_sync<1>(count); }
+__device__ __forceinline__ void states_done(int buf, int count) { buf ? bar_arrive<4>(count) : bar_arrive<3>(count); }
+__device__ __forceinline__ void states_wait(int buf, int count) { buf ? bar_sync<4>(count) : bar_sync<3>(count); }
 
-// A thread's channels.  WIDE: kVec next to each other, in one access; else (rows that
-// do not start on such a boundary) every kLanes-th, one by one, so that a half warp
-// still reads whole sectors.
+// ---------------------------------------------------------------------------
+// a block's place and its rows in shared memory
+// ---------------------------------------------------------------------------
+// Shared rows have kChannels values; a thread has kVec next to each other.  WIDE: they are
+// channels next to each other too, and a tile comes by one TMA copy.  Else (rows that
+// TMA or a thread's stores cannot address) the thread's channels are every kLanes-th, so that
+// a half warp reads and writes whole sectors, and it copies them itself.
 struct Place {
   int rank;                          // in the cluster: tiles rank, rank + cluster, ...
   int b;                             // sequence (packed: 0)
-  int c;                             // first channel
-  int run;                           // first token in a tile
+  int block_c, c;                    // the block's and the thread's first channel
   uint32_t on;                       // which channels exist (WIDE: all or none)
 };
 template <bool WIDE>
 __device__ __forceinline__ int channel(int i) { return WIDE ? i : i * kLanes; }
+// where value i of a shared row lies from the block's first channel
+template <bool WIDE>
+__device__ __forceinline__ int shared_channel(int i) { return WIDE ? i : i / kVec + i % kVec * kLanes; }
 template <bool WIDE>
 __device__ __forceinline__ Place my_place(const ScanParams& p) {
   Place w;
@@ -172,8 +185,8 @@ __device__ __forceinline__ Place my_place(const ScanParams& p) {
   const int i = blockIdx.x / p.cluster, lane = threadIdx.x % kLanes;
   w.rank = blockIdx.x - i * p.cluster;
   w.b = i / blocks;
-  w.c = (i - w.b * blocks) * kChannels + (WIDE ? lane * kVec : lane);
-  w.run = threadIdx.x / kLanes * kRun;
+  w.block_c = (i - w.b * blocks) * kChannels;
+  w.c = w.block_c + (WIDE ? lane * kVec : lane);
   w.on = 0;
 #pragma unroll
   for (int j = 0; j < kVec; ++j)
@@ -181,35 +194,36 @@ __device__ __forceinline__ Place my_place(const ScanParams& p) {
   return w;
 }
 
-// A thread's kRun rows of one tensor, in a ring of STAGES tiles.
-template <typename T, bool WIDE, int STAGES>
+// Tiles of one tensor in a ring of SLOTS.
+template <typename T, int TILE, int SLOTS>
 struct Ring {
-  static constexpr int kBytes = STAGES * kRun * kThreads * kVec * sizeof(T);
-  T* at;
-  __device__ Ring(void* base) : at(static_cast<T*>(base) + threadIdx.x * kVec) {}
-  __device__ T* place(int stage, int i) const { return at + (stage * kRun + i) * kThreads * kVec; }
-  // rows row, row + stride, ..., of which those in `mask` are wanted (the others: zeros)
-  __device__ void load(int stage, const T* row, int64_t stride, uint32_t mask, uint32_t on) const {
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      T* dst = place(stage, i);
-      const bool ok = mask >> i & 1;
-      if constexpr (WIDE) {
-        copy_async<kVec * sizeof(T)>(dst, row, ok);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const bool has = ok && (on >> j & 1);
-          if constexpr (sizeof(T) == 4) copy_async<4>(dst + j, row + channel<WIDE>(j), has);
-          else dst[j] = has ? row[channel<WIDE>(j)] : T(0.f);
-        }
-      }
-      row += stride;
-    }
+  static constexpr int kTileBytes = TILE * kChannels * sizeof(T);
+  static constexpr int kBytes = SLOTS * kTileBytes;
+  unsigned char* base;
+  __device__ T* row(int k, int i) const {
+    return reinterpret_cast<T*>(base + (k % SLOTS) * kTileBytes) + i * kChannels;
   }
-  __device__ __forceinline__ void read(int stage, int i, float2 (&v)[kPairs]) const {
+  // one thread: tile k from row t on, counted on `bar`
+  __device__ void copy(const CUtensorMap* map, int k, int c, int t, int b, uint64_t* bar) const {
+    ptx::mbar_arrive_expect_tx(bar, kTileBytes);
+    ptx::tma_load_3d(base + (k % SLOTS) * kTileBytes, map, c, t, b, bar);
+  }
+  // a thread: its rows i .. i + kRun - 1 of tile k, those in `mask` (the others: zeros)
+  __device__ void copy_own(const T* src, int64_t stride, int k, int i, uint32_t mask, uint32_t on) const {
+    T v[kRun][kVec];
+#pragma unroll
+    for (int t = 0; t < kRun; ++t)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        v[t][j] = (mask >> t & 1) && (on >> j & 1) ? src[t * stride + channel<false>(j)] : T(0.f);
+#pragma unroll
+    for (int t = 0; t < kRun; ++t)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) row(k, i + t)[threadIdx.x % kLanes * kVec + j] = v[t][j];
+  }
+  __device__ __forceinline__ void read(int k, int i, float2 (&v)[kPairs]) const {
     float t[kVec];
-    ld4(place(stage, i), t);
+    ld4(row(k, i) + threadIdx.x % kLanes * kVec, t);
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) v[j] = make_float2(t[2 * j], t[2 * j + 1]);
   }
@@ -223,7 +237,7 @@ __device__ __forceinline__ void write(T* p, uint32_t on, const float2 (&v)[kPair
     t[2 * j + 1] = v[j].y;
   }
   if constexpr (WIDE) {
-    if (on) st4(p, t);
+    st4(p, t);
   } else {
 #pragma unroll
     for (int j = 0; j < kVec; ++j)
@@ -231,7 +245,7 @@ __device__ __forceinline__ void write(T* p, uint32_t on, const float2 (&v)[kPair
   }
 }
 
-// A state (or checkpoint) row of fp32 values, any alignment; zeros without one.
+// A state row of fp32 values, any alignment; zeros without one.
 template <bool WIDE>
 __device__ __forceinline__ void load_state(const float* row, uint32_t on, float2 (&v)[kPairs]) {
   float t[kVec];
@@ -249,171 +263,200 @@ __device__ __forceinline__ void store_state(float* row, uint32_t on, const float
   }
 }
 // The state of the packed sequence at row t.
-__device__ __forceinline__ const float* state_of(const ScanParams& p, const float* base, int64_t stride, int t,
-                                                 int c) {
-  return base == nullptr ? nullptr : base + (int64_t)max(sequence_at(p.q_start, p.B, t), 0) * stride + c;
+__device__ __forceinline__ float* state_of(const ScanParams& p, const float* base, int64_t stride, int t, int c) {
+  if (base == nullptr) return nullptr;
+  return const_cast<float*>(base) + (int64_t)max(sequence_at(p.q_start, p.B, t), 0) * stride + c;
 }
 
-// Which of a thread's rows are there (bits), and for packed batches which start and end a sequence.
+// Which of rows t .. t + kRun - 1 are there (bits), and for packed batches which start and end
+// a sequence.
+constexpr uint32_t kAllRows = (1u << kRun) - 1;
 struct RowMask { uint32_t there, first, last; };
 template <bool PACKED>
-__device__ __forceinline__ RowMask row_mask(const ScanParams& p, const Place& w, int tile) {
-  constexpr uint32_t all = (1u << kRun) - 1;
+__device__ __forceinline__ RowMask row_mask(const ScanParams& p, int t) {
   RowMask m{0, 0, 0};
-  if (tile >= p.tiles || tile < 0 || !w.on) return m;
   if constexpr (PACKED) {
-    const Marks k = p.marks[tile];
-    m.there = (uint32_t)(k.owned >> w.run) & all;
-    m.first = (uint32_t)(k.first >> w.run) & all;
-    m.last = (uint32_t)(k.last >> w.run) & all;
+    if (t < 0 || t >= p.T) return m;
+    static_assert(kMarked % kRun == 0, "a run is inside one Marks");
+    const Marks* k = p.marks + t / kMarked;
+    const int at = t % kMarked;
+    m.there = (uint32_t)(k->owned >> at) & kAllRows;
+    m.first = (uint32_t)(k->first >> at) & kAllRows;
+    m.last = (uint32_t)(k->last >> at) & kAllRows;
   } else {
-    const int left = p.T - (tile * kTile + w.run);
-    m.there = left >= kRun ? all : left > 0 ? (1u << left) - 1 : 0;
+    const int left = t < 0 ? 0 : p.T - t;
+    m.there = left >= kRun ? kAllRows : left > 0 ? (1u << left) - 1 : 0;
   }
   return m;
+}
+
+// The decays of a run.  EACH: a c for every token (1 - a needs it), else one for the run.
+template <bool EACH>
+struct Decays {
+  float2 c_[EACH ? kRun : 1][kPairs], r[kRun][kPairs];
+  __device__ __forceinline__ float2 c(int t, int j) const { return c_[EACH ? t : 0][j]; }
+};
+// From the gates; also the decay over all of them, by their sum.
+template <bool EACH>
+__device__ __forceinline__ void set_decays(Decays<EACH>& a, const float2 (&g)[kRun][kPairs], float2 (&all_c)[kPairs],
+                                           float2 (&all_r)[kPairs]) {
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    float2 sum = both(0.f);
+    if constexpr (EACH) {
+#pragma unroll
+      for (int t = 0; t < kRun; ++t) {
+        const bool nx = fabsf(g[t][j].x) < kNear, ny = fabsf(g[t][j].y) < kNear;
+        a.c_[t][j] = one_if(nx, ny);
+        a.r[t][j] = decay(g[t][j], nx, ny);
+        sum = __fadd2_rn(sum, g[t][j]);
+      }
+    } else {
+      float x = 0.f, y = 0.f;
+#pragma unroll
+      for (int t = 0; t < kRun; ++t) {
+        x = fmaxf(x, fabsf(g[t][j].x));
+        y = fmaxf(y, fabsf(g[t][j].y));
+        sum = __fadd2_rn(sum, g[t][j]);
+      }
+      const bool nx = x < kNear, ny = y < kNear;
+      a.c_[0][j] = one_if(nx, ny);
+#pragma unroll
+      for (int t = 0; t < kRun; ++t) a.r[t][j] = decay(g[t][j], nx, ny);
+    }
+    const bool ax = fabsf(sum.x) < kNear, ay = fabsf(sum.y) < kNear;
+    all_c[j] = one_if(ax, ay);
+    all_r[j] = decay(sum, ax, ay);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // pieces: the decay over some tokens, and the state they give from a state of zero
 // ---------------------------------------------------------------------------
-struct Piece {
-  Decay a[kPairs];
-  float2 h[kPairs];
+struct Piece {                       // of one channel
+  float c, r, h;
 };
+// A piece inside which a packed sequence starts passes nothing on of what came before it,
+// not even a NaN: r = -infinity.
+__device__ __forceinline__ float cut() { return __int_as_float((int)0xff800000); }
 template <bool PACKED>
-__device__ __forceinline__ void pass_on(const Piece& q, float2 (&h)[kPairs]) {
-#pragma unroll
-  for (int j = 0; j < kPairs; ++j) h[j] = pass_on<PACKED>(q.a[j], h[j], q.h[j]);
+__device__ __forceinline__ float pass_on(const Piece& q, float h) {
+  const float n = fmaf(q.r, h, fmaf(q.c, h, q.h));
+  return PACKED && q.r == cut() ? q.h : n;
 }
-// `q`, and `next` behind it in the direction of the walk
+// `q`, and `next` behind it in the direction of the walk: (c1 + r1) (c2 + r2)
 template <bool PACKED>
 __device__ __forceinline__ void append(Piece& q, const Piece& next) {
-  pass_on<PACKED>(next, q.h);
-#pragma unroll
-  for (int j = 0; j < kPairs; ++j) q.a[j] = join_pieces<PACKED>(q.a[j], next.a[j]);
-}
-// Pieces in shared memory: a row of kLanes threads' c, then r, then h.
-constexpr int kPieceFloats = 3 * kChannels;
-__device__ __forceinline__ void put(float* row, int lane, const Piece& q) {
-  static_assert(kVec == 4, "a thread's channels are one float4");
-  float4* d = reinterpret_cast<float4*>(row) + lane;
-  d[0] = make_float4(q.a[0].c.x, q.a[0].c.y, q.a[1].c.x, q.a[1].c.y);
-  d[kLanes] = make_float4(q.a[0].r.x, q.a[0].r.y, q.a[1].r.x, q.a[1].r.y);
-  d[2 * kLanes] = make_float4(q.h[0].x, q.h[0].y, q.h[1].x, q.h[1].y);
-}
-__device__ __forceinline__ Piece take(const float* row, int lane) {
-  const float4* s = reinterpret_cast<const float4*>(row) + lane;
-  const float4 c = s[0], r = s[kLanes], h = s[2 * kLanes];
-  Piece q;
-  q.a[0] = {make_float2(c.x, c.y), make_float2(r.x, r.y)};
-  q.a[1] = {make_float2(c.z, c.w), make_float2(r.z, r.w)};
-  q.h[0] = make_float2(h.x, h.y);
-  q.h[1] = make_float2(h.z, h.w);
-  return q;
-}
-// The piece of lane `from` (decays of a cut piece included).
-__device__ __forceinline__ float2 shuffle(float2 v, int from) {
-  return make_float2(__shfl_sync(0xffffffffu, v.x, from), __shfl_sync(0xffffffffu, v.y, from));
-}
-__device__ __forceinline__ Piece shuffle(const Piece& q, int from) {
-  Piece o;
-#pragma unroll
-  for (int j = 0; j < kPairs; ++j) {
-    o.a[j].c = shuffle(q.a[j].c, from);
-    o.a[j].r = shuffle(q.a[j].r, from);
-    o.h[j] = shuffle(q.h[j], from);
+  q.h = pass_on<PACKED>(next, q.h);
+  const bool none = PACKED && (q.r == cut() || next.r == cut());
+  float c = q.c * next.c, r = fmaf(q.c, next.r, fmaf(next.c, q.r, q.r * next.r));
+  if (c == 1.f && r < -0.5f) {
+    c = 0.f;
+    r += 1.f;
   }
-  return o;
+  q.c = none ? 0.f : c;
+  q.r = none ? cut() : r;
 }
+
+// The parts' pieces of a tile.
+template <int PARTS>
+struct Parts {
+  float c[PARTS][kChannels], r[PARTS][kChannels], h[PARTS][kChannels];
+};
+__device__ __forceinline__ void put(float* row, const float2 (&v)[kPairs]) {
+  static_assert(kVec == 4, "a thread's channels are one float4");
+  reinterpret_cast<float4*>(row)[threadIdx.x % kLanes] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+}
+__device__ __forceinline__ void get(const float* row, float2 (&v)[kPairs]) {
+  const float4 t = reinterpret_cast<const float4*>(row)[threadIdx.x % kLanes];
+  v[0] = make_float2(t.x, t.y);
+  v[1] = make_float2(t.z, t.w);
+}
+
 // ---------------------------------------------------------------------------
 // pieces between the blocks of a cluster
 // ---------------------------------------------------------------------------
 // Every block sends its tile's piece to all of them (itself too) by st.async, which counts its
 // bytes on the receiver's barrier: nothing is fenced, so no block waits for its own stores
-// to memory as a cluster's barrier would (B = 4, T = 8192, D = 2048: 189 us with one).
+// to memory as a cluster's barrier would (B = 4, T = 8192, D = 2048: 189 us for 145).
 // Two turns of pieces, a barrier each: a block sends turn k + 2 when it has all of turn k + 1,
-// which every block sends when all its threads are done with turn k.
+// which every block sends when it is done with turn k.
+constexpr int kRowFloats = 3 * kChannels;
 __host__ __device__ constexpr size_t cluster_bytes(int cluster) {
-  return cluster > 1 ? (size_t)2 * cluster * kPieceFloats * sizeof(float) : 0;
+  return cluster > 1 ? (size_t)2 * cluster * kRowFloats * sizeof(float) : 0;
 }
-constexpr uint64_t kWaitNs = 2000000000;    // a wait that takes longer gives up (device error word 9)
 
 struct Exchange {
   uint64_t* full;                    // [2] in shared memory
-  float* pieces;                     // [2][cluster][kPieceFloats]
+  float* pieces;                     // [2][cluster][c, r, h][kChannels]
   int cluster, rank;
-  int* error;
-  uint64_t limit;
-  __device__ Exchange(uint64_t* full_, float* pieces_, const ScanParams& p, int rank_, int* error_)
-      : full(full_), pieces(pieces_), cluster(p.cluster), rank(rank_), error(error_), limit(kWaitNs) {
-    if (cluster == 1) return;
-    if (threadIdx.x == 0) {
-      ptx::mbar_init(full, 1);
-      ptx::mbar_init(full + 1, 1);
-      ptx::fence_mbar_init();
-    }
-    barrier();
+  __device__ Exchange(uint64_t* full_, float* pieces_, const ScanParams& p, int rank_)
+      : full(full_), pieces(pieces_), cluster(p.cluster), rank(rank_) {}
+  __device__ void init() const {     // one thread, before a barrier of the block and one of the cluster
+    ptx::mbar_init(full, 1);
+    ptx::mbar_init(full + 1, 1);
   }
-  static __device__ void barrier() {
-    asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+  __device__ void barrier() const {  // all threads
+    if (cluster > 1) asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
   }
-  __device__ float* row(int turn, int i) const { return pieces + ((turn & 1) * cluster + i) * kPieceFloats; }
-  // The warps' pieces joined in the direction of the walk (`back`: the last warp first), to
-  // every block: sixteen threads to a block.
-  template <bool PACKED>
-  __device__ void send(int turn, const float* warps, bool back) const {
+  __device__ float* at(int turn, int i, int ch) const {
+    return pieces + ((turn & 1) * cluster + i) * kRowFloats + ch;
+  }
+  __device__ Piece get(int turn, int i, int ch) const {
+    const float* s = at(turn, i, ch);
+    return {s[0], s[kChannels], s[2 * kChannels]};
+  }
+  __device__ void send(int turn, int ch, const Piece& q, bool arm) const {
     uint64_t* bar = full + (turn & 1);
-    if (threadIdx.x == 0 && limit) ptx::mbar_arrive_expect_tx(bar, cluster * kPieceFloats * sizeof(float));
-    const int lane = threadIdx.x % kLanes;
-    Piece q = take(warps + (back ? kWarps - 1 : 0) * kPieceFloats, lane);
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i)
-      append<PACKED>(q, take(warps + (back ? kWarps - 1 - i : i) * kPieceFloats, lane));
-    const uint32_t dst = ptx::smem_u32(row(turn, rank)) + 16 * lane, at = ptx::smem_u32(bar);
-    for (int i = threadIdx.x / kLanes; i < cluster; i += kThreads / kLanes) {
+    if (ch == 0 && arm) ptx::mbar_arrive_expect_tx(bar, cluster * kRowFloats * sizeof(float));
+    const uint32_t dst = ptx::smem_u32(at(turn, rank, ch)), mine = ptx::smem_u32(bar);
+    for (int i = 0; i < cluster; ++i) {
       uint32_t d, m;
       asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(dst), "r"(i));
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(at), "r"(i));
-      post(d, m, q.a[0].c, q.a[1].c);
-      post(d + 16 * kLanes, m, q.a[0].r, q.a[1].r);
-      post(d + 32 * kLanes, m, q.h[0], q.h[1]);
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(mine), "r"(i));
+      post(d, m, q.c);
+      post(d + 4 * kChannels, m, q.r);
+      post(d + 8 * kChannels, m, q.h);
     }
   }
-  static __device__ __forceinline__ void post(uint32_t dst, uint32_t bar, float2 a, float2 b) {
-    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
-                     dst), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "r"(bar) : "memory");
-  }
-  static __device__ __forceinline__ bool here(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(ptx::smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-  }
-  // Until all of a turn's pieces are here.  (A thread that gives up goes on, so that the block's
-  // barriers stay matched, and waits no more.)
-  __device__ void wait(int turn) {
-    uint64_t* bar = full + (turn & 1);
-    const uint32_t parity = (turn >> 1) & 1;
-    if (here(bar, parity)) return;
-    const uint64_t start = ptx::globaltimer_ns();
-    while (!here(bar, parity)) {
-      if (ptx::globaltimer_ns() - start >= limit) {
-        *error = kErrWait;
-        limit = 0;
-        return;
-      }
-    }
-  }
-  // No block leaves while another may still send to it.
-  __device__ void leave() const {
-    if (cluster > 1) barrier();
+  static __device__ __forceinline__ void post(uint32_t dst, uint32_t bar, float v) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(dst),
+                 "f"(v), "r"(bar) : "memory");
   }
 };
+
+// One channel's states (gradients) that enter a tile's parts, by the thread that carries the channel;
+// BACK: from the last part to the first.  `carry` enters the cluster's first tile of the
+// turn and becomes what leaves its last one.  What enters part i takes the place of h[i].
+template <bool PACKED, bool BACK, int PARTS>
+__device__ __forceinline__ void enter_parts(const Exchange& exchange, Patience& patience, int turn,
+                                            const Parts<PARTS>& parts, float (*h)[kChannels], uint32_t cuts,
+                                            float& carry, int ch) {
+  const auto part = [&](int i) {
+    return Piece{parts.c[i][ch], PACKED && (cuts >> i & 1) ? cut() : parts.r[i][ch], h[i][ch]};
+  };
+  float s = carry;
+  if (exchange.cluster > 1) {
+    Piece q = part(BACK ? PARTS - 1 : 0);
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) append<PACKED>(q, part(BACK ? PARTS - 1 - i : i));
+    exchange.send(turn, ch, q, patience.limit != 0);
+    patience.wait(exchange.full + (turn & 1), (turn >> 1) & 1);
+    for (int i = 0; i < exchange.cluster; ++i) {
+      const int j = BACK ? exchange.cluster - 1 - i : i;
+      if (j == exchange.rank) s = carry;
+      carry = pass_on<PACKED>(exchange.get(turn, j, ch), carry);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const int j = BACK ? PARTS - 1 - i : i;
+    const Piece q = part(j);
+    h[j][ch] = s;
+    s = pass_on<PACKED>(q, s);
+  }
+  if (exchange.cluster == 1) carry = s;
+}
 
 // ---------------------------------------------------------------------------
 // host
@@ -427,14 +470,46 @@ cudaError_t by_types(int x, int g, F f) {
   return g == KDA_DTYPE_F32 ? f(__nv_bfloat16{}, float{}) : f(__nv_bfloat16{}, __nv_bfloat16{});
 }
 
+// Calls f with the three flags as types.
+template <typename F>
+cudaError_t by_flags(bool a, bool b, bool c, F f) {
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (a) return b ? (c ? f(Yes{}, Yes{}, Yes{}) : f(Yes{}, Yes{}, No{})) : (c ? f(Yes{}, No{}, Yes{}) : f(Yes{}, No{}, No{}));
+  return b ? (c ? f(No{}, Yes{}, Yes{}) : f(No{}, Yes{}, No{})) : (c ? f(No{}, No{}, Yes{}) : f(No{}, No{}, No{}));
+}
+
+// The map of x, g or dh for tiles of `tile` rows; false where TMA cannot address its rows.
+template <typename T>
+bool encode(CUtensorMap* m, const void* base, const int64_t* stride, const ScanParams& p, int tile) {
+  if (base == nullptr) return true;
+  const EncodeTiled enc = encode_tiled();
+  const int64_t token = stride[1] * (int64_t)sizeof(T), batch = p.q_start ? 0 : stride[0] * (int64_t)sizeof(T);
+  if (!enc || reinterpret_cast<uintptr_t>(base) % 16 || token % 16 || batch % 16 || token < 0 || batch < 0)
+    return false;
+  const bool one = p.q_start != nullptr || p.B == 1;
+  if ((p.T > 1 && token == 0) || (!one && batch == 0)) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)p.D, (cuuint64_t)p.T, (cuuint64_t)(one ? 1 : p.B)};
+  const cuuint64_t strides[2] = {(cuuint64_t)(p.T > 1 ? token : 16), (cuuint64_t)(one ? 16 : batch)};
+  const cuuint32_t box[3] = {(cuuint32_t)kChannels, (cuuint32_t)tile, 1}, ones[3] = {1, 1, 1};
+  const CUtensorMapDataType dt = std::is_same<T, float>::value    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return enc(m, dt, 3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // A kernel over all channels and sequences, in clusters of p.cluster blocks, behind
 // mark_kernel where the batch is packed.
-inline cudaError_t launch_tiles(void (*kernel)(ScanParams), const ScanParams& p, size_t smem, cudaStream_t s) {
+template <typename... Maps>
+cudaError_t launch_tiles(void (*kernel)(ScanParams, Maps...), const ScanParams& p, int threads, size_t smem,
+                         cudaStream_t s, const Maps&... maps) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((p.D + kChannels - 1) / kChannels * (p.q_start ? 1 : p.B) * p.cluster));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
@@ -450,11 +525,12 @@ inline cudaError_t launch_tiles(void (*kernel)(ScanParams), const ScanParams& p,
     at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p, maps...);
 }
 
 int read_grad_device_error(bool clear);   // kda_scan_grad.cu's error word
-cudaError_t launch_grad(const ScanParams& p, int x_dtype, int g_dtype, bool wide, cudaStream_t s);
+cudaError_t launch_grad(ScanParams p, int x_dtype, int g_dtype, bool wide, cudaStream_t s);
+void choose_cluster(ScanParams& p, int tile, int slots);   // sets tiles and cluster
 
 }  // namespace scan
 }  // namespace kda

@@ -426,7 +426,7 @@ size_t mla_cache_args_size(void);
  * g is a log decay (<= 0).  States are fp32.
  *
  * kda_scan_fwd: h, state_out, and (ckpt not NULL) what kda_scan_bwd needs:
- *   kda_scan_ckpt_floats() values, the state that enters every 64th token.
+ *   kda_scan_ckpt_floats() values, the state that enters every 32nd token.
  * kda_scan_bwd: gradients dx, dg (types of x, g) and dstate_in (fp32), any of them
  *   may be NULL, from dh (type of x) and dstate_out (either may be NULL: zero).
  * kda_scan_step: one token for each of B rows: x, g, h [B, D] (T = 1, token strides

@@ -107,8 +107,8 @@ def test_scan_entry_points_refuse():
     assert lib.kda_scan_workspace_bytes(P(_scan_args())) == 0
     assert lib.kda_scan_workspace_bytes(P(_scan_args(T=65, q_start=FAKE))) == 2 * 24
     n = lib.kda_scan_ckpt_floats
-    assert n(P(_scan_args(T=64))) == 2 * 16 and n(P(_scan_args(T=65))) == 2 * 2 * 16
-    assert n(P(_scan_args(T=65, q_start=FAKE))) == 2 * 16 and n(P(_scan_args(T=0))) == 0
+    assert n(P(_scan_args(T=32))) == 2 * 16 and n(P(_scan_args(T=33))) == 2 * 2 * 16
+    assert n(P(_scan_args(T=33, q_start=FAKE))) == 2 * 16 and n(P(_scan_args(T=0))) == 0
 
 
 def _qk_args(**kw):
