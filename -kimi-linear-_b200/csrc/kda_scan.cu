@@ -59,7 +59,7 @@ using Fwd = Shape<kWarps>;
 
 struct Shared {
   Parts<Fwd::kParts> parts[2];       // of two turns
-  uint64_t x_full[kXSlots], g_full[kGSlots], exchange[2];
+  uint64_t full[kXSlots], exchange[2];
   uint8_t starts[2][Fwd::kParts];    // packed: a sequence starts in the part
 };
 
@@ -77,28 +77,34 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
   Patience patience(&g_scan_device_error);
   const int turns = (p.tiles + p.cluster - 1) / p.cluster;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kXSlots; ++i) ptx::mbar_init(sh.x_full + i, 1);
-    for (int i = 0; i < kGSlots; ++i) ptx::mbar_init(sh.g_full + i, 1);
+    for (int i = 0; i < kXSlots; ++i) ptx::mbar_init(sh.full + i, 1);
     exchange.init();
     ptx::fence_mbar_init();
   }
   __syncthreads();
   exchange.barrier();
   if (threadIdx.x >= Fwd::kWork) {
-    // a channel's state from turn to turn, and the copies
-    const int i_ch = threadIdx.x - Fwd::kWork, ch = w.block_c + shared_channel<WIDE>(i_ch);
-    const bool kept = ch < p.D, copies = WIDE && i_ch == 0;
+    // two channels' states from turn to turn, and the copies
+    const int at = threadIdx.x - Fwd::kWork;
+    const int ch0 = w.block_c + shared_channel<WIDE>(2 * at), ch1 = w.block_c + shared_channel<WIDE>(2 * at + 1);
+    const bool copies = WIDE && at == 0;
     const auto copy = [&](int k) {
       const int tile = k * p.cluster + w.rank;
       if (tile >= p.tiles) return;
-      xs.copy(&x_map, k, w.block_c, tile * Fwd::kTile, w.b, sh.x_full + k % kXSlots);
-      gs.copy(&g_map, k, w.block_c, tile * Fwd::kTile, w.b, sh.g_full + k % kGSlots);
+      uint64_t* bar = sh.full + k % kXSlots;
+      ptx::mbar_arrive_expect_tx(bar, XRing::kTileBytes + GRing::kTileBytes);
+      gs.copy(&g_map, k, w.block_c, tile * Fwd::kTile, w.b, bar);
+      xs.copy(&x_map, k, w.block_c, tile * Fwd::kTile, w.b, bar);
     };
     if (copies)
       for (int k = 0; k < 2; ++k) copy(k);
     if constexpr (PACKED) ptx::grid_dep_wait();
-    float carry = !PACKED && kept && p.state_in ? p.state_in[w.b * p.si_s + ch] : 0.f;
-    float* ckpt = p.ckpt && kept ? p.ckpt + (int64_t)w.b * p.steps * p.D + ch : nullptr;
+    float2 carry = both(0.f);
+    if (!PACKED && p.state_in) {
+      if (ch0 < p.D) carry.x = p.state_in[w.b * p.si_s + ch0];
+      if (ch1 < p.D) carry.y = p.state_in[w.b * p.si_s + ch1];
+    }
+    float* const ckpt = p.ckpt ? p.ckpt + (int64_t)w.b * p.steps * p.D : nullptr;
     for (int k = 0; k < turns; ++k) {
       const int buf = k & 1;
       pieces_wait(buf, Fwd::kThreads);
@@ -109,27 +115,28 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
 #pragma unroll
         for (int i = 0; i < Fwd::kParts; ++i) cuts |= (uint32_t)sh.starts[buf][i] << i;
       }
-      enter_parts<PACKED, false>(exchange, patience, k, sh.parts[buf], sh.parts[buf].h, cuts, carry, i_ch);
-      float kept_state[Fwd::kTile / kStep];
-#pragma unroll
-      for (int i = 0; i < Fwd::kTile / kStep; ++i) kept_state[i] = sh.parts[buf].h[i * (kStep / kRun)][i_ch];
-      states_done(buf, Fwd::kThreads);
+      Parts<Fwd::kParts>& parts = sh.parts[buf];
+      enter_parts<PACKED, false>(exchange, patience, k, parts, parts.h, cuts, carry, at);
       if (ckpt) {
 #pragma unroll
         for (int i = 0; i < Fwd::kTile / kStep; ++i) {
-          const int step = (k * p.cluster + w.rank) * (Fwd::kTile / kStep) + i;
-          if (step < p.steps) ckpt[(int64_t)step * p.D] = kept_state[i];
+          const int step = (k * p.cluster + w.rank) * (Fwd::kTile / kStep) + i, j = i * (kStep / kRun);
+          float2 s = pair(parts.h[j], at);
+          if (p.cluster > 1) s = pass_on<PACKED>({pair(parts.c[j], at), pair(parts.r[j], at), s}, pair(parts.entry, at));
+          if (step < p.steps && ch0 < p.D) ckpt[(int64_t)step * p.D + ch0] = s.x;
+          if (step < p.steps && ch1 < p.D) ckpt[(int64_t)step * p.D + ch1] = s.y;
         }
       }
+      states_done(buf, Fwd::kThreads);
     }
-    if (!PACKED && w.rank == 0 && kept) p.state_out[w.b * p.so_s + ch] = carry;
+    if (!PACKED && w.rank == 0) {
+      if (ch0 < p.D) p.state_out[w.b * p.so_s + ch0] = carry.x;
+      if (ch1 < p.D) p.state_out[w.b * p.so_s + ch1] = carry.y;
+    }
     if (copies) {                    // (a worker may have given up)
       Patience landed(&g_scan_device_error);
-      for (int k = max(turns - 2, 0); k < turns; ++k) {
-        if (k * p.cluster + w.rank >= p.tiles) continue;
-        landed.wait(sh.x_full + k % kXSlots, k / kXSlots & 1);
-        landed.wait(sh.g_full + k % kGSlots, k / kGSlots & 1);
-      }
+      for (int k = max(turns - 2, 0); k < turns; ++k)
+        if (k * p.cluster + w.rank < p.tiles) landed.wait(sh.full + k % kXSlots, k / kXSlots & 1);
     }
   } else {
     if constexpr (PACKED) ptx::grid_dep_wait();
@@ -141,31 +148,37 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     // turn k's pieces
     const auto pieces = [&](int k, int buf, Decays<COMPLEMENT>& a) {
       const int t0 = first_row(k);
+      Parts<Fwd::kParts>& parts = sh.parts[buf];
+      if (t0 - row0 >= p.T) {        // no tile: nothing changes
+        const float2 one[kPairs] = {both(1.f), both(1.f)}, zero[kPairs] = {};
+        put(parts.c[part], one);
+        put(parts.r[part], zero);
+        put(parts.h[part], zero);
+        if (PACKED && threadIdx.x % kLanes == 0) sh.starts[buf][part] = 0;
+        pieces_done(buf, Fwd::kThreads);
+        return;
+      }
       const RowMask m = row_mask<PACKED>(p, t0);
-      const bool tile_there = t0 - row0 < p.T;
       if constexpr (WIDE) {
-        if (tile_there) {
-          patience.wait(sh.x_full + k % kXSlots, k / kXSlots & 1);
-          patience.wait(sh.g_full + k % kGSlots, k / kGSlots & 1);
-        }
+        patience.wait(sh.full + k % kXSlots, k / kXSlots & 1);
       } else {
         xs.copy_own(x + (int64_t)t0 * p.x_s[1], p.x_s[1], k, row0, m.there, w.on);
         gs.copy_own(g + (int64_t)t0 * p.g_s[1], p.g_s[1], k, row0, m.there, w.on);
       }
+      // (rows past T are zeros: they change nothing; packed rows of no sequence are not)
+      if (PACKED && WIDE && m.there != kAllRows) {
+        gs.clear(k, row0, m.there);
+        xs.clear(k, row0, m.there);
+      }
       float2 gt[kRun][kPairs], all_c[kPairs], all_r[kPairs], h[kPairs];
 #pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        gs.read(k, row0 + t, gt[t]);
-        // (rows past T are zeros already where their tile has any)
-        if (PACKED ? !(m.there >> t & 1) : !tile_there) gt[t][0] = gt[t][1] = both(0.f);
-      }
+      for (int t = 0; t < kRun; ++t) gs.read(k, row0 + t, gt[t]);
       set_decays(a, gt, all_c, all_r);
       h[0] = h[1] = both(0.f);
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
         float2 v[kPairs];
         xs.read(k, row0 + t, v);
-        if (PACKED ? !(m.there >> t & 1) : !tile_there) v[0] = v[1] = both(0.f);
         if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
@@ -173,21 +186,21 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
           h[j] = apply(a.c(t, j), a.r[t][j], h[j], v[j]);
         }
       }
-      put(sh.parts[buf].c[part], all_c);
-      put(sh.parts[buf].r[part], all_r);
-      put(sh.parts[buf].h[part], h);
+      put(parts.c[part], all_c);
+      put(parts.r[part], all_r);
+      put(parts.h[part], h);
       if (PACKED && threadIdx.x % kLanes == 0) sh.starts[buf][part] = m.first != 0;
       pieces_done(buf, Fwd::kThreads);
     };
     // turn k's tokens again, from the state that enters them
     const auto states = [&](int k, int buf, const Decays<COMPLEMENT>& a) {
       const int t0 = first_row(k);
-      const RowMask m = row_mask<PACKED>(p, t0);
       states_wait(buf, Fwd::kThreads);
+      if (t0 >= p.T || (WIDE && !w.on)) return;
+      const RowMask m = row_mask<PACKED>(p, t0);
       float2 h[kPairs];
-      get(sh.parts[buf].h[part], h);
+      entered<PACKED>(sh.parts[buf], sh.parts[buf].h[part], p.cluster, part, h);
       TX* row = out + (int64_t)t0 * p.h_s[1];
-      if (WIDE && !w.on) return;
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
         float2 v[kPairs];
@@ -199,12 +212,13 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
           h[j] = apply(a.c(t, j), a.r[t][j], h[j], v[j]);
         }
         if (m.there >> t & 1) {
-          write<WIDE>(row + t * p.h_s[1], w.on, h);
+          write<WIDE>(row, w.on, h);
         } else if (PACKED && t0 + t < p.T) {
           const float2 zero[kPairs] = {};
-          write<WIDE>(row + t * p.h_s[1], w.on, zero);
+          write<WIDE>(row, w.on, zero);
         }
         if (PACKED && (m.last >> t & 1)) store_state<WIDE>(state_of(p, p.state_out, p.so_s, t0 + t, w.c), w.on, h);
+        row += p.h_s[1];
       }
     };
     // a turn's pieces before the turn before's states: those come meanwhile

@@ -2,10 +2,10 @@
 // what the scan and its gradient share.
 //
 // A decay a = exp(g) is held as c + r, with c = 1, r = a - 1 for a channel's run of kRun tokens
-// that all have |g| < 1/4, and c = 0, r = a for the others: rounding a itself to 24 bits is
+// that all have |g| < 1/8, and c = 0, r = a for the others: rounding a itself to 24 bits is
 // off by up to 2^-25 per token, always to the same side for a steady g, which a state that
-// remembers n tokens adds up to n 2^-25.  (A run with a larger |g| forgets a fifth, so that there
-// n stays below twenty.)  c h + r h is one instruction more than a product, and two channels
+// remembers n tokens adds up to n 2^-25.  (A run with a larger |g| forgets a tenth, so that there
+// n stays below forty.)  c h + r h is one instruction more than a product, and two channels
 // share each (fma.f32x2), so a thread works on pairs of channels.
 #pragma once
 
@@ -51,18 +51,17 @@ struct ScanParams {
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// exp(g): near zero, less one, the series up to g^6/6!, of which the first term left out is 2^-24 of
-// the sum at |g| = 1/4; elsewhere 2^(g log2 e) by the hardware's instruction (2^-22 of itself, and
+// exp(g): near zero, less one, the series up to g^5/5!, of which the first term left out is 2^-24 of
+// the sum at |g| = 1/8; elsewhere 2^(g log2 e) by the hardware's instruction (2^-22 of itself, and
 // 2^-24 |g| from the rounded exponent).  What is below 2^-126 is zero.
-constexpr float kNear = 0.25f;
+constexpr float kNear = 0.125f;
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float2 decay(float2 g, bool near_x, bool near_y) {
-  float2 p = __ffma2_rn(g, both(1.f / 720.f), both(1.f / 120.f));
-  p = __ffma2_rn(p, g, both(1.f / 24.f));
+  float2 p = __ffma2_rn(g, both(1.f / 120.f), both(1.f / 24.f));
   p = __ffma2_rn(p, g, both(1.f / 6.f));
   p = __ffma2_rn(p, g, both(0.5f));
   p = __ffma2_rn(p, g, both(1.f));
@@ -99,7 +98,7 @@ constexpr int kVec = 4;                       // channels of a thread
 constexpr int kPairs = kVec / 2;
 constexpr int kChannels = kLanes * kVec;      // of a block
 constexpr int kRun = 4;                       // tokens of a thread in a tile
-constexpr int kCarry = kChannels;             // threads that carry a channel's state each
+constexpr int kCarry = kChannels / 2;         // threads that carry the states of a pair of channels each
 constexpr int kMaxCluster = 8;
 constexpr uint64_t kWaitNs = 2000000000;      // a wait that takes longer gives up (device error word 9)
 
@@ -203,9 +202,8 @@ struct Ring {
   __device__ T* row(int k, int i) const {
     return reinterpret_cast<T*>(base + (k % SLOTS) * kTileBytes) + i * kChannels;
   }
-  // one thread: tile k from row t on, counted on `bar`
+  // one thread: tile k from row t on, its bytes counted on `bar`
   __device__ void copy(const CUtensorMap* map, int k, int c, int t, int b, uint64_t* bar) const {
-    ptx::mbar_arrive_expect_tx(bar, kTileBytes);
     ptx::tma_load_3d(base + (k % SLOTS) * kTileBytes, map, c, t, b, bar);
   }
   // a thread: its rows i .. i + kRun - 1 of tile k, those in `mask` (the others: zeros)
@@ -220,6 +218,15 @@ struct Ring {
     for (int t = 0; t < kRun; ++t)
 #pragma unroll
       for (int j = 0; j < kVec; ++j) row(k, i + t)[threadIdx.x % kLanes * kVec + j] = v[t][j];
+  }
+  // a thread: zeros for its rows that are not in `mask`
+  __device__ void clear(int k, int i, uint32_t mask) const {
+#pragma unroll
+    for (int t = 0; t < kRun; ++t) {
+      const float zero[kVec] = {};
+      if (!(mask >> t & 1)) st4(row(k, i + t) + threadIdx.x % kLanes * kVec, zero);
+    }
+    ptx::fence_proxy_async_smem();   // (TMA writes here again)
   }
   __device__ __forceinline__ void read(int k, int i, float2 (&v)[kPairs]) const {
     float t[kVec];
@@ -333,35 +340,34 @@ __device__ __forceinline__ void set_decays(Decays<EACH>& a, const float2 (&g)[kR
 // ---------------------------------------------------------------------------
 // pieces: the decay over some tokens, and the state they give from a state of zero
 // ---------------------------------------------------------------------------
-struct Piece {                       // of one channel
-  float c, r, h;
+struct Piece {                       // of a pair of channels
+  float2 c, r, h;
 };
 // A piece inside which a packed sequence starts passes nothing on of what came before it,
-// not even a NaN: r = -infinity.
-__device__ __forceinline__ float cut() { return __int_as_float((int)0xff800000); }
+// not even a NaN: r = -infinity (in both channels).
+__device__ __forceinline__ float2 cut() { return both(__int_as_float((int)0xff800000)); }
+__device__ __forceinline__ bool is_cut(float2 r) { return __float_as_int(r.x) == (int)0xff800000; }
 template <bool PACKED>
-__device__ __forceinline__ float pass_on(const Piece& q, float h) {
-  const float n = fmaf(q.r, h, fmaf(q.c, h, q.h));
-  return PACKED && q.r == cut() ? q.h : n;
+__device__ __forceinline__ float2 pass_on(const Piece& q, float2 h) {
+  const float2 n = apply(q.c, q.r, h, q.h);
+  return PACKED && is_cut(q.r) ? q.h : n;
 }
-// `q`, and `next` behind it in the direction of the walk: (c1 + r1) (c2 + r2)
+// `q`, and `next` behind it in the direction of the walk: (c1 + r1) (c2 + r2).  (Where c stays 1
+// through a tile its kParts <= 16 parts have decays of exp(-1/8) at least: of 1 + r >= exp(-2)
+// the rounding of r costs three bits at most.)
 template <bool PACKED>
 __device__ __forceinline__ void append(Piece& q, const Piece& next) {
   q.h = pass_on<PACKED>(next, q.h);
-  const bool none = PACKED && (q.r == cut() || next.r == cut());
-  float c = q.c * next.c, r = fmaf(q.c, next.r, fmaf(next.c, q.r, q.r * next.r));
-  if (c == 1.f && r < -0.5f) {
-    c = 0.f;
-    r += 1.f;
-  }
-  q.c = none ? 0.f : c;
+  const bool none = PACKED && (is_cut(q.r) || is_cut(next.r));
+  const float2 r = __ffma2_rn(q.c, next.r, __ffma2_rn(next.c, q.r, __fmul2_rn(q.r, next.r)));
+  q.c = __fmul2_rn(q.c, next.c);
   q.r = none ? cut() : r;
 }
 
-// The parts' pieces of a tile.
+// The parts' pieces of a tile, and (`entry`) what enters the tile.
 template <int PARTS>
 struct Parts {
-  float c[PARTS][kChannels], r[PARTS][kChannels], h[PARTS][kChannels];
+  float c[PARTS][kChannels], r[PARTS][kChannels], h[PARTS][kChannels], entry[kChannels];
 };
 __device__ __forceinline__ void put(float* row, const float2 (&v)[kPairs]) {
   static_assert(kVec == 4, "a thread's channels are one float4");
@@ -372,6 +378,7 @@ __device__ __forceinline__ void get(const float* row, float2 (&v)[kPairs]) {
   v[0] = make_float2(t.x, t.y);
   v[1] = make_float2(t.z, t.w);
 }
+__device__ __forceinline__ float2& pair(float* row, int i) { return reinterpret_cast<float2*>(row)[i]; }
 
 // ---------------------------------------------------------------------------
 // pieces between the blocks of a cluster
@@ -399,17 +406,15 @@ struct Exchange {
   __device__ void barrier() const {  // all threads
     if (cluster > 1) asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
   }
-  __device__ float* at(int turn, int i, int ch) const {
-    return pieces + ((turn & 1) * cluster + i) * kRowFloats + ch;
+  __device__ float* row(int turn, int i) const { return pieces + ((turn & 1) * cluster + i) * kRowFloats; }
+  __device__ Piece get(int turn, int i, int at) const {
+    float* s = row(turn, i);
+    return {pair(s, at), pair(s + kChannels, at), pair(s + 2 * kChannels, at)};
   }
-  __device__ Piece get(int turn, int i, int ch) const {
-    const float* s = at(turn, i, ch);
-    return {s[0], s[kChannels], s[2 * kChannels]};
-  }
-  __device__ void send(int turn, int ch, const Piece& q, bool arm) const {
+  __device__ void send(int turn, int at, const Piece& q, bool arm) const {
     uint64_t* bar = full + (turn & 1);
-    if (ch == 0 && arm) ptx::mbar_arrive_expect_tx(bar, cluster * kRowFloats * sizeof(float));
-    const uint32_t dst = ptx::smem_u32(at(turn, rank, ch)), mine = ptx::smem_u32(bar);
+    if (at == 0 && arm) ptx::mbar_arrive_expect_tx(bar, cluster * kRowFloats * sizeof(float));
+    const uint32_t dst = ptx::smem_u32(&pair(row(turn, rank), at)), mine = ptx::smem_u32(bar);
     for (int i = 0; i < cluster; ++i) {
       uint32_t d, m;
       asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(dst), "r"(i));
@@ -419,43 +424,65 @@ struct Exchange {
       post(d + 8 * kChannels, m, q.h);
     }
   }
-  static __device__ __forceinline__ void post(uint32_t dst, uint32_t bar, float v) {
-    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(dst),
-                 "f"(v), "r"(bar) : "memory");
+  static __device__ __forceinline__ void post(uint32_t dst, uint32_t bar, float2 v) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(dst),
+                 "f"(v.x), "f"(v.y), "r"(bar) : "memory");
   }
 };
 
-// One channel's states (gradients) that enter a tile's parts, by the thread that carries the channel;
-// BACK: from the last part to the first.  `carry` enters the cluster's first tile of the
-// turn and becomes what leaves its last one.  What enters part i takes the place of h[i].
+// What enters a tile's parts, by the thread that carries a pair of channels; BACK: from the last
+// part to the first.  `carry` enters the cluster's first tile of the turn and becomes what leaves its
+// last one.  Alone, a block leaves what enters part i in the place of h[i].  In a cluster it
+// leaves the piece of all parts before i in the place of part i's, since that can be done
+// before the other blocks' pieces are here, and what enters the tile in `entry`; a worker
+// puts the two together (entered()).
 template <bool PACKED, bool BACK, int PARTS>
 __device__ __forceinline__ void enter_parts(const Exchange& exchange, Patience& patience, int turn,
-                                            const Parts<PARTS>& parts, float (*h)[kChannels], uint32_t cuts,
-                                            float& carry, int ch) {
-  const auto part = [&](int i) {
-    return Piece{parts.c[i][ch], PACKED && (cuts >> i & 1) ? cut() : parts.r[i][ch], h[i][ch]};
+                                            Parts<PARTS>& parts, float (*h)[kChannels], uint32_t cuts, float2& carry,
+                                            int at) {
+  const auto part = [&](int j) {
+    return Piece{pair(parts.c[j], at), PACKED && (cuts >> j & 1) ? cut() : pair(parts.r[j], at), pair(h[j], at)};
   };
-  float s = carry;
-  if (exchange.cluster > 1) {
-    Piece q = part(BACK ? PARTS - 1 : 0);
+  if (exchange.cluster == 1) {
 #pragma unroll
-    for (int i = 1; i < PARTS; ++i) append<PACKED>(q, part(BACK ? PARTS - 1 - i : i));
-    exchange.send(turn, ch, q, patience.limit != 0);
-    patience.wait(exchange.full + (turn & 1), (turn >> 1) & 1);
-    for (int i = 0; i < exchange.cluster; ++i) {
-      const int j = BACK ? exchange.cluster - 1 - i : i;
-      if (j == exchange.rank) s = carry;
-      carry = pass_on<PACKED>(exchange.get(turn, j, ch), carry);
+    for (int i = 0; i < PARTS; ++i) {
+      const int j = BACK ? PARTS - 1 - i : i;
+      const Piece q = part(j);
+      pair(h[j], at) = carry;
+      carry = pass_on<PACKED>(q, carry);
     }
+    return;
   }
+  Piece all{both(1.f), both(0.f), both(0.f)};
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
     const int j = BACK ? PARTS - 1 - i : i;
     const Piece q = part(j);
-    h[j][ch] = s;
-    s = pass_on<PACKED>(q, s);
+    pair(parts.c[j], at) = all.c;
+    pair(parts.r[j], at) = all.r;
+    pair(h[j], at) = all.h;
+    append<PACKED>(all, q);
   }
-  if (exchange.cluster == 1) carry = s;
+  exchange.send(turn, at, all, patience.limit != 0);
+  patience.wait(exchange.full + (turn & 1), (turn >> 1) & 1);
+  for (int i = 0; i < exchange.cluster; ++i) {
+    const int j = BACK ? exchange.cluster - 1 - i : i;
+    if (j == exchange.rank) pair(parts.entry, at) = carry;
+    carry = pass_on<PACKED>(exchange.get(turn, j, at), carry);
+  }
+}
+// What enters a worker's part.
+template <bool PACKED, int PARTS>
+__device__ __forceinline__ void entered(const Parts<PARTS>& parts, const float* h, int cluster, int part,
+                                        float2 (&s)[kPairs]) {
+  get(h, s);
+  if (cluster == 1) return;
+  float2 c[kPairs], r[kPairs], e[kPairs];
+  get(parts.c[part], c);
+  get(parts.r[part], r);
+  get(parts.entry, e);
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) s[j] = pass_on<PACKED>({c[j], r[j], s[j]}, e[j]);
 }
 
 // ---------------------------------------------------------------------------

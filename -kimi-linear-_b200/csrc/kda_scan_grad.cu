@@ -21,7 +21,7 @@ using Bwd = Shape<kWarps>;
 struct Shared {
   Parts<Bwd::kParts> parts[2];
   float back[2][Bwd::kParts][kChannels];   // the parts' gradients from zero, then what enters them
-  uint64_t x_full[kXSlots], d_full[kXSlots], g_full[kGSlots], exchange[2];
+  uint64_t full[kXSlots], exchange[2];
   uint8_t ends[2][Bwd::kParts];      // packed: a sequence starts (1), ends (2) in the part
 };
 
@@ -40,11 +40,7 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
   Patience patience(&g_grad_device_error);
   const int turns = (p.tiles + p.cluster - 1) / p.cluster;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kXSlots; ++i) {
-      ptx::mbar_init(sh.x_full + i, 1);
-      ptx::mbar_init(sh.d_full + i, 1);
-    }
-    for (int i = 0; i < kGSlots; ++i) ptx::mbar_init(sh.g_full + i, 1);
+    for (int i = 0; i < kXSlots; ++i) ptx::mbar_init(sh.full + i, 1);
     exchange.init();
     ptx::fence_mbar_init();
   }
@@ -52,38 +48,49 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
   exchange.barrier();
   const auto tile_of = [&](int k) { return (turns - 1 - k) * p.cluster + w.rank; };
   if (threadIdx.x >= Bwd::kWork) {
-    // a channel's gradient from turn to turn, its states in a tile, and the copies
-    const int i_ch = threadIdx.x - Bwd::kWork, ch = w.block_c + shared_channel<WIDE>(i_ch);
-    const bool kept = ch < p.D, copies = WIDE && i_ch == 0;
+    // two channels' gradients from turn to turn, their states in a tile, and the copies
+    const int at = threadIdx.x - Bwd::kWork;
+    const int ch0 = w.block_c + shared_channel<WIDE>(2 * at), ch1 = w.block_c + shared_channel<WIDE>(2 * at + 1);
+    const bool copies = WIDE && at == 0;
     const auto copy = [&](int k) {
-      const int tile = tile_of(k);
-      uint64_t *xb = sh.x_full + k % kXSlots, *gb = sh.g_full + k % kGSlots, *db = sh.d_full + k % kXSlots;
       if (k >= turns) return;
+      const int tile = tile_of(k);
+      uint64_t* bar = sh.full + k % kXSlots;
       if (tile >= p.tiles) {         // (the first turn's may be missing: its phase passes all the same)
-        ptx::mbar_arrive(xb);
-        ptx::mbar_arrive(gb);
-        if (p.dh) ptx::mbar_arrive(db);
+        ptx::mbar_arrive(bar);
         return;
       }
-      xs.copy(&x_map, k, w.block_c, tile * Bwd::kTile, w.b, xb);
-      gs.copy(&g_map, k, w.block_c, tile * Bwd::kTile, w.b, gb);
-      if (p.dh) ds.copy(&d_map, k, w.block_c, tile * Bwd::kTile, w.b, db);
+      ptx::mbar_arrive_expect_tx(bar, (p.dh ? 2 : 1) * XRing::kTileBytes + GRing::kTileBytes);
+      gs.copy(&g_map, k, w.block_c, tile * Bwd::kTile, w.b, bar);
+      xs.copy(&x_map, k, w.block_c, tile * Bwd::kTile, w.b, bar);
+      if (p.dh) ds.copy(&d_map, k, w.block_c, tile * Bwd::kTile, w.b, bar);
     };
     if (copies)
       for (int k = 0; k < 2; ++k) copy(k);
     if constexpr (PACKED) ptx::grid_dep_wait();
-    float carry = !PACKED && kept && p.dstate_out ? p.dstate_out[w.b * p.dso_s + ch] : 0.f;
-    const float* ckpt = p.ckpt + (int64_t)w.b * p.steps * p.D + ch;
+    float2 carry = both(0.f);
+    if (!PACKED && p.dstate_out) {
+      if (ch0 < p.D) carry.x = p.dstate_out[w.b * p.dso_s + ch0];
+      if (ch1 < p.D) carry.y = p.dstate_out[w.b * p.dso_s + ch1];
+    }
     static_assert(Bwd::kTile == kStep, "a tile starts at a checkpoint");
-    // (without tokens there is no tile at all; the first turn's may be missing)
-    float next = turns > 0 && kept && tile_of(0) < p.tiles ? ckpt[(int64_t)tile_of(0) * p.D] : 0.f;
+    // (the first turn's tile may be missing)
+    const auto checkpoint = [&](int k) {
+      float2 s = both(0.f);
+      if (k >= turns || tile_of(k) >= p.tiles) return s;
+      const float* row = p.ckpt + ((int64_t)w.b * p.steps + tile_of(k)) * p.D;
+      if (ch0 < p.D) s.x = row[ch0];
+      if (ch1 < p.D) s.y = row[ch1];
+      return s;
+    };
+    float2 next = checkpoint(0);
     for (int k = 0; k < turns; ++k) {
       const int buf = k & 1;
-      float state = next;
+      float2 state = next;
       pieces_wait(buf, Bwd::kThreads);
       // the workers are done with the gates of turn k and with the other rows of turn k - 2
       if (copies && patience.limit) copy(k + 2);
-      if (k + 1 < turns && kept) next = ckpt[(int64_t)tile_of(k + 1) * p.D];
+      next = checkpoint(k + 1);
       uint32_t cuts = 0, starts = 0;
       if constexpr (PACKED) {
 #pragma unroll
@@ -92,24 +99,24 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
           cuts |= (uint32_t)(sh.ends[buf][i] >> 1) << i;
         }
       }
+      Parts<Bwd::kParts>& parts = sh.parts[buf];
 #pragma unroll
       for (int i = 0; i < Bwd::kParts; ++i) {
-        const Piece q{sh.parts[buf].c[i][i_ch], PACKED && (starts >> i & 1) ? cut() : sh.parts[buf].r[i][i_ch],
-                      sh.parts[buf].h[i][i_ch]};
-        sh.parts[buf].h[i][i_ch] = state;
+        const Piece q{pair(parts.c[i], at), PACKED && (starts >> i & 1) ? cut() : pair(parts.r[i], at),
+                      pair(parts.h[i], at)};
+        pair(parts.h[i], at) = state;
         state = pass_on<PACKED>(q, state);
       }
-      enter_parts<PACKED, true>(exchange, patience, k, sh.parts[buf], sh.back[buf], cuts, carry, i_ch);
+      enter_parts<PACKED, true>(exchange, patience, k, parts, sh.back[buf], cuts, carry, at);
       states_done(buf, Bwd::kThreads);
     }
-    if (!PACKED && p.dstate_in && w.rank == 0 && kept) p.dstate_in[w.b * p.dsi_s + ch] = carry;
+    if (!PACKED && p.dstate_in && w.rank == 0) {
+      if (ch0 < p.D) p.dstate_in[w.b * p.dsi_s + ch0] = carry.x;
+      if (ch1 < p.D) p.dstate_in[w.b * p.dsi_s + ch1] = carry.y;
+    }
     if (copies) {                    // (a worker may have given up)
       Patience landed(&g_grad_device_error);
-      for (int k = max(turns - 2, 0); k < turns; ++k) {
-        landed.wait(sh.x_full + k % kXSlots, k / kXSlots & 1);
-        landed.wait(sh.g_full + k % kGSlots, k / kGSlots & 1);
-        if (p.dh) landed.wait(sh.d_full + k % kXSlots, k / kXSlots & 1);
-      }
+      for (int k = max(turns - 2, 0); k < turns; ++k) landed.wait(sh.full + k % kXSlots, k / kXSlots & 1);
     }
   } else {
     if constexpr (PACKED) ptx::grid_dep_wait();
@@ -119,36 +126,41 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     const TX* dh = p.dh ? static_cast<const TX*>(p.dh) + w.b * p.dh_s[0] + w.c : nullptr;
     TX* const dx = p.dx ? static_cast<TX*>(p.dx) + w.b * p.dx_s[0] + w.c : nullptr;
     TG* const dg = p.dg ? static_cast<TG*>(p.dg) + w.b * p.dg_s[0] + w.c : nullptr;
-    // row t of the thread's x or dh of turn k; zeros for a row that is not there
-    const auto read = [&](const XRing& ring, int k, int t, uint32_t there, bool tile_there, float2 (&v)[kPairs]) {
-      ring.read(k, row0 + t, v);
-      if (PACKED ? !(there >> t & 1) : !tile_there) v[0] = v[1] = both(0.f);
-    };
     const auto pieces = [&](int k, int buf, Decays<COMPLEMENT>& a) {
       const int t0 = tile_of(k) * Bwd::kTile + row0;
+      Parts<Bwd::kParts>& parts = sh.parts[buf];
+      if (WIDE) patience.wait(sh.full + k % kXSlots, k / kXSlots & 1);
+      if (t0 - row0 >= p.T) {        // no tile: nothing changes
+        const float2 one[kPairs] = {both(1.f), both(1.f)}, zero[kPairs] = {};
+        put(parts.c[part], one);
+        put(parts.r[part], zero);
+        put(parts.h[part], zero);
+        put(sh.back[buf][part], zero);
+        if (PACKED && threadIdx.x % kLanes == 0) sh.ends[buf][part] = 0;
+        pieces_done(buf, Bwd::kThreads);
+        return;
+      }
       const RowMask m = row_mask<PACKED>(p, t0);
-      const bool tile_there = t0 - row0 < p.T;
-      if constexpr (WIDE) {
-        patience.wait(sh.g_full + k % kGSlots, k / kGSlots & 1);
-        patience.wait(sh.x_full + k % kXSlots, k / kXSlots & 1);
-        if (p.dh) patience.wait(sh.d_full + k % kXSlots, k / kXSlots & 1);
-      } else {
+      if constexpr (!WIDE) {
         xs.copy_own(x + (int64_t)t0 * p.x_s[1], p.x_s[1], k, row0, m.there, w.on);
         gs.copy_own(g + (int64_t)t0 * p.g_s[1], p.g_s[1], k, row0, m.there, w.on);
         if (p.dh) ds.copy_own(dh + (int64_t)t0 * p.dh_s[1], p.dh_s[1], k, row0, m.there, w.on);
       }
+      // (rows past T are zeros: they change nothing; packed rows of no sequence are not)
+      if (PACKED && WIDE && m.there != kAllRows) {
+        gs.clear(k, row0, m.there);
+        xs.clear(k, row0, m.there);
+        ds.clear(k, row0, m.there);
+      }
       float2 gt[kRun][kPairs], all_c[kPairs], all_r[kPairs], h[kPairs], u[kPairs];
 #pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        gs.read(k, row0 + t, gt[t]);
-        if (PACKED ? !(m.there >> t & 1) : !tile_there) gt[t][0] = gt[t][1] = both(0.f);
-      }
+      for (int t = 0; t < kRun; ++t) gs.read(k, row0 + t, gt[t]);
       set_decays(a, gt, all_c, all_r);
       h[0] = h[1] = u[0] = u[1] = both(0.f);
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
         float2 v[kPairs];
-        read(xs, k, t, m.there, tile_there, v);
+        xs.read(k, row0 + t, v);
         if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
@@ -159,30 +171,30 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
 #pragma unroll
       for (int t = kRun - 1; t >= 0; --t) {
         float2 d[kPairs] = {both(0.f), both(0.f)};
-        if (p.dh) read(ds, k, t, m.there, tile_there, d);
+        if (p.dh) ds.read(k, row0 + t, d);
         if (PACKED && (m.last >> t & 1)) load_state<WIDE>(state_of(p, p.dstate_out, p.dso_s, t0 + t, w.c), w.on, u);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) u[j] = times(a.c(t, j), a.r[t][j], __fadd2_rn(d[j], u[j]));
       }
-      put(sh.parts[buf].c[part], all_c);
-      put(sh.parts[buf].r[part], all_r);
-      put(sh.parts[buf].h[part], h);
+      put(parts.c[part], all_c);
+      put(parts.r[part], all_r);
+      put(parts.h[part], h);
       put(sh.back[buf][part], u);
       if (PACKED && threadIdx.x % kLanes == 0) sh.ends[buf][part] = (m.first != 0) | (m.last != 0) << 1;
       pieces_done(buf, Bwd::kThreads);
     };
     const auto grads = [&](int k, int buf, const Decays<COMPLEMENT>& a) {
       const int t0 = tile_of(k) * Bwd::kTile + row0;
-      const RowMask m = row_mask<PACKED>(p, t0);
       states_wait(buf, Bwd::kThreads);
-      if ((WIDE && !w.on) || t0 >= p.T) return;
+      if (t0 >= p.T || (WIDE && !w.on)) return;
+      const RowMask m = row_mask<PACKED>(p, t0);
       float2 h[kPairs], u[kPairs], v[kRun][kPairs];
       // a_t h_{t-1} (complement: a_t (h_{t-1} - x_t))
       get(sh.parts[buf].h[part], h);
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
         float2 xt[kPairs];
-        read(xs, k, t, m.there, true, xt);
+        xs.read(k, row0 + t, xt);
         if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
@@ -196,11 +208,13 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
           }
         }
       }
-      get(sh.back[buf][part], u);
+      entered<PACKED>(sh.parts[buf], sh.back[buf][part], p.cluster, part, u);
+      TX* dx_row = dx ? dx + (int64_t)(t0 + kRun - 1) * p.dx_s[1] : nullptr;
+      TG* dg_row = dg ? dg + (int64_t)(t0 + kRun - 1) * p.dg_s[1] : nullptr;
 #pragma unroll
       for (int t = kRun - 1; t >= 0; --t) {
         float2 d[kPairs] = {both(0.f), both(0.f)}, ox[kPairs], og[kPairs];
-        if (p.dh) read(ds, k, t, m.there, true, d);
+        if (p.dh) ds.read(k, row0 + t, d);
         if (PACKED && (m.last >> t & 1)) load_state<WIDE>(state_of(p, p.dstate_out, p.dso_s, t0 + t, w.c), w.on, u);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
@@ -213,9 +227,11 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
         const bool there = m.there >> t & 1;
         if (PACKED && !there) ox[0] = ox[1] = og[0] = og[1] = both(0.f);
         if (there || (PACKED && t0 + t < p.T)) {
-          if (dx) write<WIDE>(dx + (int64_t)(t0 + t) * p.dx_s[1], w.on, ox);
-          if (dg) write<WIDE>(dg + (int64_t)(t0 + t) * p.dg_s[1], w.on, og);
+          if (dx) write<WIDE>(dx_row, w.on, ox);
+          if (dg) write<WIDE>(dg_row, w.on, og);
         }
+        if (dx) dx_row -= p.dx_s[1];
+        if (dg) dg_row -= p.dg_s[1];
         if (PACKED && p.dstate_in && (m.first >> t & 1))
           store_state<WIDE>(state_of(p, p.dstate_in, p.dsi_s, t0 + t, w.c), w.on, u);
       }
