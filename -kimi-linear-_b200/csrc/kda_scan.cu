@@ -54,12 +54,16 @@ __global__ void __launch_bounds__(kMarked) mark_kernel(const ScanParams p, int m
 // forward
 // ---------------------------------------------------------------------------
 constexpr int kWarps = 8;
-constexpr int kXSlots = 4, kGSlots = 2;
+constexpr int kSlots = 3;
 using Fwd = Shape<kWarps>;
 
+// A thread's decays and (weighed) inputs of a turn.
+struct Run {
+  float2 a[kRun][kPairs], v[kRun][kPairs];
+};
 struct Shared {
   Parts<Fwd::kParts> parts[2];       // of two turns
-  uint64_t full[kXSlots], exchange[2];
+  uint64_t full[kSlots], exchange[2];
   uint8_t starts[2][Fwd::kParts];    // packed: a sequence starts in the part
 };
 
@@ -67,8 +71,8 @@ template <typename TX, typename TG, bool WIDE, bool PACKED, bool COMPLEMENT>
 __global__ void __launch_bounds__(Fwd::kThreads, 2)
 scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap g_map) {
   extern __shared__ __align__(128) unsigned char smem[];
-  using XRing = Ring<TX, Fwd::kTile, kXSlots>;
-  using GRing = Ring<TG, Fwd::kTile, kGSlots>;
+  using XRing = Ring<TX, Fwd::kTile, kSlots>;
+  using GRing = Ring<TG, Fwd::kTile, kSlots>;
   const XRing xs{smem};
   const GRing gs{smem + XRing::kBytes};
   Shared& sh = *reinterpret_cast<Shared*>(smem + XRing::kBytes + GRing::kBytes);
@@ -77,7 +81,7 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
   Patience patience(&g_scan_device_error);
   const int turns = (p.tiles + p.cluster - 1) / p.cluster;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kXSlots; ++i) ptx::mbar_init(sh.full + i, 1);
+    for (int i = 0; i < kSlots; ++i) ptx::mbar_init(sh.full + i, 1);
     exchange.init();
     ptx::fence_mbar_init();
   }
@@ -91,13 +95,13 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     const auto copy = [&](int k) {
       const int tile = k * p.cluster + w.rank;
       if (tile >= p.tiles) return;
-      uint64_t* bar = sh.full + k % kXSlots;
+      uint64_t* bar = sh.full + k % kSlots;
       ptx::mbar_arrive_expect_tx(bar, XRing::kTileBytes + GRing::kTileBytes);
       gs.copy(&g_map, k, w.block_c, tile * Fwd::kTile, w.b, bar);
       xs.copy(&x_map, k, w.block_c, tile * Fwd::kTile, w.b, bar);
     };
     if (copies)
-      for (int k = 0; k < 2; ++k) copy(k);
+      for (int k = 0; k < kSlots; ++k) copy(k);
     if constexpr (PACKED) ptx::grid_dep_wait();
     float2 carry = both(0.f);
     if (!PACKED && p.state_in) {
@@ -108,8 +112,8 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     for (int k = 0; k < turns; ++k) {
       const int buf = k & 1;
       pieces_wait(buf, Fwd::kThreads);
-      // the workers are done with the gates of turn k and with the inputs of turn k - 2
-      if (copies && patience.limit) copy(k + 2);
+      // the workers have read the rows of turn k
+      if (copies && patience.limit) copy(k + kSlots);
       uint32_t cuts = 0;
       if constexpr (PACKED) {
 #pragma unroll
@@ -135,8 +139,8 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     }
     if (copies) {                    // (a worker may have given up)
       Patience landed(&g_scan_device_error);
-      for (int k = max(turns - 2, 0); k < turns; ++k)
-        if (k * p.cluster + w.rank < p.tiles) landed.wait(sh.full + k % kXSlots, k / kXSlots & 1);
+      for (int k = max(turns - kSlots, 0); k < turns; ++k)
+        if (k * p.cluster + w.rank < p.tiles) landed.wait(sh.full + k % kSlots, k / kSlots & 1);
     }
   } else {
     if constexpr (PACKED) ptx::grid_dep_wait();
@@ -146,7 +150,7 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     TX* const out = static_cast<TX*>(p.h) + w.b * p.h_s[0] + w.c;
     const auto first_row = [&](int k) { return (k * p.cluster + w.rank) * Fwd::kTile + row0; };
     // turn k's pieces
-    const auto pieces = [&](int k, int buf, Decays<COMPLEMENT>& a) {
+    const auto pieces = [&](int k, int buf, Run& run) {
       const int t0 = first_row(k);
       Parts<Fwd::kParts>& parts = sh.parts[buf];
       if (t0 - row0 >= p.T) {        // no tile: nothing changes
@@ -160,7 +164,7 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       }
       const RowMask m = row_mask<PACKED>(p, t0);
       if constexpr (WIDE) {
-        patience.wait(sh.full + k % kXSlots, k / kXSlots & 1);
+        patience.wait(sh.full + k % kSlots, k / kSlots & 1);
       } else {
         xs.copy_own(x + (int64_t)t0 * p.x_s[1], p.x_s[1], k, row0, m.there, w.on);
         gs.copy_own(g + (int64_t)t0 * p.g_s[1], p.g_s[1], k, row0, m.there, w.on);
@@ -170,30 +174,32 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
         gs.clear(k, row0, m.there);
         xs.clear(k, row0, m.there);
       }
-      float2 gt[kRun][kPairs], all_c[kPairs], all_r[kPairs], h[kPairs];
-#pragma unroll
-      for (int t = 0; t < kRun; ++t) gs.read(k, row0 + t, gt[t]);
-      set_decays(a, gt, all_c, all_r);
-      h[0] = h[1] = both(0.f);
+      float2 sum[kPairs], c[kPairs], r[kPairs], h[kPairs];
+      sum[0] = sum[1] = h[0] = h[1] = both(0.f);
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
-        float2 v[kPairs];
-        xs.read(k, row0 + t, v);
+        float2 gt[kPairs];
+        gs.read(k, row0 + t, gt);
+        xs.read(k, row0 + t, run.v[t]);
         if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          if (COMPLEMENT) v[j] = __fmul2_rn(v[j], rest(a.c(t, j), a.r[t][j]));
-          h[j] = apply(a.c(t, j), a.r[t][j], h[j], v[j]);
+          run.a[t][j] = decay(gt[j]);
+          sum[j] = __fadd2_rn(sum[j], gt[j]);
+          if (COMPLEMENT) run.v[t][j] = __fmul2_rn(run.v[t][j], rest(gt[j], run.a[t][j]));
+          h[j] = __ffma2_rn(run.a[t][j], h[j], run.v[t][j]);
         }
       }
-      put(parts.c[part], all_c);
-      put(parts.r[part], all_r);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) split_decay(sum[j], c[j], r[j]);
+      put(parts.c[part], c);
+      put(parts.r[part], r);
       put(parts.h[part], h);
       if (PACKED && threadIdx.x % kLanes == 0) sh.starts[buf][part] = m.first != 0;
       pieces_done(buf, Fwd::kThreads);
     };
     // turn k's tokens again, from the state that enters them
-    const auto states = [&](int k, int buf, const Decays<COMPLEMENT>& a) {
+    const auto states = [&](int k, int buf, const Run& run) {
       const int t0 = first_row(k);
       states_wait(buf, Fwd::kThreads);
       if (t0 >= p.T || (WIDE && !w.on)) return;
@@ -203,14 +209,9 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       TX* row = out + (int64_t)t0 * p.h_s[1];
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
-        float2 v[kPairs];
-        xs.read(k, row0 + t, v);
         if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          if (COMPLEMENT) v[j] = __fmul2_rn(v[j], rest(a.c(t, j), a.r[t][j]));
-          h[j] = apply(a.c(t, j), a.r[t][j], h[j], v[j]);
-        }
+        for (int j = 0; j < kPairs; ++j) h[j] = __ffma2_rn(run.a[t][j], h[j], run.v[t][j]);
         if (m.there >> t & 1) {
           write<WIDE>(row, w.on, h);
         } else if (PACKED && t0 + t < p.T) {
@@ -222,7 +223,7 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       }
     };
     // a turn's pieces before the turn before's states: those come meanwhile
-    Decays<COMPLEMENT> a, b;
+    Run a, b;
     for (int k = 0; k <= turns; k += 2) {
       if (k < turns) pieces(k, 0, a);
       if (k > 0) states(k - 1, 1, b);
@@ -240,7 +241,7 @@ cudaError_t launch_forward(ScanParams p, int x_dtype, int g_dtype, bool wide, cu
     using TG = decltype(g);
     CUtensorMap mx, mg;
     const bool tma = wide && encode<TX>(&mx, p.x, p.x_s, p, Fwd::kTile) && encode<TG>(&mg, p.g, p.g_s, p, Fwd::kTile);
-    const size_t smem = Ring<TX, Fwd::kTile, kXSlots>::kBytes + Ring<TG, Fwd::kTile, kGSlots>::kBytes +
+    const size_t smem = Ring<TX, Fwd::kTile, kSlots>::kBytes + Ring<TG, Fwd::kTile, kSlots>::kBytes +
                         sizeof(Shared) + cluster_bytes(p.cluster);
     return by_flags(tma, p.q_start != nullptr, p.complement, [&](auto wide_, auto packed, auto complement) {
       return launch_tiles(scan_kernel<TX, TG, wide_.value, packed.value, complement.value>, p, Fwd::kThreads, smem, s,
@@ -282,11 +283,11 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, 
     }
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const bool nx = fabsf(g[i]) < kNear, ny = fabsf(g[i + 1]) < kNear;
-      const float2 r = decay(make_float2(g[i], g[i + 1]), nx, ny), c2 = one_if(nx, ny);
-      float2 v = make_float2(x[i], x[i + 1]);
-      if (p.complement) v = __fmul2_rn(v, rest(c2, r));
-      v = apply(c2, r, make_float2(h[i], h[i + 1]), v);
+      const float2 gi = make_float2(g[i], g[i + 1]);
+      float2 v = make_float2(x[i], x[i + 1]), c2, r;
+      if (p.complement) v = __fmul2_rn(v, rest(gi, decay(gi)));
+      split_decay(gi, c2, r);
+      v = pass_on<false>({c2, r, v}, make_float2(h[i], h[i + 1]));
       h[i] = v.x;
       h[i + 1] = v.y;
     }

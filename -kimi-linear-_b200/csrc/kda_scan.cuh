@@ -1,12 +1,12 @@
 // kda_scan.cuh -- gated linear recurrence: parameters, the arithmetic of its decays, and
 // what the scan and its gradient share.
 //
-// A decay a = exp(g) is held as c + r, with c = 1, r = a - 1 for a channel's run of kRun tokens
-// that all have |g| < 1/8, and c = 0, r = a for the others: rounding a itself to 24 bits is
-// off by up to 2^-25 per token, always to the same side for a steady g, which a state that
-// remembers n tokens adds up to n 2^-25.  (A run with a larger |g| forgets a tenth, so that there
-// n stays below forty.)  c h + r h is one instruction more than a product, and two channels
-// share each (fma.f32x2), so a thread works on pairs of channels.
+// Inside a run of kRun tokens a decay is a = exp(g) in 24 bits.  Over a whole run, where it leads
+// from one run to the next, it is held as c + r, c = 1 and r = a - 1 where |sum of g| is small
+// and c = 0, r = a elsewhere: a in 24 bits is off by up to 2^-25, always to the same side for a
+// steady g, which a state that remembers n runs adds up to n 2^-25.  (Rounding inside a run is not
+// carried on.)  c h + r h is one instruction more than a product, and two channels share each
+// (fma.f32x2), so a thread works on pairs of channels.
 #pragma once
 
 #include "kda_internal.cuh"
@@ -51,34 +51,38 @@ struct ScanParams {
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// exp(g): near zero, less one, the series up to g^5/5!, of which the first term left out is 2^-24 of
-// the sum at |g| = 1/8; elsewhere 2^(g log2 e) by the hardware's instruction (2^-22 of itself, and
-// 2^-24 |g| from the rounded exponent).  What is below 2^-126 is zero.
-constexpr float kNear = 0.125f;
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float2 decay(float2 g, bool near_x, bool near_y) {
+// exp(g) = 2^(g log2 e) by the hardware's instruction: off by 2^-22 of itself, and 2^-24 |g| from
+// the rounded exponent.  What is below 2^-126 is zero.
+__device__ __forceinline__ float2 decay(float2 g) {
+  const float2 e = __fmul2_rn(g, both(1.4426950408889634f));
+  return make_float2(exp2_fast(e.x), exp2_fast(e.y));
+}
+// exp(g) - 1 by its series up to g^5/5!, of which the first term left out is 2^-24 of the sum at
+// |g| = kNear.
+constexpr float kNear = 0.125f;
+__device__ __forceinline__ float2 decay_less_one(float2 g) {
   float2 p = __ffma2_rn(g, both(1.f / 120.f), both(1.f / 24.f));
   p = __ffma2_rn(p, g, both(1.f / 6.f));
   p = __ffma2_rn(p, g, both(0.5f));
   p = __ffma2_rn(p, g, both(1.f));
-  p = __fmul2_rn(p, g);
-  const float2 e = __fmul2_rn(g, both(1.4426950408889634f));
-  return make_float2(near_x ? p.x : exp2_fast(e.x), near_y ? p.y : exp2_fast(e.y));
+  return __fmul2_rn(p, g);
 }
-__device__ __forceinline__ float2 one_if(bool x, bool y) { return make_float2(x ? 1.f : 0.f, y ? 1.f : 0.f); }
-// a h + b
-__device__ __forceinline__ float2 apply(float2 c, float2 r, float2 h, float2 b) {
-  return __ffma2_rn(r, h, __ffma2_rn(c, h, b));
+// exp(g) as c + r
+__device__ __forceinline__ void split_decay(float2 g, float2& c, float2& r) {
+  const float2 p = decay_less_one(g), e = decay(g);
+  const bool x = fabsf(g.x) < kNear, y = fabsf(g.y) < kNear;
+  c = make_float2(x ? 1.f : 0.f, y ? 1.f : 0.f);
+  r = make_float2(x ? p.x : e.x, y ? p.y : e.y);
 }
-// a v
-__device__ __forceinline__ float2 times(float2 c, float2 r, float2 v) { return __ffma2_rn(r, v, __fmul2_rn(c, v)); }
-// 1 - a
-__device__ __forceinline__ float2 rest(float2 c, float2 r) {
-  return __ffma2_rn(r, both(-1.f), __ffma2_rn(c, both(-1.f), both(1.f)));
+// 1 - exp(g) to 24 bits, a = exp(g) given
+__device__ __forceinline__ float2 rest(float2 g, float2 a) {
+  const float2 p = decay_less_one(g), w = __ffma2_rn(a, both(-1.f), both(1.f));
+  return make_float2(fabsf(g.x) < kNear ? -p.x : w.x, fabsf(g.y) < kNear ? -p.y : w.y);
 }
 
 // The last sequence of a packed batch that starts at row t or before it (-1: none).  Of those
@@ -297,46 +301,6 @@ __device__ __forceinline__ RowMask row_mask(const ScanParams& p, int t) {
   return m;
 }
 
-// The decays of a run.  EACH: a c for every token (1 - a needs it), else one for the run.
-template <bool EACH>
-struct Decays {
-  float2 c_[EACH ? kRun : 1][kPairs], r[kRun][kPairs];
-  __device__ __forceinline__ float2 c(int t, int j) const { return c_[EACH ? t : 0][j]; }
-};
-// From the gates; also the decay over all of them, by their sum.
-template <bool EACH>
-__device__ __forceinline__ void set_decays(Decays<EACH>& a, const float2 (&g)[kRun][kPairs], float2 (&all_c)[kPairs],
-                                           float2 (&all_r)[kPairs]) {
-#pragma unroll
-  for (int j = 0; j < kPairs; ++j) {
-    float2 sum = both(0.f);
-    if constexpr (EACH) {
-#pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        const bool nx = fabsf(g[t][j].x) < kNear, ny = fabsf(g[t][j].y) < kNear;
-        a.c_[t][j] = one_if(nx, ny);
-        a.r[t][j] = decay(g[t][j], nx, ny);
-        sum = __fadd2_rn(sum, g[t][j]);
-      }
-    } else {
-      float x = 0.f, y = 0.f;
-#pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        x = fmaxf(x, fabsf(g[t][j].x));
-        y = fmaxf(y, fabsf(g[t][j].y));
-        sum = __fadd2_rn(sum, g[t][j]);
-      }
-      const bool nx = x < kNear, ny = y < kNear;
-      a.c_[0][j] = one_if(nx, ny);
-#pragma unroll
-      for (int t = 0; t < kRun; ++t) a.r[t][j] = decay(g[t][j], nx, ny);
-    }
-    const bool ax = fabsf(sum.x) < kNear, ay = fabsf(sum.y) < kNear;
-    all_c[j] = one_if(ax, ay);
-    all_r[j] = decay(sum, ax, ay);
-  }
-}
-
 // ---------------------------------------------------------------------------
 // pieces: the decay over some tokens, and the state they give from a state of zero
 // ---------------------------------------------------------------------------
@@ -349,12 +313,12 @@ __device__ __forceinline__ float2 cut() { return both(__int_as_float((int)0xff80
 __device__ __forceinline__ bool is_cut(float2 r) { return __float_as_int(r.x) == (int)0xff800000; }
 template <bool PACKED>
 __device__ __forceinline__ float2 pass_on(const Piece& q, float2 h) {
-  const float2 n = apply(q.c, q.r, h, q.h);
+  const float2 n = __ffma2_rn(q.r, h, __ffma2_rn(q.c, h, q.h));
   return PACKED && is_cut(q.r) ? q.h : n;
 }
-// `q`, and `next` behind it in the direction of the walk: (c1 + r1) (c2 + r2).  (Where c stays 1
-// through a tile its kParts <= 16 parts have decays of exp(-1/8) at least: of 1 + r >= exp(-2)
-// the rounding of r costs three bits at most.)
+// `q`, and `next` behind it in the direction of the walk: (c1 + r1) (c2 + r2).  (Where c stays 1 through a tile its
+// 16 parts or less have decays of exp(-1/8) at least: of 1 + r >= exp(-2) the rounding of r
+// costs three bits at most.)
 template <bool PACKED>
 __device__ __forceinline__ void append(Piece& q, const Piece& next) {
   q.h = pass_on<PACKED>(next, q.h);

@@ -18,6 +18,11 @@ constexpr int kWarps = 4;
 constexpr int kXSlots = 4, kGSlots = 2;
 using Bwd = Shape<kWarps>;
 
+// A thread's decays of a turn, and 1 - a for the complement.
+template <bool COMPLEMENT>
+struct Run {
+  float2 a[kRun][kPairs], w[COMPLEMENT ? kRun : 1][kPairs];
+};
 struct Shared {
   Parts<Bwd::kParts> parts[2];
   float back[2][Bwd::kParts][kChannels];   // the parts' gradients from zero, then what enters them
@@ -126,7 +131,17 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     const TX* dh = p.dh ? static_cast<const TX*>(p.dh) + w.b * p.dh_s[0] + w.c : nullptr;
     TX* const dx = p.dx ? static_cast<TX*>(p.dx) + w.b * p.dx_s[0] + w.c : nullptr;
     TG* const dg = p.dg ? static_cast<TG*>(p.dg) + w.b * p.dg_s[0] + w.c : nullptr;
-    const auto pieces = [&](int k, int buf, Decays<COMPLEMENT>& a) {
+    // d_t = dh_t + u_t in the place of d_{t+1} (for the last token of the run: of u_t)
+    const auto add_later = [&](int k, int t, int t0, const RowMask& m, const Run<COMPLEMENT>& run, float2 (&u)[kPairs]) {
+      float2 d[kPairs] = {both(0.f), both(0.f)};
+      if (p.dh) ds.read(k, row0 + t, d);
+      const bool last = PACKED && (m.last >> t & 1);
+      if (last) load_state<WIDE>(state_of(p, p.dstate_out, p.dso_s, t0 + t, w.c), w.on, u);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j)
+        u[j] = t == kRun - 1 || last ? __fadd2_rn(d[j], u[j]) : __ffma2_rn(run.a[t + 1 < kRun ? t + 1 : t][j], u[j], d[j]);
+    };
+    const auto pieces = [&](int k, int buf, Run<COMPLEMENT>& run) {
       const int t0 = tile_of(k) * Bwd::kTile + row0;
       Parts<Bwd::kParts>& parts = sh.parts[buf];
       if (WIDE) patience.wait(sh.full + k % kXSlots, k / kXSlots & 1);
@@ -152,38 +167,39 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
         xs.clear(k, row0, m.there);
         ds.clear(k, row0, m.there);
       }
-      float2 gt[kRun][kPairs], all_c[kPairs], all_r[kPairs], h[kPairs], u[kPairs];
-#pragma unroll
-      for (int t = 0; t < kRun; ++t) gs.read(k, row0 + t, gt[t]);
-      set_decays(a, gt, all_c, all_r);
-      h[0] = h[1] = u[0] = u[1] = both(0.f);
+      float2 sum[kPairs], c[kPairs], r[kPairs], h[kPairs], u[kPairs];
+      sum[0] = sum[1] = h[0] = h[1] = u[0] = u[1] = both(0.f);
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
-        float2 v[kPairs];
+        float2 gt[kPairs], v[kPairs];
+        gs.read(k, row0 + t, gt);
         xs.read(k, row0 + t, v);
         if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          if (COMPLEMENT) v[j] = __fmul2_rn(v[j], rest(a.c(t, j), a.r[t][j]));
-          h[j] = apply(a.c(t, j), a.r[t][j], h[j], v[j]);
+          run.a[t][j] = decay(gt[j]);
+          sum[j] = __fadd2_rn(sum[j], gt[j]);
+          if (COMPLEMENT) {
+            run.w[t][j] = rest(gt[j], run.a[t][j]);
+            v[j] = __fmul2_rn(v[j], run.w[t][j]);
+          }
+          h[j] = __ffma2_rn(run.a[t][j], h[j], v[j]);
         }
       }
 #pragma unroll
-      for (int t = kRun - 1; t >= 0; --t) {
-        float2 d[kPairs] = {both(0.f), both(0.f)};
-        if (p.dh) ds.read(k, row0 + t, d);
-        if (PACKED && (m.last >> t & 1)) load_state<WIDE>(state_of(p, p.dstate_out, p.dso_s, t0 + t, w.c), w.on, u);
+      for (int t = kRun - 1; t >= 0; --t) add_later(k, t, t0, m, run, u);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) u[j] = times(a.c(t, j), a.r[t][j], __fadd2_rn(d[j], u[j]));
-      }
-      put(parts.c[part], all_c);
-      put(parts.r[part], all_r);
+      for (int j = 0; j < kPairs; ++j) u[j] = __fmul2_rn(run.a[0][j], u[j]);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) split_decay(sum[j], c[j], r[j]);
+      put(parts.c[part], c);
+      put(parts.r[part], r);
       put(parts.h[part], h);
       put(sh.back[buf][part], u);
       if (PACKED && threadIdx.x % kLanes == 0) sh.ends[buf][part] = (m.first != 0) | (m.last != 0) << 1;
       pieces_done(buf, Bwd::kThreads);
     };
-    const auto grads = [&](int k, int buf, const Decays<COMPLEMENT>& a) {
+    const auto grads = [&](int k, int buf, const Run<COMPLEMENT>& run) {
       const int t0 = tile_of(k) * Bwd::kTile + row0;
       states_wait(buf, Bwd::kThreads);
       if (t0 >= p.T || (WIDE && !w.on)) return;
@@ -198,13 +214,12 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
         if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          const float2 c = a.c(t, j), r = a.r[t][j];
           if (COMPLEMENT) {
-            v[t][j] = times(c, r, __ffma2_rn(xt[j], both(-1.f), h[j]));
-            h[j] = apply(c, r, h[j], __fmul2_rn(rest(c, r), xt[j]));
+            v[t][j] = __fmul2_rn(run.a[t][j], __ffma2_rn(xt[j], both(-1.f), h[j]));
+            h[j] = __ffma2_rn(run.a[t][j], h[j], __fmul2_rn(run.w[t][j], xt[j]));
           } else {
-            v[t][j] = times(c, r, h[j]);
-            h[j] = __fadd2_rn(v[t][j], xt[j]);
+            v[t][j] = __fmul2_rn(run.a[t][j], h[j]);
+            h[j] = __ffma2_rn(run.a[t][j], h[j], xt[j]);
           }
         }
       }
@@ -213,16 +228,12 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       TG* dg_row = dg ? dg + (int64_t)(t0 + kRun - 1) * p.dg_s[1] : nullptr;
 #pragma unroll
       for (int t = kRun - 1; t >= 0; --t) {
-        float2 d[kPairs] = {both(0.f), both(0.f)}, ox[kPairs], og[kPairs];
-        if (p.dh) ds.read(k, row0 + t, d);
-        if (PACKED && (m.last >> t & 1)) load_state<WIDE>(state_of(p, p.dstate_out, p.dso_s, t0 + t, w.c), w.on, u);
+        float2 ox[kPairs], og[kPairs];
+        add_later(k, t, t0, m, run, u);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          const float2 c = a.c(t, j), r = a.r[t][j];
-          d[j] = __fadd2_rn(d[j], u[j]);
-          ox[j] = COMPLEMENT ? __fmul2_rn(rest(c, r), d[j]) : d[j];
-          og[j] = __fmul2_rn(v[t][j], d[j]);
-          u[j] = times(c, r, d[j]);
+          ox[j] = COMPLEMENT ? __fmul2_rn(run.w[t][j], u[j]) : u[j];
+          og[j] = __fmul2_rn(v[t][j], u[j]);
         }
         const bool there = m.there >> t & 1;
         if (PACKED && !there) ox[0] = ox[1] = og[0] = og[1] = both(0.f);
@@ -232,11 +243,13 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
         }
         if (dx) dx_row -= p.dx_s[1];
         if (dg) dg_row -= p.dg_s[1];
-        if (PACKED && p.dstate_in && (m.first >> t & 1))
-          store_state<WIDE>(state_of(p, p.dstate_in, p.dsi_s, t0 + t, w.c), w.on, u);
+        if (PACKED && p.dstate_in && (m.first >> t & 1)) {
+          const float2 out[kPairs] = {__fmul2_rn(run.a[t][0], u[0]), __fmul2_rn(run.a[t][1], u[1])};
+          store_state<WIDE>(state_of(p, p.dstate_in, p.dsi_s, t0 + t, w.c), w.on, out);
+        }
       }
     };
-    Decays<COMPLEMENT> a, b;
+    Run<COMPLEMENT> a, b;
     for (int k = 0; k <= turns; k += 2) {
       if (k < turns) pieces(k, 0, a);
       if (k > 0) grads(k - 1, 1, b);
