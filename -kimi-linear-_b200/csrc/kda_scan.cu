@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(kMarked) mark_kernel(const ScanParams p, int m
     const uint32_t first = __ballot_sync(0xffffffffu, owned && p.q_start[max(b, 0)] == t);
     const uint32_t last = __ballot_sync(0xffffffffu, owned && end == t + 1);
     const uint32_t own = __ballot_sync(0xffffffffu, owned);
+    marks[blockIdx.x].sequence[threadIdx.x] = max(b, 0);
     if (threadIdx.x % 32 == 0) {
       uint32_t* m = reinterpret_cast<uint32_t*>(marks + blockIdx.x) + threadIdx.x / 32;
       m[0] = first;
@@ -53,29 +54,36 @@ __global__ void __launch_bounds__(kMarked) mark_kernel(const ScanParams p, int m
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-constexpr int kWarps = 8;
-constexpr int kSlots = 3;
-using Fwd = Shape<kWarps>;
+// Long sequences, one block an SM: fewer and larger exchanges.  Short ones, two blocks: one
+// starts or ends while the other works.
+using Long = Shape<16, 4, 1>;
+using Short = Shape<8, 1, 2>;
+// tiles in flight or in use: as many as fit
+constexpr int kMaxSlots = 3;
+template <typename TX, typename TG, typename SHAPE>
+constexpr int kSlotsOf = sizeof(TX) + sizeof(TG) > 6 && SHAPE::kTile == 128 ? 2 : 3;
 
 // A thread's decays and (weighed) inputs of a turn.
 struct Run {
   float2 a[kRun][kPairs], v[kRun][kPairs];
 };
+template <typename SHAPE>
 struct Shared {
-  Parts<Fwd::kParts> parts[2];       // of two turns
-  uint64_t full[kSlots], exchange[2];
-  uint8_t starts[2][Fwd::kParts];    // packed: a sequence starts in the part
+  Parts<SHAPE> parts[2];             // of two turns
+  uint64_t full[kMaxSlots], exchange[2];
+  TileRows<SHAPE> rows;              // packed
 };
 
-template <typename TX, typename TG, bool WIDE, bool PACKED, bool COMPLEMENT>
-__global__ void __launch_bounds__(Fwd::kThreads, 2)
+template <typename TX, typename TG, typename Fwd, bool WIDE, bool PACKED, bool COMPLEMENT>
+__global__ void __launch_bounds__(Fwd::kThreads, Fwd::kBlocks)
 scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap g_map) {
   extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int kSlots = kSlotsOf<TX, TG, Fwd>;
   using XRing = Ring<TX, Fwd::kTile, kSlots>;
   using GRing = Ring<TG, Fwd::kTile, kSlots>;
   const XRing xs{smem};
   const GRing gs{smem + XRing::kBytes};
-  Shared& sh = *reinterpret_cast<Shared*>(smem + XRing::kBytes + GRing::kBytes);
+  Shared<Fwd>& sh = *reinterpret_cast<Shared<Fwd>*>(smem + XRing::kBytes + GRing::kBytes);
   const Place w = my_place<WIDE>(p);
   const Exchange exchange(sh.exchange, reinterpret_cast<float*>(&sh + 1), p, w.rank);
   Patience patience(&g_scan_device_error);
@@ -85,13 +93,21 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     exchange.init();
     ptx::fence_mbar_init();
   }
+  const auto first_row = [&](int k, int part) { return (k * p.cluster + w.rank) * Fwd::kTile + part * kRun; };
+  if constexpr (PACKED) {
+    ptx::grid_dep_wait();
+    if (threadIdx.x < 2 * Fwd::kParts) {
+      const int k = threadIdx.x / Fwd::kParts, part = threadIdx.x % Fwd::kParts;
+      sh.rows.bits[k][part] = packed_rows(p, first_row(k, part));
+    }
+  }
   __syncthreads();
   exchange.barrier();
   if (threadIdx.x >= Fwd::kWork) {
     // two channels' states from turn to turn, and the copies
-    const int at = threadIdx.x - Fwd::kWork;
+    const int at = threadIdx.x % 32, warp = (threadIdx.x - Fwd::kWork) / 32;
     const int ch0 = w.block_c + shared_channel<WIDE>(2 * at), ch1 = w.block_c + shared_channel<WIDE>(2 * at + 1);
-    const bool copies = WIDE && at == 0;
+    const bool copies = WIDE && warp == 0 && at == 0;
     const auto copy = [&](int k) {
       const int tile = k * p.cluster + w.rank;
       if (tile >= p.tiles) return;
@@ -102,7 +118,6 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     };
     if (copies)
       for (int k = 0; k < kSlots; ++k) copy(k);
-    if constexpr (PACKED) ptx::grid_dep_wait();
     float2 carry = both(0.f);
     if (!PACKED && p.state_in) {
       if (ch0 < p.D) carry.x = p.state_in[w.b * p.si_s + ch0];
@@ -114,26 +129,30 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       pieces_wait(buf, Fwd::kThreads);
       // the workers have read the rows of turn k
       if (copies && patience.limit) copy(k + kSlots);
-      uint32_t cuts = 0;
+      uint32_t cuts = 0, ahead = 0;
       if constexpr (PACKED) {
-#pragma unroll
-        for (int i = 0; i < Fwd::kParts; ++i) cuts |= (uint32_t)sh.starts[buf][i] << i;
+        cuts = sh.rows.starts(k);
+        if (warp == Fwd::kCarryWarps - 1 && at < Fwd::kParts) ahead = packed_rows(p, first_row(k + 2, at));
       }
-      Parts<Fwd::kParts>& parts = sh.parts[buf];
-      enter_parts<PACKED, false>(exchange, patience, k, parts, parts.h, cuts, carry, at);
+      Parts<Fwd>& parts = sh.parts[buf];
+      enter_parts<PACKED, false>(exchange, patience, k, parts, parts.h, cuts, carry, warp, at, [] {});
       if (ckpt) {
+        // the checkpoints that are in this warp's share of the parts
+        constexpr int N = Fwd::kParts / Fwd::kCarryWarps;
 #pragma unroll
-        for (int i = 0; i < Fwd::kTile / kStep; ++i) {
-          const int step = (k * p.cluster + w.rank) * (Fwd::kTile / kStep) + i, j = i * (kStep / kRun);
-          float2 s = pair(parts.h[j], at);
-          if (p.cluster > 1) s = pass_on<PACKED>({pair(parts.c[j], at), pair(parts.r[j], at), s}, pair(parts.entry, at));
+        for (int i = 0; i < N; ++i) {
+          const int j = warp * N + i;
+          if (j % (kStep / kRun)) continue;
+          const int step = (k * p.cluster + w.rank) * (Fwd::kTile / kStep) + j / (kStep / kRun);
+          const float2 s = pair(parts.h[j], at);
           if (step < p.steps && ch0 < p.D) ckpt[(int64_t)step * p.D + ch0] = s.x;
           if (step < p.steps && ch1 < p.D) ckpt[(int64_t)step * p.D + ch1] = s.y;
         }
       }
+      if (PACKED && warp == Fwd::kCarryWarps - 1 && at < Fwd::kParts) sh.rows.bits[(k + 2) & 3][at] = ahead;
       states_done(buf, Fwd::kThreads);
     }
-    if (!PACKED && w.rank == 0) {
+    if (!PACKED && w.rank == 0 && warp == 0) {
       if (ch0 < p.D) p.state_out[w.b * p.so_s + ch0] = carry.x;
       if (ch1 < p.D) p.state_out[w.b * p.so_s + ch1] = carry.y;
     }
@@ -143,26 +162,23 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
         if (k * p.cluster + w.rank < p.tiles) landed.wait(sh.full + k % kSlots, k / kSlots & 1);
     }
   } else {
-    if constexpr (PACKED) ptx::grid_dep_wait();
     const int part = threadIdx.x / kLanes, row0 = part * kRun;
     const TX* x = static_cast<const TX*>(p.x) + w.b * p.x_s[0] + w.c;
     const TG* g = static_cast<const TG*>(p.g) + w.b * p.g_s[0] + w.c;
     TX* const out = static_cast<TX*>(p.h) + w.b * p.h_s[0] + w.c;
-    const auto first_row = [&](int k) { return (k * p.cluster + w.rank) * Fwd::kTile + row0; };
     // turn k's pieces
     const auto pieces = [&](int k, int buf, Run& run) {
-      const int t0 = first_row(k);
-      Parts<Fwd::kParts>& parts = sh.parts[buf];
+      const int t0 = first_row(k, part);
+      Parts<Fwd>& parts = sh.parts[buf];
       if (t0 - row0 >= p.T) {        // no tile: nothing changes
         const float2 one[kPairs] = {both(1.f), both(1.f)}, zero[kPairs] = {};
         put(parts.c[part], one);
         put(parts.r[part], zero);
         put(parts.h[part], zero);
-        if (PACKED && threadIdx.x % kLanes == 0) sh.starts[buf][part] = 0;
         pieces_done(buf, Fwd::kThreads);
         return;
       }
-      const RowMask m = row_mask<PACKED>(p, t0);
+      const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
       if constexpr (WIDE) {
         patience.wait(sh.full + k % kSlots, k / kSlots & 1);
       } else {
@@ -195,17 +211,16 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       put(parts.c[part], c);
       put(parts.r[part], r);
       put(parts.h[part], h);
-      if (PACKED && threadIdx.x % kLanes == 0) sh.starts[buf][part] = m.first != 0;
       pieces_done(buf, Fwd::kThreads);
     };
     // turn k's tokens again, from the state that enters them
     const auto states = [&](int k, int buf, const Run& run) {
-      const int t0 = first_row(k);
+      const int t0 = first_row(k, part);
       states_wait(buf, Fwd::kThreads);
       if (t0 >= p.T || (WIDE && !w.on)) return;
-      const RowMask m = row_mask<PACKED>(p, t0);
+      const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
       float2 h[kPairs];
-      entered<PACKED>(sh.parts[buf], sh.parts[buf].h[part], p.cluster, part, h);
+      get(sh.parts[buf].h[part], h);
       TX* row = out + (int64_t)t0 * p.h_s[1];
 #pragma unroll
       for (int t = 0; t < kRun; ++t) {
@@ -234,20 +249,33 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
   exchange.barrier();                // no block leaves while another may still send to it
 }
 
-cudaError_t launch_forward(ScanParams p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
-  choose_cluster(p, Fwd::kTile, 2 * 148);
+template <typename Fwd>
+cudaError_t launch_shape(const ScanParams& p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
   return by_types(x_dtype, g_dtype, [&](auto x, auto g) {
     using TX = decltype(x);
     using TG = decltype(g);
+    constexpr int kSlots = kSlotsOf<TX, TG, Fwd>;
     CUtensorMap mx, mg;
     const bool tma = wide && encode<TX>(&mx, p.x, p.x_s, p, Fwd::kTile) && encode<TG>(&mg, p.g, p.g_s, p, Fwd::kTile);
     const size_t smem = Ring<TX, Fwd::kTile, kSlots>::kBytes + Ring<TG, Fwd::kTile, kSlots>::kBytes +
-                        sizeof(Shared) + cluster_bytes(p.cluster);
+                        sizeof(Shared<Fwd>) + cluster_bytes(p.cluster);
     return by_flags(tma, p.q_start != nullptr, p.complement, [&](auto wide_, auto packed, auto complement) {
-      return launch_tiles(scan_kernel<TX, TG, wide_.value, packed.value, complement.value>, p, Fwd::kThreads, smem, s,
-                          mx, mg);
+      return launch_tiles(scan_kernel<TX, TG, Fwd, wide_.value, packed.value, complement.value>, p, Fwd::kThreads, smem,
+                          s, mx, mg);
     });
   });
+}
+cudaError_t launch_forward(ScanParams p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
+  // (blocks: a sequence's channels, before clusters.  us, Long and Short: 4 x 8192 x 2048 f16, 128 blocks, 84
+  // and 127; 1 x 1024 x 2048, 32 blocks, 8.0 and 9.0; 8 x 4096 x 2048 bf16, 256 blocks, 74 and 69; 64 x 512 x
+  // 2048 f16, 2048 blocks, 100 and 87)
+  const bool is_long = (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels) <= kSms;
+  if (is_long) {
+    choose_cluster<Long>(p);
+    return launch_shape<Long>(p, x_dtype, g_dtype, wide, s);
+  }
+  choose_cluster<Short>(p);
+  return launch_shape<Short>(p, x_dtype, g_dtype, wide, s);
 }
 
 constexpr int kStepThreads = 128;
@@ -442,12 +470,6 @@ int run_step(const KdaScanArgs* a, void* stream) {
 }
 
 }  // namespace
-
-void choose_cluster(ScanParams& p, int tile, int slots) {
-  p.tiles = (p.T + tile - 1) / tile;
-  const int64_t blocks = (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels);
-  p.cluster = (int)max((int64_t)1, min((int64_t)min(kMaxCluster, p.tiles), slots / blocks));
-}
 
 int read_device_error(bool clear) {
   const int grad = read_grad_device_error(clear);

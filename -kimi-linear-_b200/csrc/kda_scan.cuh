@@ -20,9 +20,10 @@ constexpr int kErrWait = 9;       // device error word: a wait for a cluster's p
 constexpr int kStep = 32;         // tokens between two checkpoints of the state
 constexpr int kMarked = 64;       // rows of a packed batch that one Marks describes
 
-// What kMarked rows of a packed batch are, a bit a row.
+// What kMarked rows of a packed batch are, a bit a row; and each row's sequence.
 struct Marks {
   uint64_t first, last, owned;      // of a sequence; by any sequence
+  int sequence[kMarked];            // (that of the last row before it where it is not owned, or 0)
 };
 
 // Device-side view of KdaScanArgs (strides in elements).
@@ -102,17 +103,19 @@ constexpr int kVec = 4;                       // channels of a thread
 constexpr int kPairs = kVec / 2;
 constexpr int kChannels = kLanes * kVec;      // of a block
 constexpr int kRun = 4;                       // tokens of a thread in a tile
-constexpr int kCarry = kChannels / 2;         // threads that carry the states of a pair of channels each
 constexpr int kMaxCluster = 8;
+constexpr int kSms = 148;
 constexpr uint64_t kWaitNs = 2000000000;      // a wait that takes longer gives up (device error word 9)
 
-// A block's working warps and what follows from their number.
-template <int WARPS>
+// A block: WORK warps that do the tokens, and CARRY warps that carry states from tile to tile
+// (a lane has a pair of channels, a warp its share of the parts).
+template <int WORK, int CARRY, int BLOCKS>
 struct Shape {
-  static constexpr int kWork = WARPS * 32;
-  static constexpr int kThreads = kWork + kCarry;
+  static constexpr int kWork = WORK * 32, kCarryWarps = CARRY, kCarry = CARRY * 32, kThreads = kWork + kCarry;
+  static constexpr int kBlocks = BLOCKS;               // on an SM
   static constexpr int kParts = kWork / kLanes;        // half warps, each with kRun tokens of a tile
   static constexpr int kTile = kParts * kRun;
+  static_assert(kParts % CARRY == 0, "shares of the parts");
 };
 
 // ---------------------------------------------------------------------------
@@ -147,6 +150,11 @@ struct Patience {
     }
   }
 };
+// a barrier of the carrying threads alone
+template <int THREADS>
+__device__ __forceinline__ void carry_sync() {
+  asm volatile("barrier.cta.sync 5, %0;" ::"n"(THREADS) : "memory");
+}
 // The block's named barriers, two of each kind (buf 0 and 1): the workers' pieces are there (the
 // workers go on, the carrying threads wait); the states that enter the parts are there (the
 // other way round).
@@ -276,30 +284,47 @@ __device__ __forceinline__ void store_state(float* row, uint32_t on, const float
 // The state of the packed sequence at row t.
 __device__ __forceinline__ float* state_of(const ScanParams& p, const float* base, int64_t stride, int t, int c) {
   if (base == nullptr) return nullptr;
-  return const_cast<float*>(base) + (int64_t)max(sequence_at(p.q_start, p.B, t), 0) * stride + c;
+  return const_cast<float*>(base) + p.marks[t / kMarked].sequence[t % kMarked] * stride + c;
 }
 
 // Which of rows t .. t + kRun - 1 are there (bits), and for packed batches which start and end
-// a sequence.
+// a sequence; held as there | first << kRun | last << 2 kRun.
 constexpr uint32_t kAllRows = (1u << kRun) - 1;
-struct RowMask { uint32_t there, first, last; };
-template <bool PACKED>
-__device__ __forceinline__ RowMask row_mask(const ScanParams& p, int t) {
-  RowMask m{0, 0, 0};
-  if constexpr (PACKED) {
-    if (t < 0 || t >= p.T) return m;
-    static_assert(kMarked % kRun == 0, "a run is inside one Marks");
-    const Marks* k = p.marks + t / kMarked;
-    const int at = t % kMarked;
-    m.there = (uint32_t)(k->owned >> at) & kAllRows;
-    m.first = (uint32_t)(k->first >> at) & kAllRows;
-    m.last = (uint32_t)(k->last >> at) & kAllRows;
-  } else {
-    const int left = t < 0 ? 0 : p.T - t;
-    m.there = left >= kRun ? kAllRows : left > 0 ? (1u << left) - 1 : 0;
-  }
+struct RowMask {
+  uint32_t there, first, last;
+  __device__ RowMask() : there(0), first(0), last(0) {}
+  __device__ explicit RowMask(uint32_t bits)
+      : there(bits & kAllRows), first(bits >> kRun & kAllRows), last(bits >> 2 * kRun & kAllRows) {}
+};
+__device__ __forceinline__ uint32_t packed_rows(const ScanParams& p, int t) {
+  if (t < 0 || t >= p.T) return 0;
+  static_assert(kMarked % kRun == 0, "a run is inside one Marks");
+  const Marks& k = p.marks[t / kMarked];
+  const int at = t % kMarked;
+  return (uint32_t)(k.owned >> at) & kAllRows | ((uint32_t)(k.first >> at) & kAllRows) << kRun |
+         ((uint32_t)(k.last >> at) & kAllRows) << 2 * kRun;
+}
+__device__ __forceinline__ RowMask batch_rows(const ScanParams& p, int t) {
+  RowMask m;
+  const int left = t < 0 ? 0 : p.T - t;
+  m.there = left >= kRun ? kAllRows : left > 0 ? (1u << left) - 1 : 0;
   return m;
 }
+// A packed tile's rows, by part, fetched two turns ahead by the carrying threads: a worker that
+// fetched its own would wait for memory in every turn.
+template <typename SHAPE>
+struct TileRows {
+  uint16_t bits[4][SHAPE::kParts];   // of turn k at k & 3
+  __device__ RowMask of(int k, int part) const { return RowMask(bits[k & 3][part]); }
+  // (warp-wide) which parts have a row in which a sequence starts (ends)
+  __device__ uint32_t starts(int k) const { return parts_with(k, kRun); }
+  __device__ uint32_t ends(int k) const { return parts_with(k, 2 * kRun); }
+  __device__ uint32_t parts_with(int k, int shift) const {
+    const int lane = threadIdx.x % 32;
+    const uint32_t b = lane < SHAPE::kParts ? bits[k & 3][lane] : 0;
+    return __ballot_sync(0xffffffffu, (b >> shift & kAllRows) != 0);
+  }
+};
 
 // ---------------------------------------------------------------------------
 // pieces: the decay over some tokens, and the state they give from a state of zero
@@ -328,10 +353,11 @@ __device__ __forceinline__ void append(Piece& q, const Piece& next) {
   q.r = none ? cut() : r;
 }
 
-// The parts' pieces of a tile, and (`entry`) what enters the tile.
-template <int PARTS>
+// The parts' pieces of a tile, and those of the carrying warps' shares of them.
+template <typename SHAPE>
 struct Parts {
-  float c[PARTS][kChannels], r[PARTS][kChannels], h[PARTS][kChannels], entry[kChannels];
+  float c[SHAPE::kParts][kChannels], r[SHAPE::kParts][kChannels], h[SHAPE::kParts][kChannels];
+  float share[SHAPE::kCarryWarps][3][kChannels];
 };
 __device__ __forceinline__ void put(float* row, const float2 (&v)[kPairs]) {
   static_assert(kVec == 4, "a thread's channels are one float4");
@@ -375,11 +401,12 @@ struct Exchange {
     float* s = row(turn, i);
     return {pair(s, at), pair(s + kChannels, at), pair(s + 2 * kChannels, at)};
   }
-  __device__ void send(int turn, int at, const Piece& q, bool arm) const {
+  // carrying warp `warp` of `warps` sends to blocks warp, warp + warps, ...
+  __device__ void send(int turn, int warp, int warps, int at, const Piece& q, bool arm) const {
     uint64_t* bar = full + (turn & 1);
-    if (at == 0 && arm) ptx::mbar_arrive_expect_tx(bar, cluster * kRowFloats * sizeof(float));
+    if (warp == 0 && at == 0 && arm) ptx::mbar_arrive_expect_tx(bar, cluster * kRowFloats * sizeof(float));
     const uint32_t dst = ptx::smem_u32(&pair(row(turn, rank), at)), mine = ptx::smem_u32(bar);
-    for (int i = 0; i < cluster; ++i) {
+    for (int i = warp; i < cluster; i += warps) {
       uint32_t d, m;
       asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(dst), "r"(i));
       asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(mine), "r"(i));
@@ -394,59 +421,69 @@ struct Exchange {
   }
 };
 
-// What enters a tile's parts, by the thread that carries a pair of channels; BACK: from the last
-// part to the first.  `carry` enters the cluster's first tile of the turn and becomes what leaves its
-// last one.  Alone, a block leaves what enters part i in the place of h[i].  In a cluster it
-// leaves the piece of all parts before i in the place of part i's, since that can be done
-// before the other blocks' pieces are here, and what enters the tile in `entry`; a worker
-// puts the two together (entered()).
-template <bool PACKED, bool BACK, int PARTS>
+// Puts what enters part i of a tile in the place of h[i]: lane `at` of carrying warp `warp` has a pair
+// of channels in its share of the parts; BACK: from the last part to the first.  `carry` (the
+// same in all warps) enters the cluster's first tile of the turn and becomes what leaves its
+// last one.  `meanwhile` is done while the other blocks' pieces are on their way.
+template <bool PACKED, bool BACK, typename SHAPE, typename F>
 __device__ __forceinline__ void enter_parts(const Exchange& exchange, Patience& patience, int turn,
-                                            Parts<PARTS>& parts, float (*h)[kChannels], uint32_t cuts, float2& carry,
-                                            int at) {
+                                            Parts<SHAPE>& parts, float (*h)[kChannels], uint32_t cuts, float2& carry,
+                                            int warp, int at, F meanwhile) {
+  constexpr int W = SHAPE::kCarryWarps, N = SHAPE::kParts / W;
+  const int share = BACK ? W - 1 - warp : warp;        // the warp-th in the direction of the walk
+  const auto place = [&](int i) { return share * N + (BACK ? N - 1 - i : i); };
   const auto part = [&](int j) {
     return Piece{pair(parts.c[j], at), PACKED && (cuts >> j & 1) ? cut() : pair(parts.r[j], at), pair(h[j], at)};
   };
-  if (exchange.cluster == 1) {
+  float2 s = carry;
+  const bool alone = exchange.cluster == 1;
+  if (W > 1 || !alone) {
+    const Piece none{both(1.f), both(0.f), both(0.f)};
+    Piece all = none, before = none;                   // of the tile; of the shares before this warp's
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
-      const int j = BACK ? PARTS - 1 - i : i;
-      const Piece q = part(j);
-      pair(h[j], at) = carry;
-      carry = pass_on<PACKED>(q, carry);
+    for (int i = 0; i < N; ++i) append<PACKED>(all, part(place(i)));
+    if constexpr (W > 1) {
+      pair(parts.share[warp][0], at) = all.c;
+      pair(parts.share[warp][1], at) = all.r;
+      pair(parts.share[warp][2], at) = all.h;
+      carry_sync<SHAPE::kCarry>();
+      all = none;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if (i == warp) before = all;
+        append<PACKED>(all, {pair(parts.share[i][0], at), pair(parts.share[i][1], at), pair(parts.share[i][2], at)});
+      }
     }
-    return;
-  }
-  Piece all{both(1.f), both(0.f), both(0.f)};
+    if (alone) {
+      carry = pass_on<PACKED>(all, carry);
+      meanwhile();
+    } else {
+      exchange.send(turn, warp, W, at, all, patience.limit != 0);
+      meanwhile();
+      patience.wait(exchange.full + (turn & 1), (turn >> 1) & 1);
+      Piece others[kMaxCluster];
 #pragma unroll
-  for (int i = 0; i < PARTS; ++i) {
-    const int j = BACK ? PARTS - 1 - i : i;
+      for (int i = 0; i < kMaxCluster; ++i)
+        if (i < exchange.cluster) others[i] = exchange.get(turn, BACK ? exchange.cluster - 1 - i : i, at);
+      const int me = BACK ? exchange.cluster - 1 - exchange.rank : exchange.rank;
+#pragma unroll
+      for (int i = 0; i < kMaxCluster; ++i) {
+        if (i == me) s = carry;
+        if (i < exchange.cluster) carry = pass_on<PACKED>(others[i], carry);
+      }
+    }
+    s = pass_on<PACKED>(before, s);
+  } else {
+    meanwhile();
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = place(i);
     const Piece q = part(j);
-    pair(parts.c[j], at) = all.c;
-    pair(parts.r[j], at) = all.r;
-    pair(h[j], at) = all.h;
-    append<PACKED>(all, q);
+    pair(h[j], at) = s;
+    s = pass_on<PACKED>(q, s);
   }
-  exchange.send(turn, at, all, patience.limit != 0);
-  patience.wait(exchange.full + (turn & 1), (turn >> 1) & 1);
-  for (int i = 0; i < exchange.cluster; ++i) {
-    const int j = BACK ? exchange.cluster - 1 - i : i;
-    if (j == exchange.rank) pair(parts.entry, at) = carry;
-    carry = pass_on<PACKED>(exchange.get(turn, j, at), carry);
-  }
-}
-// What enters a worker's part.
-template <bool PACKED, int PARTS>
-__device__ __forceinline__ void entered(const Parts<PARTS>& parts, const float* h, int cluster, int part,
-                                        float2 (&s)[kPairs]) {
-  get(h, s);
-  if (cluster == 1) return;
-  float2 c[kPairs], r[kPairs], e[kPairs];
-  get(parts.c[part], c);
-  get(parts.r[part], r);
-  get(parts.entry, e);
-#pragma unroll
-  for (int j = 0; j < kPairs; ++j) s[j] = pass_on<PACKED>({c[j], r[j], s[j]}, e[j]);
+  if (W == 1 && alone) carry = s;
 }
 
 // ---------------------------------------------------------------------------
@@ -468,6 +505,15 @@ cudaError_t by_flags(bool a, bool b, bool c, F f) {
   using No = std::false_type;
   if (a) return b ? (c ? f(Yes{}, Yes{}, Yes{}) : f(Yes{}, Yes{}, No{})) : (c ? f(Yes{}, No{}, Yes{}) : f(Yes{}, No{}, No{}));
   return b ? (c ? f(No{}, Yes{}, Yes{}) : f(No{}, Yes{}, No{})) : (c ? f(No{}, No{}, Yes{}) : f(No{}, No{}, No{}));
+}
+
+// Sets tiles and cluster: as many blocks to a sequence as the device holds at once, and has
+// tiles for.
+template <typename SHAPE>
+void choose_cluster(ScanParams& p) {
+  p.tiles = (p.T + SHAPE::kTile - 1) / SHAPE::kTile;
+  const int64_t blocks = (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels);
+  p.cluster = (int)max((int64_t)1, min((int64_t)min(kMaxCluster, p.tiles), kSms * SHAPE::kBlocks / blocks));
 }
 
 // The map of x, g or dh for tiles of `tile` rows; false where TMA cannot address its rows.
@@ -520,8 +566,7 @@ cudaError_t launch_tiles(void (*kernel)(ScanParams, Maps...), const ScanParams& 
 }
 
 int read_grad_device_error(bool clear);   // kda_scan_grad.cu's error word
-cudaError_t launch_grad(ScanParams p, int x_dtype, int g_dtype, bool wide, cudaStream_t s);
-void choose_cluster(ScanParams& p, int tile, int slots);   // sets tiles and cluster
+cudaError_t launch_grad(const ScanParams& p, int x_dtype, int g_dtype, bool wide, cudaStream_t s);
 
 }  // namespace scan
 }  // namespace kda

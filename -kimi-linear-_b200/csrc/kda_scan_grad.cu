@@ -5,6 +5,8 @@
 // It needs h_{t-1} in 32 bits: h is in x's type, so a tile's states are computed again from
 // the checkpoint that the forward pass left at its start.  The blocks, threads and pieces are
 // those of scan_kernel (kda_scan.cu), the tiles taken from the last to the first.
+#include <type_traits>
+
 #include "kda_scan.cuh"
 
 namespace kda {
@@ -14,24 +16,26 @@ __device__ int g_grad_device_error = 0;
 
 namespace {
 
-constexpr int kWarps = 4;
+// As in the scan; the long shape's tiles are shorter where values have 32 bits, so that they fit.
+template <typename TX>
+using Long = std::conditional_t<sizeof(TX) == 4, Shape<8, 4, 1>, Shape<12, 4, 1>>;
+using Short = Shape<4, 1, 3>;
 constexpr int kXSlots = 4, kGSlots = 2;
-using Bwd = Shape<kWarps>;
-
 // A thread's decays of a turn, and 1 - a for the complement.
 template <bool COMPLEMENT>
 struct Run {
   float2 a[kRun][kPairs], w[COMPLEMENT ? kRun : 1][kPairs];
 };
+template <typename SHAPE>
 struct Shared {
-  Parts<Bwd::kParts> parts[2];
-  float back[2][Bwd::kParts][kChannels];   // the parts' gradients from zero, then what enters them
+  Parts<SHAPE> parts[2];
+  float back[2][SHAPE::kParts][kChannels];   // the parts' gradients from zero, then what enters them
   uint64_t full[kXSlots], exchange[2];
-  uint8_t ends[2][Bwd::kParts];      // packed: a sequence starts (1), ends (2) in the part
+  TileRows<SHAPE> rows;                      // packed
 };
 
-template <typename TX, typename TG, bool WIDE, bool PACKED, bool COMPLEMENT>
-__global__ void __launch_bounds__(Bwd::kThreads, 3)
+template <typename TX, typename TG, typename Bwd, bool WIDE, bool PACKED, bool COMPLEMENT>
+__global__ void __launch_bounds__(Bwd::kThreads, Bwd::kBlocks)
 scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
                  const __grid_constant__ CUtensorMap g_map, const __grid_constant__ CUtensorMap d_map) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -39,7 +43,7 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
   using GRing = Ring<TG, Bwd::kTile, kGSlots>;
   const XRing xs{smem}, ds{smem + XRing::kBytes};
   const GRing gs{smem + 2 * XRing::kBytes};
-  Shared& sh = *reinterpret_cast<Shared*>(smem + 2 * XRing::kBytes + GRing::kBytes);
+  Shared<Bwd>& sh = *reinterpret_cast<Shared<Bwd>*>(smem + 2 * XRing::kBytes + GRing::kBytes);
   const Place w = my_place<WIDE>(p);
   const Exchange exchange(sh.exchange, reinterpret_cast<float*>(&sh + 1), p, w.rank);
   Patience patience(&g_grad_device_error);
@@ -49,14 +53,22 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     exchange.init();
     ptx::fence_mbar_init();
   }
+  const auto tile_of = [&](int k) { return (turns - 1 - k) * p.cluster + w.rank; };
+  const auto first_row = [&](int k, int part) { return tile_of(k) * Bwd::kTile + part * kRun; };
+  if constexpr (PACKED) {
+    ptx::grid_dep_wait();
+    if (threadIdx.x < 2 * Bwd::kParts) {
+      const int k = threadIdx.x / Bwd::kParts, part = threadIdx.x % Bwd::kParts;
+      sh.rows.bits[k][part] = packed_rows(p, first_row(k, part));
+    }
+  }
   __syncthreads();
   exchange.barrier();
-  const auto tile_of = [&](int k) { return (turns - 1 - k) * p.cluster + w.rank; };
   if (threadIdx.x >= Bwd::kWork) {
     // two channels' gradients from turn to turn, their states in a tile, and the copies
-    const int at = threadIdx.x - Bwd::kWork;
+    const int at = threadIdx.x % 32, warp = (threadIdx.x - Bwd::kWork) / 32;
     const int ch0 = w.block_c + shared_channel<WIDE>(2 * at), ch1 = w.block_c + shared_channel<WIDE>(2 * at + 1);
-    const bool copies = WIDE && at == 0;
+    const bool copies = WIDE && warp == 0 && at == 0;
     const auto copy = [&](int k) {
       if (k >= turns) return;
       const int tile = tile_of(k);
@@ -72,18 +84,17 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     };
     if (copies)
       for (int k = 0; k < 2; ++k) copy(k);
-    if constexpr (PACKED) ptx::grid_dep_wait();
     float2 carry = both(0.f);
     if (!PACKED && p.dstate_out) {
       if (ch0 < p.D) carry.x = p.dstate_out[w.b * p.dso_s + ch0];
       if (ch1 < p.D) carry.y = p.dstate_out[w.b * p.dso_s + ch1];
     }
-    static_assert(Bwd::kTile == kStep, "a tile starts at a checkpoint");
+    static_assert(Bwd::kTile % kStep == 0, "a tile starts at a checkpoint");
     // (the first turn's tile may be missing)
     const auto checkpoint = [&](int k) {
       float2 s = both(0.f);
       if (k >= turns || tile_of(k) >= p.tiles) return s;
-      const float* row = p.ckpt + ((int64_t)w.b * p.steps + tile_of(k)) * p.D;
+      const float* row = p.ckpt + ((int64_t)w.b * p.steps + tile_of(k) * (Bwd::kTile / kStep)) * p.D;
       if (ch0 < p.D) s.x = row[ch0];
       if (ch1 < p.D) s.y = row[ch1];
       return s;
@@ -96,26 +107,28 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       // the workers are done with the gates of turn k and with the other rows of turn k - 2
       if (copies && patience.limit) copy(k + 2);
       next = checkpoint(k + 1);
-      uint32_t cuts = 0, starts = 0;
+      uint32_t cuts = 0, starts = 0, ahead = 0;
       if constexpr (PACKED) {
+        starts = sh.rows.starts(k);
+        cuts = sh.rows.ends(k);
+        if (warp == Bwd::kCarryWarps - 1 && at < Bwd::kParts) ahead = packed_rows(p, first_row(k + 2, at));
+      }
+      Parts<Bwd>& parts = sh.parts[buf];
+      enter_parts<PACKED, true>(exchange, patience, k, parts, sh.back[buf], cuts, carry, warp, at, [&] {
+        // the states that enter the parts, by the last warp
+        if (warp != Bwd::kCarryWarps - 1) return;
 #pragma unroll
         for (int i = 0; i < Bwd::kParts; ++i) {
-          starts |= (uint32_t)(sh.ends[buf][i] & 1) << i;
-          cuts |= (uint32_t)(sh.ends[buf][i] >> 1) << i;
+          const Piece q{pair(parts.c[i], at), PACKED && (starts >> i & 1) ? cut() : pair(parts.r[i], at),
+                        pair(parts.h[i], at)};
+          pair(parts.h[i], at) = state;
+          state = pass_on<PACKED>(q, state);
         }
-      }
-      Parts<Bwd::kParts>& parts = sh.parts[buf];
-#pragma unroll
-      for (int i = 0; i < Bwd::kParts; ++i) {
-        const Piece q{pair(parts.c[i], at), PACKED && (starts >> i & 1) ? cut() : pair(parts.r[i], at),
-                      pair(parts.h[i], at)};
-        pair(parts.h[i], at) = state;
-        state = pass_on<PACKED>(q, state);
-      }
-      enter_parts<PACKED, true>(exchange, patience, k, parts, sh.back[buf], cuts, carry, at);
+      });
+      if (PACKED && warp == Bwd::kCarryWarps - 1 && at < Bwd::kParts) sh.rows.bits[(k + 2) & 3][at] = ahead;
       states_done(buf, Bwd::kThreads);
     }
-    if (!PACKED && p.dstate_in && w.rank == 0) {
+    if (!PACKED && p.dstate_in && w.rank == 0 && warp == 0) {
       if (ch0 < p.D) p.dstate_in[w.b * p.dsi_s + ch0] = carry.x;
       if (ch1 < p.D) p.dstate_in[w.b * p.dsi_s + ch1] = carry.y;
     }
@@ -124,7 +137,6 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       for (int k = max(turns - 2, 0); k < turns; ++k) landed.wait(sh.full + k % kXSlots, k / kXSlots & 1);
     }
   } else {
-    if constexpr (PACKED) ptx::grid_dep_wait();
     const int part = threadIdx.x / kLanes, row0 = part * kRun;
     const TX* x = static_cast<const TX*>(p.x) + w.b * p.x_s[0] + w.c;
     const TG* g = static_cast<const TG*>(p.g) + w.b * p.g_s[0] + w.c;
@@ -142,8 +154,8 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
         u[j] = t == kRun - 1 || last ? __fadd2_rn(d[j], u[j]) : __ffma2_rn(run.a[t + 1 < kRun ? t + 1 : t][j], u[j], d[j]);
     };
     const auto pieces = [&](int k, int buf, Run<COMPLEMENT>& run) {
-      const int t0 = tile_of(k) * Bwd::kTile + row0;
-      Parts<Bwd::kParts>& parts = sh.parts[buf];
+      const int t0 = first_row(k, part);
+      Parts<Bwd>& parts = sh.parts[buf];
       if (WIDE) patience.wait(sh.full + k % kXSlots, k / kXSlots & 1);
       if (t0 - row0 >= p.T) {        // no tile: nothing changes
         const float2 one[kPairs] = {both(1.f), both(1.f)}, zero[kPairs] = {};
@@ -151,11 +163,10 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
         put(parts.r[part], zero);
         put(parts.h[part], zero);
         put(sh.back[buf][part], zero);
-        if (PACKED && threadIdx.x % kLanes == 0) sh.ends[buf][part] = 0;
         pieces_done(buf, Bwd::kThreads);
         return;
       }
-      const RowMask m = row_mask<PACKED>(p, t0);
+      const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
       if constexpr (!WIDE) {
         xs.copy_own(x + (int64_t)t0 * p.x_s[1], p.x_s[1], k, row0, m.there, w.on);
         gs.copy_own(g + (int64_t)t0 * p.g_s[1], p.g_s[1], k, row0, m.there, w.on);
@@ -196,14 +207,13 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       put(parts.r[part], r);
       put(parts.h[part], h);
       put(sh.back[buf][part], u);
-      if (PACKED && threadIdx.x % kLanes == 0) sh.ends[buf][part] = (m.first != 0) | (m.last != 0) << 1;
       pieces_done(buf, Bwd::kThreads);
     };
     const auto grads = [&](int k, int buf, const Run<COMPLEMENT>& run) {
-      const int t0 = tile_of(k) * Bwd::kTile + row0;
+      const int t0 = first_row(k, part);
       states_wait(buf, Bwd::kThreads);
       if (t0 >= p.T || (WIDE && !w.on)) return;
-      const RowMask m = row_mask<PACKED>(p, t0);
+      const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
       float2 h[kPairs], u[kPairs], v[kRun][kPairs];
       // a_t h_{t-1} (complement: a_t (h_{t-1} - x_t))
       get(sh.parts[buf].h[part], h);
@@ -223,7 +233,7 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
           }
         }
       }
-      entered<PACKED>(sh.parts[buf], sh.back[buf][part], p.cluster, part, u);
+      get(sh.back[buf][part], u);
       TX* dx_row = dx ? dx + (int64_t)(t0 + kRun - 1) * p.dx_s[1] : nullptr;
       TG* dg_row = dg ? dg + (int64_t)(t0 + kRun - 1) * p.dg_s[1] : nullptr;
 #pragma unroll
@@ -272,20 +282,31 @@ int read_grad_device_error(bool clear) {
   return v;
 }
 
-cudaError_t launch_grad(ScanParams p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
-  choose_cluster(p, Bwd::kTile, 3 * 148);
+namespace {
+template <typename TX, typename TG, typename Bwd>
+cudaError_t launch_shape(ScanParams p, bool wide, cudaStream_t s) {
+  choose_cluster<Bwd>(p);
+  CUtensorMap mx, mg, md;
+  const bool tma = wide && encode<TX>(&mx, p.x, p.x_s, p, Bwd::kTile) && encode<TG>(&mg, p.g, p.g_s, p, Bwd::kTile) &&
+                   encode<TX>(&md, p.dh, p.dh_s, p, Bwd::kTile);
+  const size_t smem = 2 * Ring<TX, Bwd::kTile, kXSlots>::kBytes + Ring<TG, Bwd::kTile, kGSlots>::kBytes +
+                      sizeof(Shared<Bwd>) + cluster_bytes(p.cluster);
+  return by_flags(tma, p.q_start != nullptr, p.complement, [&](auto wide_, auto packed, auto complement) {
+    return launch_tiles(scan_grad_kernel<TX, TG, Bwd, wide_.value, packed.value, complement.value>, p, Bwd::kThreads,
+                        smem, s, mx, mg, md);
+  });
+}
+}  // namespace
+
+cudaError_t launch_grad(const ScanParams& p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
+  // (us, Long and Short: 4 x 8192 x 2048 bf16, 128 blocks, 152 and 165; 1 x 4096 x 2048, 32 blocks, 27 and 31;
+  // 16 x 2048 x 2048, 512 blocks, 166 and 205; 64 x 512 x 2048, 2048 blocks, 178 and 155)
+  const bool is_long =
+      (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels) <= kSms || p.T >= 1024;
   return by_types(x_dtype, g_dtype, [&](auto x, auto g) {
     using TX = decltype(x);
     using TG = decltype(g);
-    CUtensorMap mx, mg, md;
-    const bool tma = wide && encode<TX>(&mx, p.x, p.x_s, p, Bwd::kTile) &&
-                     encode<TG>(&mg, p.g, p.g_s, p, Bwd::kTile) && encode<TX>(&md, p.dh, p.dh_s, p, Bwd::kTile);
-    const size_t smem = 2 * Ring<TX, Bwd::kTile, kXSlots>::kBytes + Ring<TG, Bwd::kTile, kGSlots>::kBytes +
-                        sizeof(Shared) + cluster_bytes(p.cluster);
-    return by_flags(tma, p.q_start != nullptr, p.complement, [&](auto wide_, auto packed, auto complement) {
-      return launch_tiles(scan_grad_kernel<TX, TG, wide_.value, packed.value, complement.value>, p, Bwd::kThreads,
-                          smem, s, mx, mg, md);
-    });
+    return is_long ? launch_shape<TX, TG, Long<TX>>(p, wide, s) : launch_shape<TX, TG, Short>(p, wide, s);
   });
 }
 
