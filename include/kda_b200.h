@@ -488,7 +488,7 @@ size_t kda_scan_args_size(void);
  * kda_qk_bwd: dx and dw (w's type; NULL: not wanted) from x and dy.  It needs
  * kda_qk_partial_floats() fp32 values of scratch where a dw is wanted, and adds in a
  * fixed order.
- * Requires D <= 512, R even and <= D, eps >= 1e-12.
+ * Requires D <= 512, R even and <= D, B T <= 2^30, eps >= 1e-12.
  */
 enum { KDA_NORM_NONE = 0, KDA_NORM_RMS = 1, KDA_NORM_L2 = 2 };
 typedef struct KdaQkArgs {

@@ -105,7 +105,7 @@ def test_scan_entry_points_refuse():
     assert lib.kda_scan_step(P(_scan_args(**{**step, "state_in": FAKE + 64}, scatter=1)), None) == L.KDA_ERR_STRIDE
     assert lib.kda_scan_step(P(_scan_args(**{**step, "B": 0})), None) == L.KDA_OK
     assert lib.kda_scan_workspace_bytes(P(_scan_args())) == 0
-    assert lib.kda_scan_workspace_bytes(P(_scan_args(T=65, q_start=FAKE))) == 2 * 24
+    assert lib.kda_scan_workspace_bytes(P(_scan_args(T=65, q_start=FAKE))) > 0
     n = lib.kda_scan_ckpt_floats
     assert n(P(_scan_args(T=32))) == 2 * 16 and n(P(_scan_args(T=33))) == 2 * 2 * 16
     assert n(P(_scan_args(T=33, q_start=FAKE))) == 2 * 16 and n(P(_scan_args(T=0))) == 0
@@ -139,6 +139,7 @@ def test_qk_entry_points_refuse():
                 (dict(R=7), L.KDA_ERR_SHAPE), (dict(R=18), L.KDA_ERR_SHAPE), (dict(R=-2), L.KDA_ERR_SHAPE),
                 (dict(norm=3), L.KDA_ERR_SHAPE), (dict(eps=0.0), L.KDA_ERR_SHAPE),
                 (dict(eps=float("nan")), L.KDA_ERR_SHAPE), (dict(heads0=-1), L.KDA_ERR_SHAPE),
+                (dict(B=1 << 16, T=1 << 15), L.KDA_ERR_SHAPE),
                 (dict(io_dtype=3), L.KDA_ERR_DTYPE), (dict(w_dtype=-1), L.KDA_ERR_DTYPE),
                 (dict(inv_freq=None), L.KDA_ERR_NULL_POINTER), (dict(x0=None), L.KDA_ERR_NULL_POINTER),
                 (dict(x1=FAKE + 1), L.KDA_ERR_ALIGNMENT), (dict(w0=FAKE + 2), L.KDA_ERR_ALIGNMENT),
@@ -151,6 +152,6 @@ def test_qk_entry_points_refuse():
     assert lib.kda_qk_bwd(P(_qk_args(dw0=FAKE)), None) == L.KDA_ERR_NULL_POINTER
     assert lib.kda_qk_bwd(P(_qk_args(dw0=FAKE, w0=FAKE)), None) == L.KDA_ERR_WORKSPACE
     need = lib.kda_qk_partial_floats(P(_qk_args()))
-    assert need > 0 and need % (6 * 16) == 0
+    assert need > 0 and need % 16 == 0
     assert lib.kda_qk_bwd(P(_qk_args(dw0=FAKE, w0=FAKE, partial=FAKE, partial_floats=need - 1)),
                           None) == L.KDA_ERR_WORKSPACE
