@@ -29,7 +29,7 @@ constexpr int kThreads = 128;
 constexpr int kMaxD = 512;
 constexpr int kItems = kMaxD / 32;
 constexpr int kSms = 148;
-template <bool GRAD> constexpr int kUnroll = GRAD ? 1 : 2;   // rows of a thread on their way in head_kernel
+constexpr int kUnroll = 2;   // rows of a thread on their way in head_kernel
 
 // Device-side view of KdaQkArgs (strides in elements).
 struct QkParams {
@@ -241,9 +241,10 @@ __global__ void __launch_bounds__(kThreads) row_kernel(const QkParams p) {
 // ---------------------------------------------------------------------------
 // rows of 2 VEC N channels
 // ---------------------------------------------------------------------------
-constexpr int kHeadThreads = 512;        // of a block, at most
-// Blocks of 256 threads that an SM takes: registers for the rows on their way
-// (the gradient holds twice as many, and its weights' sums).
+constexpr int kHeadThreads = 256;        // of a block, at most
+// Blocks that an SM takes.  4 x 8192 tokens of 32 heads of 128, f16: three blocks 92 us, two
+// 111, four (one row of a thread at a time) 100; the gradient with two 136, with three (which
+// spill) 178; with one row at a time 158.
 template <bool GRAD> constexpr int kHeadBlocks = GRAD ? 2 : 3;
 
 struct HeadShape {
@@ -349,10 +350,10 @@ __device__ __forceinline__ Rate row_rate(const QkParams& p, const Row<VEC>& x) {
 // `together`-th token from s / heads on.  A block's tokens are of one sequence, or of sequences
 // that lie one behind the other (p.span tokens).
 template <typename T, int VEC, int LANES, bool GRAD, bool INTERLEAVED>
-__global__ void __launch_bounds__(kHeadThreads, kHeadBlocks<GRAD> * 256 / kHeadThreads)
+__global__ void __launch_bounds__(kHeadThreads, kHeadBlocks<GRAD>)
 head_kernel(const QkParams p, const HeadShape hs) {
   extern __shared__ __align__(16) unsigned char shared[];
-  constexpr int UNROLL = kUnroll<GRAD>;
+  constexpr int UNROLL = kUnroll;
   using R = Raw<T, VEC>;
   const int pairs = p.R / 2, turned = pairs / VEC;               // of a row: lanes that are turned
   float4* const angles = reinterpret_cast<float4*>(shared);      // [2][batch][VEC / 2][turned]
@@ -599,11 +600,11 @@ HeadShape head_shape(const QkParams& p, int vec, bool grad) {
   const int all = p.heads[0] + p.heads[1], most = kHeadThreads / h.lanes;
   h.groups = (all + most - 1) / most;
   h.heads = (all + h.groups - 1) / h.groups;
-  // (256 threads are enough for a block that has few heads; small calls get more blocks)
-  h.together = max(1, min(256 / h.lanes / h.heads, (p.tokens + kSms - 1) / kSms));
+  // (small calls get more blocks)
+  h.together = max(1, min(most / h.heads, (p.tokens + kSms - 1) / kSms));
   h.threads = (h.heads * h.together * h.lanes + 31) / 32 * 32;
   // angles for several turns, four for every thread or so
-  const int turn = h.together * (grad ? kUnroll<true> : kUnroll<false>);
+  const int turn = h.together * kUnroll;
   h.batch = turn * max(1, min(8, 4 * h.threads / max(1, turn * p.R / 2)));
   h.smem = (size_t)(p.R / 2) * (sizeof(double) + 2 * h.batch * sizeof(float2));
   if (grad) h.smem = max(h.smem, (size_t)h.together * h.heads * p.D * sizeof(float));
@@ -656,7 +657,7 @@ bool plan(const KdaQkArgs* a, QkParams& p, bool grad, HeadShape& h) {
     join(p, grad);
     h = head_shape(p, vec, grad);
     // as many blocks as the GPU takes at once, so that all end together
-    cut(p, h.groups, h.together, kSms * max(1, (grad ? kHeadBlocks<true> : kHeadBlocks<false>) * 256 / h.threads));
+    cut(p, h.groups, h.together, kSms * ((grad ? kHeadBlocks<true> : kHeadBlocks<false>) * kHeadThreads / h.threads));
   } else {
     cut(p, p.heads[0] + p.heads[1], kThreads / 32 * 4, kSms * 16);
   }
