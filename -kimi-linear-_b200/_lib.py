@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -264,6 +265,9 @@ class KdaScanArgs(ctypes.Structure):
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
+    # the fields in order, for one pack() (setting them one by one costs as much as a launch)
+    PACK = struct.Struct("@10i31q")
+
 
 _I64x3x2 = _I64x3 * 2
 _P2 = ctypes.c_void_p * 2
@@ -291,6 +295,8 @@ class KdaQkArgs(ctypes.Structure):
         ("dw", _P2),
         ("partial", ctypes.c_void_p), ("partial_floats", ctypes.c_size_t),
     ]
+
+    PACK = struct.Struct("@14if1i42q")
 
 
 class KdaLibraryError(RuntimeError):

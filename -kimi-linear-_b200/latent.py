@@ -38,7 +38,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DT, KdaError, _call
+from .ops import _DT, _launch
 
 _HALF = (torch.float16, torch.bfloat16)
 _I64x2 = ctypes.c_int64 * 2
@@ -194,17 +194,6 @@ def _args(fn, cache, block_table, lens, q_start, N):
     if q_start is not None:
         a.q_start = q_start.data_ptr()
     return a
-
-
-def _launch(fn, entry, a, dev):
-    """Call a C entry point on the current stream of ``dev`` (:func:`ops._call`
-    with less host work: these calls can be a few microseconds long)."""
-    index = dev.index
-    if torch.cuda.current_device() != index:
-        return _call(fn, entry, a, dev)
-    st = entry(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
-    if st != _lib.KDA_OK:
-        raise KdaError(fn, st)
 
 
 def _rows(fn, name, t, N, width):

@@ -168,6 +168,16 @@ def _call(fn_name, entry, args, dev):
         raise KdaError(fn_name, st)
 
 
+def _launch(fn, entry, a, dev):
+    """:func:`_call` with less host work, for calls that are a few microseconds long."""
+    index = dev.index
+    if torch.cuda.current_device() != index:
+        return _call(fn, entry, a, dev)
+    st = entry(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
+    if st != _lib.KDA_OK:
+        raise KdaError(fn, st)
+
+
 def kda_chunkwise(q, k, v, g, beta, initial_state=None, chunk_size=64, tile_size=0,
                   state_dtype=None, *, inplace=False):
     """Chunkwise KDA forward -- drop-in for ``kimi_linear/kda.py:58``.

@@ -25,9 +25,9 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DT, _call, _check_tensors, _needs_grad
+from .ops import _DT, _check_tensors, _launch, _needs_grad
 
-_I64x2 = ctypes.c_int64 * 2
+_NONE2, _NONE3 = (0, 0), (0, 0, 0)
 
 
 def _unit(t):
@@ -36,8 +36,24 @@ def _unit(t):
 
 
 def _bt(t, packed):
-    """(batch, token) strides."""
-    return _I64x2(0, t.stride(0)) if packed else _I64x2(t.stride(0), t.stride(1))
+    """Pointer and (batch, token) strides."""
+    if packed:
+        return t.data_ptr(), 0, t.stride(0)
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _rows(t):
+    """Pointer and stride of the rows of a state."""
+    return t.data_ptr(), t.stride(0)
+
+
+def _args(B, T, x, g, complement, xs, gs, state=_NONE2, q_start=0, slots=0, h=_NONE3, S=_NONE2, ckpt=0,
+          dh=_NONE3, dS=_NONE2, dx=_NONE3, dg=_NONE3, dstate=_NONE2, num_states=0, scatter=0):
+    """The argument block, but for the workspace: pointers with their strides."""
+    return _lib.KdaScanArgs.from_buffer_copy(_lib.KdaScanArgs.PACK.pack(
+        _lib.ABI_VERSION, B, T, x.shape[-1], _DT[x.dtype], _DT[g.dtype], 1 if complement else 0,
+        num_states, scatter, 0, *xs, *gs, *state, q_start, slots, *h, *S, ckpt, *dh, *dS, *dx, *dg, *dstate,
+        0, 0))
 
 
 def _check(fn, x, g, state, rows, others=()):
@@ -72,29 +88,12 @@ def _batch(fn, x, q_start):
     return q_start.shape[0] - 1
 
 
-def _fill(x, g, state, q_start, complement):
-    packed = q_start is not None
-    a = _lib.KdaScanArgs()
-    a.abi_version = _lib.ABI_VERSION
-    a.B = q_start.shape[0] - 1 if packed else x.shape[0]
-    a.T, a.D = x.shape[-2], x.shape[-1]
-    a.x_dtype, a.g_dtype = _DT[x.dtype], _DT[g.dtype]
-    a.complement = 1 if complement else 0
-    a.x, a.x_stride = x.data_ptr(), _bt(x, packed)
-    a.g, a.g_stride = g.data_ptr(), _bt(g, packed)
-    if state is not None:
-        a.state_in, a.state_in_stride = state.data_ptr(), state.stride(0)
-    if packed:
-        a.q_start = q_start.data_ptr()
-    return a
-
-
 def _workspace(a, q_start):
     """Scratch for a packed batch, set in ``a``; the caller holds it through the call."""
     if q_start is None:
         return None
     need = int(_lib.load().kda_scan_workspace_bytes(ctypes.byref(a)))
-    ws = torch.empty((need + 7) // 8, device=q_start.device, dtype=torch.int64)
+    ws = q_start.new_empty(((need + 7) // 8,), dtype=torch.int64)
     a.workspace, a.workspace_bytes = ws.data_ptr(), need
     return ws
 
@@ -102,21 +101,21 @@ def _workspace(a, q_start):
 def _forward(x, g, state, q_start, complement, keep):
     """``(h, S, checkpoints)`` for operands that :func:`_check` has passed;
     ``keep``: checkpoints for the backward pass are wanted."""
+    packed = q_start is not None
     x, g = _unit(x), _unit(g)
     state = None if state is None else _unit(state.float())
-    a = _fill(x, g, state, q_start, complement)
-    h = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    S = torch.empty((a.B, a.D), device=x.device, dtype=torch.float32)
-    a.h, a.h_stride = h.data_ptr(), _bt(h, q_start is not None)
-    a.state_out, a.state_out_stride = S.data_ptr(), a.D
+    B, T, D = q_start.shape[0] - 1 if packed else x.shape[0], x.shape[-2], x.shape[-1]
+    h = x.new_empty(x.shape)
+    S = x.new_empty((B, D), dtype=torch.float32)
     lib = _lib.load()
+    a = _args(B, T, x, g, complement, _bt(x, packed), _bt(g, packed), _NONE2 if state is None else _rows(state),
+              q_start.data_ptr() if packed else 0, 0, _bt(h, packed), (S.data_ptr(), D))
     ckpt = None
     if keep:
-        ckpt = torch.empty(int(lib.kda_scan_ckpt_floats(ctypes.byref(a))), device=x.device,
-                           dtype=torch.float32)
+        ckpt = S.new_empty((int(lib.kda_scan_ckpt_floats(ctypes.byref(a))),))
         a.ckpt = ckpt.data_ptr()
     ws = _workspace(a, q_start)  # noqa: F841
-    _call("gated_scan", lib.kda_scan_fwd, a, x.device)
+    _launch("gated_scan", lib.kda_scan_fwd, a, x.device)
     return h, S, ckpt
 
 
@@ -163,26 +162,21 @@ def _backward(x, g, state, q_start, complement, ckpt, dh, dS, need):
     packed = q_start is not None
     x, g = _unit(x), _unit(g)
     state32 = None if state is None else _unit(state.float())
-    a = _fill(x, g, state32, q_start, complement)
-    a.ckpt = ckpt.data_ptr()
+    B, T, D = q_start.shape[0] - 1 if packed else x.shape[0], x.shape[-2], x.shape[-1]
     if dh is not None:
         dh = _unit(dh.to(x.dtype))
-        a.dh, a.dh_stride = dh.data_ptr(), _bt(dh, packed)
     if dS is not None:
         dS = _unit(dS.float())
-        a.dstate_out, a.dstate_out_stride = dS.data_ptr(), dS.stride(0)
-    dx = dg = dstate = None
-    if need[0]:
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        a.dx, a.dx_stride = dx.data_ptr(), _bt(dx, packed)
-    if need[1]:
-        dg = torch.empty(g.shape, device=x.device, dtype=g.dtype)
-        a.dg, a.dg_stride = dg.data_ptr(), _bt(dg, packed)
-    if need[2] and state is not None:
-        dstate = torch.empty(state.shape, device=x.device, dtype=torch.float32)
-        a.dstate_in, a.dstate_in_stride = dstate.data_ptr(), a.D
+    dx = x.new_empty(x.shape) if need[0] else None
+    dg = g.new_empty(g.shape) if need[1] else None
+    dstate = ckpt.new_empty((B, D)) if need[2] and state is not None else None
+    three = lambda t: _NONE3 if t is None else _bt(t, packed)  # noqa: E731
+    two = lambda t: _NONE2 if t is None else _rows(t)  # noqa: E731
+    a = _args(B, T, x, g, complement, _bt(x, packed), _bt(g, packed), two(state32),
+              q_start.data_ptr() if packed else 0, ckpt=ckpt.data_ptr(), dh=three(dh), dS=two(dS), dx=three(dx),
+              dg=three(dg), dstate=two(dstate))
     ws = _workspace(a, q_start)  # noqa: F841
-    _call("gated_scan_backward", _lib.load().kda_scan_bwd, a, x.device)
+    _launch("gated_scan_backward", _lib.load().kda_scan_bwd, a, x.device)
     return dx, dg, None if dstate is None else dstate.to(state.dtype)
 
 
@@ -244,21 +238,10 @@ def gated_step(x, g, state=None, slots=None, *, complement=False, inplace=False)
     elif state is not None:
         state = _unit(state)
     x, g = _unit(x), _unit(g)
-    h = torch.empty(shape, device=dev, dtype=x.dtype)
-    S = state if inplace else torch.empty((B, D), device=dev, dtype=torch.float32)
-    a = _lib.KdaScanArgs()
-    a.abi_version = _lib.ABI_VERSION
-    a.B, a.T, a.D = B, 1, D
-    a.x_dtype, a.g_dtype = _DT[x.dtype], _DT[g.dtype]
-    a.complement = 1 if complement else 0
-    a.scatter = 1 if inplace else 0
-    a.x, a.x_stride[0] = x.data_ptr(), x.stride(0)
-    a.g, a.g_stride[0] = g.data_ptr(), g.stride(0)
-    a.h, a.h_stride[0] = h.data_ptr(), D
-    if state is not None:
-        a.state_in, a.state_in_stride = state.data_ptr(), state.stride(0)
-    a.state_out, a.state_out_stride = S.data_ptr(), S.stride(0)
-    if slots is not None:
-        a.slots, a.num_states = slots.data_ptr(), rows
-    _call(fn, _lib.load().kda_scan_step, a, dev)
+    h = x.new_empty(shape)
+    S = state if inplace else x.new_empty((B, D), dtype=torch.float32)
+    a = _args(B, 1, x, g, complement, (x.data_ptr(), x.stride(0), 0), (g.data_ptr(), g.stride(0), 0),
+              _NONE2 if state is None else _rows(state), 0, 0 if slots is None else slots.data_ptr(),
+              (h.data_ptr(), D, 0), _rows(S), num_states=0 if slots is None else rows, scatter=1 if inplace else 0)
+    _launch(fn, _lib.load().kda_scan_step, a, dev)
     return h, S

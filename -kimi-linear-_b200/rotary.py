@@ -20,22 +20,31 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DT, _call, _check_tensors, _needs_grad
+from .ops import _DT, _check_tensors, _launch, _needs_grad
 
 NORMS = {None: _lib.NORM_NONE, "rms": _lib.NORM_RMS, "l2": _lib.NORM_L2}
 MAX_D = 512
+_NONE = (0, 0, 0, 0)              # pointer and strides of an operand that is not there
 
 
 def _unit(t):
     return t if t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
 
 
-def _put(a, name, i, t):
+def _bth(t):
     """Pointer and (batch, token, head) strides of a [B, T, H, D] or [N, H, D] tensor."""
-    getattr(a, name)[i] = t.data_ptr()
-    s = t.stride()
-    st = getattr(a, name + "_stride")[i]
-    st[0], st[1], st[2] = (0, s[0], s[1]) if t.dim() == 3 else (s[0], s[1], s[2])
+    if t is None:
+        return _NONE
+    return (t.data_ptr(), 0, *t.stride()[:2]) if t.dim() == 3 else (t.data_ptr(), *t.stride()[:3])
+
+
+def _two(q, k):
+    """As the argument block has them: both pointers, then both strides."""
+    q, k = _bth(q), _bth(k)
+    return (q[0], k[0], *q[1:], *k[1:])
+
+
+_NONE2 = _two(None, None)
 
 
 def _check(fn, q, k, wq, wk, norm, eps, positions, inv_freq, others=()):
@@ -80,55 +89,40 @@ def _check(fn, q, k, wq, wk, norm, eps, positions, inv_freq, others=()):
     return dev
 
 
-def _fill(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved):
-    """The argument block but for outputs and gradients, and what must stay alive with it."""
-    a = _lib.KdaQkArgs()
-    a.abi_version = _lib.ABI_VERSION
+def _args(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, y=_NONE2, dy=_NONE2, dx=_NONE2, dw=(0, 0)):
+    """The argument block, but for the partial sums, and what must stay alive with it."""
     packed = q.dim() == 3
-    a.B, a.T = (1, q.shape[0]) if packed else q.shape[:2]
-    a.D = q.shape[-1]
-    a.heads[0] = q.shape[-2]
-    a.heads[1] = 0 if k is None else k.shape[-2]
-    a.io_dtype = _DT[q.dtype]
-    a.norm, a.interleaved = NORMS[norm], 1 if interleaved else 0
-    a.eps = float(eps)
-    keep = []
-    _put(a, "x", 0, q)
-    if k is not None:
-        _put(a, "x", 1, k)
-    for i, w in enumerate((wq, wk)):
-        if w is not None:
-            w = w.detach().contiguous()
-            keep.append(w)
-            a.w[i], a.w_dtype, a.w_heads = w.data_ptr(), _DT[w.dtype], 1 if w.dim() == 2 else 0
+    B, T = (1, q.shape[0]) if packed else q.shape[:2]
+    ws = [None if w is None else w.detach().contiguous() for w in (wq, wk)]
+    w = ws[0] if ws[0] is not None else ws[1]
+    R = 0
     if inv_freq is not None:
         inv_freq = inv_freq.detach().contiguous()
-        keep.append(inv_freq)
-        a.R, a.inv_freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
-    a.pos_step = 1
+        R = 2 * inv_freq.shape[0]
+    pos, wide, step, ps = 0, 0, 1, (0, 0)
     if positions is not None:
-        a.positions, a.pos_64 = positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0
-        s = positions.stride()
+        pos, wide, s = positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0, positions.stride()
         if positions.dim() == 2:
-            a.pos_stride[0], a.pos_stride[1], a.pos_step = s[0], s[1], 0
+            ps, step = s, 0
         elif packed:
-            a.pos_stride[1], a.pos_step = s[0], 0
+            ps, step = (0, s[0]), 0
         else:
-            a.pos_stride[0] = s[0]
-    return a, keep
+            ps = (s[0], 0)
+    a = _lib.KdaQkArgs.from_buffer_copy(_lib.KdaQkArgs.PACK.pack(
+        _lib.ABI_VERSION, B, T, q.shape[-1], R, q.shape[-2], 0 if k is None else k.shape[-2], _DT[q.dtype],
+        _lib.DTYPE_F32 if w is None else _DT[w.dtype], NORMS[norm], 1 if interleaved else 0,
+        0 if w is None or w.dim() == 1 else 1, wide, step, float(eps), 0, *_two(q, k),
+        *(0 if t is None else t.data_ptr() for t in ws), pos, *ps,
+        0 if inv_freq is None else inv_freq.data_ptr(), *y, *dy, *dx, *dw, 0, 0))
+    return a, (ws, inv_freq)
 
 
 def _forward(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved):
     q, k = _unit(q), None if k is None else _unit(k)
-    a, keep = _fill(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved)
-    outs = []
-    for i, t in enumerate((q, k)):
-        out = None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype)
-        if out is not None:
-            _put(a, "y", i, out)
-        outs.append(out)
-    _call("qk_norm_rope", _lib.load().kda_qk_fwd, a, q.device)
-    return tuple(outs)
+    oq, ok = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    a, keep = _args(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, y=_two(oq, ok))
+    _launch("qk_norm_rope", _lib.load().kda_qk_fwd, a, q.device)
+    return oq, ok
 
 
 def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, *, norm="rms", eps=1e-6, positions=None,
@@ -180,28 +174,19 @@ class _QkNormRope(torch.autograd.Function):
 
 def _backward(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, dq, dk, need):
     q, k = _unit(q), None if k is None else _unit(k)
-    a, keep = _fill(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved)
-    outs = [None] * 4
-    for i, (t, d) in enumerate(((q, dq), (k, dk))):
-        if t is None:
-            continue
-        d = _unit(d.to(t.dtype))
-        keep.append(d)
-        _put(a, "dy", i, d)
-        outs[i] = torch.empty(t.shape, device=t.device, dtype=t.dtype)
-        _put(a, "dx", i, outs[i])
-    for i, w in enumerate((wq, wk)):
-        if w is not None and need[2 + i]:
-            outs[2 + i] = torch.empty(w.shape, device=w.device, dtype=w.dtype)
-            a.dw[i] = outs[2 + i].data_ptr()
+    dq = _unit(dq.to(q.dtype))
+    dk = None if k is None else _unit(dk.to(k.dtype))
+    oq, ok = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    dw = [w.new_empty(w.shape) if w is not None and n else None for w, n in ((wq, need[2]), (wk, need[3]))]
+    a, keep = _args(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, dy=_two(dq, dk), dx=_two(oq, ok),
+                    dw=[0 if w is None else w.data_ptr() for w in dw])
     lib = _lib.load()
     if a.dw[0] or a.dw[1]:
         n = int(lib.kda_qk_partial_floats(ctypes.byref(a)))
-        partial = torch.empty(n, device=q.device, dtype=torch.float32)
-        keep.append(partial)
+        partial = q.new_empty((n,), dtype=torch.float32)
         a.partial, a.partial_floats = partial.data_ptr(), n
-    _call("qk_norm_rope_backward", lib.kda_qk_bwd, a, q.device)
-    return tuple(outs)
+    _launch("qk_norm_rope_backward", lib.kda_qk_bwd, a, q.device)
+    return oq, ok, *dw
 
 
 def qk_norm_rope_backward(dq, dk, q, k=None, q_weight=None, k_weight=None, *, norm="rms", eps=1e-6,
