@@ -39,6 +39,7 @@ import torch
 
 from . import _lib
 from .ops import _DT, _launch
+from .rotary import qk_norm_rope
 
 _HALF = (torch.float16, torch.bfloat16)
 _I64x2 = ctypes.c_int64 * 2
@@ -318,7 +319,10 @@ def mla_step(module, x, q_nope, q_rope, c_kv, k_rope, state, use_cache):
     ``q_nope`` ``[B, T, H, DN]``, ``q_rope`` ``[B, T, H, DR]`` and ``k_rope``
     ``[B, T, DR]`` (rotated; None without a rope part), ``c_kv`` ``[B, T, KVL]``.
     ``state``: ``cache`` (a :class:`LatentCache`), ``block_table`` and ``lens``;
-    the pages for ``lens + T`` tokens must be in the table.  ``lens`` is advanced
+    the pages for ``lens + T`` tokens must be in the table.  With ``inv_freq`` fp32
+    ``[R / 2]`` in ``state``, ``q_rope`` and ``k_rope`` come before their rotation and are
+    rotated by their tokens' positions, ``lens`` and on, read on the device (by
+    :func:`rotary.qk_norm_rope`; ``interleaved`` in ``state`` as there).  ``lens`` is advanced
     by ``T`` on the device (a step that raises takes that back), the tokens are
     appended, the queries folded into the latent space by the module's own
     ``kv_b_proj`` weight (cast on every step unless it is in the cache's type),
@@ -333,6 +337,13 @@ def mla_step(module, x, q_nope, q_rope, c_kv, k_rope, state, use_cache):
                            f"rope_dim {cache.rope_dim}")
     dt = cache.dtype
     w = module.kv_b_proj.weight.detach().to(dt).view(H, DN + DV, KVL)
+    inv_freq = state.get("inv_freq")
+    if inv_freq is not None:
+        if not cache.rope_dim:
+            raise RuntimeError("mla_step: inv_freq for a cache without a rope part")
+        q_rope, k_rope = qk_norm_rope(q_rope.reshape(B, T, H, cache.rope_dim),
+                                      k_rope.reshape(B, T, 1, cache.rope_dim), norm=None, positions=lens,
+                                      inv_freq=inv_freq, interleaved=state.get("interleaved", False))
     lens.add_(T)
     try:
         if cache.rope_dim:

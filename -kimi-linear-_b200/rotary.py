@@ -5,7 +5,7 @@ Every head of a token is normalised (root mean square with an optional weight, a
 ``HeadwiseRMSNorm``, ``kimi_linear/kda.py:258-279``; or to length one, as ``l2norm``,
 ``kda.py:313-325``; or not at all), and its first ``R`` channels are rotated by the
 token's position: what stands between a layer's projections and its attention or
-recurrence.
+recurrence (:func:`latent.mla_step` rotates its rope parts with it).
 
 :func:`qk_norm_rope` is differentiable in queries, keys and weights;
 :func:`qk_norm_rope_backward` is the gradient that autograd calls.  CUDA tensors only

@@ -87,6 +87,30 @@ def test_batch(cuda_dev, tx, tg, complement, B, T, D):
         close(v.reshape(w.shape), w, e, n)
 
 
+@pytest.mark.parametrize("tx,tg", [(F32, F32), (F16, F32), (BF16, BF16)], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("B,T,D", [(80, 70, 128), (150, 3, 40), (1, 200, 9536), (76, 1030, 128), (149, 1, 64),
+                                   (3, 140, 9480)])
+def test_more_blocks_than_the_gpu_takes(cuda_dev, tx, tg, B, T, D):
+    """The blocks of many sequences or channels, short and long; as a batch and packed."""
+    kb = pkg()
+    complement = tx == F16
+    x, g, s0, dh, dS = inputs(B * T, D, tx, tg, B + T, B, cuda_dev)
+    wide = lambda t: t.view(B, T, D).transpose(0, 1).reshape(T, B * D)  # noqa: E731
+    want, err = expected(wide(x), wide(g), s0.view(1, -1), wide(dh), dS.view(1, -1), [(0, T)], complement)
+    back = lambda t: t.view(T, B, D).transpose(0, 1)  # noqa: E731
+    dev = lambda t: t.to(cuda_dev)  # noqa: E731
+    for q in (None, dev(torch.arange(0, B * T + 1, T, dtype=torch.int32))):
+        rows = (B, T, D) if q is None else (B * T, D)
+        leaves = [dev(x).view(rows).requires_grad_(), dev(g).view(rows).requires_grad_(),
+                  dev(s0).requires_grad_()]
+        h, S = kb.gated_scan(*leaves, q, complement=complement)
+        got = [h, S, *torch.autograd.grad([h, S], leaves, [dev(dh).view(rows), dev(dS)])]
+        for i, (n, v) in enumerate(zip(NAMES, got)):
+            states = i in (1, 4)
+            w, e = (t.view(B, D) if states else back(t) for t in (want[i], err[i]))
+            close(v.reshape(w.shape), w, e, n)
+
+
 STARTS = {
     "one": (50, [0, 50]),
     "ragged": (300, [0, 1, 2, 66, 66, 194, 300]),
