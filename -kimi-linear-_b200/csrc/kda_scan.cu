@@ -126,13 +126,17 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     float* const ckpt = p.ckpt ? p.ckpt + (int64_t)w.b * p.steps * p.D : nullptr;
     for (int k = 0; k < turns; ++k) {
       const int buf = k & 1;
+      // (packed: rows of two turns on, asked for while the workers are busy; they are done with turn
+      // k - 2, whose place these take, when turn k's pieces are there)
+      const bool fetches = PACKED && warp == Fwd::kCarryWarps - 1 && at < Fwd::kParts;
+      const uint32_t ahead = fetches ? packed_rows(p, first_row(k + 2, at)) : 0;
       pieces_wait(buf, Fwd::kThreads);
+      if (fetches) sh.rows.bits[(k + 2) & 3][at] = ahead;
       // the workers have read the rows of turn k
       if (copies && patience.limit) copy(k + kSlots);
-      uint32_t cuts = 0, ahead = 0;
+      uint32_t cuts = 0;
       if constexpr (PACKED) {
         cuts = sh.rows.starts(k);
-        if (warp == Fwd::kCarryWarps - 1 && at < Fwd::kParts) ahead = packed_rows(p, first_row(k + 2, at));
       }
       Parts<Fwd>& parts = sh.parts[buf];
       enter_parts<PACKED, false>(exchange, patience, k, parts, parts.h, cuts, carry, warp, at, [] {});
@@ -149,7 +153,6 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
           if (step < p.steps && ch1 < p.D) ckpt[(int64_t)step * p.D + ch1] = s.y;
         }
       }
-      if (PACKED && warp == Fwd::kCarryWarps - 1 && at < Fwd::kParts) sh.rows.bits[(k + 2) & 3][at] = ahead;
       states_done(buf, Fwd::kThreads);
     }
     if (!PACKED && w.rank == 0 && warp == 0) {
@@ -179,6 +182,7 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
         return;
       }
       const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
+      const bool plain = PACKED && m.plain();
       if constexpr (WIDE) {
         patience.wait(sh.full + k % kSlots, k / kSlots & 1);
       } else {
@@ -192,20 +196,23 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       }
       float2 sum[kPairs], c[kPairs], r[kPairs], h[kPairs];
       sum[0] = sum[1] = h[0] = h[1] = both(0.f);
+      by_rows<PACKED>(plain, [&](auto each) {
+        constexpr bool EACH = decltype(each)::value;
 #pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        float2 gt[kPairs];
-        gs.read(k, row0 + t, gt);
-        xs.read(k, row0 + t, run.v[t]);
-        if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
+        for (int t = 0; t < kRun; ++t) {
+          float2 gt[kPairs];
+          gs.read(k, row0 + t, gt);
+          xs.read(k, row0 + t, run.v[t]);
+          if (EACH && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          run.a[t][j] = decay(gt[j]);
-          sum[j] = __fadd2_rn(sum[j], gt[j]);
-          if (COMPLEMENT) run.v[t][j] = __fmul2_rn(run.v[t][j], rest(gt[j], run.a[t][j]));
-          h[j] = __ffma2_rn(run.a[t][j], h[j], run.v[t][j]);
+          for (int j = 0; j < kPairs; ++j) {
+            run.a[t][j] = decay(gt[j]);
+            sum[j] = __fadd2_rn(sum[j], gt[j]);
+            if (COMPLEMENT) run.v[t][j] = __fmul2_rn(run.v[t][j], rest(gt[j], run.a[t][j]));
+            h[j] = __ffma2_rn(run.a[t][j], h[j], run.v[t][j]);
+          }
         }
-      }
+      });
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) split_decay(sum[j], c[j], r[j]);
       put(parts.c[part], c);
@@ -217,25 +224,29 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     const auto states = [&](int k, int buf, const Run& run) {
       const int t0 = first_row(k, part);
       states_wait(buf, Fwd::kThreads);
-      if (t0 >= p.T || (WIDE && !w.on)) return;
       const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
+      const bool plain = PACKED && m.plain();      // (before any lane leaves)
+      if (t0 >= p.T || (WIDE && !w.on)) return;
       float2 h[kPairs];
       get(sh.parts[buf].h[part], h);
       TX* row = out + (int64_t)t0 * p.h_s[1];
+      by_rows<PACKED>(plain, [&](auto each) {
+        constexpr bool EACH = decltype(each)::value;
 #pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
+        for (int t = 0; t < kRun; ++t) {
+          if (EACH && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) h[j] = __ffma2_rn(run.a[t][j], h[j], run.v[t][j]);
-        if (m.there >> t & 1) {
-          write<WIDE>(row, w.on, h);
-        } else if (PACKED && t0 + t < p.T) {
-          const float2 zero[kPairs] = {};
-          write<WIDE>(row, w.on, zero);
+          for (int j = 0; j < kPairs; ++j) h[j] = __ffma2_rn(run.a[t][j], h[j], run.v[t][j]);
+          if ((PACKED && !EACH) || (m.there >> t & 1)) {
+            write<WIDE>(row, w.on, h);
+          } else if (EACH && t0 + t < p.T) {
+            const float2 zero[kPairs] = {};
+            write<WIDE>(row, w.on, zero);
+          }
+          if (EACH && (m.last >> t & 1)) store_state<WIDE>(state_of(p, p.state_out, p.so_s, t0 + t, w.c), w.on, h);
+          row += p.h_s[1];
         }
-        if (PACKED && (m.last >> t & 1)) store_state<WIDE>(state_of(p, p.state_out, p.so_s, t0 + t, w.c), w.on, h);
-        row += p.h_s[1];
-      }
+      });
     };
     // a turn's pieces before the turn before's states: those come meanwhile
     Run a, b;

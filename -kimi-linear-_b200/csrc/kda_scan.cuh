@@ -9,6 +9,8 @@
 // (fma.f32x2), so a thread works on pairs of channels.
 #pragma once
 
+#include <type_traits>
+
 #include "kda_internal.cuh"
 #include "tc_ptx.cuh"
 
@@ -295,7 +297,23 @@ struct RowMask {
   __device__ RowMask() : there(0), first(0), last(0) {}
   __device__ explicit RowMask(uint32_t bits)
       : there(bits & kAllRows), first(bits >> kRun & kAllRows), last(bits >> 2 * kRun & kAllRows) {}
+  // (warp-wide: all lanes of the warp have to ask) all rows are there, and no sequence starts or ends
+  __device__ __forceinline__ bool plain() const {
+    return __all_sync(0xffffffffu, there == kAllRows && (first | last) == 0);
+  }
 };
+// Calls f with whether the rows have to be looked at one by one: branches between the rows of a
+// run keep the next rows' reads behind them (one sequence of 16000 tokens of 2048 channels, f16,
+// packed: OLD).
+template <bool PACKED, typename F>
+__device__ __forceinline__ void by_rows(bool plain, F f) {
+  if constexpr (PACKED) {
+    if (plain) f(std::false_type{});
+    else f(std::true_type{});
+  } else {
+    f(std::false_type{});
+  }
+}
 __device__ __forceinline__ uint32_t packed_rows(const ScanParams& p, int t) {
   if (t < 0 || t >= p.T) return 0;
   static_assert(kMarked % kRun == 0, "a run is inside one Marks");
@@ -440,8 +458,13 @@ __device__ __forceinline__ void enter_parts(const Exchange& exchange, Patience& 
   if (W > 1 || !alone) {
     const Piece none{both(1.f), both(0.f), both(0.f)};
     Piece all = none, before = none;                   // of the tile; of the shares before this warp's
+    if (PACKED && cuts != 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) append<PACKED>(all, part(place(i)));
+      for (int i = 0; i < N; ++i) append<PACKED>(all, part(place(i)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) append<false>(all, part(place(i)));
+    }
     if constexpr (W > 1) {
       pair(parts.share[warp][0], at) = all.c;
       pair(parts.share[warp][1], at) = all.r;
@@ -476,13 +499,17 @@ __device__ __forceinline__ void enter_parts(const Exchange& exchange, Patience& 
   } else {
     meanwhile();
   }
+  const auto enter = [&](auto cut_) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int j = place(i);
-    const Piece q = part(j);
-    pair(h[j], at) = s;
-    s = pass_on<PACKED>(q, s);
-  }
+    for (int i = 0; i < N; ++i) {
+      const int j = place(i);
+      const Piece q = part(j);
+      pair(h[j], at) = s;
+      s = pass_on<decltype(cut_)::value>(q, s);
+    }
+  };
+  if (PACKED && cuts != 0) enter(std::true_type{});
+  else enter(std::false_type{});
   if (W == 1 && alone) carry = s;
 }
 

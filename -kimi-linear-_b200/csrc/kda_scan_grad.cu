@@ -103,15 +103,19 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     for (int k = 0; k < turns; ++k) {
       const int buf = k & 1;
       float2 state = next;
+      // (packed: rows of two turns on, asked for while the workers are busy; they are done with turn
+      // k - 2, whose place these take, when turn k's pieces are there)
+      const bool fetches = PACKED && warp == Bwd::kCarryWarps - 1 && at < Bwd::kParts;
+      const uint32_t ahead = fetches ? packed_rows(p, first_row(k + 2, at)) : 0;
       pieces_wait(buf, Bwd::kThreads);
+      if (fetches) sh.rows.bits[(k + 2) & 3][at] = ahead;
       // the workers are done with the gates of turn k and with the other rows of turn k - 2
       if (copies && patience.limit) copy(k + 2);
       next = checkpoint(k + 1);
-      uint32_t cuts = 0, starts = 0, ahead = 0;
+      uint32_t cuts = 0, starts = 0;
       if constexpr (PACKED) {
         starts = sh.rows.starts(k);
         cuts = sh.rows.ends(k);
-        if (warp == Bwd::kCarryWarps - 1 && at < Bwd::kParts) ahead = packed_rows(p, first_row(k + 2, at));
       }
       Parts<Bwd>& parts = sh.parts[buf];
       enter_parts<PACKED, true>(exchange, patience, k, parts, sh.back[buf], cuts, carry, warp, at, [&] {
@@ -125,7 +129,6 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
           state = pass_on<PACKED>(q, state);
         }
       });
-      if (PACKED && warp == Bwd::kCarryWarps - 1 && at < Bwd::kParts) sh.rows.bits[(k + 2) & 3][at] = ahead;
       states_done(buf, Bwd::kThreads);
     }
     if (!PACKED && p.dstate_in && w.rank == 0 && warp == 0) {
@@ -144,10 +147,11 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     TX* const dx = p.dx ? static_cast<TX*>(p.dx) + w.b * p.dx_s[0] + w.c : nullptr;
     TG* const dg = p.dg ? static_cast<TG*>(p.dg) + w.b * p.dg_s[0] + w.c : nullptr;
     // d_t = dh_t + u_t in the place of d_{t+1} (for the last token of the run: of u_t)
-    const auto add_later = [&](int k, int t, int t0, const RowMask& m, const Run<COMPLEMENT>& run, float2 (&u)[kPairs]) {
+    const auto add_later = [&](auto each, int k, int t, int t0, const RowMask& m, const Run<COMPLEMENT>& run,
+                               float2 (&u)[kPairs]) {
       float2 d[kPairs] = {both(0.f), both(0.f)};
       if (p.dh) ds.read(k, row0 + t, d);
-      const bool last = PACKED && (m.last >> t & 1);
+      const bool last = decltype(each)::value && (m.last >> t & 1);
       if (last) load_state<WIDE>(state_of(p, p.dstate_out, p.dso_s, t0 + t, w.c), w.on, u);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j)
@@ -167,6 +171,7 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
         return;
       }
       const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
+      const bool plain = PACKED && m.plain();
       if constexpr (!WIDE) {
         xs.copy_own(x + (int64_t)t0 * p.x_s[1], p.x_s[1], k, row0, m.there, w.on);
         gs.copy_own(g + (int64_t)t0 * p.g_s[1], p.g_s[1], k, row0, m.there, w.on);
@@ -180,25 +185,28 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       }
       float2 sum[kPairs], c[kPairs], r[kPairs], h[kPairs], u[kPairs];
       sum[0] = sum[1] = h[0] = h[1] = u[0] = u[1] = both(0.f);
+      by_rows<PACKED>(plain, [&](auto each) {
+        constexpr bool EACH = decltype(each)::value;
 #pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        float2 gt[kPairs], v[kPairs];
-        gs.read(k, row0 + t, gt);
-        xs.read(k, row0 + t, v);
-        if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
+        for (int t = 0; t < kRun; ++t) {
+          float2 gt[kPairs], v[kPairs];
+          gs.read(k, row0 + t, gt);
+          xs.read(k, row0 + t, v);
+          if (EACH && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          run.a[t][j] = decay(gt[j]);
-          sum[j] = __fadd2_rn(sum[j], gt[j]);
-          if (COMPLEMENT) {
-            run.w[t][j] = rest(gt[j], run.a[t][j]);
-            v[j] = __fmul2_rn(v[j], run.w[t][j]);
+          for (int j = 0; j < kPairs; ++j) {
+            run.a[t][j] = decay(gt[j]);
+            sum[j] = __fadd2_rn(sum[j], gt[j]);
+            if (COMPLEMENT) {
+              run.w[t][j] = rest(gt[j], run.a[t][j]);
+              v[j] = __fmul2_rn(v[j], run.w[t][j]);
+            }
+            h[j] = __ffma2_rn(run.a[t][j], h[j], v[j]);
           }
-          h[j] = __ffma2_rn(run.a[t][j], h[j], v[j]);
         }
-      }
 #pragma unroll
-      for (int t = kRun - 1; t >= 0; --t) add_later(k, t, t0, m, run, u);
+        for (int t = kRun - 1; t >= 0; --t) add_later(each, k, t, t0, m, run, u);
+      });
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) u[j] = __fmul2_rn(run.a[0][j], u[j]);
 #pragma unroll
@@ -212,52 +220,56 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     const auto grads = [&](int k, int buf, const Run<COMPLEMENT>& run) {
       const int t0 = first_row(k, part);
       states_wait(buf, Bwd::kThreads);
-      if (t0 >= p.T || (WIDE && !w.on)) return;
       const RowMask m = PACKED ? sh.rows.of(k, part) : batch_rows(p, t0);
-      float2 h[kPairs], u[kPairs], v[kRun][kPairs];
-      // a_t h_{t-1} (complement: a_t (h_{t-1} - x_t))
-      get(sh.parts[buf].h[part], h);
+      const bool plain = PACKED && m.plain();      // (before any lane leaves)
+      if (t0 >= p.T || (WIDE && !w.on)) return;
+      by_rows<PACKED>(plain, [&](auto each) {
+        constexpr bool EACH = decltype(each)::value;
+        float2 h[kPairs], u[kPairs], v[kRun][kPairs];
+        // a_t h_{t-1} (complement: a_t (h_{t-1} - x_t))
+        get(sh.parts[buf].h[part], h);
 #pragma unroll
-      for (int t = 0; t < kRun; ++t) {
-        float2 xt[kPairs];
-        xs.read(k, row0 + t, xt);
-        if (PACKED && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
+        for (int t = 0; t < kRun; ++t) {
+          float2 xt[kPairs];
+          xs.read(k, row0 + t, xt);
+          if (EACH && (m.first >> t & 1)) load_state<WIDE>(state_of(p, p.state_in, p.si_s, t0 + t, w.c), w.on, h);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          if (COMPLEMENT) {
-            v[t][j] = __fmul2_rn(run.a[t][j], __ffma2_rn(xt[j], both(-1.f), h[j]));
-            h[j] = __ffma2_rn(run.a[t][j], h[j], __fmul2_rn(run.w[t][j], xt[j]));
-          } else {
-            v[t][j] = __fmul2_rn(run.a[t][j], h[j]);
-            h[j] = __ffma2_rn(run.a[t][j], h[j], xt[j]);
+          for (int j = 0; j < kPairs; ++j) {
+            if (COMPLEMENT) {
+              v[t][j] = __fmul2_rn(run.a[t][j], __ffma2_rn(xt[j], both(-1.f), h[j]));
+              h[j] = __ffma2_rn(run.a[t][j], h[j], __fmul2_rn(run.w[t][j], xt[j]));
+            } else {
+              v[t][j] = __fmul2_rn(run.a[t][j], h[j]);
+              h[j] = __ffma2_rn(run.a[t][j], h[j], xt[j]);
+            }
           }
         }
-      }
-      get(sh.back[buf][part], u);
-      TX* dx_row = dx ? dx + (int64_t)(t0 + kRun - 1) * p.dx_s[1] : nullptr;
-      TG* dg_row = dg ? dg + (int64_t)(t0 + kRun - 1) * p.dg_s[1] : nullptr;
+        get(sh.back[buf][part], u);
+        TX* dx_row = dx ? dx + (int64_t)(t0 + kRun - 1) * p.dx_s[1] : nullptr;
+        TG* dg_row = dg ? dg + (int64_t)(t0 + kRun - 1) * p.dg_s[1] : nullptr;
 #pragma unroll
-      for (int t = kRun - 1; t >= 0; --t) {
-        float2 ox[kPairs], og[kPairs];
-        add_later(k, t, t0, m, run, u);
+        for (int t = kRun - 1; t >= 0; --t) {
+          float2 ox[kPairs], og[kPairs];
+          add_later(each, k, t, t0, m, run, u);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          ox[j] = COMPLEMENT ? __fmul2_rn(run.w[t][j], u[j]) : u[j];
-          og[j] = __fmul2_rn(v[t][j], u[j]);
+          for (int j = 0; j < kPairs; ++j) {
+            ox[j] = COMPLEMENT ? __fmul2_rn(run.w[t][j], u[j]) : u[j];
+            og[j] = __fmul2_rn(v[t][j], u[j]);
+          }
+          const bool there = (PACKED && !EACH) || (m.there >> t & 1);
+          if (EACH && !there) ox[0] = ox[1] = og[0] = og[1] = both(0.f);
+          if (there || (EACH && t0 + t < p.T)) {
+            if (dx) write<WIDE>(dx_row, w.on, ox);
+            if (dg) write<WIDE>(dg_row, w.on, og);
+          }
+          if (dx) dx_row -= p.dx_s[1];
+          if (dg) dg_row -= p.dg_s[1];
+          if (EACH && p.dstate_in && (m.first >> t & 1)) {
+            const float2 out[kPairs] = {__fmul2_rn(run.a[t][0], u[0]), __fmul2_rn(run.a[t][1], u[1])};
+            store_state<WIDE>(state_of(p, p.dstate_in, p.dsi_s, t0 + t, w.c), w.on, out);
+          }
         }
-        const bool there = m.there >> t & 1;
-        if (PACKED && !there) ox[0] = ox[1] = og[0] = og[1] = both(0.f);
-        if (there || (PACKED && t0 + t < p.T)) {
-          if (dx) write<WIDE>(dx_row, w.on, ox);
-          if (dg) write<WIDE>(dg_row, w.on, og);
-        }
-        if (dx) dx_row -= p.dx_s[1];
-        if (dg) dg_row -= p.dg_s[1];
-        if (PACKED && p.dstate_in && (m.first >> t & 1)) {
-          const float2 out[kPairs] = {__fmul2_rn(run.a[t][0], u[0]), __fmul2_rn(run.a[t][1], u[1])};
-          store_state<WIDE>(state_of(p, p.dstate_in, p.dsi_s, t0 + t, w.c), w.on, out);
-        }
-      }
+      });
     };
     Run<COMPLEMENT> a, b;
     for (int k = 0; k <= turns; k += 2) {
