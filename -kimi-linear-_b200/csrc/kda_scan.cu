@@ -1,15 +1,19 @@
 // kda_scan.cu -- gated linear recurrence h_t = a_t h_{t-1} + w_t x_t: scan, single-token
 // step, and the C entry points (include/kda_b200.h); its gradient is in kda_scan_grad.cu.
 //
-// A block walks a sequence's tiles of kTile tokens for kChannels channels: a half warp reads a
-// row, a thread has kRun tokens of kVec channels.  Each thread runs over its tokens from a
-// state of zero, which gives its piece's decay and its piece's state; the pieces are joined
-// (half warps by shuffles, warps through shared memory, and where a sequence has more
-// tiles than there are blocks otherwise, the tiles of a cluster's blocks through
-// distributed shared memory), and each thread runs over its tokens again from the state that
-// enters them.  The gradient does the same in both directions at once.  Rows come by cp.async
-// into places that only the thread that asked for them reads, kStages tiles deep, so that
-// nothing waits for a load but the tile it is for.
+// A block walks a sequence's tiles of kTile tokens for kChannels channels.  Its working warps
+// read a tile from shared memory, where TMA copies put it two or three turns ahead: a half warp has a
+// row, a thread kRun tokens of kVec channels.  Each thread runs over its tokens from a state of
+// zero, which gives its piece: a decay and a state.  The carrying warps join the pieces of the
+// tile, and of the cluster's blocks that have the sequence's neighbouring tiles (Exchange), and
+// give back the state that enters each piece; from it the threads run over their tokens again,
+// one turn later, while the carrying warps are busy with the next tile.
+//
+// Memory bounds it where there are blocks enough: 4 x 8192 x 2048, f16 with fp32 decays, 1 - a:
+// 83 us, 98 % of what a copy reaches.  A single sequence of 2048 channels has 32 blocks and their
+// clusters, 128 SMs, and is bound by the exchange of a turn: 32768 tokens, bf16: 90 us, 68 %.  Packed
+// rows cost the marks (4.5 us) and the look at them: 16000 tokens, f16: 71 us, unpacked 50.  Rows that
+// TMA cannot address are copied by their threads: 4 x 1000 x 2047: 33 us, 31 %.
 #include <cstring>
 
 #include "kda_scan.cuh"

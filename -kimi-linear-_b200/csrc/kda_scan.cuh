@@ -303,8 +303,9 @@ struct RowMask {
   }
 };
 // Calls f with whether the rows have to be looked at one by one: branches between the rows of a
-// run keep the next rows' reads behind them (one sequence of 16000 tokens of 2048 channels, f16,
-// packed: OLD).
+// run keep the next rows' reads behind them.  (Packed 16000 tokens of 2048 channels, f16: 23
+// sequences, gradient 132 us to 120; of one 130 to 113; of 128, where most tiles have a boundary,
+// 152 to 176.)
 template <bool PACKED, typename F>
 __device__ __forceinline__ void by_rows(bool plain, F f) {
   if constexpr (PACKED) {

@@ -155,3 +155,19 @@ def test_qk_entry_points_refuse():
     assert need > 0 and need % 16 == 0
     assert lib.kda_qk_bwd(P(_qk_args(dw0=FAKE, w0=FAKE, partial=FAKE, partial_floats=need - 1)),
                           None) == L.KDA_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("rope_dim", [0, 64])
+def test_mla_step_with_frequencies_refuses(rope_dim):
+    """Frequencies without a rope part, and rope parts on the CPU, before the lengths change."""
+    from test_latent_step_host import _step_args
+
+    args = _step_args(DR=rope_dim)
+    state = args[6]
+    state["inv_freq"] = torch.ones(32)
+    if rope_dim:
+        state["cache"] = pkg().LatentCache(2, 16, 128, rope_dim, device="cpu")
+        args[3], args[5] = torch.zeros(2, 1, 2, rope_dim), torch.zeros(2, 1, rope_dim)
+    with pytest.raises(RuntimeError):
+        pkg().latent.mla_step(*args, True)
+    assert state["lens"].tolist() == [3, 5]
