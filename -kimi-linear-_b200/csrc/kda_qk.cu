@@ -9,8 +9,9 @@
 //
 // Memory bounds both at length.  A lane has two groups of 16 bytes of a row (or 8, where
 // the rows are aligned to no more): those that the rotation pairs (i and i + R / 2), or
-// neighbours, so that a pair is always in one lane.  (With 8 bytes a group always, the address
-// and loop instructions were 190 for eight channels of 16 bits and bound the kernel; now 121.)
+// neighbours, so that a pair is always in one lane.  (With 8 bytes a group always, instructions,
+// 216 for eight channels of 16 bits with their rotation, bound the kernel; now 121.  4 x 8192 tokens of
+// 32 heads of 128, f16: 92 us, 89 % of what a copy reaches; gradient 136 us, 90 %.)
 // Rows of one token share its angles: a block has the heads of a few tokens side by side and
 // puts cosines and sines into shared memory for a batch of tokens.  (head_kernel)  Rows that
 // this does not fit (head sizes or strides that are no multiples of the groups) have a warp
