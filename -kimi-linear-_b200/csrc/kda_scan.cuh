@@ -3,12 +3,13 @@
 //
 // Inside a run of kRun tokens a decay is a = exp(g) in 24 bits.  Over a whole run, where it leads
 // from one run to the next, it is held as c + r, c = 1 and r = a - 1 where |sum of g| is small
-// and c = 0, r = a elsewhere: a in 24 bits is off by up to 2^-25, always to the same side for a
+// and c = 0 (or next to it), r = a elsewhere: a in 24 bits is off by up to 2^-25, always to the same side for a
 // steady g, which a state that remembers n runs adds up to n 2^-25.  (Rounding inside a run is not
 // carried on.)  c h + r h is one instruction more than a product, and two channels share each
 // (fma.f32x2), so a thread works on pairs of channels.
 #pragma once
 
+#include <cfloat>
 #include <type_traits>
 
 #include "kda_internal.cuh"
@@ -60,7 +61,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 // exp(g) = 2^(g log2 e) by the hardware's instruction: off by 2^-22 of itself, and 2^-24 |g| from
-// the rounded exponent.  What is below 2^-126 is zero.
+// the rounded exponent.  What is below 2^-126 is zero (which makes an infinite state a NaN).
 __device__ __forceinline__ float2 decay(float2 g) {
   const float2 e = __fmul2_rn(g, both(1.4426950408889634f));
   return make_float2(exp2_fast(e.x), exp2_fast(e.y));
@@ -75,11 +76,13 @@ __device__ __forceinline__ float2 decay_less_one(float2 g) {
   p = __ffma2_rn(p, g, both(1.f));
   return __fmul2_rn(p, g);
 }
-// exp(g) as c + r
+// exp(g) as c + r.  c is zero for g = -infinity alone: below kNear it is the smallest number, which
+// adds nothing to a finite state and keeps an infinite one (pass_on).
+constexpr float kLeast = 0x1p-149f;
 __device__ __forceinline__ void split_decay(float2 g, float2& c, float2& r) {
   const float2 p = decay_less_one(g), e = decay(g);
   const bool x = fabsf(g.x) < kNear, y = fabsf(g.y) < kNear;
-  c = make_float2(x ? 1.f : 0.f, y ? 1.f : 0.f);
+  c = make_float2(x ? 1.f : g.x < -FLT_MAX ? 0.f : kLeast, y ? 1.f : g.y < -FLT_MAX ? 0.f : kLeast);
   r = make_float2(x ? p.x : e.x, y ? p.y : e.y);
 }
 // 1 - exp(g) to 24 bits, a = exp(g) given
@@ -355,10 +358,14 @@ struct Piece {                       // of a pair of channels
 // not even a NaN: r = -infinity (in both channels).
 __device__ __forceinline__ float2 cut() { return both(__int_as_float((int)0xff800000)); }
 __device__ __forceinline__ bool is_cut(float2 r) { return __float_as_int(r.x) == (int)0xff800000; }
+// What a state h in front of a piece is behind it.  An infinite h stays infinite under any decay but
+// zero: c h says so, and r h, which may be infinite the other way or no number, is left out.  (The
+// choice is four cycles in a chain of some twenty a turn: 4 x 8192 x 2048 f16 85 us, without 82.)
 template <bool PACKED>
 __device__ __forceinline__ float2 pass_on(const Piece& q, float2 h) {
-  const float2 n = __ffma2_rn(q.r, h, __ffma2_rn(q.c, h, q.h));
-  return PACKED && is_cut(q.r) ? q.h : n;
+  const float2 t = __ffma2_rn(q.c, h, q.h), n = __ffma2_rn(q.r, h, t);
+  const float2 v = make_float2(isinf(h.x) ? t.x : n.x, isinf(h.y) ? t.y : n.y);
+  return PACKED && is_cut(q.r) ? q.h : v;
 }
 // `q`, and `next` behind it in the direction of the walk: (c1 + r1) (c2 + r2).  (Where c stays 1 through a tile its
 // 16 parts or less have decays of exp(-1/8) at least: of 1 + r >= exp(-2) the rounding of r
@@ -368,7 +375,7 @@ __device__ __forceinline__ void append(Piece& q, const Piece& next) {
   q.h = pass_on<PACKED>(next, q.h);
   const bool none = PACKED && (is_cut(q.r) || is_cut(next.r));
   const float2 r = __ffma2_rn(q.c, next.r, __ffma2_rn(next.c, q.r, __fmul2_rn(q.r, next.r)));
-  q.c = __fmul2_rn(q.c, next.c);
+  q.c = make_float2(fminf(q.c.x, next.c.x), fminf(q.c.y, next.c.y));   // (of 1, kLeast and 0: the product)
   q.r = none ? cut() : r;
 }
 
@@ -457,25 +464,28 @@ __device__ __forceinline__ void enter_parts(const Exchange& exchange, Patience& 
   float2 s = carry;
   const bool alone = exchange.cluster == 1;
   if (W > 1 || !alone) {
-    const Piece none{both(1.f), both(0.f), both(0.f)};
-    Piece all = none, before = none;                   // of the tile; of the shares before this warp's
+    Piece all, before{both(1.f), both(0.f), both(0.f)};   // of the tile; of the shares before this warp's (none)
+    all = part(place(0));
     if (PACKED && cuts != 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) append<PACKED>(all, part(place(i)));
+      for (int i = 1; i < N; ++i) append<PACKED>(all, part(place(i)));
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) append<false>(all, part(place(i)));
+      for (int i = 1; i < N; ++i) append<false>(all, part(place(i)));
     }
     if constexpr (W > 1) {
       pair(parts.share[warp][0], at) = all.c;
       pair(parts.share[warp][1], at) = all.r;
       pair(parts.share[warp][2], at) = all.h;
       carry_sync<SHAPE::kCarry>();
-      all = none;
+      const auto share_of = [&](int i) {
+        return Piece{pair(parts.share[i][0], at), pair(parts.share[i][1], at), pair(parts.share[i][2], at)};
+      };
+      all = share_of(0);
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
+      for (int i = 1; i < W; ++i) {
         if (i == warp) before = all;
-        append<PACKED>(all, {pair(parts.share[i][0], at), pair(parts.share[i][1], at), pair(parts.share[i][2], at)});
+        append<PACKED>(all, share_of(i));
       }
     }
     if (alone) {

@@ -1,0 +1,98 @@
+"""Gated recurrence on the GPU, beyond the ordinary: states and inputs that are not finite."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import pkg
+from oracle import recurrence_oracle as R
+from test_gpu_recurrence import BF16, F16, F32, NAMES, close, expected
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+def close_or_same(got, want, bound, what):
+    """:func:`close` where the 64-bit value is finite, and elsewhere the same infinity or a NaN."""
+    finite = torch.isfinite(want)
+    g = got.detach().cpu()
+    assert torch.isfinite(bound[finite]).all(), what
+    close(g[finite], want[finite], bound[finite], what)
+    for name, is_it in (("nan", torch.isnan), ("inf", lambda t: t == INF), ("-inf", lambda t: t == -INF)):
+        bad = is_it(g.double()) != is_it(want)
+        assert not bad.any(), (what, name, int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+def sprinkled(rows, D, tx, tg, seqs, seed):
+    """Gates down to -3 a token, some of them zero, and infinities in a tenth of the channels of each of
+    inputs, states and output gradients."""
+    gen = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    x, s0, dh, dS = rnd(rows, D), rnd(seqs, D), rnd(rows, D), rnd(seqs, D)
+    g = -torch.exp(torch.empty(rows, D).uniform_(-6.0, 1.1, generator=gen))
+    g[:, ::5] = -3.0                                   # (over 128 tokens: a decay of e^-384)
+    g[torch.rand(rows, D, generator=gen) < 0.02] = 0.0
+    for t in (x, s0, dh, dS):
+        some = torch.rand(D, generator=gen) < 0.1
+        at = torch.randint(0, t.shape[0], (D,), generator=gen)[some]
+        t[at, some] = INF * (1 - 2 * torch.randint(0, 2, (int(some.sum()),), generator=gen)).float()
+    # an infinity that a gate of -inf meets
+    if rows > 3:
+        x[rows // 3, 1], g[rows // 2, 1] = INF, -INF
+        dh[rows // 2, 2], g[rows // 3, 2] = INF, -INF
+    return x.to(tx), g.to(tg), s0, dh.to(tx), dS
+
+
+@pytest.mark.parametrize("complement", [False, True], ids=["plain", "complement"])
+@pytest.mark.parametrize("tx,tg", [(F32, F32), (F16, F32), (BF16, BF16)], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("B,T,D", [(1, 1, 64), (2, 5, 40), (1, 131, 37), (2, 700, 64), (1, 2300, 128), (100, 300, 64),
+                                   (160, 200, 64), (240, 150, 64)])
+def test_infinities(cuda_dev, B, T, D, tx, tg, complement):
+    """What 64 bits give: infinities stay until they meet their opposite or a decay of zero."""
+    kb = pkg()
+    data = sprinkled(T, B * D, tx, tg, 1, T + D)       # the batch's channels side by side
+    want, err = expected(*data, [(0, T)], complement)
+    split = lambda t: t.view(-1, B, D).transpose(0, 1)  # noqa: E731
+    dev = lambda t: split(t).contiguous().to(cuda_dev)  # noqa: E731
+    x, g, s0, dh, dS = data
+    leaves = [dev(x).requires_grad_(), dev(g).requires_grad_(), dev(s0)[:, 0].contiguous().requires_grad_()]
+    h, S = kb.gated_scan(*leaves, complement=complement)
+    got = [h, S, *torch.autograd.grad([h, S], leaves, [dev(dh), dev(dS)[:, 0]])]
+    for i, (n, v, w, e) in enumerate(zip(NAMES, got, want, err)):
+        w, e = split(w), split(e)
+        close_or_same(v, w[:, 0] if i in (1, 4) else w, e[:, 0] if i in (1, 4) else e, n)
+
+
+@pytest.mark.parametrize("tx,tg", [(F32, F32), (F16, F32), (BF16, BF16)], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("N,D,q", [(300, 128, [3, 4, 40, 40, 171, 290]), (2600, 64, [0, 1300, 1301, 2590]),
+                                   (3000, 40, list(range(0, 3000, 9))), (200, 9536, [0, 77, 200])],
+                         ids=["ragged", "long", "short", "wide"])
+def test_infinities_packed(cuda_dev, N, D, q, tx, tg):
+    kb = pkg()
+    data = sprinkled(N, D, tx, tg, len(q) - 1, N)
+    want, err = expected(*data, list(zip(q, q[1:])), D == 40)
+    x, g, s0, dh, dS = (t.to(cuda_dev) for t in data)
+    starts = torch.tensor(q, dtype=torch.int32, device=cuda_dev)
+    got = [*kb.gated_scan(x, g, s0, starts, complement=D == 40),
+           *kb.recurrence.gated_scan_backward(x, g, s0, dh, dS, starts, complement=D == 40)]
+    for n, v, w, e in zip(NAMES, got, want, err):
+        close_or_same(v, w, e, n)
+
+
+@pytest.mark.parametrize("complement", [False, True], ids=["plain", "complement"])
+def test_infinities_step(cuda_dev, complement):
+    kb = pkg()
+    gs = [0.0, -0.01, -0.5, -3.0, -80.0, -INF]
+    xs = [0.0, 1.0, INF, -INF, float("nan")]
+    ss = [1.0, INF, -INF, float("nan")]
+    grid = torch.cartesian_prod(*(torch.tensor(v) for v in (gs, xs, ss)))
+    for D in (len(grid), 1):
+        g, x, s = (c.view(-1, D) for c in grid.t())
+        want = torch.stack([R.scan(x[b:b + 1].double(), g[b:b + 1].double(), s[b].double(), complement)[1]
+                            for b in range(x.shape[0])])
+        h, S = kb.gated_step(x.contiguous().to(cuda_dev), g.contiguous().to(cuda_dev), s.contiguous().to(cuda_dev),
+                             complement=complement)
+        for v in (h, S):
+            close_or_same(v, want, torch.full_like(want, 32 * R.U), "step")
