@@ -96,3 +96,56 @@ def test_infinities_step(cuda_dev, complement):
                              complement=complement)
         for v in (h, S):
             close_or_same(v, want, torch.full_like(want, 32 * R.U), "step")
+
+
+def test_weight_of_the_complement(cuda_dev):
+    """One token from a state of zero, x = 1: the weight 1 - e^g by itself.  Nearer than 1/2 it is a
+    product g (1 + g q): U for the product, U for the sum behind it (it is above 0.78, its half step below
+    U), 0.2 U for those further in, 0.12 U for what q leaves out: 2.4 U.  Farther out it is 1 - a: a, from
+    an exponent off by 1.5 U |g| and an instruction off by 4 U, is off by (4 + 1.5 |g|) U of itself, and
+    the difference rounds once.  In the scan and in the step."""
+    kb = pkg()
+    gen = torch.Generator().manual_seed(3)
+    edges = torch.tensor([0.125, 0.25, 0.5, 1.0, 0.03125])
+    g = -torch.cat([torch.exp(torch.empty(20000).uniform_(-9.0, 3.0, generator=gen)),
+                    torch.empty(20000).uniform_(0.1, 0.6, generator=gen), edges, edges.nextafter(torch.zeros(5)),
+                    edges.nextafter(torch.ones(5))])[None]
+    want = -torch.expm1(g.double())
+    a = torch.exp(g.double())
+    bar = torch.where(g > -0.5, 2.4 * want, (4 - 1.5 * g.double()) * a + want) * R.U
+    x, gd = torch.ones_like(g, device=cuda_dev), g.to(cuda_dev)
+    outs = [*kb.gated_step(x, gd, complement=True), *kb.gated_scan(x[None], gd[None], complement=True)]
+    for got in outs:
+        err = (got.view_as(g).cpu().double() - want).abs()
+        bad = err > bar
+        assert not bad.any(), (int(bad.sum()), float((err / want / R.U)[bad].max()), g[bad][:4])
+
+
+@pytest.mark.parametrize("complement", [False, True], ids=["plain", "complement"])
+@pytest.mark.parametrize("packed", [False, True])
+def test_steady_gates_at_the_seams(cuda_dev, packed, complement):
+    """Gates that stay on either side of where a decay is held in two parts (a run of four tokens: 1/8)
+    and where 1 - a is worked out in another way (1/2), over thousands of tokens; and the same by steps."""
+    kb = pkg()
+    T = 3000
+    at = torch.tensor([1 / 32, 1 / 8, 1 / 2, 0.2499, 0.2501, 0.2])
+    g = -torch.cat([at, at.nextafter(torch.zeros(6)), at.nextafter(torch.ones(6)), at * (1 - 1e-3), at * (1 + 1e-3)])
+    g = torch.cat([g, torch.tensor([-1e-6, -3e-4])])[None].expand(T, -1).contiguous()
+    D = g.shape[1]
+    gen = torch.Generator().manual_seed(6)
+    x, dh = 1 + 0.1 * torch.randn(T, D, generator=gen), torch.randn(T, D, generator=gen)
+    q = [0, 1100, 1131, T] if packed else [0, T]
+    s0, dS = torch.randn(len(q) - 1, D, generator=gen), torch.randn(len(q) - 1, D, generator=gen)
+    want, err = expected(x, g, s0, dh, dS, list(zip(q, q[1:])), complement)
+    dev = lambda t: t.to(cuda_dev)  # noqa: E731
+    args = [dev(x), dev(g), dev(s0)] if packed else [dev(x)[None], dev(g)[None], dev(s0)]
+    starts = dev(torch.tensor(q, dtype=torch.int32)) if packed else None
+    got = [*kb.gated_scan(*args, starts, complement=complement),
+           *kb.recurrence.gated_scan_backward(*args, dev(dh).view_as(args[0]), dev(dS), starts, complement=complement)]
+    for n, v, w, e in zip(NAMES, got, want, err):
+        close(v.view_as(w), w, e, n)
+    if not packed:
+        state = dev(s0).clone()
+        for t in range(300):
+            h, _ = kb.gated_step(args[0][:, t], args[1][:, t], state, complement=complement, inplace=True)
+        close(state, want[0][299:300], err[0][299:300], "steps")
