@@ -90,12 +90,18 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       if (ch0 < p.D) carry.x = p.dstate_out[w.b * p.dso_s + ch0];
       if (ch1 < p.D) carry.y = p.dstate_out[w.b * p.dso_s + ch1];
     }
-    static_assert(Bwd::kTile % kStep == 0, "a tile starts at a checkpoint");
-    // (the first turn's tile may be missing)
+    // the states that enter the parts: a checkpoint's by a warp, the last first, so that the warps that
+    // copy and send have the least
+    static_assert(Bwd::kTile % kStep == 0 && kStep % kRun == 0, "a tile starts at a checkpoint");
+    constexpr int kSteps = Bwd::kTile / kStep, kStepParts = kStep / kRun;
+    static_assert(kSteps <= Bwd::kCarryWarps, "a warp for every checkpoint");
+    const int step = Bwd::kCarryWarps - 1 - warp;
+    // (the first turn's tile may be missing, and the last steps of its last one)
     const auto checkpoint = [&](int k) {
       float2 s = both(0.f);
-      if (k >= turns || tile_of(k) >= p.tiles) return s;
-      const float* row = p.ckpt + ((int64_t)w.b * p.steps + tile_of(k) * (Bwd::kTile / kStep)) * p.D;
+      const int i = tile_of(k) * kSteps + step;
+      if (k >= turns || step >= kSteps || i >= p.steps) return s;
+      const float* row = p.ckpt + ((int64_t)w.b * p.steps + i) * p.D;
       if (ch0 < p.D) s.x = row[ch0];
       if (ch1 < p.D) s.y = row[ch1];
       return s;
@@ -120,10 +126,10 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       }
       Parts<Bwd>& parts = sh.parts[buf];
       enter_parts<PACKED, true>(exchange, patience, k, parts, sh.back[buf], cuts, carry, warp, at, [&] {
-        // the states that enter the parts, by the last warp
-        if (warp != Bwd::kCarryWarps - 1) return;
+        if (step >= kSteps) return;
 #pragma unroll
-        for (int i = 0; i < Bwd::kParts; ++i) {
+        for (int j = 0; j < kStepParts; ++j) {
+          const int i = step * kStepParts + j;
           const Piece q{pair(parts.c[i], at), PACKED && (starts >> i & 1) ? cut() : pair(parts.r[i], at),
                         pair(parts.h[i], at)};
           pair(parts.h[i], at) = state;
