@@ -39,6 +39,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -253,6 +254,13 @@ def kda_recurrent(q, k, v, g, beta, state=None, state_dtype=None, *, inplace=Fal
 def _needs_grad(*ts):
     return torch.is_grad_enabled() and any(
         isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
+
+
+def _no_tangents(fn, *ts):
+    """Refuses forward-mode dual tensors, whose tangents the kernels would drop without a word."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{fn}: there is no forward-mode derivative; pass the primal of a dual tensor")
 
 
 class _KdaFunction(torch.autograd.Function):

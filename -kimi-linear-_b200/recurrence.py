@@ -25,7 +25,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DT, _check_tensors, _launch, _needs_grad
+from .ops import _DT, _check_tensors, _launch, _needs_grad, _no_tangents
 
 _NONE2, _NONE3 = (0, 0), (0, 0, 0)
 
@@ -58,6 +58,7 @@ def _args(B, T, x, g, complement, xs, gs, state=_NONE2, q_start=0, slots=0, h=_N
 
 def _check(fn, x, g, state, rows, others=()):
     """Device of the operands, after checks of types and shapes."""
+    _no_tangents(fn, x, g, state, *(t for _, t in others))
     dev = _check_tensors(fn, [("x", x), ("g", g), ("state", state), *others])
     if g is None or x.shape != g.shape:
         raise RuntimeError(f"{fn}: x {tuple(x.shape)} and g "

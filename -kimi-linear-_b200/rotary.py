@@ -20,7 +20,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DT, _check_tensors, _launch, _needs_grad
+from .ops import _DT, _check_tensors, _launch, _needs_grad, _no_tangents
 
 NORMS = {None: _lib.NORM_NONE, "rms": _lib.NORM_RMS, "l2": _lib.NORM_L2}
 MAX_D = 512
@@ -48,6 +48,7 @@ _NONE2 = _two(None, None)
 
 
 def _check(fn, q, k, wq, wk, norm, eps, positions, inv_freq, others=()):
+    _no_tangents(fn, q, k, wq, wk, inv_freq, *(t for _, t in others))
     dev = _check_tensors(fn, [("q", q), ("k", k), ("q_weight", wq), ("k_weight", wk), *others])
     if q is None or q.dim() not in (3, 4):
         raise RuntimeError(f"{fn}: expected q [B, T, H, D] or [N, H, D]")

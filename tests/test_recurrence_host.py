@@ -171,3 +171,33 @@ def test_mla_step_with_frequencies_refuses(rope_dim):
     with pytest.raises(RuntimeError):
         pkg().latent.mla_step(*args, True)
     assert state["lens"].tolist() == [3, 5]
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor that needs no gradient would come back without its tangent."""
+    from torch.autograd import forward_ad
+
+    kb = pkg()
+    z = lambda *s: torch.zeros(*s)  # noqa: E731
+    calls = [
+        (kb.gated_scan, [z(1, 2, 4), z(1, 2, 4), z(1, 4)]),
+        (kb.recurrence.gated_scan_backward, [z(1, 2, 4), z(1, 2, 4), z(1, 4), z(1, 2, 4), z(1, 4)]),
+        (kb.gated_step, [z(2, 4), z(2, 4), z(2, 4)]),
+        (kb.qk_norm_rope, [z(1, 2, 3, 4), z(1, 2, 1, 4), z(4), z(4)]),
+        (kb.rotary.qk_norm_rope_backward, [z(1, 2, 3, 4), z(1, 2, 1, 4), z(1, 2, 3, 4), z(1, 2, 1, 4), z(4), z(4)]),
+    ]
+    for fn, args in calls:
+        for i in range(len(args)):
+            with forward_ad.dual_level():
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    fn(*dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(lambda t: fn(t, *args[1:])[0], (args[0],), (torch.ones_like(args[0]),))
+        # inside a level, tensors without a tangent get as far as without one (no CPU path)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="CUDA"):
+            fn(*args)
+    with forward_ad.dual_level():
+        freq = forward_ad.make_dual(z(2), torch.ones(2))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            kb.qk_norm_rope(z(1, 2, 3, 4), inv_freq=freq)
