@@ -370,7 +370,7 @@ int validate(const KdaScanArgs* a, Pass pass) {
   const bool tokens = a->T > 0 && (a->B > 0 || a->q_start != nullptr);
   if (tokens && (!a->x || !a->g || (pass != Pass::kBackward && !a->h))) return KDA_ERR_NULL_POINTER;
   if (a->B > 0 && pass != Pass::kBackward && !a->state_out) return KDA_ERR_NULL_POINTER;
-  if (tokens && pass == Pass::kBackward && a->B > 0 && !a->ckpt) return KDA_ERR_NULL_POINTER;
+  if (tokens && pass == Pass::kBackward && !a->ckpt) return KDA_ERR_NULL_POINTER;
   if (misaligned(a->x, xs) || misaligned(a->h, xs) || misaligned(a->dh, xs) || misaligned(a->dx, xs) ||
       misaligned(a->g, gs) || misaligned(a->dg, gs) || misaligned(a->state_in, 4) ||
       misaligned(a->state_out, 4) || misaligned(a->dstate_out, 4) || misaligned(a->dstate_in, 4) ||

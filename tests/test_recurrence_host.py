@@ -201,3 +201,12 @@ def test_forward_mode_tangents_are_refused():
         freq = forward_ad.make_dual(z(2), torch.ones(2))
         with pytest.raises(RuntimeError, match="forward-mode"):
             kb.qk_norm_rope(z(1, 2, 3, 4), inv_freq=freq)
+
+
+def test_backward_wants_checkpoints_for_rows_without_sequences():
+    """Packed rows of no sequence are walked too, from the checkpoints."""
+    L = pkg()._lib
+    lib = L.load()
+    packed = dict(B=0, q_start=FAKE, workspace=FAKE, workspace_bytes=1 << 20, ckpt=None)
+    assert lib.kda_scan_bwd(ctypes.byref(_scan_args(**packed)), None) == L.KDA_ERR_NULL_POINTER
+    assert lib.kda_scan_bwd(ctypes.byref(_scan_args(**packed, T=0)), None) == L.KDA_OK
