@@ -322,7 +322,8 @@ def mla_step(module, x, q_nope, q_rope, c_kv, k_rope, state, use_cache):
     the pages for ``lens + T`` tokens must be in the table.  With ``inv_freq`` fp32
     ``[R / 2]`` in ``state``, ``q_rope`` and ``k_rope`` come before their rotation and are
     rotated by their tokens' positions, ``lens`` and on, read on the device (by
-    :func:`rotary.qk_norm_rope`; ``interleaved`` in ``state`` as there).  ``lens`` is advanced
+    :func:`rotary.qk_norm_rope`; ``interleaved`` in ``state`` as there; parts of two types
+    in fp32).  ``lens`` is advanced
     by ``T`` on the device (a step that raises takes that back), the tokens are
     appended, the queries folded into the latent space by the module's own
     ``kv_b_proj`` weight (cast on every step unless it is in the cache's type),
@@ -341,6 +342,8 @@ def mla_step(module, x, q_nope, q_rope, c_kv, k_rope, state, use_cache):
     if inv_freq is not None:
         if not cache.rope_dim:
             raise RuntimeError("mla_step: inv_freq for a cache without a rope part")
+        if q_rope.dtype != k_rope.dtype or q_rope.dtype not in _DT:
+            q_rope, k_rope = q_rope.float(), k_rope.float()
         q_rope, k_rope = qk_norm_rope(q_rope.reshape(B, T, H, cache.rope_dim),
                                       k_rope.reshape(B, T, 1, cache.rope_dim), norm=None, positions=lens,
                                       inv_freq=inv_freq, interleaved=state.get("interleaved", False))

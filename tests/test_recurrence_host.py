@@ -210,3 +210,26 @@ def test_backward_wants_checkpoints_for_rows_without_sequences():
     packed = dict(B=0, q_start=FAKE, workspace=FAKE, workspace_bytes=1 << 20, ckpt=None)
     assert lib.kda_scan_bwd(ctypes.byref(_scan_args(**packed)), None) == L.KDA_ERR_NULL_POINTER
     assert lib.kda_scan_bwd(ctypes.byref(_scan_args(**packed, T=0)), None) == L.KDA_OK
+
+
+@pytest.mark.parametrize("tq,tk", [(torch.float32, torch.bfloat16), (torch.float16, torch.bfloat16),
+                                   (torch.float64, torch.float64), (torch.bfloat16, torch.bfloat16)])
+def test_mla_step_rotates_in_one_type(tq, tk, monkeypatch):
+    """Rope parts of two types, which a step without frequencies takes, reach the rotation in one."""
+    from test_latent_step_host import _step_args
+
+    kb, seen = pkg(), []
+
+    def rotation(q, k, **kw):
+        seen.append((q.dtype, k.dtype))
+        raise InterruptedError
+
+    monkeypatch.setattr(kb.latent, "qk_norm_rope", rotation)
+    args = _step_args(DR=64)
+    args[6].update(inv_freq=torch.ones(32), cache=kb.LatentCache(2, 16, 128, 64, device="cpu"))
+    args[3], args[5] = torch.zeros(2, 1, 2, 64, dtype=tq), torch.zeros(2, 1, 64, dtype=tk)
+    with pytest.raises(InterruptedError):
+        kb.latent.mla_step(*args, True)
+    same = tq == tk and tq != torch.float64
+    assert seen == [(tq, tk) if same else (torch.float32,) * 2]
+    assert args[6]["lens"].tolist() == [3, 5]
