@@ -89,6 +89,13 @@ def _batch(fn, x, q_start):
     return q_start.shape[0] - 1
 
 
+def _read_as_float(state):
+    """A floating state of a type that the kernels do not take, in fp32."""
+    if isinstance(state, torch.Tensor) and state.is_floating_point() and state.dtype not in _DT:
+        return state.float()
+    return state
+
+
 def _workspace(a, q_start):
     """Scratch for a packed batch, set in ``a``; the caller holds it through the call."""
     if q_start is None:
@@ -130,9 +137,10 @@ def gated_scan(x, g, initial_state=None, q_start=None, *, complement=False):
     no sequence and give zeros; a sequence without rows gives its initial state.
 
     Differentiable in ``x``, ``g`` and ``initial_state``.  ``x`` f32, f16 or bf16,
-    ``g`` fp32 or ``x``'s type.  A state of any type is read as fp32."""
+    ``g`` fp32 or ``x``'s type.  A state of any floating type is read as fp32."""
     fn = "gated_scan"
     B = _batch(fn, x, q_start)
+    initial_state = _read_as_float(initial_state)
     if _needs_grad(x, g, initial_state):
         with torch.no_grad():
             _check(fn, x, g, initial_state, B)
@@ -189,13 +197,15 @@ def gated_scan_backward(x, g, initial_state, dh, dS, q_start=None, *, complement
     the call that it differentiates."""
     fn = "gated_scan_backward"
     B = _batch(fn, x, q_start)
+    given, initial_state = initial_state, _read_as_float(initial_state)
     _check(fn, x, g, initial_state, B, [("dh", dh), ("dS", dS)])
     if dh is not None and dh.shape != x.shape:
         raise RuntimeError(f"{fn}: dh shape {tuple(dh.shape)} != {tuple(x.shape)}")
     if dS is not None and tuple(dS.shape) != (B, x.shape[-1]):
         raise RuntimeError(f"{fn}: dS shape {tuple(dS.shape)} != {(B, x.shape[-1])}")
     ckpt = _forward(x, g, initial_state, q_start, complement, True)[2]
-    return _backward(x, g, initial_state, q_start, bool(complement), ckpt, dh, dS, (True, True, True))
+    dx, dg, dstate = _backward(x, g, initial_state, q_start, bool(complement), ckpt, dh, dS, (True, True, True))
+    return dx, dg, None if dstate is None else dstate.to(given.dtype)
 
 
 def gated_step(x, g, state=None, slots=None, *, complement=False, inplace=False):

@@ -149,3 +149,26 @@ def test_steady_gates_at_the_seams(cuda_dev, packed, complement):
         for t in range(300):
             h, _ = kb.gated_step(args[0][:, t], args[1][:, t], state, complement=complement, inplace=True)
         close(state, want[0][299:300], err[0][299:300], "steps")
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_state_of_64_bits(cuda_dev, packed):
+    """Read as fp32, its gradient in its own type."""
+    kb = pkg()
+    gen = torch.Generator().manual_seed(2)
+    x, g = torch.randn(2, 50, 24, generator=gen), -torch.rand(2, 50, 24, generator=gen)
+    x, g, s0 = x.to(cuda_dev), g.to(cuda_dev), torch.randn(2, 24, generator=gen, dtype=torch.float64).to(cuda_dev)
+    q = torch.tensor([0, 50, 100], dtype=torch.int32, device=cuda_dev) if packed else None
+    if packed:
+        x, g = x.view(100, 24), g.view(100, 24)
+    want = kb.gated_scan(x, g, s0.float(), q)
+    assert all(torch.equal(a, b) for a, b in zip(kb.gated_scan(x, g, s0, q), want))
+    ones = [torch.ones_like(t) for t in want]
+    ref = kb.recurrence.gated_scan_backward(x, g, s0.float(), *ones, q)
+    got = kb.recurrence.gated_scan_backward(x, g, s0, *ones, q)
+    leaf = s0.clone().requires_grad_()
+    auto, = torch.autograd.grad(kb.gated_scan(x, g, leaf, q), leaf, ones)
+    assert got[2].dtype == auto.dtype == torch.float64
+    assert all(torch.equal(a, b.to(a.dtype)) for a, b in zip((*got, auto), (*ref, ref[2])))
+    with pytest.raises(TypeError):
+        kb.gated_scan(x, g, s0.long(), q)
