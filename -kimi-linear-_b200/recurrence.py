@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .ops import _DT, _check_tensors, _launch, _needs_grad, _no_tangents
@@ -255,4 +256,6 @@ def gated_step(x, g, state=None, slots=None, *, complement=False, inplace=False)
               _NONE2 if state is None else _rows(state), 0, 0 if slots is None else slots.data_ptr(),
               (h.data_ptr(), D, 0), _rows(S), num_states=0 if slots is None else rows, scatter=1 if inplace else 0)
     _launch(fn, _lib.load().kda_scan_step, a, dev)
+    if inplace:
+        increment_version(state)     # (autograd notices where it has kept the old states)
     return h, S

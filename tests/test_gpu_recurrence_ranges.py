@@ -172,3 +172,27 @@ def test_state_of_64_bits(cuda_dev, packed):
     assert all(torch.equal(a, b.to(a.dtype)) for a, b in zip((*got, auto), (*ref, ref[2])))
     with pytest.raises(TypeError):
         kb.gated_scan(x, g, s0.long(), q)
+
+
+def test_step_in_place_is_seen_by_autograd(cuda_dev):
+    """A scan's backward pass reads its initial states: written over by a step, it refuses as for any other
+    operation in place; a step that writes elsewhere leaves it alone."""
+    kb = pkg()
+    gen = torch.Generator(device=cuda_dev).manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=cuda_dev)  # noqa: E731
+    x, g, pool = rnd(60, 16).requires_grad_(), -rnd(60, 16).abs(), rnd(3, 16)
+    q = torch.tensor([0, 20, 20, 60], dtype=torch.int32, device=cuda_dev)
+    for inplace in (False, True):
+        h, _ = kb.gated_scan(x, g, pool, q)
+        with torch.no_grad():
+            before = pool._version
+            _, S = kb.gated_step(x[:3], g[:3], pool, inplace=inplace)
+        assert (pool._version > before) == inplace and (S is pool) == inplace
+        if inplace:
+            with pytest.raises(RuntimeError, match="inplace"):
+                h.sum().backward()
+        else:
+            h.sum().backward()
+    with torch.inference_mode():
+        held = rnd(3, 16)
+        kb.gated_step(x[:3], g[:3], held, inplace=True)
