@@ -248,7 +248,7 @@ class KdaScanArgs(ctypes.Structure):
         ("x_dtype", ctypes.c_int32), ("g_dtype", ctypes.c_int32),
         ("complement", ctypes.c_int32),
         ("num_states", ctypes.c_int32), ("scatter", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
+        ("hasty", ctypes.c_int32),
         ("x", ctypes.c_void_p), ("x_stride", _I64x2),
         ("g", ctypes.c_void_p), ("g_stride", _I64x2),
         ("state_in", ctypes.c_void_p), ("state_in_stride", ctypes.c_int64),

@@ -76,6 +76,7 @@ struct Shared {
   Parts<SHAPE> parts[2];             // of two turns
   uint64_t full[kMaxSlots], exchange[2];
   TileRows<SHAPE> rows;              // packed
+  int lost;                          // a worker has gone on without its rows
 };
 
 template <typename TX, typename TG, typename Fwd, bool WIDE, bool PACKED, bool COMPLEMENT>
@@ -90,11 +91,12 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
   Shared<Fwd>& sh = *reinterpret_cast<Shared<Fwd>*>(smem + XRing::kBytes + GRing::kBytes);
   const Place w = my_place<WIDE>(p);
   const Exchange exchange(sh.exchange, reinterpret_cast<float*>(&sh + 1), p, w.rank);
-  Patience patience(&g_scan_device_error);
+  Patience patience(&g_scan_device_error, &sh.lost, p.hasty);
   const int turns = (p.tiles + p.cluster - 1) / p.cluster;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) ptx::mbar_init(sh.full + i, 1);
     exchange.init();
+    sh.lost = 0;
     ptx::fence_mbar_init();
   }
   const auto first_row = [&](int k, int part) { return (k * p.cluster + w.rank) * Fwd::kTile + part * kRun; };
@@ -112,8 +114,10 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     const int at = threadIdx.x % 32, warp = (threadIdx.x - Fwd::kWork) / 32;
     const int ch0 = w.block_c + shared_channel<WIDE>(2 * at), ch1 = w.block_c + shared_channel<WIDE>(2 * at + 1);
     const bool copies = WIDE && warp == 0 && at == 0;
+    int asked = 0;                   // turns whose copies have been asked for
     const auto copy = [&](int k) {
       const int tile = k * p.cluster + w.rank;
+      asked = k + 1;
       if (tile >= p.tiles) return;
       uint64_t* bar = sh.full + k % kSlots;
       ptx::mbar_arrive_expect_tx(bar, XRing::kTileBytes + GRing::kTileBytes);
@@ -137,7 +141,7 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       pieces_wait(buf, Fwd::kThreads);
       if (fetches) sh.rows.bits[(k + 2) & 3][at] = ahead;
       // the workers have read the rows of turn k
-      if (copies && patience.limit) copy(k + kSlots);
+      if (copies && !patience.gone && *const_cast<volatile int*>(&sh.lost) == 0) copy(k + kSlots);
       uint32_t cuts = 0;
       if constexpr (PACKED) {
         cuts = sh.rows.starts(k);
@@ -164,9 +168,8 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
       if (ch1 < p.D) p.state_out[w.b * p.so_s + ch1] = carry.y;
     }
     if (copies) {                    // (a worker may have given up)
-      Patience landed(&g_scan_device_error);
-      for (int k = max(turns - kSlots, 0); k < turns; ++k)
-        if (k * p.cluster + w.rank < p.tiles) landed.wait(sh.full + k % kSlots, k / kSlots & 1);
+      for (int k = max(asked - kSlots, 0); k < asked; ++k)
+        if (k * p.cluster + w.rank < p.tiles) patience.land(sh.full + k % kSlots, k / kSlots & 1);
     }
   } else {
     const int part = threadIdx.x / kLanes, row0 = part * kRun;
@@ -262,6 +265,7 @@ scan_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map, const
     }
   }
   exchange.barrier();                // no block leaves while another may still send to it
+  if (exchange.cluster > 1) patience.linger();
 }
 
 template <typename Fwd>
@@ -402,6 +406,7 @@ ScanParams to_params(const KdaScanArgs* a) {
   p.dg = a->dg; std::memcpy(p.dg_s, a->dg_stride, sizeof(p.dg_s));
   p.dstate_in = a->dstate_in; p.dsi_s = a->dstate_in_stride;
   p.cluster = 1;
+  p.hasty = a->hasty != 0;
   p.slots = a->slots; p.num_states = a->num_states; p.scatter = a->scatter != 0;
   return p;
 }

@@ -49,6 +49,7 @@ struct ScanParams {
   float* dstate_in; int64_t dsi_s;
   const Marks* marks;               // packed: of all rows, made by mark_kernel
   int cluster;                      // blocks that share a sequence's tiles
+  bool hasty;                       // waits give up at once
   // step
   const int* slots; int num_states; bool scatter;
 };
@@ -123,6 +124,7 @@ constexpr int kRun = 4;                       // tokens of a thread in a tile
 constexpr int kMaxCluster = 8;
 constexpr int kSms = 148;
 constexpr uint64_t kWaitNs = 2000000000;      // a wait that takes longer gives up (device error word 9)
+constexpr uint64_t kLingerNs = 1000000;
 
 // A block: WORK warps that do the tokens, and CARRY warps that carry states from tile to tile
 // (a lane has a pair of channels, a warp its share of the parts).
@@ -153,18 +155,33 @@ __device__ __forceinline__ bool here(uint64_t* bar, uint32_t parity) {
 // waits no more.
 struct Patience {
   int* error;
-  uint64_t limit;
-  __device__ explicit Patience(int* error_) : error(error_), limit(kWaitNs) {}
+  int* lost;                         // the block's: rows that have not come must not be asked for again
+  bool gone;                         // given up
+  __device__ Patience(int* error_, int* lost_, bool gone_) : error(error_), lost(lost_), gone(gone_) {}
   __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
     if (here(bar, parity)) return;
     const uint64_t start = ptx::globaltimer_ns();
-    while (!here(bar, parity)) {
-      if (ptx::globaltimer_ns() - start >= limit) {
-        *error = kErrWait;
-        limit = 0;
-        return;
-      }
+    while (!gone && !here(bar, parity)) gone = ptx::globaltimer_ns() - start >= kWaitNs;
+    if (gone) {
+      *error = kErrWait;
+      *lost = 1;
     }
+  }
+  // what is in flight as the block leaves, whoever has given up
+  __device__ __forceinline__ void land(uint64_t* bar, uint32_t parity) {
+    const uint64_t start = ptx::globaltimer_ns();
+    while (!here(bar, parity)) {
+      if (ptx::globaltimer_ns() - start < kWaitNs) continue;
+      *error = kErrWait;
+      return;
+    }
+  }
+  // One that has given up stays, behind the cluster's last barrier, until what the others had sent
+  // by then has landed in its block's memory: no barrier of its own counts that any more.
+  __device__ __forceinline__ void linger() const {
+    if (!gone) return;
+    const uint64_t start = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - start < kLingerNs) {}
   }
 };
 // a barrier of the carrying threads alone
@@ -439,10 +456,11 @@ struct Exchange {
     float* s = row(turn, i);
     return {pair(s, at), pair(s + kChannels, at), pair(s + 2 * kChannels, at)};
   }
-  // carrying warp `warp` of `warps` sends to blocks warp, warp + warps, ...
-  __device__ void send(int turn, int warp, int warps, int at, const Piece& q, bool arm) const {
+  // carrying warp `warp` of `warps` sends to blocks warp, warp + warps, ...  (A thread that has given up
+  // must not: the turn's barriers might still be in use by the turn before the last.)
+  __device__ void send(int turn, int warp, int warps, int at, const Piece& q) const {
     uint64_t* bar = full + (turn & 1);
-    if (warp == 0 && at == 0 && arm) ptx::mbar_arrive_expect_tx(bar, cluster * kRowFloats * sizeof(float));
+    if (warp == 0 && at == 0) ptx::mbar_arrive_expect_tx(bar, cluster * kRowFloats * sizeof(float));
     const uint32_t dst = ptx::smem_u32(&pair(row(turn, rank), at)), mine = ptx::smem_u32(bar);
     for (int i = warp; i < cluster; i += warps) {
       uint32_t d, m;
@@ -504,7 +522,7 @@ __device__ __forceinline__ void enter_parts(const Exchange& exchange, Patience& 
       carry = pass_on<PACKED>(all, carry);
       meanwhile();
     } else {
-      exchange.send(turn, warp, W, at, all, patience.limit != 0);
+      if (!patience.gone) exchange.send(turn, warp, W, at, all);
       meanwhile();
       patience.wait(exchange.full + (turn & 1), (turn >> 1) & 1);
       Piece others[kMaxCluster];

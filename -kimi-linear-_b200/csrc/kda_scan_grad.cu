@@ -33,6 +33,7 @@ struct Shared {
   float back[2][SHAPE::kParts][kChannels];   // the parts' gradients from zero, then what enters them
   uint64_t full[kXSlots], exchange[2];
   TileRows<SHAPE> rows;                      // packed
+  int lost;                                  // a worker has gone on without its rows
 };
 
 template <typename TX, typename TG, typename Bwd, bool WIDE, bool PACKED, bool COMPLEMENT>
@@ -47,11 +48,12 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
   Shared<Bwd>& sh = *reinterpret_cast<Shared<Bwd>*>(smem + 2 * XRing::kBytes + GRing::kBytes);
   const Place w = my_place<WIDE>(p);
   const Exchange exchange(sh.exchange, reinterpret_cast<float*>(&sh + 1), p, w.rank);
-  Patience patience(&g_grad_device_error);
+  Patience patience(&g_grad_device_error, &sh.lost, p.hasty);
   const int turns = (p.tiles + p.cluster - 1) / p.cluster;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kXSlots; ++i) ptx::mbar_init(sh.full + i, 1);
     exchange.init();
+    sh.lost = 0;
     ptx::fence_mbar_init();
   }
   const auto tile_of = [&](int k) { return (turns - 1 - k) * p.cluster + w.rank; };
@@ -70,8 +72,10 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     const int at = threadIdx.x % 32, warp = (threadIdx.x - Bwd::kWork) / 32;
     const int ch0 = w.block_c + shared_channel<WIDE>(2 * at), ch1 = w.block_c + shared_channel<WIDE>(2 * at + 1);
     const bool copies = WIDE && warp == 0 && at == 0;
+    int asked = 0;                   // turns whose copies have been asked for
     const auto copy = [&](int k) {
       if (k >= turns) return;
+      asked = k + 1;
       const int tile = tile_of(k);
       uint64_t* bar = sh.full + k % kXSlots;
       if (tile >= p.tiles) {         // (the first turn's may be missing: its phase passes all the same)
@@ -117,7 +121,7 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       pieces_wait(buf, Bwd::kThreads);
       if (fetches) sh.rows.bits[(k + 2) & 3][at] = ahead;
       // the workers are done with the gates of turn k and with the other rows of turn k - 2
-      if (copies && patience.limit) copy(k + 2);
+      if (copies && !patience.gone && *const_cast<volatile int*>(&sh.lost) == 0) copy(k + 2);
       next = checkpoint(k + 1);
       uint32_t cuts = 0, starts = 0;
       if constexpr (PACKED) {
@@ -143,8 +147,7 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
       if (ch1 < p.D) p.dstate_in[w.b * p.dsi_s + ch1] = carry.y;
     }
     if (copies) {                    // (a worker may have given up)
-      Patience landed(&g_grad_device_error);
-      for (int k = max(turns - 2, 0); k < turns; ++k) landed.wait(sh.full + k % kXSlots, k / kXSlots & 1);
+      for (int k = max(asked - kXSlots, 0); k < asked; ++k) patience.land(sh.full + k % kXSlots, k / kXSlots & 1);
     }
   } else {
     const int part = threadIdx.x / kLanes, row0 = part * kRun;
@@ -287,6 +290,7 @@ scan_grad_kernel(const ScanParams p, const __grid_constant__ CUtensorMap x_map,
     }
   }
   exchange.barrier();                // no block leaves while another may still send to it
+  if (exchange.cluster > 1) patience.linger();
 }
 
 }  // namespace

@@ -442,7 +442,8 @@ typedef struct KdaScanArgs {
   int32_t x_dtype, g_dtype;    /* g: fp32 or x's type */
   int32_t complement;
   int32_t num_states, scatter; /* step only */
-  int32_t reserved;
+  int32_t hasty;               /* 0; 1: waits inside kda_scan_fwd and kda_scan_bwd give up at once, not after 2 s
+                                * (their error path, for tests) */
   /* strides in elements (batch, token), unit channel stride */
   const void* x;  int64_t x_stride[2];
   const void* g;  int64_t g_stride[2];

@@ -196,3 +196,40 @@ def test_step_in_place_is_seen_by_autograd(cuda_dev):
     with torch.inference_mode():
         held = rnd(3, 16)
         kb.gated_step(x[:3], g[:3], held, inplace=True)
+
+
+@pytest.mark.parametrize("tx", [F32, BF16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("B,T,D,seqs", [(1, 3000, 128, 0), (2, 700, 64, 0), (100, 700, 64, 0), (160, 300, 64, 0),
+                                        (240, 300, 64, 0), (1, 2600, 64, 7), (1, 1000, 37, 0)])
+def test_waits_that_give_up(cuda_dev, monkeypatch, B, T, D, seqs, tx):
+    """Told not to wait, the kernels give up: the calls return, the error word says so, and the next calls
+    give what they gave before."""
+    kb = pkg()
+    kb.device_error()
+    gen = torch.Generator(device=cuda_dev).manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=cuda_dev)  # noqa: E731
+    rows = (T, D) if seqs else (B, T, D)
+    x, g, dh = rnd(rows).to(tx), -rnd(rows).abs(), rnd(rows).to(tx)
+    s0, dS = rnd(seqs or B, D), rnd(seqs or B, D)
+    q = torch.linspace(0, T, seqs + 1).int().to(cuda_dev) if seqs else None
+
+    def both():
+        leaves = [t.clone().requires_grad_() for t in (x, g, s0)]
+        h, S = kb.gated_scan(*leaves, q)
+        return [h, S, *torch.autograd.grad([h, S], leaves, [dh, dS])]
+
+    want, plain = both(), kb.recurrence._args
+
+    def hasty(*a, **kw):
+        out = plain(*a, **kw)
+        out.hasty = 1
+        return out
+
+    monkeypatch.setattr(kb.recurrence, "_args", hasty)
+    for call in (lambda: kb.gated_scan(x, g, s0, q),
+                 lambda: kb.recurrence._backward(x, g, s0, q, False, rnd(2 * B * T * D), dh, dS, (True,) * 3)):
+        call()
+        assert kb.device_error() == 9
+    monkeypatch.setattr(kb.recurrence, "_args", plain)
+    assert all(torch.equal(a, b) for a, b in zip(both(), want))
+    assert kb.device_error() == 0
