@@ -233,3 +233,71 @@ def test_waits_that_give_up(cuda_dev, monkeypatch, B, T, D, seqs, tx):
     monkeypatch.setattr(kb.recurrence, "_args", plain)
     assert all(torch.equal(a, b) for a, b in zip(both(), want))
     assert kb.device_error() == 0
+
+
+@pytest.mark.parametrize("tx,tg", [(F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("complement", [False, True], ids=["plain", "complement"])
+@pytest.mark.parametrize("B,T,D,packed", [(1, 8 * 128 * 5 + 37, 64, False), (1, 4500, 2048, False), (40, 900, 128, False),
+                                          (100, 1021, 64, False), (1, 8 * 128 * 5 + 37, 72, True)])
+def test_long_shape_past_its_ring(cuda_dev, B, T, D, packed, complement, tx, tg):
+    """Sequences of 16 bits that a block goes through in more turns than it has rows in shared memory for: in
+    clusters of eight, four, one; rows by TMA, and 64 channels with a rest of eight.  (Subsets of the channels go
+    to the oracle: they do not meet.)"""
+    kb = pkg()
+    # (a few channels at the edges and in between)
+    some = sorted({0, 1, 31, 63, D - 1, D // 2, 64 % D, 65 % D})
+    gen = torch.Generator(device=cuda_dev).manual_seed(T + D)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=cuda_dev)  # noqa: E731
+    x, dh = rnd(B, T, D).to(tx), rnd(B, T, D).to(tx)
+    g = (-torch.exp(torch.empty(B, T, D, device=cuda_dev).uniform_(-9.0, 1.5, generator=gen))).to(tg)
+    s0, dS = rnd(B, D), rnd(B, D)
+    cuts = [3, 700, 700, 3000, T - 11] if packed else None
+    if packed:
+        s0, dS = rnd(4, D), rnd(4, D)
+    rows = (T, D) if packed else (B, T, D)
+    starts = torch.tensor(cuts, dtype=torch.int32, device=cuda_dev) if packed else None
+    leaves = [x.view(rows).requires_grad_(), g.view(rows).requires_grad_(), s0.requires_grad_()]
+    h, S = kb.gated_scan(*leaves, starts, complement=complement)
+    got = [h, S, *torch.autograd.grad([h, S], leaves, [dh.view(rows), dS])]
+    for b in ([0] if packed else sorted({0, B // 2, B - 1})):
+        pick = lambda t: t.detach().cpu()[..., some]  # noqa: E731
+        seq = lambda t: pick(t.view(B, T, D)[b])  # noqa: E731
+        st = (lambda t: pick(t)) if packed else (lambda t: pick(t[b:b + 1]))  # noqa: E731
+        want, err = expected(seq(x), seq(g), st(s0), seq(dh), st(dS), list(zip(cuts, cuts[1:])) if packed else [(0, T)],
+                             complement)
+        for i, (n, v, w, e) in enumerate(zip(NAMES, got, want, err)):
+            close(st(v) if i in (1, 4) else seq(v), w, e, n)
+
+
+def test_empty_calls(cuda_dev):
+    """Shapes, and states that go through, one by one."""
+    kb = pkg()
+    for B, T, D in ((0, 5, 4), (2, 0, 4), (2, 5, 0), (0, 0, 4), (2, 0, 0)):
+        x, s0 = torch.zeros(B, T, D, device=cuda_dev), torch.randn(B, D, device=cuda_dev)
+        h, S = kb.gated_scan(x, x, s0)
+        assert h.shape == (B, T, D)
+        assert S.shape == (B, D)
+        dx, dg, ds = kb.recurrence.gated_scan_backward(x, x, s0, x, s0)
+        assert dx.shape == dg.shape == (B, T, D)
+        assert ds.shape == (B, D)
+        if T == 0:
+            assert torch.equal(S, s0)
+            assert torch.equal(ds, s0)
+        assert all(t.numel() == 0 for t in (h, dx, dg))
+
+
+def test_refusals_without_a_gradient(cuda_dev):
+    """The same refusals on the way that records nothing, and on the one that does."""
+    kb = pkg()
+    z = lambda *s, dt=F32: torch.zeros(*s, dtype=dt, device=cuda_dev)  # noqa: E731
+    x, s, q = z(2, 5, 4), z(2, 4), torch.zeros(3, dtype=torch.int32, device=cuda_dev)
+    cases = [((x, z(2, 5, 3)), RuntimeError), ((x, x, z(2, 3)), RuntimeError), ((x, x, z(3, 4)), RuntimeError),
+             ((z(5, 4), z(5, 4)), RuntimeError), ((x, x, s, q), RuntimeError), ((x, z(2, 5, 4, dt=F16)), TypeError),
+             ((z(5, 4), z(5, 4), s, q.long()), RuntimeError), ((z(5, 4), z(5, 4), s, q.cpu()), RuntimeError),
+             ((x, x.cpu()), RuntimeError), ((x, x, s.cpu()), RuntimeError)]
+    for args, exc in cases:
+        assert not any(t.requires_grad for t in args)
+        with pytest.raises(exc):
+            kb.gated_scan(*args)
+        with pytest.raises(exc):
+            kb.gated_scan(args[0].clone().requires_grad_(), *args[1:])
