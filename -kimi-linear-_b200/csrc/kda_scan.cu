@@ -10,9 +10,9 @@
 // one turn later, while the carrying warps are busy with the next tile.
 //
 // Memory bounds it where there are blocks enough: 4 x 8192 x 2048, f16 with fp32 decays, 1 - a:
-// 83 us, 98 % of what a copy reaches.  A single sequence of 2048 channels has 32 blocks and their
-// clusters, 128 SMs, and is bound by the exchange of a turn: 32768 tokens, bf16: 90 us, 68 %.  Packed
-// rows cost the marks (4.5 us) and the look at them: 16000 tokens, f16: 71 us, unpacked 50.  Rows that
+// 86 us, 96 % of what a copy reaches (without 1 - a 80 us).  A single sequence of 2048 channels has 32 blocks and
+// their clusters, 128 SMs, and is bound by the exchange of a turn: 32768 tokens, bf16: 96 us, 64 %.  Packed
+// rows cost the marks (4.5 us) and the look at them: 16000 tokens, f16: 74 us, unpacked 50.  Rows that
 // TMA cannot address are copied by their threads: 4 x 1000 x 2047: 33 us, 31 %.
 #include <cstring>
 
@@ -285,9 +285,9 @@ cudaError_t launch_shape(const ScanParams& p, int x_dtype, int g_dtype, bool wid
   });
 }
 cudaError_t launch_forward(ScanParams p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
-  // (blocks: a sequence's channels, before clusters.  us, Long and Short: 4 x 8192 x 2048 f16, 128 blocks, 84
-  // and 127; 1 x 1024 x 2048, 32 blocks, 8.0 and 9.0; 8 x 4096 x 2048 bf16, 256 blocks, 74 and 69; 64 x 512 x
-  // 2048 f16, 2048 blocks, 100 and 87)
+  // (blocks: a sequence's channels, before clusters.  us, Long and Short, as the shapes came: 4 x 8192 x 2048
+  // f16, 128 blocks, 84 and 127; 1 x 1024 x 2048, 32 blocks, 8.0 and 9.0; 8 x 4096 x 2048 bf16, 256 blocks, 74
+  // and 69; 64 x 512 x 2048 f16, 2048 blocks, 100 and 87)
   const bool is_long = (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels) <= kSms;
   if (is_long) {
     choose_cluster<Long>(p);

@@ -135,6 +135,7 @@ struct Shape {
   static constexpr int kParts = kWork / kLanes;        // half warps, each with kRun tokens of a tile
   static constexpr int kTile = kParts * kRun;
   static_assert(kParts % CARRY == 0, "shares of the parts");
+  static_assert(kParts <= 32, "append() counts on it");
 };
 
 // ---------------------------------------------------------------------------
@@ -337,7 +338,7 @@ struct RowMask {
 // Calls f with whether the rows have to be looked at one by one: branches between the rows of a
 // run keep the next rows' reads behind them.  (Packed 16000 tokens of 2048 channels, f16: 23
 // sequences, gradient 132 us to 120; of one 130 to 113; of 128, where most tiles have a boundary,
-// 152 to 176.)
+// 152 to 176: documents of 100 tokens pay for those of 700 and more.)
 template <bool PACKED, typename F>
 __device__ __forceinline__ void by_rows(bool plain, F f) {
   if constexpr (PACKED) {
@@ -397,8 +398,8 @@ __device__ __forceinline__ float2 pass_on(const Piece& q, float2 h) {
   return PACKED && is_cut(q.r) ? q.h : v;
 }
 // `q`, and `next` behind it in the direction of the walk: (c1 + r1) (c2 + r2).  (Where c stays 1 through a tile its
-// 16 parts or less have decays of exp(-1/8) at least: of 1 + r >= exp(-2) the rounding of r
-// costs three bits at most.)
+// 32 parts or less have decays of exp(-1/8) at least: of 1 + r >= exp(-4) a rounding of r costs six
+// bits at most, 27 x 2^-24 of what a state of 128 tokens keeps; those tokens' own roundings come to more.)
 template <bool PACKED>
 __device__ __forceinline__ void append(Piece& q, const Piece& next) {
   q.h = pass_on<PACKED>(next, q.h);
@@ -430,7 +431,8 @@ __device__ __forceinline__ float2& pair(float* row, int i) { return reinterpret_
 // ---------------------------------------------------------------------------
 // Every block sends its tile's piece to all of them (itself too) by st.async, which counts its
 // bytes on the receiver's barrier: nothing is fenced, so no block waits for its own stores
-// to memory as a cluster's barrier would (B = 4, T = 8192, D = 2048: 189 us for 145).
+// to memory as a cluster's barrier would (in the first tiled kernel, 4 x 8192 x 2048: 189 us with a
+// barrier, 145 with this).
 // Two turns of pieces, a barrier each: a block sends turn k + 2 when it has all of turn k + 1,
 // which every block sends when it is done with turn k.
 constexpr int kRowFloats = 3 * kChannels;
@@ -575,8 +577,9 @@ cudaError_t by_flags(bool a, bool b, bool c, F f) {
   return b ? (c ? f(No{}, Yes{}, Yes{}) : f(No{}, Yes{}, No{})) : (c ? f(No{}, No{}, Yes{}) : f(No{}, No{}, No{}));
 }
 
-// Sets tiles and cluster: as many blocks to a sequence as the device holds at once, and has
-// tiles for.
+// Sets tiles and cluster: as many blocks to a sequence as there are SMs for, and tiles.  (The SMs of a cluster lie
+// together, so that not every count of clusters that 148 SMs have room for is there at once: 32768 tokens,
+// bf16, take 96 us with 32 x 4 blocks of 2048 channels, but 157 with 29 x 5 of 1856.)
 template <typename SHAPE>
 void choose_cluster(ScanParams& p) {
   p.tiles = (p.T + SHAPE::kTile - 1) / SHAPE::kTile;

@@ -5,7 +5,7 @@
 // It needs h_{t-1} in 32 bits: h is in x's type, so a tile's states are computed again from
 // the checkpoint that the forward pass left at its start.  The blocks, threads and pieces are
 // those of scan_kernel (kda_scan.cu), the tiles taken from the last to the first.
-// Memory bounds it: 4 x 8192 x 2048, bf16 with fp32 decays: 154 us, 93 % of what a copy reaches.
+// Memory bounds it: 4 x 8192 x 2048, bf16 with fp32 decays: 157 us, 91 % of what a copy reaches.
 #include <type_traits>
 
 #include "kda_scan.cuh"
@@ -322,7 +322,7 @@ cudaError_t launch_shape(ScanParams p, bool wide, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_grad(const ScanParams& p, int x_dtype, int g_dtype, bool wide, cudaStream_t s) {
-  // (us, Long and Short: 4 x 8192 x 2048 bf16, 128 blocks, 152 and 165; 1 x 4096 x 2048, 32 blocks, 27 and 31;
+  // (us, Long and Short, as the shapes came: 4 x 8192 x 2048 bf16, 128 blocks, 152 and 165; 1 x 4096 x 2048, 32 blocks, 27 and 31;
   // 16 x 2048 x 2048, 512 blocks, 166 and 205; 64 x 512 x 2048, 2048 blocks, 178 and 155)
   const bool is_long =
       (int64_t)(p.q_start ? 1 : p.B) * ((p.D + kChannels - 1) / kChannels) <= kSms || p.T >= 1024;

@@ -5,13 +5,16 @@ Restates the definitions of ``include/kda_b200.h`` (KdaScanArgs, KdaQkArgs) in
 float64 torch, token by token and head by head, each value with a bound on what
 fp32 arithmetic may add to it.  Only ``tests/`` may import it.
 
-Bounds of the recurrence.  ``U = 2^-24``.  One token's decay is off by at most ``4 U`` (expf: 2
-units in the last place) of itself, its product and sum by ``2 U`` of the magnitudes that
-go in; joining pieces of a sequence by their decays adds two roundings a join and, where a
-decay is the exponential of a sum of eight ``g``, ``7 U |sum of g|``.  There is at most one join
-a token, so a token adds at most ``(8 + 8 |g|) U`` of the magnitude ``m_t = a_t m_{t-1} +
-|w_t x_t|``, and the error obeys ``e_t = a_t e_{t-1} + (8 + 8 |g_t|) U m_t``.  ``1 - a`` is
-off by ``4 U a / (1 - a) <= 15 U`` of itself where ``a <= exp(-1/4)``, and by less where a - 1 is held.
+Bounds of the recurrence.  ``U = 2^-24``.  One token's decay is off by at most ``(4 + 1.5 |g|) U`` of itself (the
+exponent ``g log2 e`` by its rounding and its constant's, the power of two by ``4 U``), its product and sum by
+``U`` of the magnitudes that go in: ``(5 + 1.5 |g|) U``.  From one run of four tokens to the next a state is multiplied by
+the exponential of the run's sum ``G``, off by ``(4 + 1.5 |G|) U`` and by ``3 U |G|`` for the sum, in two roundings: ``(6 + 4.5
+|G|) U`` a run.  Joining runs' decays before they meet a state rounds each product: at most ``3 x 27 U`` a run where the
+two-part decay has become small (``1 + r >= exp(-4)``), which only a state of 32 runs has, and less than one
+``U`` a token before.  So a token adds at most ``(8 + 8 |g|) U`` of the magnitude ``m_t = a_t m_{t-1} + |w_t x_t|``, and the
+error obeys ``e_t = a_t e_{t-1} + (8 + 8 |g_t|) U m_t``.  ``1 - a`` is off by ``2.4 U`` of itself nearer than ``|g| = 1/2``, and
+beyond by ``(4 + 1.5 |g|) U a / (1 - a) + U <= 8.4 U``; with the product by ``x``, and as a value that is multiplied again,
+below ``15 U``.
 """
 
 from __future__ import annotations
