@@ -38,6 +38,18 @@ cudaError_t launch_dependent(void (*k)(Params...), dim3 grid, int threads, size_
   return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...);
 }
 
+// For the entry points' checks.
+inline int size_of(int dt) { return dt == KDA_DTYPE_F32 ? 4 : 2; }
+inline bool misaligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+// of the current device
+inline int check_device() {
+  int dev = 0, major = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
+    return KDA_ERR_LAUNCH;
+  return major == 10 ? KDA_OK : KDA_ERR_ARCH;
+}
+
 namespace mla {
 int read_device_error(bool clear);   // the MLA kernels' error word (mla_decode.cu)
 }

@@ -526,9 +526,6 @@ __global__ void __launch_bounds__(1024) weight_kernel(const QkParams p, int64_t 
   else st(static_cast<__nv_bfloat16*>(p.dw[which]) + at, (float)s);
 }
 
-int size_of(int dt) { return dt == KDA_DTYPE_F32 ? 4 : 2; }
-bool misaligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
-
 int validate(const KdaQkArgs* a) {
   if (a == nullptr) return KDA_ERR_NULL_POINTER;
   if (a->abi_version != KDA_B200_ABI_VERSION) return KDA_ERR_SHAPE;
@@ -663,14 +660,6 @@ bool plan(const KdaQkArgs* a, QkParams& p, bool grad, HeadShape& h) {
     cut(p, p.heads[0] + p.heads[1], kThreads / 32 * 4, kSms * 16);
   }
   return vec != 0;
-}
-
-int check_device() {
-  int dev = 0, major = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
-    return KDA_ERR_LAUNCH;
-  return major == 10 ? KDA_OK : KDA_ERR_ARCH;
 }
 
 template <bool GRAD>

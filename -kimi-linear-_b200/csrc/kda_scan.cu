@@ -350,9 +350,6 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, 
   }
 }
 
-int size_of(int dt) { return dt == KDA_DTYPE_F32 ? 4 : 2; }
-bool misaligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
-
 enum class Pass { kForward, kBackward, kToken };
 
 int validate_sizes(const KdaScanArgs* a) {
@@ -409,14 +406,6 @@ ScanParams to_params(const KdaScanArgs* a) {
   p.hasty = a->hasty != 0;
   p.slots = a->slots; p.num_states = a->num_states; p.scatter = a->scatter != 0;
   return p;
-}
-
-int check_device() {
-  int dev = 0, major = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
-    return KDA_ERR_LAUNCH;
-  return major == 10 ? KDA_OK : KDA_ERR_ARCH;
 }
 
 size_t workspace_bytes(const KdaScanArgs* a) {

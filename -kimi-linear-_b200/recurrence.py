@@ -26,14 +26,9 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from .ops import _DT, _check_tensors, _launch, _needs_grad, _no_tangents
+from .ops import _DT, _check_tensors, _inner_contig, _launch, _needs_grad, _no_tangents
 
 _NONE2, _NONE3 = (0, 0), (0, 0, 0)
-
-
-def _unit(t):
-    """``t`` with a unit innermost stride."""
-    return t if t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
 
 
 def _bt(t, packed):
@@ -111,8 +106,8 @@ def _forward(x, g, state, q_start, complement, keep):
     """``(h, S, checkpoints)`` for operands that :func:`_check` has passed;
     ``keep``: checkpoints for the backward pass are wanted."""
     packed = q_start is not None
-    x, g = _unit(x), _unit(g)
-    state = None if state is None else _unit(state.float())
+    x, g = _inner_contig(x), _inner_contig(g)
+    state = None if state is None else _inner_contig(state.float())
     B, T, D = q_start.shape[0] - 1 if packed else x.shape[0], x.shape[-2], x.shape[-1]
     h = x.new_empty(x.shape)
     S = x.new_empty((B, D), dtype=torch.float32)
@@ -170,13 +165,13 @@ class _GatedScan(torch.autograd.Function):
 
 def _backward(x, g, state, q_start, complement, ckpt, dh, dS, need):
     packed = q_start is not None
-    x, g = _unit(x), _unit(g)
-    state32 = None if state is None else _unit(state.float())
+    x, g = _inner_contig(x), _inner_contig(g)
+    state32 = None if state is None else _inner_contig(state.float())
     B, T, D = q_start.shape[0] - 1 if packed else x.shape[0], x.shape[-2], x.shape[-1]
     if dh is not None:
-        dh = _unit(dh.to(x.dtype))
+        dh = _inner_contig(dh.to(x.dtype))
     if dS is not None:
-        dS = _unit(dS.float())
+        dS = _inner_contig(dS.float())
     dx = x.new_empty(x.shape) if need[0] else None
     dg = g.new_empty(g.shape) if need[1] else None
     dstate = ckpt.new_empty((B, D)) if need[2] and state is not None else None
@@ -248,8 +243,8 @@ def gated_step(x, g, state=None, slots=None, *, complement=False, inplace=False)
             raise RuntimeError(f"{fn}: inplace needs states with a unit innermost stride that do not "
                                f"overlap")
     elif state is not None:
-        state = _unit(state)
-    x, g = _unit(x), _unit(g)
+        state = _inner_contig(state)
+    x, g = _inner_contig(x), _inner_contig(g)
     h = x.new_empty(shape)
     S = state if inplace else x.new_empty((B, D), dtype=torch.float32)
     a = _args(B, 1, x, g, complement, (x.data_ptr(), x.stride(0), 0), (g.data_ptr(), g.stride(0), 0),

@@ -20,15 +20,11 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DT, _check_tensors, _launch, _needs_grad, _no_tangents
+from .ops import _DT, _check_tensors, _inner_contig, _launch, _needs_grad, _no_tangents
 
 NORMS = {None: _lib.NORM_NONE, "rms": _lib.NORM_RMS, "l2": _lib.NORM_L2}
 MAX_D = 512
 _NONE = (0, 0, 0, 0)              # pointer and strides of an operand that is not there
-
-
-def _unit(t):
-    return t if t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
 
 
 def _bth(t):
@@ -119,7 +115,7 @@ def _args(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, y=_NONE2, d
 
 
 def _forward(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved):
-    q, k = _unit(q), None if k is None else _unit(k)
+    q, k = _inner_contig(q), None if k is None else _inner_contig(k)
     oq, ok = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
     a, keep = _args(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, y=_two(oq, ok))
     _launch("qk_norm_rope", _lib.load().kda_qk_fwd, a, q.device)
@@ -174,9 +170,9 @@ class _QkNormRope(torch.autograd.Function):
 
 
 def _backward(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, dq, dk, need):
-    q, k = _unit(q), None if k is None else _unit(k)
-    dq = _unit(dq.to(q.dtype))
-    dk = None if k is None else _unit(dk.to(k.dtype))
+    q, k = _inner_contig(q), None if k is None else _inner_contig(k)
+    dq = _inner_contig(dq.to(q.dtype))
+    dk = None if k is None else _inner_contig(dk.to(k.dtype))
     oq, ok = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
     dw = [w.new_empty(w.shape) if w is not None and n else None for w, n in ((wq, need[2]), (wk, need[3]))]
     a, keep = _args(q, k, wq, wk, norm, eps, positions, inv_freq, interleaved, dy=_two(dq, dk), dx=_two(oq, ok),
