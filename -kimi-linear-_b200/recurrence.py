@@ -133,7 +133,8 @@ def gated_scan(x, g, initial_state=None, q_start=None, *, complement=False):
     no sequence and give zeros; a sequence without rows gives its initial state.
 
     Differentiable in ``x``, ``g`` and ``initial_state``.  ``x`` f32, f16 or bf16,
-    ``g`` fp32 or ``x``'s type.  A state of any floating type is read as fp32."""
+    ``g`` fp32 or ``x``'s type.  A state of any floating type is read as fp32.  What is not finite
+    goes on as the formula has it, but that a decay below 2^-126 counts as zero."""
     fn = "gated_scan"
     B = _batch(fn, x, q_start)
     initial_state = _read_as_float(initial_state)

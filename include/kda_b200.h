@@ -423,7 +423,7 @@ size_t mla_cache_args_size(void);
  * rows q_start[b] .. q_start[b + 1] - 1; q_start ascends, rows outside
  * q_start[0] .. q_start[B] - 1 get zeros.  h_{-1} is state_in [B, D] or zero,
  * state_out [B, D] each sequence's last h (state_in where it has no token).
- * g is a log decay (<= 0).  States are fp32.
+ * g is a log decay (<= 0; an exponential below 2^-126 may count as zero).  States are fp32.
  *
  * kda_scan_fwd: h, state_out, and (ckpt not NULL) what kda_scan_bwd needs:
  *   kda_scan_ckpt_floats() values, the state that enters every 32nd token.
